@@ -198,8 +198,20 @@ typedef enum loom_kv_layout {
  * BF16 / FP32. */
 typedef enum loom_kv_dtype {
   LOOM_KV_DTYPE_BF16 = 0,
-  LOOM_KV_DTYPE_FP8_E4M3 = 1
+  LOOM_KV_DTYPE_FP8_E4M3 = 1,
+  /* OCP MXFP4 (no reference counterpart).  A row of 128 values is 64 bytes of
+   * E2M1 codes (value 2i in the low nibble of byte i; 0, 0.5, 1, 1.5, 2, 3, 4, 6
+   * and their negatives) and 4 E8M0 scale bytes, one per 32 values: value =
+   * code * 2^(scale - 127), and a scale of 255 makes its block NaN.  Pages are
+   * u8 [pool, P, Hkv, 64] (NHD) or [pool, Hkv, P, 64] (HND); the scales lie apart,
+   * u8 [pool, Hkv, P, 4] for both layouts.  68 bytes per row against 256 in BF16.
+   * Paged decode (loom_paged_decode_enqueue_mxfp4), the normed append
+   * (loom_norm_rope_append_*) and the read back (loom_paged_kv_read_*) take
+   * them; paged prefill and the reference-shaped append do not. */
+  LOOM_KV_DTYPE_MXFP4 = 2
 } loom_kv_dtype_t;
+#define LOOM_MXFP4_ROW_BYTES 64u  /* code bytes of a row of 128 values */
+#define LOOM_MXFP4_ROW_SCALES 4u  /* scale bytes of a row */
 
 /* ------------------------------------------------------------------------ */
 /* Paged batch-decode contract, crates/loom-infer/src/attention/paged_decode/mod.rs */
@@ -525,6 +537,34 @@ loom_status_t loom_paged_decode_enqueue_bf16(const loom_paged_decode_plan_t *pla
                                              loom_command_scope_t *scope,
                                              const loom_bf16_paged_batch_decode_args_t *args,
                                              loom_error_t *err);
+
+/* Operands over MXFP4 pages (no reference counterpart). */
+typedef struct loom_mxfp4_paged_batch_decode_args {
+  loom_handle_t query;         /* Read<bf16>  [B, Hq, 128] */
+  loom_handle_t key_pages;     /* Read<u8>    [pool, P, Hkv, 64] or [pool, Hkv, P, 64] */
+  loom_handle_t value_pages;   /* Read<u8>    likewise */
+  loom_handle_t key_scales;    /* Read<u8>    [pool, Hkv, P, 4] */
+  loom_handle_t value_scales;  /* Read<u8>    [pool, Hkv, P, 4] */
+  loom_handle_t page_indptr;   /* Read<i32>   [B+1] */
+  loom_handle_t page_indices;  /* Read<i32>   [>= B] */
+  loom_handle_t last_page_len; /* Read<i32>   [B] */
+  loom_handle_t output;        /* Write<bf16> [B, Hq, 128] */
+  loom_handle_t lse;           /* Write<f32>  [B, Hq], log2 domain */
+  loom_handle_t workspace;     /* Write<u8>   [plan workspace_bytes], or {0, 0}: the states lie
+                                  in the queue's workspace, as for
+                                  loom_paged_decode_enqueue_bf16 */
+} loom_mxfp4_paged_batch_decode_args_t;
+
+/* Paged decode of a plan whose spec names LOOM_KV_DTYPE_MXFP4: the same command,
+ * guards and algorithms over dequantised rows.  The codes become BF16 exactly, so
+ * O and LSE are those of the BF16 command over the values the pages hold.  Q, the
+ * pages, the scales, O and LSE on 4-byte boundaries.  The other enqueue forms
+ * refuse such a plan (LOOM_NULL_ARGUMENT "K_scales"), this one plans over BF16 and
+ * FP8 pages (LOOM_NULL_ARGUMENT "args"). */
+loom_status_t loom_paged_decode_enqueue_mxfp4(const loom_paged_decode_plan_t *plan,
+                                              loom_command_scope_t *scope,
+                                              const loom_mxfp4_paged_batch_decode_args_t *args,
+                                              loom_error_t *err);
 
 /* No counterpart in the reference.  For callers that cannot allocate device
  * memory at all (code under HIP graph capture, tight serving loops, harnesses
@@ -1020,6 +1060,123 @@ loom_status_t loom_rope_append_enqueue_bf16(const loom_rope_append_plan_t *plan,
 loom_status_t loom_rope_append_tokens_enqueue_bf16(
     const loom_rope_append_plan_t *plan, loom_command_scope_t *scope,
     const loom_bf16_rope_paged_kv_append_tokens_args_t *args, loom_error_t *err);
+
+/* ------------------------------------------------------------------------ */
+/* Norms of the query and key heads with the rotation and the paged append, in */
+/* one command (no reference counterpart).                                     */
+/*   y = x * w / sqrt(mean(x^2) + norm_eps)   per head of 128, norms only      */
+/*   NeoX rotation of y by position * rope_theta^(-2j/128), j = 0..63           */
+/* Q is rounded to BF16 once, K rows and the V rows (unchanged) go to their      */
+/* page slots as BF16, FP8 E4M3 or MXFP4.  Unlike the reference-shaped append's,  */
+/* the angle is a 64-bit product, so far positions keep their phase; K rows for   */
+/* MXFP4 pages are normed and rotated in 64 bits, so that which of two codes a    */
+/* value gets does not hang on the order of 32-bit sums.  MXFP4: of a block of   */
+/* 32 values the scale is 2^e, e = clamp(floor(log2 max|v|) - 2, -126, 125); a    */
+/* code is v / 2^e rounded to nearest even and saturated at 6; a block with a NaN  */
+/* or an infinity gets scale 255 and codes 0.                                     */
+typedef struct loom_norm_rope_append_spec {
+  loom_paged_decode_spec_t paged; /* layout, page size and element type of the pages */
+  uint64_t tokens;                /* the batch for the one-token form */
+  double rope_theta;
+  float norm_eps;                 /* 0: no norms */
+  int32_t explicit_tokens;        /* 0: one token per request, at kv_len - 1 */
+} loom_norm_rope_append_spec_t;
+
+/* `paged` as from loom_paged_decode_spec_new and its setters.  explicit_tokens = 0
+ * takes tokens = batch_size (LOOM_LENGTH_MISMATCH otherwise), explicit_tokens = 1
+ * any 1 .. LOOM_APPEND_MAX_TOKENS_EXTENDED tokens.  LOOM_INVALID_ROPE_THETA unless
+ * rope_theta is finite and greater than one; LOOM_INVALID_EPSILON unless norm_eps
+ * is 0 (no norms) or finite and positive. */
+loom_status_t loom_norm_rope_append_spec_new(const loom_paged_decode_spec_t *paged, uint64_t tokens,
+                                             int32_t explicit_tokens, double rope_theta,
+                                             float norm_eps, loom_norm_rope_append_spec_t *out,
+                                             loom_error_t *err);
+/* The plan (the append plan type: free and get_info as for the others; flags:
+ * LOOM_PLAN_PAGE_INDICES_CAPACITY and the append flags).  The reference-shaped and
+ * extended append enqueues refuse it (LOOM_NULL_ARGUMENT "args"). */
+loom_status_t loom_rope_provider_plan_norm_paged_append(const loom_rope_provider_t *provider,
+                                                        const loom_norm_rope_append_spec_t *spec,
+                                                        uint32_t flags,
+                                                        loom_rope_append_plan_t **out,
+                                                        loom_error_t *err);
+
+typedef struct loom_norm_rope_append_args {
+  loom_handle_t query;         /* Read<bf16> [T, Hq, 128] */
+  loom_handle_t key;           /* Read<bf16> [T, Hkv, 128] */
+  loom_handle_t value;         /* Read<bf16> [T, Hkv, 128] */
+  loom_handle_t batch_indices; /* Read<i32>  [T] (explicit form) */
+  loom_handle_t positions;     /* Read<i32>  [T] (explicit form) */
+  loom_handle_t page_indptr;   /* Read<i32>  [B+1] */
+  loom_handle_t page_indices;  /* Read<i32>  [>= B] */
+  loom_handle_t last_page_len; /* Read<i32>  [B] */
+  loom_handle_t query_norm;    /* Read<bf16> [128], the norms' weights; {0, 0} without norms */
+  loom_handle_t key_norm;      /* Read<bf16> [128] */
+  loom_handle_t query_output;  /* Write<bf16> [T, Hq, 128] */
+  loom_handle_t key_pages;     /* Write<bf16 or u8>, as the spec's element type has them */
+  loom_handle_t value_pages;
+  loom_handle_t key_scales;    /* Write<u8> [pool, Hkv, P, 4] for MXFP4 pages, else {0, 0} */
+  loom_handle_t value_scales;
+  loom_handle_t kv_scales;     /* Read<f32> [2] for FP8 pages, else {0, 0} */
+  loom_handle_t workspace;     /* Write<u8> [workspace_bytes], zero before its first command, or
+                                  {0, 0}: the queue's own */
+} loom_norm_rope_append_args_t;
+
+/* One command with the append's guards: invalid device metadata leaves every
+ * output untouched. */
+loom_status_t loom_norm_rope_append_enqueue(const loom_rope_append_plan_t *plan,
+                                            loom_command_scope_t *scope,
+                                            const loom_norm_rope_append_args_t *args,
+                                            loom_error_t *err);
+
+/* ------------------------------------------------------------------------ */
+/* Reading MXFP4 pages back (no reference counterpart): rows [start, start + n)  */
+/* of every request as BF16 rows [nnz_kv, Hkv, 128], n = kv_indptr[r + 1] -       */
+/* kv_indptr[r], as a ragged prefill reads them: a chunk of a prompt attends to    */
+/* its cached prefix that way.  Values that BF16 holds (all but those of scales   */
+/* above 252) come back exactly.                                                 */
+typedef struct loom_paged_kv_read_spec {
+  loom_paged_decode_spec_t paged; /* kv_dtype LOOM_KV_DTYPE_MXFP4; query heads unused */
+  uint64_t nnz_kv;                /* rows of the outputs */
+} loom_paged_kv_read_spec_t;
+/* LOOM_PLAN_INVALID_OPTION "kv_dtype" for other pages. */
+loom_status_t loom_paged_kv_read_spec_new(const loom_paged_decode_spec_t *paged, uint64_t nnz_kv,
+                                          loom_paged_kv_read_spec_t *out, loom_error_t *err);
+
+typedef struct loom_paged_kv_read_plan loom_paged_kv_read_plan_t;
+/* `flags`: 0 or LOOM_PLAN_PAGE_INDICES_CAPACITY. */
+loom_status_t loom_prefill_provider_plan_paged_kv_read(const loom_prefill_provider_t *provider,
+                                                       const loom_paged_kv_read_spec_t *spec,
+                                                       uint32_t flags,
+                                                       loom_paged_kv_read_plan_t **out,
+                                                       loom_error_t *err);
+void loom_paged_kv_read_plan_free(loom_paged_kv_read_plan_t *plan);
+
+typedef struct loom_paged_kv_read_args {
+  loom_handle_t key_pages;     /* Read<u8>  [pool, P, Hkv, 64] or [pool, Hkv, P, 64] */
+  loom_handle_t value_pages;
+  loom_handle_t key_scales;    /* Read<u8>  [pool, Hkv, P, 4] */
+  loom_handle_t value_scales;
+  loom_handle_t page_indptr;   /* Read<i32> [B+1] */
+  loom_handle_t page_indices;  /* Read<i32> [>= B] */
+  loom_handle_t last_page_len; /* Read<i32> [B] */
+  loom_handle_t kv_indptr;     /* Read<i32> [B+1]: output rows of each request, from 0 on, at
+                                  most nnz_kv in all; a request may have none */
+  loom_handle_t kv_start;      /* Read<i32> [B]: first token of each request, or {0, 0}: 0 */
+  loom_handle_t key;           /* Write<bf16> [nnz_kv, Hkv, 128] */
+  loom_handle_t value;         /* Write<bf16> [nnz_kv, Hkv, 128] */
+} loom_paged_kv_read_args_t;
+
+/* One command, one kernel, no workspace.  Device guards: kv_indptr that does not
+ * start at 0 or ends above nnz_kv, or a page_indptr with wrong ends, leaves every
+ * output untouched; a request with an invalid page range, last-page length or
+ * kv_indptr range, or rows outside its tokens, leaves its rows untouched, and so
+ * does a row whose page index is out of range.  Rows from kv_indptr[B] on are left
+ * as they are.  Requires a nondecreasing kv_indptr: of one that is not, some
+ * requests' rows may be left untouched. */
+loom_status_t loom_paged_kv_read_enqueue(const loom_paged_kv_read_plan_t *plan,
+                                         loom_command_scope_t *scope,
+                                         const loom_paged_kv_read_args_t *args,
+                                         loom_error_t *err);
 
 /* ------------------------------------------------------------------------ */
 /* Graph capture and replay, crates/loom-infer-cuda/src/graph/mod.rs           */

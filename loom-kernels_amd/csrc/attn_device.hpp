@@ -180,6 +180,24 @@ __device__ __forceinline__ uint32_t fp8_e4m3_from_f32(float x) {
   return s | code;
 }
 
+// MXFP4 storage.
+// Eight E2M1 codes with one E8M0 scale as BF16 pairs.  `scale`: the scale byte
+// in bits 23..30 (v_cvt_scalef32_pk_bf16_fp4 takes its scale's exponent and
+// ignores the other bits); exact, 2^-127 and the NaN scale among them.
+__device__ __forceinline__ u32x4 mx4x8_to_bf16x8(uint32_t w, uint32_t scale) {
+  const float s = __uint_as_float(scale);
+  u32x4 o;
+  o[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 0));
+  o[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 1));
+  o[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 2));
+  o[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 3));
+  return o;
+}
+// Byte b of a row's scale word moved to bits 23..30.
+__device__ __forceinline__ uint32_t mx_scale(uint32_t word, int b) {
+  return __builtin_amdgcn_alignbit(word, word, 8 * b + 9);
+}
+
 // OR of `p` over a workgroup of W waves with one barrier (HIP's
 // __syncthreads_or takes three and an LDS atomic): each wave publishes its
 // ballot in slots[wave].  `slots` belongs to one call site, and that site must

@@ -404,7 +404,8 @@ loom_status_t loom_paged_decode_spec_with_kv_dtype(const loom_paged_decode_spec_
                                                    loom_paged_decode_spec_t *out,
                                                    loom_error_t *err) {
   if (!spec || !out) return fail(err, LOOM_NULL_ARGUMENT, "spec");
-  if (kv_dtype != LOOM_KV_DTYPE_BF16 && kv_dtype != LOOM_KV_DTYPE_FP8_E4M3)
+  if (kv_dtype != LOOM_KV_DTYPE_BF16 && kv_dtype != LOOM_KV_DTYPE_FP8_E4M3 &&
+      kv_dtype != LOOM_KV_DTYPE_MXFP4)
     return fail(err, LOOM_PLAN_INVALID_OPTION, "kv_dtype", kv_dtype);
   *out = *spec;
   out->kv_dtype = kv_dtype;
@@ -850,6 +851,62 @@ loom_status_t loom_ragged_prefill_causal_kv_end(const loom_ragged_prefill_spec_t
   if ((int64_t)query_index >= ql) return LOOM_EMPTY_RAGGED_REQUEST;
   *end = (uint64_t)((int64_t)kv[request] + kl - ql + (int64_t)query_index + 1);
   return LOOM_OK;
+}
+
+// ---- normed append and read back (no reference counterpart) ------------------------
+// The geometry of an embedded paged spec: what spec_new and its setters let through.
+static loom_status_t check_paged(const loom_paged_decode_spec_t *p, loom_error_t *err) {
+  loom_paged_decode_spec_t t;
+  loom_status_t rc =
+      loom_paged_decode_spec_new(p->batch_size, p->max_num_pages, p->num_query_heads,
+                                 p->num_kv_heads, loom::kHeadDim, loom::kPageSize, &t, err);
+  if (rc) return rc;
+  if ((rc = loom_paged_decode_spec_with_kv_layout(p, p->kv_layout, &t, err))) return rc;
+  if ((rc = loom_paged_decode_spec_with_kv_dtype(p, p->kv_dtype, &t, err))) return rc;
+  return loom_paged_decode_spec_with_page_size(p, p->page_size ? p->page_size : LOOM_PAGE_SIZE, &t,
+                                               err);
+}
+
+loom_status_t loom_norm_rope_append_spec_new(const loom_paged_decode_spec_t *paged, uint64_t tokens,
+                                             int32_t explicit_tokens, double rope_theta,
+                                             float norm_eps, loom_norm_rope_append_spec_t *out,
+                                             loom_error_t *err) {
+  if (!paged || !out) return fail(err, LOOM_NULL_ARGUMENT, "paged");
+  const loom_status_t rc = check_paged(paged, err);
+  if (rc) return rc;
+  if (tokens == 0) return fail(err, LOOM_ZERO_DIMENSION);
+  if (explicit_tokens && tokens > LOOM_APPEND_MAX_TOKENS_EXTENDED)
+    return fail(err, LOOM_UNSUPPORTED_APPEND_TOKEN_COUNT, nullptr, LOOM_APPEND_MAX_TOKENS_EXTENDED,
+                tokens);
+  if (!explicit_tokens && tokens != paged->batch_size)
+    return fail(err, LOOM_LENGTH_MISMATCH, "tokens", paged->batch_size, tokens);
+  if (!std::isfinite(rope_theta) || rope_theta <= 1.0)
+    return fail(err, LOOM_INVALID_ROPE_THETA, nullptr, 0, 0, 0, 0, rope_theta);
+  if (!std::isfinite(norm_eps) || norm_eps < 0.0f)
+    return fail(err, LOOM_INVALID_EPSILON, nullptr, 0, 0, 0, 0, norm_eps);
+  out->paged = *paged;
+  out->tokens = tokens;
+  out->rope_theta = rope_theta;
+  out->norm_eps = norm_eps;
+  out->explicit_tokens = explicit_tokens ? 1 : 0;
+  return loom::ok(err);
+}
+
+loom_status_t loom_paged_kv_read_spec_new(const loom_paged_decode_spec_t *paged, uint64_t nnz_kv,
+                                          loom_paged_kv_read_spec_t *out, loom_error_t *err) {
+  if (!paged || !out) return fail(err, LOOM_NULL_ARGUMENT, "paged");
+  const loom_status_t rc = check_paged(paged, err);
+  if (rc) return rc;
+  if (paged->kv_dtype != LOOM_KV_DTYPE_MXFP4)
+    return fail(err, LOOM_PLAN_INVALID_OPTION, "kv_dtype", paged->kv_dtype);
+  uint64_t t;
+  if (nnz_kv == 0) return fail(err, LOOM_ZERO_DIMENSION);
+  if (nnz_kv > (uint64_t)INT32_MAX || mul_ovf(nnz_kv, paged->num_kv_heads, &t) ||
+      mul_ovf(t, loom::kHeadDim, &t))
+    return fail(err, LOOM_ELEMENT_COUNT_OVERFLOW);
+  out->paged = *paged;
+  out->nnz_kv = nnz_kv;
+  return loom::ok(err);
 }
 
 }  // extern "C"

@@ -1,0 +1,241 @@
+// Reading MXFP4 pages back as BF16 rows for gfx950 (no reference counterpart).
+//
+// out[kv_indptr[r] + i] = codes * 2^(scale - 127) of token kv_start[r] + i of
+// request r, for K and V and every kv-head: the contiguous rows that a ragged
+// prefill reads.
+//
+// Each head's row is 68 bytes read and 256 written, twice (K and V), with no
+// arithmetic but the conversion, so the kernel is bound by the memory rate, four
+// fifths of it writes.  One workgroup takes 16 output rows: its first wave finds
+// their requests and pages (three dependent round trips, whatever the batch), then
+// 16 lanes per head row load 4 code bytes each and store 16 bytes, K and V
+// together, the heads of a row contiguous.
+#include <hip/hip_runtime.h>
+
+#include "attn_device.hpp"
+#include "loom_internal.hpp"
+
+using loom::fail;
+using namespace loom_dev;
+
+namespace {
+
+constexpr int kReadThreads = 256;
+constexpr int kReadRows = 16;  // output rows per workgroup
+
+struct ReadArgs {
+  const uint8_t *k;
+  const uint8_t *v;
+  const uint8_t *k_mx;
+  const uint8_t *v_mx;
+  const int32_t *indptr;
+  const int32_t *indices;
+  const int32_t *last;
+  const int32_t *kv_indptr;
+  const int32_t *kv_start;  // null: every request from its first token on
+  uint16_t *k_out;
+  uint16_t *v_out;
+  int64_t pool;
+  int64_t n_indices;
+  int32_t indices_capacity;
+  int32_t batch;
+  int32_t hkv;
+  int32_t nnz;
+  int32_t page_rows;
+  int32_t head_bytes;  // NHD: 64; HND pages: page_rows * 64
+  int32_t row_bytes;   // NHD: hkv * 64; HND pages: 64
+};
+
+// Largest request r <= batch with kv_indptr[r] <= t, by one wave: 64 entries a
+// round trip.  (kv_indptr[0] = 0 <= t.)  Wave-uniform.
+__device__ __forceinline__ int request_of(const ReadArgs &a, int t, int lane) {
+  int lo = 0, n = a.batch + 1;  // the answer is one of [lo, lo + n)
+  while (n > 1) {
+    const int step = (n + 63) / 64;
+    const int at = lane * step;
+    const bool le = at < n && a.kv_indptr[lo + at] <= t;
+    const int k = __builtin_popcountll(__builtin_amdgcn_ballot_w64(le));
+    const int skip = max(k - 1, 0) * step;  // entries 0 .. k - 1 of this round are <= t
+    lo += skip;
+    n = min(step, n - skip);
+  }
+  return lo;
+}
+
+__global__ __launch_bounds__(kReadThreads) void paged_kv_read_kernel(ReadArgs a) {
+  __shared__ int32_t s_page[kReadRows], s_off[kReadRows];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int t0 = (int)blockIdx.x * kReadRows;
+  const int rows = min(kReadRows, a.nnz - t0);
+  if (tid < 64) {
+    const int32_t ip0 = a.indptr[0], ipB = a.indptr[a.batch];
+    const int32_t kv0 = a.kv_indptr[0], kvB = a.kv_indptr[a.batch];
+    const bool ok = ip0 == 0 && ipB >= 0 && kv0 == 0 && kvB >= 0 && kvB <= a.nnz &&
+                    (a.indices_capacity ? (int64_t)ipB <= a.n_indices : (int64_t)ipB == a.n_indices);
+    int page = -1, off = 0;
+    if (ok) {
+      const int r0 = uni(request_of(a, t0, lane));
+      // Row j belongs to request r0 + the number of later starts that are <= its
+      // index; more than 64 of those (empty requests): searched again.
+      const int32_t next = r0 + 1 + lane <= a.batch ? a.kv_indptr[r0 + 1 + lane] : INT32_MAX;
+      int r = r0;
+#pragma unroll
+      for (int j = 0; j < kReadRows; ++j) {
+        const int more = __builtin_popcountll(__builtin_amdgcn_ballot_w64(next <= t0 + j));
+        const int rj = more < 64 ? r0 + more : request_of(a, t0 + j, lane);
+        if (lane == j) r = rj;
+      }
+      if (lane < rows && r < a.batch) {
+        const int t = t0 + lane;
+        const int32_t st = a.indptr[r], en = a.indptr[r + 1], tl = a.last[r];
+        const int32_t b = a.kv_indptr[r], e = a.kv_indptr[r + 1];
+        const int32_t start = a.kv_start ? a.kv_start[r] : 0;
+        const int64_t kv_len = ((int64_t)en - st - 1) * a.page_rows + tl;
+        if (st >= 0 && en > st && en <= ipB && tl >= 1 && tl <= a.page_rows && b >= 0 && b <= t &&
+            t < e && start >= 0 && (int64_t)start + (e - b) <= kv_len) {
+          const int p = start + (t - b);
+          const int32_t idx = a.indices[st + p / a.page_rows];
+          if (idx >= 0 && (int64_t)idx < a.pool) {
+            page = idx;
+            off = p % a.page_rows;
+          }
+        }
+      }
+    }
+    if (lane < kReadRows) {
+      s_page[lane] = page;
+      s_off[lane] = off;
+    }
+  }
+  __syncthreads();
+  const int c = tid & 15;
+  const int64_t page_bytes = (int64_t)a.page_rows * a.hkv * 64;
+#pragma unroll 2
+  for (int i = tid >> 4; i < rows * a.hkv; i += kReadThreads / 16) {
+    const int j = i / a.hkv, h = i - j * a.hkv;
+    const int page = s_page[j], off = s_off[j];
+    if (page < 0) continue;
+    const int64_t at =
+        page * page_bytes + (int64_t)h * a.head_bytes + (int64_t)off * a.row_bytes + c * 4;
+    const int64_t sc = ((((int64_t)page * a.hkv + h) * a.page_rows + off) << 2) + (c >> 2);
+    const uint32_t kc = *reinterpret_cast<const uint32_t *>(a.k + at);
+    const uint32_t vc = *reinterpret_cast<const uint32_t *>(a.v + at);
+    const uint32_t ks = a.k_mx[sc], vs = a.v_mx[sc];
+    const int64_t out = ((int64_t)(t0 + j) * a.hkv + h) * 128 + c * 8;
+    *reinterpret_cast<u32x4 *>(a.k_out + out) = mx4x8_to_bf16x8(kc, ks << 23);
+    *reinterpret_cast<u32x4 *>(a.v_out + out) = mx4x8_to_bf16x8(vc, vs << 23);
+  }
+}
+
+}  // namespace
+
+struct loom_paged_kv_read_plan {
+  loom_paged_kv_read_spec_t spec{};
+  uint32_t flags = 0;
+};
+
+extern "C" {
+
+loom_status_t loom_prefill_provider_plan_paged_kv_read(const loom_prefill_provider_t *provider,
+                                                       const loom_paged_kv_read_spec_t *spec,
+                                                       uint32_t flags,
+                                                       loom_paged_kv_read_plan_t **out,
+                                                       loom_error_t *err) {
+  if (!provider || !spec || !out) return fail(err, LOOM_NULL_ARGUMENT, "provider");
+  if (flags & ~LOOM_PLAN_PAGE_INDICES_CAPACITY)
+    return fail(err, LOOM_PLAN_INVALID_OPTION, "flags", flags);
+  loom_paged_kv_read_spec_t s;
+  const loom_status_t rc = loom_paged_kv_read_spec_new(&spec->paged, spec->nnz_kv, &s, err);
+  if (rc) return rc;
+  // requests and heads are indexed in 32 bits
+  if (s.paged.batch_size >= (uint64_t)INT32_MAX)
+    return fail(err, LOOM_PLAN_STATE_COUNT_OUT_OF_RANGE, "K/V read batch", s.paged.batch_size);
+  if (s.paged.num_kv_heads > (uint64_t)INT32_MAX / (64 * 64))
+    return fail(err, LOOM_PLAN_STATE_COUNT_OUT_OF_RANGE, "K/V read heads", s.paged.num_kv_heads);
+  auto *p = new loom_paged_kv_read_plan;
+  p->spec = s;
+  p->flags = flags;
+  *out = p;
+  return loom::ok(err);
+}
+
+void loom_paged_kv_read_plan_free(loom_paged_kv_read_plan_t *p) { delete p; }
+
+loom_status_t loom_paged_kv_read_enqueue(const loom_paged_kv_read_plan_t *plan,
+                                         loom_command_scope_t *scope,
+                                         const loom_paged_kv_read_args_t *args,
+                                         loom_error_t *err) {
+  if (!plan || !scope || !args) return fail(err, LOOM_NULL_ARGUMENT, "plan");
+  const loom_paged_decode_spec_t &s = plan->spec.paged;
+  const loom::OperandSpec ops[11] = {
+      {"K_pages", LOOM_DTYPE_U8, false},      {"V_pages", LOOM_DTYPE_U8, false},
+      {"K_scales", LOOM_DTYPE_U8, false},     {"V_scales", LOOM_DTYPE_U8, false},
+      {"page_indptr", LOOM_DTYPE_I32, false}, {"page_indices", LOOM_DTYPE_I32, false},
+      {"last_page_len", LOOM_DTYPE_I32, false}, {"kv_indptr", LOOM_DTYPE_I32, false},
+      {"K", LOOM_DTYPE_BF16, true},           {"V", LOOM_DTYPE_BF16, true},
+      {"kv_start", LOOM_DTYPE_I32, false}};
+  const loom_handle_t hs[11] = {args->key_pages,    args->value_pages,  args->key_scales,
+                                args->value_scales, args->page_indptr,  args->page_indices,
+                                args->last_page_len, args->kv_indptr,   args->key,
+                                args->value,        args->kv_start};
+  const int n = args->kv_start.set_id != 0 ? 11 : 10;
+  const loom::Lease *l[11];
+  loom_status_t rc = loom::resolve_command(scope, hs, ops, n, l, err);
+  if (rc) return rc;
+  const uint64_t page_rows = s.page_size ? s.page_size : loom::kPageSize;
+  const uint64_t rows = s.max_num_pages * page_rows * s.num_kv_heads;
+  const uint64_t on = plan->spec.nnz_kv * s.num_kv_heads * loom::kHeadDim;
+  const uint64_t want[11] = {rows * LOOM_MXFP4_ROW_BYTES,
+                             rows * LOOM_MXFP4_ROW_BYTES,
+                             rows * LOOM_MXFP4_ROW_SCALES,
+                             rows * LOOM_MXFP4_ROW_SCALES,
+                             s.batch_size + 1,
+                             0,
+                             s.batch_size,
+                             s.batch_size + 1,
+                             on,
+                             on,
+                             s.batch_size};
+  for (int i = 0; i < n; ++i) {
+    if (i == 5) {
+      if (l[5]->numel < s.batch_size)
+        return fail(err, LOOM_ENQ_PAGE_INDICES_TOO_SHORT, nullptr, s.batch_size, l[5]->numel);
+      continue;
+    }
+    if (l[i]->numel != want[i])
+      return fail(err, LOOM_ENQ_LENGTH_MISMATCH, ops[i].name, want[i], l[i]->numel);
+  }
+  // 4-byte boundaries, as for the other commands over pages (16-byte accesses
+  // need no more on gfx950).
+  for (int i : {0, 1, 2, 3, 8, 9})
+    if (l[i]->ptr % 4 != 0)
+      return fail(err, LOOM_ENQ_MISALIGNED_BUFFER, ops[i].name, (int64_t)l[i]->ptr, 4);
+  ReadArgs a{};
+  a.k = (const uint8_t *)l[0]->ptr;
+  a.v = (const uint8_t *)l[1]->ptr;
+  a.k_mx = (const uint8_t *)l[2]->ptr;
+  a.v_mx = (const uint8_t *)l[3]->ptr;
+  a.indptr = (const int32_t *)l[4]->ptr;
+  a.indices = (const int32_t *)l[5]->ptr;
+  a.last = (const int32_t *)l[6]->ptr;
+  a.kv_indptr = (const int32_t *)l[7]->ptr;
+  a.kv_start = n == 11 ? (const int32_t *)l[10]->ptr : nullptr;
+  a.k_out = (uint16_t *)l[8]->ptr;
+  a.v_out = (uint16_t *)l[9]->ptr;
+  a.pool = (int64_t)s.max_num_pages;
+  a.n_indices = (int64_t)l[5]->numel;
+  a.indices_capacity = (plan->flags & LOOM_PLAN_PAGE_INDICES_CAPACITY) ? 1 : 0;
+  a.batch = (int32_t)s.batch_size;
+  a.hkv = (int32_t)s.num_kv_heads;
+  a.nnz = (int32_t)plan->spec.nnz_kv;
+  a.page_rows = (int32_t)page_rows;
+  const bool hnd = s.kv_layout == LOOM_KV_LAYOUT_HND;
+  a.head_bytes = hnd ? a.page_rows * 64 : 64;
+  a.row_bytes = hnd ? 64 : a.hkv * 64;
+  const unsigned grid = (unsigned)((plan->spec.nnz_kv + kReadRows - 1) / kReadRows);
+  hipLaunchKernelGGL(paged_kv_read_kernel, dim3(grid), dim3(kReadThreads), 0, scope->queue->stream,
+                     a);
+  return loom::record_launch(scope, hipGetLastError(), err);
+}
+
+}  // extern "C"

@@ -173,6 +173,16 @@ struct AppendArgs {
   float inv_freq[64];
 };
 
+// Operands of the normed append (loom_norm_rope_append_*) beside those.
+struct NormAppendArgs : AppendArgs {
+  const uint16_t *q_norm;  // [128] weights of the head norms; null: no norms
+  const uint16_t *k_norm;
+  uint8_t *k_mx;  // MXFP4 pages: E8M0 bytes [pool, Hkv, page_rows, 4]
+  uint8_t *v_mx;
+  float eps;
+  double inv_freq64[64];
+};
+
 // Request and token geometry shared by both kernels.  Returns false for any
 // invalid mapping; on success fills the physical slot.
 // Entries of page_indices that belong to the page table: all of them, or the
@@ -495,12 +505,250 @@ __device__ __forceinline__ void apply_row(const AppendArgs &a, int t, int64_t pa
   }
 }
 
+// ---- the normed append ----------------------------------------------------------
+// Row c ^ 8 of the same 16 lanes (a rotation by 8), and sums over the 16 lanes
+// and maxima over 4 of them (the lanes of one MXFP4 block), on DPP.
+__device__ __forceinline__ uint32_t dpp_other_half(uint32_t x) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x128, 0xf, 0xf, false);
+}
+template <int CTRL>
+__device__ __forceinline__ float dpp_f32(float x) {
+  return __uint_as_float(
+      (uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(x), CTRL, 0xf, 0xf, false));
+}
+template <int CTRL>
+__device__ __forceinline__ double dpp_f64(double x) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo =
+      (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, 0xf, 0xf, false);
+  const uint32_t hi =
+      (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, 0xf, 0xf, false);
+  return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
+}
+__device__ __forceinline__ float dpp_value(float x, int) { return dpp_f32<0x128>(x); }
+__device__ __forceinline__ double dpp_value(double x, int) { return dpp_f64<0x128>(x); }
+__device__ __forceinline__ float row_sum(float x) {
+  x += dpp_f32<0x128>(x);
+  x += dpp_f32<0x124>(x);
+  x += dpp_f32<0x122>(x);
+  return x + dpp_f32<0x121>(x);
+}
+__device__ __forceinline__ double row_sum(double x) {
+  x += dpp_f64<0x128>(x);
+  x += dpp_f64<0x124>(x);
+  x += dpp_f64<0x122>(x);
+  return x + dpp_f64<0x121>(x);
+}
+__device__ __forceinline__ uint32_t block_max(uint32_t x) {  // over lanes 4i .. 4i + 3
+  x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0xB1, 0xf, 0xf, false));
+  return max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x4E, 0xf, 0xf, false));
+}
+
+__device__ __forceinline__ float bf16_at(const u32x4 &x, int i) {
+  return __uint_as_float((i & 1) ? (x[i >> 1] & 0xffff0000u) : (x[i >> 1] << 16));
+}
+
+// The 8 values of lane c of a head row: normed by `w` (the lane's 8 weights)
+// when `norm`, and rotated; computed in F (float or double).  `sn`, `cs`: the
+// token's 64 sines and cosines.
+template <class F>
+__device__ __forceinline__ void norm_rotate(const u32x4 &x, const u32x4 &w, bool norm, F eps, int c,
+                                            const F *sn, const F *cs, F (&y)[8]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) y[i] = (F)bf16_at(x, i);
+  if (norm) {
+    F ss = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) ss += y[i] * y[i];
+    const F r = (F)1 / sqrt(row_sum(ss) * (F)(1.0 / 128.0) + eps);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = y[i] * r * (F)bf16_at(w, i);
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int pair = (c * 8 + i) & 63;
+    const F other = dpp_value(y[i], 0);
+    // first half: first*cos - second*sin; second half: second*cos + first*sin
+    y[i] = y[i] * cs[pair] + (c < 8 ? -other : other) * sn[pair];
+  }
+}
+
+// Scale byte of an MXFP4 block whose largest magnitude has binary exponent
+// `ex` (floor(log2)): 2^(ex - 2), kept in the range whose codes BF16 can hold.
+__device__ __forceinline__ int mx_exponent(int ex) { return min(max(ex - 2, -126), 125); }
+
+__device__ __forceinline__ uint32_t mx_pack8(const float (&f)[8], float scale) {
+  uint32_t w = 0;
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, f[0], f[1], scale, 0);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, f[2], f[3], scale, 1);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, f[4], f[5], scale, 2);
+  return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, f[6], f[7], scale, 3);
+}
+
+// MXFP4 codes (8 per lane) and the block's scale byte of a row of BF16 values.
+// v_cvt_scalef32_pk_fp4_f32 divides by the scale, rounds to nearest even and
+// saturates at 6 (checked over every finite FP32 input).
+__device__ __forceinline__ uint32_t mx_encode(const u32x4 &v, uint32_t *byte) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) m = max(m, max(v[e] & 0x7fffu, (v[e] >> 16) & 0x7fffu));
+  m = block_max(m);
+  if (m >= 0x7f80u) {  // an infinity or a NaN in the block
+    *byte = 255u;
+    return 0u;
+  }
+  const int e = mx_exponent((int)(m >> 7) - 127);
+  *byte = (uint32_t)(e + 127);
+  float f[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) f[i] = bf16_at(v, i);
+  return mx_pack8(f, __uint_as_float((uint32_t)(e + 127) << 23));
+}
+// The same of 64-bit values.  Each goes to FP32 with the bits that FP32 drops
+// collected in its last one (round to odd), from which the code rounds as from
+// the value itself.
+__device__ __forceinline__ uint32_t mx_encode(const double (&y)[8], uint32_t *byte) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    m = max(m, (uint32_t)(__builtin_bit_cast(uint64_t, y[i]) >> 32) & 0x7fffffffu);
+  m = block_max(m);
+  if (m >= 0x7ff00000u) {
+    *byte = 255u;
+    return 0u;
+  }
+  const int e = mx_exponent((int)(m >> 20) - 1023);
+  *byte = (uint32_t)(e + 127);
+  float f[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, y[i]);
+    const uint32_t hi = (uint32_t)(u >> 32), lo = (uint32_t)u;
+    // exponent of y / 2^e in FP32's bias; below it the code is 0
+    const int ex = (int)((hi >> 20) & 0x7ffu) - (e + 1023 - 127);
+    const uint32_t mant = (hi & 0xfffffu) << 3 | lo >> 29 | ((lo << 3) != 0u ? 1u : 0u);
+    f[i] = __uint_as_float((hi & 0x80000000u) | (ex > 0 ? (uint32_t)ex << 23 | mant : 0u));
+  }
+  return mx_pack8(f, 1.0f);
+}
+
+// Forms of the append kernels: the reference's (BF16 or FP8 pages), and the
+// normed one over each kind of page.
+enum KvForm : int { kKvBf16 = 0, kKvFp8 = 1, kKvMx4 = 2 };
+
+template <bool FP8>
+struct RefForm {
+  using Args = AppendArgs;
+  static constexpr int kWavesPerEu = 6;
+  struct Angles {
+    float cos[64], sin[64];
+  };
+  struct Weights {};
+  static __device__ __forceinline__ Weights weights(const Args &, int) { return {}; }
+  static __device__ __forceinline__ void sincos(const Args &a, int pos, int tid, Angles &s) {
+    token_sincos(a, pos, tid, s.sin, s.cos);
+  }
+  static __device__ __forceinline__ void row(const Args &a, const Weights &, int t, int64_t page,
+                                             int off, int row, int c, const Angles &s,
+                                             const RowSlice &sl) {
+    apply_row<FP8>(a, t, page, off, row, c, s.sin, s.cos, sl);
+  }
+};
+
+template <int KV>
+struct NormForm {
+  using Args = NormAppendArgs;
+  static constexpr int kWavesPerEu = KV == kKvMx4 ? 4 : 5;
+  struct Angles {
+    float cos[64], sin[64];
+    double cos64[KV == kKvMx4 ? 64 : 1], sin64[KV == kKvMx4 ? 64 : 1];
+  };
+  struct Weights {
+    u32x4 q, k;
+  };
+  static __device__ __forceinline__ Weights weights(const Args &a, int c) {
+    Weights w = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+    if (a.q_norm) {
+      w.q = *reinterpret_cast<const u32x4 *>(a.q_norm + c * 8);
+      w.k = *reinterpret_cast<const u32x4 *>(a.k_norm + c * 8);
+    }
+    return w;
+  }
+  static __device__ __forceinline__ void sincos(const Args &a, int pos, int tid, Angles &s) {
+    if (tid < 64) {
+      const double angle = (double)pos * a.inv_freq64[tid];
+      const double sn = sin(angle), cs = cos(angle);
+      s.sin[tid] = (float)sn;
+      s.cos[tid] = (float)cs;
+      if constexpr (KV == kKvMx4) {
+        s.sin64[tid] = sn;
+        s.cos64[tid] = cs;
+      }
+    }
+  }
+  static __device__ __forceinline__ void row(const Args &a, const Weights &w, int t, int64_t page,
+                                             int off, int row, int c, const Angles &s,
+                                             const RowSlice &sl) {
+    const bool norm = a.q_norm != nullptr;
+    if (row < a.hq) {
+      float y[8];
+      norm_rotate<float>(sl.x, w.q, norm, a.eps, c, s.sin, s.cos, y);
+      u32x4 o;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = loom_dev::bf16x2_pack(y[2 * e], y[2 * e + 1]);
+      __builtin_nontemporal_store(
+          o, reinterpret_cast<u32x4 *>(a.q_out + ((int64_t)t * a.hq + row) * 128 + c * 8));
+      return;
+    }
+    const int kh = row - a.hq;
+    const int64_t at =
+        page * a.page_rows * a.hkv * 128 + (int64_t)kh * a.head_elems + (int64_t)off * a.row_elems;
+    if constexpr (KV == kKvMx4) {
+      double y[8];
+      norm_rotate<double>(sl.x, w.k, norm, (double)a.eps, c, s.sin64, s.cos64, y);
+      uint32_t kb, vb;
+      const uint32_t k4 = mx_encode(y, &kb), v4 = mx_encode(sl.v, &vb);
+      uint8_t *kp = reinterpret_cast<uint8_t *>(a.k_pages) + at / 2 + c * 4;
+      uint8_t *vp = reinterpret_cast<uint8_t *>(a.v_pages) + at / 2 + c * 4;
+      *reinterpret_cast<uint32_t *>(kp) = k4;
+      *reinterpret_cast<uint32_t *>(vp) = v4;
+      if ((c & 3) == 0) {
+        const int64_t sc = (((page * a.hkv + kh) * a.page_rows + off) << 2) + (c >> 2);
+        a.k_mx[sc] = (uint8_t)kb;
+        a.v_mx[sc] = (uint8_t)vb;
+      }
+    } else {
+      float y[8];
+      norm_rotate<float>(sl.x, w.k, norm, a.eps, c, s.sin, s.cos, y);
+      if constexpr (KV == kKvFp8) {
+        const float ks = a.kv_scales[0], vs = a.kv_scales[1];
+        loom_dev::u32x2 k8 = {0, 0}, v8 = {0, 0};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          k8[i >> 2] |= loom_dev::fp8_e4m3_from_f32(y[i] / ks) << (8 * (i & 3));
+          v8[i >> 2] |= loom_dev::fp8_e4m3_from_f32(bf16_at(sl.v, i) / vs) << (8 * (i & 3));
+        }
+        uint8_t *kp = reinterpret_cast<uint8_t *>(a.k_pages) + at + c * 8;
+        uint8_t *vp = reinterpret_cast<uint8_t *>(a.v_pages) + at + c * 8;
+        __builtin_nontemporal_store(k8, reinterpret_cast<loom_dev::u32x2 *>(kp));
+        __builtin_nontemporal_store(v8, reinterpret_cast<loom_dev::u32x2 *>(vp));
+      } else {
+        u32x4 o;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = loom_dev::bf16x2_pack(y[2 * e], y[2 * e + 1]);
+        __builtin_nontemporal_store(o, reinterpret_cast<u32x4 *>(a.k_pages + at + c * 8));
+        __builtin_nontemporal_store(sl.v, reinterpret_cast<u32x4 *>(a.v_pages + at + c * 8));
+      }
+    }
+  }
+};
+
 // Rotates the Q/K rows of token t and scatters its K/V rows into slot
 // (page, off).
-template <bool FP8>
-__device__ __forceinline__ void apply_token(const AppendArgs &a, int t, int64_t page, int off,
-                                            int tid, const float *s_sin, const float *s_cos,
-                                            const RowSlices &pre) {
+template <class Form>
+__device__ __forceinline__ void apply_token(const typename Form::Args &a, int t, int64_t page,
+                                            int off, int tid, const typename Form::Angles &s,
+                                            const typename Form::Weights &w, const RowSlices &pre) {
   const int c = tid & 15;
   const int rows = a.hq + a.hkv;
   int row = tid >> 4;
@@ -510,12 +758,12 @@ __device__ __forceinline__ void apply_token(const AppendArgs &a, int t, int64_t 
     if (it == kPreloadRows) {
       for (; row < rows; row += kApplyThreads / 16) {
         const RowSlice one = load_slice(a, t, row, c);
-        apply_row<FP8>(a, t, page, off, row, c, s_sin, s_cos, one);
+        Form::row(a, w, t, page, off, row, c, s, one);
       }
       break;
     }
     if (row >= rows) break;
-    apply_row<FP8>(a, t, page, off, row, c, s_sin, s_cos, pre.r[it]);
+    Form::row(a, w, t, page, off, row, c, s, pre.r[it]);
     row += kApplyThreads / 16;
   }
 }
@@ -554,12 +802,12 @@ __device__ __forceinline__ void apply_token(const AppendArgs &a, int t, int64_t 
 // Same-address atomics of many workgroups serialize (about 0.1 us each here),
 // so there is no shared counter: every polled word has a few readers and one
 // writer.
-template <bool FP8>
-__global__ __launch_bounds__(kApplyThreads) __attribute__((amdgpu_waves_per_eu(6)))
-void append_validated_kernel(AppendArgs a) {
+template <class Form>
+__global__ __launch_bounds__(kApplyThreads) __attribute__((amdgpu_waves_per_eu(Form::kWavesPerEu)))
+void append_validated_kernel(typename Form::Args a) {
   __shared__ int32_t s_ip[kValidateLdsBatch + 1], s_last[kValidateLdsBatch];
   __shared__ uint32_t s_or[kValidateThreads / 64];
-  __shared__ float s_cos[64], s_sin[64];
+  __shared__ typename Form::Angles s_angles;
   __shared__ int s_bad;
   const int tid = threadIdx.x;
   const WsLayout w = ws_layout(a.ws);
@@ -638,7 +886,8 @@ void append_validated_kernel(AppendArgs a) {
   // memory system is not yet flooded with the command's row traffic, and the
   // rows still arrive before the verdicts.
   const RowSlices first = load_first_slices(a, t, tid);
-  token_sincos(a, pos, tid, s_sin, s_cos);
+  const typename Form::Weights w8 = Form::weights(a, tid & 15);
+  Form::sincos(a, pos, tid, s_angles);
   if (tid < 64) {  // wave 0 polls copy t % kSignalCopies
     const uint64_t *copy = w.signals + (t % kSignalCopies) * kMaxValidateBlocks;
     int polls = 0, ready = 0, valid = 0;
@@ -661,7 +910,7 @@ void append_validated_kernel(AppendArgs a) {
     }
   }
   __syncthreads();
-  if (!s_bad) apply_token<FP8>(a, t, page, off, tid, s_sin, s_cos, first);
+  if (!s_bad) apply_token<Form>(a, t, page, off, tid, s_angles, w8, first);
 }
 
 // Two-launch form (plan flag LOOM_PLAN_APPEND_TWO_LAUNCH), for callers that
@@ -687,10 +936,10 @@ __global__ __launch_bounds__(kValidateThreads) void append_validate_kernel(Appen
     __hip_atomic_store(a.ws + kWsVerdicts + b, bad ? 0u : 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
-template <bool FP8>
-__global__ __launch_bounds__(kApplyThreads) __attribute__((amdgpu_waves_per_eu(6)))
-void append_apply_kernel(AppendArgs a) {
-  __shared__ float s_cos[64], s_sin[64];
+template <class Form>
+__global__ __launch_bounds__(kApplyThreads) __attribute__((amdgpu_waves_per_eu(Form::kWavesPerEu)))
+void append_apply_kernel(typename Form::Args a) {
+  __shared__ typename Form::Angles s_angles;
   __shared__ uint32_t s_ok[kApplyThreads / 64];
   const int tid = threadIdx.x;
   const int t = blockIdx.x;
@@ -704,28 +953,30 @@ void append_apply_kernel(AppendArgs a) {
   const int64_t pages = table_pages(a, a.indptr[a.batch]);
   if (!token_slot_apply(a, t, tid, pages, &r, &pos, &page, &off)) pos = 0, page = 0;
   const RowSlices first = load_first_slices(a, t, tid);
-  token_sincos(a, pos, tid, s_sin, s_cos);
+  const typename Form::Weights w8 = Form::weights(a, tid & 15);
+  Form::sincos(a, pos, tid, s_angles);
   // empty this workgroup's share of the table the validation kernel filled
   if (!ep.broken) {
     uint32_t *table = ws_layout(a.ws).tables + (ep.epoch & 1u) * kTableSlots;
     for (int i = t * kApplyThreads + tid; i < kTableSlots; i += a.tokens * kApplyThreads) table[i] = 0u;
   }
   if (loom_dev::block_or(!ok, s_ok)) return;
-  apply_token<FP8>(a, t, page, off, tid, s_sin, s_cos, first);
+  apply_token<Form>(a, t, page, off, tid, s_angles, w8, first);
 }
 
 // Small commands (T <= 64 tokens, <= 4096 page indices): one launch.  Every
 // workgroup (one per token) validates the whole command itself, as the
 // reference's kernels do, and applies its own token only if all of it is
 // valid, so the all-or-nothing guard needs no second kernel.
-template <bool FP8>
-__global__ __launch_bounds__(kApplyThreads) void append_fused_small_kernel(AppendArgs a) {
-  __shared__ float s_cos[64], s_sin[64];
+template <class Form>
+__global__ __launch_bounds__(kApplyThreads) void append_fused_small_kernel(typename Form::Args a) {
+  __shared__ typename Form::Angles s_angles;
   __shared__ __align__(16) uint32_t s_keys[kFusedMaxTokens];
   __shared__ uint32_t s_bad[kApplyThreads / 64], s_dup[kApplyThreads / 64];
   const int tid = threadIdx.x;
   const int t = blockIdx.x;
   const RowSlices first = load_first_slices(a, t, tid);
+  const typename Form::Weights w8 = Form::weights(a, tid & 15);
   // Wave 1 takes this workgroup's token position straight from the metadata
   // and computes its (sin, cos) pairs while wave 0 walks the validation's
   // dependent loads.  Nothing is written unless the validation passes, and
@@ -739,7 +990,7 @@ __global__ __launch_bounds__(kApplyThreads) void append_fused_small_kernel(Appen
       const int32_t st = a.indptr[t], en = a.indptr[t + 1], tl = a.last[t];
       pos_t = (en - st - 1) * a.page_rows + tl - 1;
     }
-    token_sincos(a, pos_t, tid - 64, s_sin, s_cos);
+    Form::sincos(a, pos_t, tid - 64, s_angles);
   }
 
   int bad = 0;
@@ -783,8 +1034,8 @@ __global__ __launch_bounds__(kApplyThreads) void append_fused_small_kernel(Appen
   if (loom_dev::block_or(dup != 0, s_dup)) return;
   const uint32_t key = s_keys[t];
   // key = page * page_rows + row
-  apply_token<FP8>(a, t, key / (uint32_t)a.page_rows, (int)(key % (uint32_t)a.page_rows), tid, s_sin,
-              s_cos, first);
+  apply_token<Form>(a, t, key / (uint32_t)a.page_rows, (int)(key % (uint32_t)a.page_rows), tid,
+                    s_angles, w8, first);
 }
 
 }  // namespace
@@ -805,6 +1056,9 @@ struct loom_rope_append_plan {
   uint32_t kv_dtype = LOOM_KV_DTYPE_BF16;
   uint32_t page_rows = 16;
   float inv_freq[64];
+  bool normed = false;  // a plan of loom_rope_provider_plan_norm_paged_append
+  float norm_eps = 0;   // 0: no norms
+  double inv_freq64[64];
 };
 
 extern "C" {
@@ -823,15 +1077,18 @@ loom_status_t loom_rope_provider_load(int device, loom_rope_provider_t **out, lo
 
 void loom_rope_provider_free(loom_rope_provider_t *p) { delete p; }
 
+// `norm`: the normed append's spec, which alone takes MXFP4 pages.
 static loom_status_t make_plan(const loom_paged_decode_spec_t &s, uint64_t tokens,
                                bool explicit_tokens, uint32_t flags,
-                               loom_rope_append_plan_t **out, loom_error_t *err) {
+                               loom_rope_append_plan_t **out, loom_error_t *err,
+                               const loom_norm_rope_append_spec_t *norm = nullptr) {
   if (flags & ~(LOOM_PLAN_PAGE_INDICES_CAPACITY | LOOM_PLAN_APPEND_TWO_LAUNCH |
                 LOOM_PLAN_APPEND_TEST_NO_WAIT))
     return fail(err, LOOM_PLAN_INVALID_OPTION, "flags", flags);
   if (s.kv_layout != LOOM_KV_LAYOUT_NHD && s.kv_layout != LOOM_KV_LAYOUT_HND)
     return fail(err, LOOM_PLAN_INVALID_OPTION, "kv_layout", s.kv_layout);
-  if (s.kv_dtype != LOOM_KV_DTYPE_BF16 && s.kv_dtype != LOOM_KV_DTYPE_FP8_E4M3)
+  if (s.kv_dtype != LOOM_KV_DTYPE_BF16 && s.kv_dtype != LOOM_KV_DTYPE_FP8_E4M3 &&
+      !(norm && s.kv_dtype == LOOM_KV_DTYPE_MXFP4))
     return fail(err, LOOM_PLAN_INVALID_OPTION, "kv_dtype", s.kv_dtype);
   // rope/mod.rs:628-682: states = tokens * (Hq + Hkv) must fit the grid.
   uint64_t rows = s.num_query_heads + s.num_kv_heads, states;
@@ -868,6 +1125,12 @@ static loom_status_t make_plan(const loom_paged_decode_spec_t &s, uint64_t token
     const float exponent = 2.0f * (float)i / 128.0f;
     p->inv_freq[i] = std::pow(10000.0f, -exponent) / 1.0f;
   }
+  if (norm) {
+    p->normed = true;
+    p->norm_eps = norm->norm_eps;
+    for (int i = 0; i < 64; ++i)
+      p->inv_freq64[i] = std::pow(norm->rope_theta, -2.0 * (double)i / 128.0);
+  }
   *out = p;
   return loom::ok(err);
 }
@@ -901,6 +1164,20 @@ loom_status_t loom_rope_provider_plan_bf16_paged_append_tokens_flags(
   return make_plan(spec->paged, spec->tokens, true, flags, out, err);
 }
 
+loom_status_t loom_rope_provider_plan_norm_paged_append(const loom_rope_provider_t *provider,
+                                                        const loom_norm_rope_append_spec_t *spec,
+                                                        uint32_t flags,
+                                                        loom_rope_append_plan_t **out,
+                                                        loom_error_t *err) {
+  if (!provider || !spec || !out) return fail(err, LOOM_NULL_ARGUMENT, "provider");
+  loom_norm_rope_append_spec_t s;  // a spec that spec_new would refuse is refused here too
+  const loom_status_t rc =
+      loom_norm_rope_append_spec_new(&spec->paged, spec->tokens, spec->explicit_tokens,
+                                     spec->rope_theta, spec->norm_eps, &s, err);
+  if (rc) return rc;
+  return make_plan(s.paged, s.tokens, s.explicit_tokens != 0, flags, out, err, &s);
+}
+
 void loom_rope_append_plan_free(loom_rope_append_plan_t *p) { delete p; }
 
 void loom_rope_append_plan_get_info(const loom_rope_append_plan_t *p,
@@ -912,9 +1189,43 @@ void loom_rope_append_plan_get_info(const loom_rope_append_plan_t *p,
 
 namespace {
 
-// enqueue_into, rope/mod.rs:758-830 / :846-934.  `hs_all` holds the thirteen
-// handles of loom_rope_append_args_t; with `queue_ws` the validation words
-// live in the command queue's zero-initialised workspace and the workspace
+// Operands of an append command, in the order of its handles: the thirteen of
+// loom_rope_append_args_t, then the normed append's.
+constexpr int kAppendOperands = 17;
+
+// The kernels of one form.  Commands of at most kFusedMaxTokens tokens and
+// kFusedMaxIndices page indices: one launch in which every workgroup validates.
+// Others: the validation workgroups first, then one per token (the plan's bounds
+// keep both within the workspace layout), or the two-launch form.
+template <class Form>
+loom_status_t launch_append(const loom_rope_append_plan_t *plan, loom_command_scope_t *scope,
+                            const typename Form::Args &a, loom_error_t *err) {
+  hipStream_t stream = scope->queue->stream;
+  const dim3 threads(kApplyThreads);
+  if (a.tokens <= kFusedMaxTokens && a.n_indices <= kFusedMaxIndices) {
+    hipLaunchKernelGGL(append_fused_small_kernel<Form>, dim3((unsigned)a.tokens), threads, 0, stream,
+                       a);
+    return loom::record_launch(scope, hipGetLastError(), err);
+  }
+  const int grid = a.validate_blocks + a.tokens;
+  if (a.validate_blocks > kMaxValidateBlocks || grid > kMaxGrid)
+    return fail(err, LOOM_PLAN_STATE_COUNT_OUT_OF_RANGE, "RoPE validation grid", grid);
+  if (plan->flags & LOOM_PLAN_APPEND_TWO_LAUNCH) {
+    hipLaunchKernelGGL(append_validate_kernel, dim3((unsigned)a.validate_blocks),
+                       dim3(kValidateThreads), 0, stream, a);
+    hipError_t e = hipGetLastError();
+    if (e == hipSuccess) {
+      hipLaunchKernelGGL(append_apply_kernel<Form>, dim3((unsigned)a.tokens), threads, 0, stream, a);
+      e = hipGetLastError();
+    }
+    return loom::record_launch(scope, e, err);
+  }
+  hipLaunchKernelGGL(append_validated_kernel<Form>, dim3((unsigned)grid), threads, 0, stream, a);
+  return loom::record_launch(scope, hipGetLastError(), err);
+}
+
+// enqueue_into, rope/mod.rs:758-830 / :846-934.  With `queue_ws` the validation
+// words live in the command queue's zero-initialised workspace and the workspace
 // handle is not an operand.
 loom_status_t rope_append_enqueue_impl(const loom_rope_append_plan_t *plan,
                                        loom_command_scope_t *scope, const loom_handle_t *hs_all,
@@ -923,32 +1234,39 @@ loom_status_t rope_append_enqueue_impl(const loom_rope_append_plan_t *plan,
   const bool ex = pi.explicit_tokens != 0;
   // Operand order of Bf16RopePagedKvAppend{,Tokens}Args (rope/mod.rs:963-1047).
   const bool fp8 = plan->kv_dtype == LOOM_KV_DTYPE_FP8_E4M3;
-  if (fp8 && queue_ws)  // the reference-shaped args carry no scales
+  const bool mx4 = plan->kv_dtype == LOOM_KV_DTYPE_MXFP4;
+  const bool norms = plan->normed && plan->norm_eps != 0.0f;
+  if (fp8 && queue_ws && !plan->normed)  // the reference-shaped args carry no scales
     return fail(err, LOOM_ENQ_LENGTH_MISMATCH, "kv_scales", 2, 0);
-  const loom_dtype_t kv_t = fp8 ? LOOM_DTYPE_U8 : LOOM_DTYPE_BF16;
-  loom::OperandSpec ops[13] = {
+  const loom_dtype_t kv_t = fp8 || mx4 ? LOOM_DTYPE_U8 : LOOM_DTYPE_BF16;
+  const loom::OperandSpec ops[kAppendOperands] = {
       {"query", LOOM_DTYPE_BF16, false},        {"key", LOOM_DTYPE_BF16, false},
       {"value", LOOM_DTYPE_BF16, false},        {"batch_indices", LOOM_DTYPE_I32, false},
       {"positions", LOOM_DTYPE_I32, false},     {"page_indptr", LOOM_DTYPE_I32, false},
       {"page_indices", LOOM_DTYPE_I32, false},  {"last_page_len", LOOM_DTYPE_I32, false},
       {"query_output", LOOM_DTYPE_BF16, true},  {"key_pages", kv_t, true},
       {"value_pages", kv_t, true},              {"workspace", LOOM_DTYPE_U8, true},
-      {"kv_scales", LOOM_DTYPE_F32, false}};
+      {"kv_scales", LOOM_DTYPE_F32, false},     {"query_norm", LOOM_DTYPE_BF16, false},
+      {"key_norm", LOOM_DTYPE_BF16, false},     {"key_scales", LOOM_DTYPE_U8, true},
+      {"value_scales", LOOM_DTYPE_U8, true}};
   // The one-token form has no batch_indices/positions operands; only FP8
-  // plans take kv_scales.
-  loom::OperandSpec sel_ops[13];
-  loom_handle_t sel[13];
-  int map[13];
+  // plans take kv_scales, only MXFP4 plans the scale bytes.
+  loom::OperandSpec sel_ops[kAppendOperands];
+  loom_handle_t sel[kAppendOperands];
+  int map[kAppendOperands];
   int n = 0;
-  for (int i = 0; i < 13; ++i) {
+  for (int i = 0; i < kAppendOperands; ++i) {
+    map[i] = -1;
     if (!ex && (i == 3 || i == 4)) continue;
     if (queue_ws && i == 11) continue;
     if (!fp8 && i == 12) continue;
+    if (!norms && (i == 13 || i == 14)) continue;
+    if (!mx4 && i >= 15) continue;
     sel_ops[n] = ops[i];
     sel[n] = hs_all[i];
     map[i] = n++;
   }
-  const loom::Lease *l[13];
+  const loom::Lease *l[kAppendOperands];
   loom_status_t rc = loom::resolve_command(scope, sel, sel_ops, n, l, err);
   if (rc) return rc;
   if (fp8 && l[map[12]]->numel != 2)
@@ -956,7 +1274,9 @@ loom_status_t rope_append_enqueue_impl(const loom_rope_append_plan_t *plan,
   auto L = [&](int i) { return l[map[i]]; };
   const uint64_t T = pi.tokens, B = pi.batch_size, hq = pi.num_query_heads,
                  hkv = pi.num_kv_heads;
-  const uint64_t kvn = plan->max_num_pages * plan->page_rows * hkv * loom::kHeadDim;
+  const uint64_t pool_rows = plan->max_num_pages * plan->page_rows * hkv;
+  const uint64_t kvn = pool_rows * (mx4 ? LOOM_MXFP4_ROW_BYTES : loom::kHeadDim);
+  const uint64_t scn = pool_rows * LOOM_MXFP4_ROW_SCALES;
   struct Want {
     int i;
     uint64_t n;
@@ -964,10 +1284,11 @@ loom_status_t rope_append_enqueue_impl(const loom_rope_append_plan_t *plan,
   const Want wants[] = {{0, T * hq * 128}, {1, T * hkv * 128}, {2, T * hkv * 128},
                         {3, T},           {4, T},             {5, B + 1},
                         {7, B},           {8, T * hq * 128},  {9, kvn},
-                        {10, kvn},        {11, pi.workspace_bytes}};
+                        {10, kvn},        {11, pi.workspace_bytes},
+                        {13, 128},        {14, 128},          {15, scn},
+                        {16, scn}};
   for (const Want &w : wants) {
-    if (!ex && (w.i == 3 || w.i == 4)) continue;
-    if (queue_ws && w.i == 11) continue;
+    if (map[w.i] < 0) continue;
     if (w.i == 7) {  // page_indices precedes last_page_len in the reference order
       if (L(6)->numel < B)
         return fail(err, LOOM_ENQ_PAGE_INDICES_TOO_SHORT, nullptr, B, L(6)->numel);
@@ -991,7 +1312,7 @@ loom_status_t rope_append_enqueue_impl(const loom_rope_append_plan_t *plan,
     ws = (uint32_t *)L(11)->ptr;
   }
 
-  AppendArgs a{};
+  NormAppendArgs a{};
   a.q = (const uint16_t *)L(0)->ptr;
   a.k = (const uint16_t *)L(1)->ptr;
   a.v = (const uint16_t *)L(2)->ptr;
@@ -1032,33 +1353,20 @@ loom_status_t rope_append_enqueue_impl(const loom_rope_append_plan_t *plan,
   a.validate_blocks = (int32_t)vblocks;
   a.status = scope->queue->status_dev;
   a.poll_limit = (plan->flags & LOOM_PLAN_APPEND_TEST_NO_WAIT) ? 0 : kPollLimit;
-  hipStream_t stream = scope->queue->stream;
-  if (T <= (uint64_t)kFusedMaxTokens && (int64_t)L(6)->numel <= kFusedMaxIndices) {
-    hipLaunchKernelGGL(fp8 ? append_fused_small_kernel<true> : append_fused_small_kernel<false>,
-                       dim3((unsigned)T), dim3(kApplyThreads), 0,
-                       stream, a);
-    return loom::record_launch(scope, hipGetLastError(), err);
+  if (!plan->normed)
+    return fp8 ? launch_append<RefForm<true>>(plan, scope, a, err)
+               : launch_append<RefForm<false>>(plan, scope, a, err);
+  a.q_norm = norms ? (const uint16_t *)L(13)->ptr : nullptr;
+  a.k_norm = norms ? (const uint16_t *)L(14)->ptr : nullptr;
+  a.eps = plan->norm_eps;
+  for (int i = 0; i < 64; ++i) a.inv_freq64[i] = plan->inv_freq64[i];
+  if (mx4) {
+    a.k_mx = (uint8_t *)L(15)->ptr;
+    a.v_mx = (uint8_t *)L(16)->ptr;
+    return launch_append<NormForm<kKvMx4>>(plan, scope, a, err);
   }
-  // One launch: the validation workgroups first, then one per token (the
-  // plan's bounds keep both within the workspace layout).
-  const uint64_t grid = vblocks + T;
-  if (vblocks > (uint64_t)kMaxValidateBlocks || grid > (uint64_t)kMaxGrid)
-    return fail(err, LOOM_PLAN_STATE_COUNT_OUT_OF_RANGE, "RoPE validation grid", grid);
-  if (plan->flags & LOOM_PLAN_APPEND_TWO_LAUNCH) {
-    hipLaunchKernelGGL(append_validate_kernel, dim3((unsigned)vblocks), dim3(kValidateThreads), 0,
-                       stream, a);
-    hipError_t e = hipGetLastError();
-    if (e == hipSuccess) {
-      hipLaunchKernelGGL(fp8 ? append_apply_kernel<true> : append_apply_kernel<false>,
-                         dim3((unsigned)T), dim3(kApplyThreads), 0, stream, a);
-      e = hipGetLastError();
-    }
-    return loom::record_launch(scope, e, err);
-  }
-  hipLaunchKernelGGL(fp8 ? append_validated_kernel<true> : append_validated_kernel<false>,
-                     dim3((unsigned)grid), dim3(kApplyThreads), 0, stream, a);
-  hipError_t e = hipGetLastError();
-  return loom::record_launch(scope, e, err);
+  return fp8 ? launch_append<NormForm<kKvFp8>>(plan, scope, a, err)
+             : launch_append<NormForm<kKvBf16>>(plan, scope, a, err);
 }
 
 }  // namespace
@@ -1069,11 +1377,13 @@ loom_status_t loom_rope_append_enqueue(const loom_rope_append_plan_t *plan,
                                        loom_command_scope_t *scope,
                                        const loom_rope_append_args_t *args, loom_error_t *err) {
   if (!plan || !scope || !args) return fail(err, LOOM_NULL_ARGUMENT, "plan");
-  const loom_handle_t hs[13] = {args->query,        args->key,           args->value,
-                                args->batch_indices, args->positions,    args->page_indptr,
-                                args->page_indices, args->last_page_len, args->query_output,
-                                args->key_pages,    args->value_pages,   args->workspace,
-                                args->kv_scales};
+  if (plan->normed)  // the normed plan takes its own args
+    return fail(err, LOOM_NULL_ARGUMENT, "args");
+  const loom_handle_t hs[kAppendOperands] = {
+      args->query,        args->key,           args->value,        args->batch_indices,
+      args->positions,    args->page_indptr,   args->page_indices, args->last_page_len,
+      args->query_output, args->key_pages,     args->value_pages,  args->workspace,
+      args->kv_scales};
   return rope_append_enqueue_impl(plan, scope, hs, false, err);
 }
 
@@ -1082,10 +1392,10 @@ loom_status_t loom_rope_append_enqueue_bf16(const loom_rope_append_plan_t *plan,
                                             const loom_bf16_rope_paged_kv_append_args_t *args,
                                             loom_error_t *err) {
   if (!plan || !scope || !args) return fail(err, LOOM_NULL_ARGUMENT, "plan");
-  if (plan->info.explicit_tokens)  // the tokens plan takes the tokens args
+  if (plan->normed || plan->info.explicit_tokens)  // the tokens plan takes the tokens args
     return fail(err, LOOM_NULL_ARGUMENT, "args");
   const loom_handle_t none{0, 0};
-  const loom_handle_t hs[13] = {args->query,        args->key,           args->value,
+  const loom_handle_t hs[kAppendOperands] = {args->query,        args->key,           args->value,
                                 none,               none,                args->page_indptr,
                                 args->page_indices, args->last_page_len, args->query_output,
                                 args->key_pages,    args->value_pages,   none,
@@ -1097,15 +1407,31 @@ loom_status_t loom_rope_append_tokens_enqueue_bf16(
     const loom_rope_append_plan_t *plan, loom_command_scope_t *scope,
     const loom_bf16_rope_paged_kv_append_tokens_args_t *args, loom_error_t *err) {
   if (!plan || !scope || !args) return fail(err, LOOM_NULL_ARGUMENT, "plan");
-  if (!plan->info.explicit_tokens)  // the one-token plan takes the one-token args
+  if (plan->normed || !plan->info.explicit_tokens)  // the one-token plan takes the one-token args
     return fail(err, LOOM_NULL_ARGUMENT, "args");
   const loom_handle_t none{0, 0};
-  const loom_handle_t hs[13] = {args->query,        args->key,           args->value,
+  const loom_handle_t hs[kAppendOperands] = {args->query,        args->key,           args->value,
                                 args->batch_indices, args->positions,    args->page_indptr,
                                 args->page_indices, args->last_page_len, args->query_output,
                                 args->key_pages,    args->value_pages,   none,
                                 none};
   return rope_append_enqueue_impl(plan, scope, hs, true, err);
+}
+
+loom_status_t loom_norm_rope_append_enqueue(const loom_rope_append_plan_t *plan,
+                                            loom_command_scope_t *scope,
+                                            const loom_norm_rope_append_args_t *args,
+                                            loom_error_t *err) {
+  if (!plan || !scope || !args) return fail(err, LOOM_NULL_ARGUMENT, "plan");
+  if (!plan->normed)  // the other plans take their own args
+    return fail(err, LOOM_NULL_ARGUMENT, "args");
+  const loom_handle_t hs[kAppendOperands] = {
+      args->query,        args->key,         args->value,        args->batch_indices,
+      args->positions,    args->page_indptr, args->page_indices, args->last_page_len,
+      args->query_output, args->key_pages,   args->value_pages,  args->workspace,
+      args->kv_scales,    args->query_norm,  args->key_norm,     args->key_scales,
+      args->value_scales};
+  return rope_append_enqueue_impl(plan, scope, hs, args->workspace.set_id == 0, err);
 }
 
 }  // extern "C"

@@ -62,9 +62,14 @@ def _layout_code(kv_layout) -> int:
     return KV_LAYOUTS[kv_layout]
 
 
-# K/V page element types (loom_kv_dtype_t): BF16, or OCP FP8 E4M3 bytes with
-# per-tensor [k_scale, v_scale] (no reference counterpart).
-KV_DTYPES = {"bf16": 0, "fp8_e4m3": 1}
+# K/V page element types (loom_kv_dtype_t): BF16, OCP FP8 E4M3 bytes with
+# per-tensor [k_scale, v_scale], or OCP MXFP4 (64 bytes of E2M1 codes per row of
+# 128 values, and one E8M0 scale byte per 32 values in tensors of their own; paged
+# decode, the normed append and the read back).  The last two have no reference
+# counterpart.
+KV_DTYPES = {"bf16": 0, "fp8_e4m3": 1, "mxfp4": 2}
+MXFP4_ROW_BYTES = 64  # code bytes of a row
+MXFP4_ROW_SCALES = 4  # scale bytes of a row
 
 
 def _set_paged_layout(c_paged, kv_layout, kv_dtype="bf16", kv_page_size=None):
@@ -267,7 +272,12 @@ class Bf16PagedBatchDecodeSpec:
     page_size = property(lambda s: s._c.page_size or PAGE_SIZE)
     gqa_group_size = property(lambda s: s.num_query_heads // s.num_kv_heads)
     query_numel = property(lambda s: s.batch_size * s.num_query_heads * HEAD_DIM)
-    kv_pages_numel = property(lambda s: s.max_num_pages * s.page_size * s.num_kv_heads * HEAD_DIM)
+    # elements of each K/V pages operand (bytes of codes for MXFP4 pages)
+    kv_pages_numel = property(lambda s: s.max_num_pages * s.page_size * s.num_kv_heads
+                              * (MXFP4_ROW_BYTES if s.kv_dtype == "mxfp4" else HEAD_DIM))
+    # bytes of each MXFP4 scale operand [pool, Hkv, page_size, 4]
+    mx_scales_numel = property(lambda s: s.max_num_pages * s.page_size * s.num_kv_heads
+                               * MXFP4_ROW_SCALES)
     output_numel = property(lambda s: s.query_numel)
     lse_numel = property(lambda s: s.batch_size * s.num_query_heads)
     page_indptr_numel = property(lambda s: s.batch_size + 1)
@@ -356,6 +366,63 @@ class Bf16RopePagedKvAppendTokensSpec:
         _call(lib().loom_rope_append_tokens_validate_metadata, C.byref(self._c), bi, nbi, ps,
               nps, ip, nip, ix, nix, ln, nln, slots)
         return [(slots[2 * t], slots[2 * t + 1]) for t in range(self.tokens)]
+
+
+class NormRopePagedKvAppendSpec:
+    """Norms of the query and key heads, rotation and paged append in one command
+    (no reference counterpart): K/V pages in BF16, FP8 E4M3 or MXFP4.  `norm_eps`
+    None: no norms.  `explicit_tokens` False: one token per request at kv_len - 1
+    (tokens = batch_size)."""
+
+    def __init__(self, tokens, batch_size, max_num_pages, num_query_heads, num_kv_heads,
+                 head_dim=HEAD_DIM, page_size=PAGE_SIZE, kv_layout="NHD", kv_dtype="bf16",
+                 kv_page_size=None, rope_theta=10000.0, norm_eps=None, explicit_tokens=True):
+        if norm_eps is not None and not norm_eps > 0:  # 0 means "no norms" in the C spec
+            raise ContractError(3, "InvalidEpsilon",
+                                f"RMSNorm epsilon must be finite and positive, got {norm_eps:g}",
+                                None, (0, 0, 0, 0), float(norm_eps), 0)
+        self.paged = Bf16PagedBatchDecodeSpec(batch_size, max_num_pages, num_query_heads,
+                                              num_kv_heads, head_dim, page_size, kv_layout,
+                                              kv_dtype, kv_page_size)
+        self._c = _ffi.NormRopeAppendSpec()
+        _call(lib().loom_norm_rope_append_spec_new, C.byref(self.paged._c), tokens,
+              1 if explicit_tokens else 0, float(rope_theta),
+              0.0 if norm_eps is None else float(norm_eps), C.byref(self._c))
+
+    tokens = property(lambda s: s._c.tokens)
+    rope_theta = property(lambda s: s._c.rope_theta)
+    norm_eps = property(lambda s: s._c.norm_eps or None)
+    explicit_tokens = property(lambda s: bool(s._c.explicit_tokens))
+    batch_size = property(lambda s: s.paged.batch_size)
+    max_num_pages = property(lambda s: s.paged.max_num_pages)
+    num_query_heads = property(lambda s: s.paged.num_query_heads)
+    num_kv_heads = property(lambda s: s.paged.num_kv_heads)
+    query_numel = property(lambda s: s.tokens * s.num_query_heads * HEAD_DIM)
+    key_numel = property(lambda s: s.tokens * s.num_kv_heads * HEAD_DIM)
+    value_numel = key_numel
+    query_output_numel = query_numel
+    kv_pages_numel = property(lambda s: s.paged.kv_pages_numel)
+    mx_scales_numel = property(lambda s: s.paged.mx_scales_numel)
+
+
+class PagedKvReadSpec:
+    """Rows of an MXFP4 paged cache read back as BF16 [nnz_kv, Hkv, 128], ragged by
+    kv_indptr (no reference counterpart)."""
+
+    def __init__(self, batch_size, nnz_kv, max_num_pages, num_kv_heads, head_dim=HEAD_DIM,
+                 page_size=PAGE_SIZE, kv_layout="NHD", kv_dtype="mxfp4", kv_page_size=None):
+        self.paged = Bf16PagedBatchDecodeSpec(batch_size, max_num_pages, num_kv_heads,
+                                              num_kv_heads, head_dim, page_size, kv_layout,
+                                              kv_dtype, kv_page_size)
+        self._c = _ffi.PagedKvReadSpec()
+        _call(lib().loom_paged_kv_read_spec_new, C.byref(self.paged._c), nnz_kv, C.byref(self._c))
+
+    nnz_kv = property(lambda s: s._c.nnz_kv)
+    batch_size = property(lambda s: s.paged.batch_size)
+    num_kv_heads = property(lambda s: s.paged.num_kv_heads)
+    output_numel = property(lambda s: s.nnz_kv * s.num_kv_heads * HEAD_DIM)
+    kv_pages_numel = property(lambda s: s.paged.kv_pages_numel)
+    mx_scales_numel = property(lambda s: s.paged.mx_scales_numel)
 
 
 def _wrap_paged(c_spec) -> Bf16PagedBatchDecodeSpec:
@@ -627,6 +694,30 @@ class Bf16PagedBatchDecodeArgs:
         object.__setattr__(self, "_ref", C.byref(c))
 
 
+@dataclass(frozen=True)
+class Mxfp4PagedBatchDecodeArgs:
+    """Operands of a paged decode over MXFP4 pages (a spec with kv_dtype="mxfp4"; no
+    reference counterpart).  Without a `workspace` the split-KV states live in the
+    command queue's."""
+    query: Read
+    key_pages: Read
+    value_pages: Read
+    key_scales: Read
+    value_scales: Read
+    page_indptr: Read
+    page_indices: Read
+    last_page_len: Read
+    output: Write
+    lse: Write
+    workspace: Optional[Write] = None
+
+    def __post_init__(self):
+        c = _ffi.Mxfp4PagedBatchDecodeArgs(*[
+            _h(getattr(self, f)) for f, _ in _ffi.Mxfp4PagedBatchDecodeArgs._fields_])
+        object.__setattr__(self, "_struct", c)
+        object.__setattr__(self, "_ref", C.byref(c))
+
+
 class Bf16PagedBatchDecodePlan:
     def __init__(self, ptr, spec):
         self._p = ptr
@@ -645,7 +736,12 @@ class Bf16PagedBatchDecodePlan:
     def workspace_bytes(self) -> int:
         return self.info.workspace_bytes
 
-    def enqueue_into(self, scope: CommandScope, args: Bf16PagedBatchDecodeArgs):
+    def enqueue_into(self, scope: CommandScope, args):
+        """`args`: Bf16PagedBatchDecodeArgs, or Mxfp4PagedBatchDecodeArgs for a plan over
+        MXFP4 pages."""
+        if isinstance(args, Mxfp4PagedBatchDecodeArgs):
+            _enqueue(_ffi.load().loom_paged_decode_enqueue_mxfp4, self._p, scope._p, args._ref)
+            return
         fn = (_ffi.load().loom_paged_decode_enqueue_bf16 if args.reference_shaped
               else _ffi.load().loom_paged_decode_enqueue)
         _enqueue(fn, self._p, scope._p, args._ref)
@@ -654,7 +750,7 @@ class Bf16PagedBatchDecodePlan:
         """The same command with the split-KV workspace in the library's static
         per-device scratch: allocates nothing (no reference counterpart).
         Commands that overlap in time on one device race."""
-        if not args.reference_shaped:
+        if not getattr(args, "reference_shaped", False):
             raise TypeError("the allocation-free enqueue takes the reference's eight operands")
         _enqueue(_ffi.load().loom_paged_decode_enqueue_bf16_no_alloc, self._p, scope._p,
                  args._ref)
@@ -1101,6 +1197,47 @@ class Bf16RaggedPrefillPlan:
             pass
 
 
+@dataclass(frozen=True)
+class PagedKvReadArgs:
+    """Operands of the read back; `kv_start` [B]: each request's first token (none: 0)."""
+    key_pages: Read
+    value_pages: Read
+    key_scales: Read
+    value_scales: Read
+    page_indptr: Read
+    page_indices: Read
+    last_page_len: Read
+    kv_indptr: Read
+    key: Write
+    value: Write
+    kv_start: Optional[Read] = None
+
+    def __post_init__(self):
+        c = _ffi.PagedKvReadArgs(*[_h(getattr(self, f)) for f, _ in _ffi.PagedKvReadArgs._fields_])
+        object.__setattr__(self, "_struct", c)
+        object.__setattr__(self, "_ref", C.byref(c))
+
+
+class PagedKvReadPlan:
+    def __init__(self, ptr, spec):
+        self._p = ptr
+        self._spec = spec
+
+    def spec(self):
+        return self._spec
+
+    def enqueue_into(self, scope: CommandScope, args: PagedKvReadArgs):
+        _enqueue(_ffi.load().loom_paged_kv_read_enqueue, self._p, scope._p, args._ref)
+
+    def __del__(self):
+        try:
+            if getattr(self, "_p", None):
+                lib().loom_paged_kv_read_plan_free(self._p)
+                self._p = None
+        except Exception:  # interpreter shutdown: module globals are gone
+            pass
+
+
 class PrefillProvider:
     """prefill.rs:2278-2410 (the paged and ragged plans)."""
 
@@ -1139,6 +1276,15 @@ class PrefillProvider:
         _call(lib().loom_prefill_provider_plan_bf16_ragged, self._p, C.byref(spec._c),
               C.byref(opt), C.byref(out))
         return Bf16RaggedPrefillPlan(out.value, spec)
+
+    def plan_paged_kv_read(self, spec: PagedKvReadSpec,
+                           indices_capacity: bool = False) -> PagedKvReadPlan:
+        """MXFP4 pages read back as the contiguous BF16 rows of a ragged prefill (no
+        reference counterpart)."""
+        out = C.c_void_p()
+        _call(lib().loom_prefill_provider_plan_paged_kv_read, self._p, C.byref(spec._c),
+              PLAN_PAGE_INDICES_CAPACITY if indices_capacity else 0, C.byref(out))
+        return PagedKvReadPlan(out.value, spec)
 
     def __del__(self):
         try:
@@ -1202,6 +1348,37 @@ def Bf16RopePagedKvAppendTokensArgs(query, key, value, batch_indices, positions,
                                      workspace, batch_indices, positions, kv_scales)
 
 
+@dataclass(frozen=True)
+class NormRopePagedKvAppendArgs:
+    """Operands of the normed append (no reference counterpart).  `batch_indices` and
+    `positions` for explicit tokens, `query_norm` and `key_norm` (Read<bf16> [128]) with
+    norms, `key_scales` and `value_scales` for MXFP4 pages, `kv_scales` for FP8 pages; a
+    `workspace` of the caller's, or the command queue's."""
+    query: Read
+    key: Read
+    value: Read
+    page_indptr: Read
+    page_indices: Read
+    last_page_len: Read
+    query_output: Write
+    key_pages: Write
+    value_pages: Write
+    batch_indices: Optional[Read] = None
+    positions: Optional[Read] = None
+    query_norm: Optional[Read] = None
+    key_norm: Optional[Read] = None
+    key_scales: Optional[Write] = None
+    value_scales: Optional[Write] = None
+    kv_scales: Optional[Read] = None
+    workspace: Optional[Write] = None
+
+    def __post_init__(self):
+        c = _ffi.NormRopeAppendArgs(*[
+            _h(getattr(self, f)) for f, _ in _ffi.NormRopeAppendArgs._fields_])
+        object.__setattr__(self, "_struct", c)
+        object.__setattr__(self, "_ref", C.byref(c))
+
+
 class Bf16RopePagedKvAppendPlan:
     def __init__(self, ptr, spec):
         self._p = ptr
@@ -1216,8 +1393,12 @@ class Bf16RopePagedKvAppendPlan:
     def workspace_bytes(self) -> int:
         return self.info.workspace_bytes
 
-    def enqueue_into(self, scope: CommandScope, args: Bf16RopePagedKvAppendArgs):
-        if not args.reference_shaped:
+    def enqueue_into(self, scope: CommandScope, args):
+        """`args`: Bf16RopePagedKvAppendArgs, or NormRopePagedKvAppendArgs for a plan of
+        plan_norm_paged_append."""
+        if isinstance(args, NormRopePagedKvAppendArgs):
+            fn = _ffi.load().loom_norm_rope_append_enqueue
+        elif not args.reference_shaped:
             fn = _ffi.load().loom_rope_append_enqueue
         elif args.batch_indices is None:
             fn = _ffi.load().loom_rope_append_enqueue_bf16
@@ -1263,6 +1444,14 @@ class RopeProvider:
         _call(lib().loom_rope_provider_plan_bf16_paged_append_tokens_flags, self._p,
               C.byref(spec._c), (PLAN_PAGE_INDICES_CAPACITY if indices_capacity else 0) | flags,
               C.byref(out))
+        return Bf16RopePagedKvAppendPlan(out.value, spec)
+
+    def plan_norm_paged_append(self, spec: NormRopePagedKvAppendSpec,
+                               indices_capacity: bool = False, flags: int = 0):
+        """The normed append (no reference counterpart), with the same `flags`."""
+        out = C.c_void_p()
+        _call(lib().loom_rope_provider_plan_norm_paged_append, self._p, C.byref(spec._c),
+              (PLAN_PAGE_INDICES_CAPACITY if indices_capacity else 0) | flags, C.byref(out))
         return Bf16RopePagedKvAppendPlan(out.value, spec)
 
     def __del__(self):

@@ -59,6 +59,12 @@ class Bf16PagedBatchDecodeArgs(C.Structure):
                                       "page_indices", "last_page_len", "output", "lse")]
 
 
+class Mxfp4PagedBatchDecodeArgs(C.Structure):
+    _fields_ = [(n, Handle) for n in ("query", "key_pages", "value_pages", "key_scales",
+                                      "value_scales", "page_indptr", "page_indices",
+                                      "last_page_len", "output", "lse", "workspace")]
+
+
 class SingleDecodeSpec(C.Structure):
     _fields_ = [("kv_len", u64), ("num_query_heads", u64), ("num_kv_heads", u64),
                 ("softmax_scale", f32)]
@@ -139,6 +145,29 @@ class Bf16RopePagedKvAppendTokensArgs(C.Structure):
                                       "query_output", "key_pages", "value_pages")]
 
 
+class NormRopeAppendSpec(C.Structure):
+    _fields_ = [("paged", PagedDecodeSpec), ("tokens", u64), ("rope_theta", C.c_double),
+                ("norm_eps", f32), ("explicit_tokens", i32)]
+
+
+class NormRopeAppendArgs(C.Structure):
+    _fields_ = [(n, Handle) for n in ("query", "key", "value", "batch_indices", "positions",
+                                      "page_indptr", "page_indices", "last_page_len",
+                                      "query_norm", "key_norm", "query_output", "key_pages",
+                                      "value_pages", "key_scales", "value_scales", "kv_scales",
+                                      "workspace")]
+
+
+class PagedKvReadSpec(C.Structure):
+    _fields_ = [("paged", PagedDecodeSpec), ("nnz_kv", u64)]
+
+
+class PagedKvReadArgs(C.Structure):
+    _fields_ = [(n, Handle) for n in ("key_pages", "value_pages", "key_scales", "value_scales",
+                                      "page_indptr", "page_indices", "last_page_len", "kv_indptr",
+                                      "kv_start", "key", "value")]
+
+
 P = C.POINTER
 pi32 = P(i32)
 E = P(Error)
@@ -203,6 +232,7 @@ SIGNATURES = {
     "loom_paged_decode_enqueue": (i32, [vp, vp, P(PagedDecodeArgs), E]),
     "loom_paged_decode_enqueue_bf16": (i32, [vp, vp, P(Bf16PagedBatchDecodeArgs), E]),
     "loom_paged_decode_enqueue_bf16_no_alloc": (i32, [vp, vp, P(Bf16PagedBatchDecodeArgs), E]),
+    "loom_paged_decode_enqueue_mxfp4": (i32, [vp, vp, P(Mxfp4PagedBatchDecodeArgs), E]),
     "loom_single_decode_spec_new": (i32, [u64] * 4 + [P(SingleDecodeSpec), E]),
     "loom_single_decode_split_k_spec_new": (
         i32, [P(SingleDecodeSpec), u64, P(SingleDecodeSplitKSpec), E]),
@@ -252,6 +282,15 @@ SIGNATURES = {
     "loom_rope_append_enqueue_bf16": (i32, [vp, vp, P(Bf16RopePagedKvAppendArgs), E]),
     "loom_rope_append_tokens_enqueue_bf16": (
         i32, [vp, vp, P(Bf16RopePagedKvAppendTokensArgs), E]),
+    "loom_norm_rope_append_spec_new": (
+        i32, [P(PagedDecodeSpec), u64, i32, C.c_double, f32, P(NormRopeAppendSpec), E]),
+    "loom_rope_provider_plan_norm_paged_append": (
+        i32, [vp, P(NormRopeAppendSpec), u32, P(vp), E]),
+    "loom_norm_rope_append_enqueue": (i32, [vp, vp, P(NormRopeAppendArgs), E]),
+    "loom_paged_kv_read_spec_new": (i32, [P(PagedDecodeSpec), u64, P(PagedKvReadSpec), E]),
+    "loom_prefill_provider_plan_paged_kv_read": (i32, [vp, P(PagedKvReadSpec), u32, P(vp), E]),
+    "loom_paged_kv_read_plan_free": (None, [vp]),
+    "loom_paged_kv_read_enqueue": (i32, [vp, vp, P(PagedKvReadArgs), E]),
     "loom_graph_queue_new": (i32, [C.c_int, u64, P(vp), E]),
     "loom_graph_queue_free": (None, [vp]),
     "loom_graph_queue_bindings": (i32, [vp, u64, P(vp), E]),
