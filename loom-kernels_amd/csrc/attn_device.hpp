@@ -104,6 +104,26 @@ __device__ __forceinline__ void lds_load4(__amdgpu_buffer_rsrc_t r, void *lds, i
                "s"(m0), "s"(r)
                : "m0", "memory");
 }
+// The same, nontemporal or not.
+template <bool NT>
+__device__ __forceinline__ void lds_load16_at(__amdgpu_buffer_rsrc_t r, uint32_t lds_addr,
+                                              int byte_offset) {
+  if constexpr (!NT) {
+    lds_load16_at(r, lds_addr, byte_offset);
+  } else {
+    const uint32_t m0 = __builtin_amdgcn_readfirstlane(lds_addr);
+    asm volatile("s_mov_b32 m0, %1\n\tbuffer_load_dwordx4 %0, %2, 0 offen nt lds" ::"v"(byte_offset),
+                 "s"(m0), "s"(r)
+                 : "m0", "memory");
+  }
+}
+__device__ __forceinline__ void lds_load4_at(__amdgpu_buffer_rsrc_t r, uint32_t lds_addr,
+                                             int byte_offset) {
+  const uint32_t m0 = __builtin_amdgcn_readfirstlane(lds_addr);
+  asm volatile("s_mov_b32 m0, %1\n\tbuffer_load_dword %0, %2, 0 offen lds" ::"v"(byte_offset),
+               "s"(m0), "s"(r)
+               : "m0", "memory");
+}
 #pragma clang diagnostic pop
 
 // Transposing 8-byte LDS read (ds_read_b64_tr_b16): within each 16 lanes,

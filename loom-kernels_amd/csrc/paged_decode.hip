@@ -41,6 +41,7 @@
 
 #include "attn_device.hpp"
 #include "loom_internal.hpp"
+#include "mx4_decode.hpp"
 
 using loom::fail;
 using namespace loom_dev;
@@ -99,24 +100,14 @@ constexpr int kDepth = LOOM_DECODE_DEPTH;
 #ifndef LOOM_DECODE_SPLIT_WAVES_PER_4CU_FP8
 #define LOOM_DECODE_SPLIT_WAVES_PER_4CU_FP8 32
 #endif
-#ifndef LOOM_DECODE_SPLIT_WAVES_PER_4CU_MX4
-#define LOOM_DECODE_SPLIT_WAVES_PER_4CU_MX4 32
-#endif
 #ifndef LOOM_DECODE_SPLIT_DEPTH_FP8
 #define LOOM_DECODE_SPLIT_DEPTH_FP8 3
 #endif
-// What the pages hold: BF16, FP8 E4M3 with per-tensor scales, or MXFP4.
-enum KvForm : int { kKvBf16 = 0, kKvFp8 = 1, kKvMx4 = 2 };
-#ifndef LOOM_DECODE_SPLIT_DEPTH_MX4
-#define LOOM_DECODE_SPLIT_DEPTH_MX4 4
-#endif
 // Pages in flight per wave of the split kernel (FP8 pages take half the
 // registers per page).
-template <int KV>
+template <bool FP8>
 constexpr int split_depth() {
-  return KV == kKvMx4   ? LOOM_DECODE_SPLIT_DEPTH_MX4
-         : KV == kKvFp8 ? LOOM_DECODE_SPLIT_DEPTH_FP8
-                        : LOOM_DECODE_SPLIT_DEPTH;
+  return FP8 ? LOOM_DECODE_SPLIT_DEPTH_FP8 : LOOM_DECODE_SPLIT_DEPTH;
 }
 // Normalizer written into a state whose pages failed the guard.
 constexpr float kPoisonNormalizer = -1.0f;
@@ -167,10 +158,6 @@ struct DecodeArgs {
   // FP8 E4M3 pages: device [k_scale, v_scale] (K = fp8 * k_scale, V = fp8 *
   // v_scale); null for BF16 pages.
   const float *__restrict__ kv_scales;
-  // MXFP4 pages: E8M0 bytes [pool, Hkv, P, 4], one per 32 dims of a row
-  // (head-major for either page layout); null otherwise.
-  const uint8_t *__restrict__ k_mx;
-  const uint8_t *__restrict__ v_mx;
   // Direct kernel: workgroups per (request, kv-head, tile).  1: the workgroup
   // writes O and LSE; more: each writes the state of its share of the
   // request's blocks to states[((split * B + r) * Hq + qh) * kStateStride]
@@ -189,7 +176,7 @@ __device__ __forceinline__ bool batch_pages_ok(const DecodeArgs &a, int32_t ipB)
 
 
 
-template <int GT, int KV>
+template <int GT>
 struct Smem {
   int64_t incl[kLdsPrefix];           // inclusive page prefix, requests < kLdsPrefix
   int32_t req_st[kLdsPrefix];         // indptr[r] and last_page_len[r], same requests
@@ -198,10 +185,8 @@ struct Smem {
   int64_t wave_tot[kWaves];
   // Per-wave K tile: 16 token rows of 256 bytes padded to kKRowBytes so the
   // MFMA fragment reads (16 rows, same column) hit 16 distinct bank groups.
-  // (MXFP4 pages keep both in registers.)
-  uint8_t ktile[kWaves][KV == kKvMx4 ? 16 : kKTileBytes];
-  // per wave: MFMA B fragments of its query tile
-  u32x4 qfrag[kWaves][KV == kKvMx4 ? 1 : 4][KV == kKvMx4 ? 1 : 64];
+  uint8_t ktile[kWaves][kKTileBytes];
+  u32x4 qfrag[kWaves][4][64];  // per wave: MFMA B fragments of its query tile
 };
 
 // One page of K and V for one wave, both as whole 256-byte rows: lane
@@ -253,21 +238,8 @@ struct PageRegs8 {
   u32x2 v[4];
 };
 
-// The same 16 rows in MXFP4: 64 bytes of E2M1 codes per row of one kv-head
-// (even dim in the low nibble) and 4 E8M0 scale bytes.  K as the A fragment of
-// S = K·Qᵀ wants it: lane (col, quad) holds dims 32 quad + [0, 32) of row col,
-// one scale block, and that row's scale word.  V as in the other forms: 8 dims
-// from 8 col on of rows 4 quad + j, and those rows' scale words.
-struct PageRegs4 {
-  u32x4 k;
-  uint32_t v[4];
-  uint32_t ks;
-  u32x4 vs;
-};
-
-template <int KV>
-using PageBuf = typename std::conditional<
-    KV == kKvMx4, PageRegs4, typename std::conditional<KV == kKvFp8, PageRegs8, PageRegs>::type>::type;
+template <bool FP8>
+using PageBuf = typename std::conditional<FP8, PageRegs8, PageRegs>::type;
 
 __device__ __forceinline__ void load_rows(PageRegs8 &r, const DecodeArgs &a, int64_t elem0,
                                           int valid_rows, int lane, int kvh) {
@@ -291,31 +263,6 @@ __device__ __forceinline__ void load_rows(PageRegs8 &r, const DecodeArgs &a, int
 __device__ __forceinline__ void load_page(PageRegs8 &r, const DecodeArgs &a, int page, int sub,
                                           int valid_rows, int lane, int kvh) {
   load_rows(r, a, block_elem(a, page, sub), valid_rows, lane, kvh);
-}
-
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t bytes_rsrc(const uint8_t *base, int bytes) {
-  return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(base), 0, bytes, 0x00020000);
-}
-__device__ __forceinline__ void load_page(PageRegs4 &r, const DecodeArgs &a, int page, int sub,
-                                          int valid_rows, int lane, int kvh) {
-  const int col = lane & 15, quad = lane >> 4;
-  const int64_t first = (block_elem(a, page, sub) + (int64_t)kvh * a.head_elems) >> 1;
-  const int64_t sfirst = (((int64_t)page * a.hkv + kvh) * a.page_rows + sub * 16) * 4;
-  const int stride = a.row_elems >> 1;
-  const int bytes = valid_rows > 0 ? (valid_rows - 1) * stride + 64 : 0;
-  const int sbytes = valid_rows * 4;
-  const __amdgpu_buffer_rsrc_t rk = bytes_rsrc(reinterpret_cast<const uint8_t *>(a.k) + first, bytes);
-  const __amdgpu_buffer_rsrc_t rv = bytes_rsrc(reinterpret_cast<const uint8_t *>(a.v) + first, bytes);
-  const __amdgpu_buffer_rsrc_t rks = bytes_rsrc(a.k_mx + sfirst, sbytes);
-  const __amdgpu_buffer_rsrc_t rvs = bytes_rsrc(a.v_mx + sfirst, sbytes);
-  r.k = __builtin_bit_cast(
-      u32x4, __builtin_amdgcn_raw_buffer_load_b128(rk, col * stride + quad * 16, 0, 0));
-  r.ks = __builtin_amdgcn_raw_buffer_load_b32(rks, col * 4, 0, 0);
-#pragma unroll
-  for (int j = 0; j < 4; ++j)
-    r.v[j] = __builtin_amdgcn_raw_buffer_load_b32(rv, (quad * 4 + j) * stride + col * 4, 0, 0);
-  r.vs = __builtin_bit_cast(u32x4,
-                            __builtin_amdgcn_raw_buffer_load_b128(rvs, quad * 16, 0, 0));
 }
 
 // K and V row words (BF16 pairs) of a page in either form; FP8 E4M3 bytes
@@ -366,15 +313,14 @@ __device__ __forceinline__ int64_t team_of(int64_t total, int64_t v, int teams) 
 // Both products run on MFMA; the accumulator acc[e][i] holds O[query column
 // col][dim 32 quad + 8 i + e] (unnormalized), so every lane owns 32 output
 // dims of one query column and its softmax state is the column's.
-template <int GT, int KV = kKvBf16>
+template <int GT>
 struct WaveDecoder {
   const DecodeArgs &a;
   uint8_t *kt;          // this wave's K tile (16 rows of kKRowBytes)
-  u32x4 (*qfrag)[64];   // [4][64] MFMA B fragments of the query tile (not for MXFP4)
+  u32x4 (*qfrag)[64];   // [4][64] MFMA B fragments of the query tile
   int lane, col, quad, kvh;
   float m_run, l_run;
   f32x4 acc[8];
-  u32x4 q_regs[4];  // MXFP4: the query fragments
 
   __device__ void reset() {
     m_run = -INFINITY;
@@ -386,21 +332,12 @@ struct WaveDecoder {
   // Q fragment: column `col` is query head qh0 + col (zero beyond gcount);
   // MFMA c contracts dims 32c + 8*quad + [0, 8), the slices the K fragments
   // read.  `prefetched` lets the caller issue other loads before the LDS write.
-  // MXFP4: MFMA c contracts dims 32 quad + 8 c + [0, 8), so that a lane's K
-  // codes are one scale block.
   __device__ void load_q(int r, int qh0, int gcount, u32x4 (&qr)[4]) const {
-    constexpr bool kMx = KV == kKvMx4;
-    const uint16_t *qp = a.q + ((int64_t)r * a.hq + qh0 + col) * 128 + quad * (kMx ? 32 : 8);
+    const uint16_t *qp = a.q + ((int64_t)r * a.hq + qh0 + col) * 128 + quad * 8;
 #pragma unroll
-    for (int c = 0; c < 4; ++c)
-      qr[c] = col < gcount ? load16(qp + c * (kMx ? 8 : 32)) : u32x4{0, 0, 0, 0};
+    for (int c = 0; c < 4; ++c) qr[c] = col < gcount ? load16(qp + c * 32) : u32x4{0, 0, 0, 0};
   }
   __device__ void store_q(const u32x4 (&qr)[4]) {
-    if constexpr (KV == kKvMx4) {
-#pragma unroll
-      for (int c = 0; c < 4; ++c) q_regs[c] = qr[c];
-      return;
-    }
 #pragma unroll
     for (int c = 0; c < 4; ++c) qfrag[c][lane] = qr[c];
     wave_lds_fence();
@@ -412,16 +349,6 @@ struct WaveDecoder {
   template <class Page>
   __device__ void process(const Page &pr, int rows) {
     u32x4 kf[4];
-    f32x4 s = {0.f, 0.f, 0.f, 0.f};
-    if constexpr (KV == kKvMx4) {
-      const uint32_t ks = mx_scale(pr.ks, quad);
-#pragma unroll
-      for (int c = 0; c < 4; ++c) kf[c] = mx4x8_to_bf16x8(pr.k[c], ks);
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-        s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(kf[c]), as_bf16x8(q_regs[c]), s, 0, 0,
-                                                    0);
-    } else {
     // K rows -> LDS tile -> MFMA A fragments (lane: token row `col`, dims
     // 32c + 8*quad + [0, 8)).
 #pragma unroll
@@ -431,11 +358,11 @@ struct WaveDecoder {
 #pragma unroll
     for (int c = 0; c < 4; ++c)
       kf[c] = *reinterpret_cast<const u32x4 *>(kt + col * kKRowBytes + (c * 4 + quad) * 16);
+    f32x4 s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int c = 0; c < 4; ++c)
       s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(kf[c]), as_bf16x8(qfrag[c][lane]), s,
                                                   0, 0, 0);
-    }
     // s[i] = S[token 4 quad + i][query column col]
     float sv[4];
 #pragma unroll
@@ -471,12 +398,7 @@ struct WaveDecoder {
     // zeros and have zero weight.
     u32x4 vw[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if constexpr (KV == kKvMx4)
-        vw[j] = mx4x8_to_bf16x8(pr.v[j], mx_scale(pr.vs[j], col >> 2));
-      else
-        vw[j] = v_words(pr, j);
-    }
+    for (int j = 0; j < 4; ++j) vw[j] = v_words(pr, j);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const int w = e >> 1;
@@ -491,18 +413,20 @@ struct WaveDecoder {
   // each step issues the loads of the block kDepth-1 steps ahead before
   // consuming the current one.  Loads past the end have no valid rows and
   // touch no memory; the unrolled buffer rotation lets the compiler wait for
-  // exactly the oldest block's loads.  load(buf, i, rows) issues the loads of
-  // block i; i and rows_of(i) are wave-uniform.
-  template <class Load, class RowsOf>
-  __device__ void stream(int n, Load load, RowsOf rows_of) {
-    PageBuf<KV> buf[kDepth];
+  // exactly the oldest block's loads.  tok_of(i) (element offset of block i's
+  // first row for kv-head 0)
+  // and rows_of(i) must be wave-uniform.
+  template <bool FP8 = false, class TokOf, class RowsOf>
+  __device__ void stream(int n, TokOf tok_of, RowsOf rows_of) {
+    PageBuf<FP8> buf[kDepth];
 #pragma unroll
-    for (int j = 0; j < kDepth - 1; ++j) load(buf[j], j, rows_of(j));
+    for (int j = 0; j < kDepth - 1; ++j) load_rows(buf[j], a, tok_of(j), rows_of(j), lane, kvh);
     int i = 0;
     while (true) {
 #pragma unroll
       for (int s = 0; s < kDepth; ++s) {
-        load(buf[(s + kDepth - 1) % kDepth], i + kDepth - 1, rows_of(i + kDepth - 1));
+        load_rows(buf[(s + kDepth - 1) % kDepth], a, tok_of(i + kDepth - 1),
+                  rows_of(i + kDepth - 1), lane, kvh);
         process(buf[s], rows_of(i));
         if (++i >= n) return;
       }
@@ -517,7 +441,7 @@ struct WaveDecoder {
 // Normalized output of one query column: the 32 dims acc[e][i] (dim
 // 32 quad + 8 i + e) divided by the normalizer, times V's scale on FP8 pages,
 // as BF16 at o[0..32).
-template <int KV>
+template <bool FP8>
 __device__ __forceinline__ void store_out_row(uint16_t *o, const f32x4 (&acc)[8], float l,
                                               float v_scale) {
 #pragma unroll
@@ -526,7 +450,7 @@ __device__ __forceinline__ void store_out_row(uint16_t *o, const f32x4 (&acc)[8]
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       float x0 = acc[2 * e][i] / l, x1 = acc[2 * e + 1][i] / l;
-      if constexpr (KV == kKvFp8) {
+      if constexpr (FP8) {
         x0 *= v_scale;
         x1 *= v_scale;
       }
@@ -557,14 +481,14 @@ __device__ __forceinline__ int active_teams(int64_t total, int teams) {
   return (int)max<int64_t>(1, min<int64_t>(teams, by_pages));
 }
 
-template <int GT, int KV = kKvBf16>
+template <int GT, bool FP8 = false>
 __global__ __launch_bounds__(kThreads, LOOM_DECODE_SPLIT_WAVES) void paged_decode_split_kv_kernel(
     DecodeArgs a) {
-  __shared__ Smem<GT, KV> sm;
-  constexpr int kSD = split_depth<KV>();
+  __shared__ Smem<GT> sm;
+  constexpr int kSD = split_depth<FP8>();
   // FP8 pages: K's scale folds into the score scale, V's into the output.
   float v_scale = 1.0f;
-  if constexpr (KV == kKvFp8) {
+  if constexpr (FP8) {
     a.scale_log2 *= a.kv_scales[0];
     v_scale = a.kv_scales[1];
   }
@@ -708,7 +632,7 @@ __global__ __launch_bounds__(kThreads, LOOM_DECODE_SPLIT_WAVES) void paged_decod
     tl_out = uni(tl_out);
     return uni(c);
   };
-  WaveDecoder<GT, KV> w{a, kt, reinterpret_cast<u32x4(*)[64]>(sm.qfrag[wave]), lane, col, quad, kvh};
+  WaveDecoder<GT> w{a, kt, sm.qfrag[wave], lane, col, quad, kvh};
   const int64_t qh_base = (int64_t)kvh * a.group + g_base;
 
   // ---- one continuous page stream over [v_begin, v_end) --------------------
@@ -812,7 +736,7 @@ __global__ __launch_bounds__(kThreads, LOOM_DECODE_SPLIT_WAVES) void paged_decod
       // invalid page index leaves the request's sentinels untouched.
       if (!bad && mine) {
         uint16_t *o = a.out + ((int64_t)rr * a.hq + qh_base + col) * 128 + quad * 32;
-        store_out_row<KV>(o, acc, l_tot, v_scale);
+        store_out_row<FP8>(o, acc, l_tot, v_scale);
         if (quad == 0) a.lse[(int64_t)rr * a.hq + qh_base + col] = m_run + __log2f(l_tot);
       }
     } else {
@@ -844,7 +768,7 @@ __global__ __launch_bounds__(kThreads, LOOM_DECODE_SPLIT_WAVES) void paged_decod
   // Pipeline: page v+kSD-1 is issued before page v is consumed; the
   // unrolled buffer rotation lets the compiler wait for exactly the oldest
   // page's loads.
-  PageBuf<KV> buf[kSD];
+  PageBuf<FP8> buf[kSD];
   int brows[kSD];
 #pragma unroll
   for (int j = 0; j < kSD - 1; ++j) {
@@ -899,10 +823,10 @@ stream_done:
 // is launch- and latency-bound.  With a.splits > 1 each request's blocks are
 // cut into a.splits equal ranges, one workgroup each, which write states for
 // paged_decode_direct_merge_kernel instead of O and LSE.
-template <int GT, int W = kWaves, int KV = kKvBf16>
+template <int GT, int W = kWaves>
 struct DirectSmem {
-  uint8_t ktile[W][KV == kKvMx4 ? 16 : kKTileBytes];
-  u32x4 qfrag[W][KV == kKvMx4 ? 1 : 4][KV == kKvMx4 ? 1 : 64];
+  uint8_t ktile[W][kKTileBytes];
+  u32x4 qfrag[W][4][64];
   float wm[W][GT];
   float wl[W][GT];
   float wacc[W][GT][128];
@@ -913,18 +837,18 @@ struct DirectSmem {
 // more pages, so each wave streams fewer of them).
 // Waves per SIMD the direct kernel's LDS allows (160 KiB per CU), at most the
 // register target.
-template <int GT, int W, int KV>
+template <int GT, int W>
 constexpr int direct_waves_per_eu() {
-  const int per_cu = (int)((160 * 1024) / sizeof(DirectSmem<GT, W, KV>)) * W / 4;
+  const int per_cu = (int)((160 * 1024) / sizeof(DirectSmem<GT, W>)) * W / 4;
   return per_cu < 1 ? 1 : per_cu < waves_per_eu<GT>() ? per_cu : waves_per_eu<GT>();
 }
 
-template <int GT, int W, int KV = kKvBf16>
-__global__ __launch_bounds__(W * 64, (direct_waves_per_eu<GT, W, KV>())) void paged_decode_direct_kernel(
+template <int GT, int W, bool FP8 = false>
+__global__ __launch_bounds__(W * 64, (direct_waves_per_eu<GT, W>())) void paged_decode_direct_kernel(
     DecodeArgs a) {
-  __shared__ DirectSmem<GT, W, KV> sm;
+  __shared__ DirectSmem<GT, W> sm;
   float v_scale = 1.0f;
-  if constexpr (KV == kKvFp8) {
+  if constexpr (FP8) {
     a.scale_log2 *= a.kv_scales[0];
     v_scale = a.kv_scales[1];
   }
@@ -949,8 +873,7 @@ __global__ __launch_bounds__(W * 64, (direct_waves_per_eu<GT, W, KV>())) void pa
   auto poison = [&]() {
     if (a.splits > 1 && tid < gcount) state_of(tid)[1] = kPoisonNormalizer;
   };
-  WaveDecoder<GT, KV> w{a, sm.ktile[wave], reinterpret_cast<u32x4(*)[64]>(sm.qfrag[wave]),
-                        lane, col, quad, kvh};
+  WaveDecoder<GT> w{a, sm.ktile[wave], sm.qfrag[wave], lane, col, quad, kvh};
   // One round trip for the guard words (decode.rs:233-246 global, :430-478
   // per request), the query tile and, when the page-index array has at most
   // 128 entries (as direct plans' tables do), the whole array (two words per
@@ -997,16 +920,15 @@ __global__ __launch_bounds__(W * 64, (direct_waves_per_eu<GT, W, KV>())) void pa
       const int n = min(mine - s0, 64);
       const int ok = (idx >= 0 && (int64_t)idx < a.pool) ? 1 : 0;
       bad |= __ballot(lane < n && !ok) != 0;
-      auto load = [&](PageBuf<KV> &b, int i, int rows) {
+      auto tok_of = [&](int i) {
         const int j = min(i, n - 1);
-        load_page(b, a, __builtin_amdgcn_readlane(idx, j), (lo + wave + W * (s0 + j)) & bmask, rows,
-                  lane, kvh);
+        return block_elem(a, __builtin_amdgcn_readlane(idx, j), (lo + wave + W * (s0 + j)) & bmask);
       };
       auto rows_of = [&](int i) {
         if (i >= n || !__builtin_amdgcn_readlane(ok, i)) return 0;
         return lo + wave + W * (s0 + i) == cnt - 1 ? tl_rows : 16;
       };
-      w.stream(n, load, rows_of);
+      w.template stream<FP8>(n, tok_of, rows_of);
     }
   }
   const float l_tot = w.reduce();
@@ -1047,7 +969,7 @@ __global__ __launch_bounds__(W * 64, (direct_waves_per_eu<GT, W, KV>())) void pa
       continue;
     }
     float o = O / L;
-    if constexpr (KV == kKvFp8) o *= v_scale;
+    if constexpr (FP8) o *= v_scale;
     a.out[((int64_t)r * a.hq + qh_base + g) * 128 + d] = f32_to_bf16(o);
     if (d == 0) a.lse[(int64_t)r * a.hq + qh_base + g] = M + __log2f(L);
   }
@@ -1195,15 +1117,14 @@ __global__ __launch_bounds__(kThreads, waves_per_eu<GT>()) void single_decode_ke
   }
   w.reset();
   if (mine > 0) {
-    auto load = [&](PageRegs &b, int i, int rows) {
-      load_rows(b, a, token_elem(a, (int64_t)(wave + kWaves * min(i, mine - 1)) * 16), rows, lane,
-                kvh);
+    auto tok_of = [&](int i) {
+      return token_elem(a, (int64_t)(wave + kWaves * min(i, mine - 1)) * 16);
     };
     auto rows_of = [&](int i) {
       if (i >= mine) return 0;
       return (int)min<int64_t>(16, kv_len - (int64_t)(wave + kWaves * i) * 16);
     };
-    w.stream(mine, load, rows_of);
+    w.stream(mine, tok_of, rows_of);
   }
   const float l_tot = w.reduce();
   if (col < GT) {
@@ -1265,13 +1186,11 @@ __global__ __launch_bounds__(kThreads, waves_per_eu<GT>()) void single_decode_sp
   // state NaN.  (One with no other token stores the empty state.)
   w.m_run = -FLT_MAX;
   const int nb = (int)((end - start + 15) / 16);
-  auto load = [&](PageRegs &b, int i, int rows) {
-    load_rows(b, a, token_elem(a, start + (int64_t)min(i, nb - 1) * 16), rows, lane, kvh);
-  };
+  auto tok_of = [&](int i) { return token_elem(a, start + (int64_t)min(i, nb - 1) * 16); };
   auto rows_of = [&](int i) {
     return i >= nb ? 0 : (int)min<int64_t>(16, end - start - (int64_t)i * 16);
   };
-  w.stream(nb, load, rows_of);
+  w.stream(nb, tok_of, rows_of);
   const float l_tot = w.reduce();
   const int64_t qh_base = (int64_t)kvh * a.group + g_base;
   if (col < gcount) {
@@ -1421,39 +1340,39 @@ DecodeArgs single_args(const loom_single_decode_spec_t &s, uint32_t gtiles, uint
 }  // namespace
 
 namespace {
-template <int KV>
+template <bool FP8>
 void launch_direct(const loom_paged_decode_plan_info_t &pi, dim3 g3, dim3 bd, hipStream_t stream,
                    const DecodeArgs &a) {
   if (pi.block_threads == 4 * 64) {
     switch (pi.group_tile) {
-      case 1: hipLaunchKernelGGL((paged_decode_direct_kernel<1, 4, KV>), g3, bd, 0, stream, a); break;
-      case 2: hipLaunchKernelGGL((paged_decode_direct_kernel<2, 4, KV>), g3, bd, 0, stream, a); break;
-      case 4: hipLaunchKernelGGL((paged_decode_direct_kernel<4, 4, KV>), g3, bd, 0, stream, a); break;
-      default: hipLaunchKernelGGL((paged_decode_direct_kernel<8, 4, KV>), g3, bd, 0, stream, a); break;
+      case 1: hipLaunchKernelGGL((paged_decode_direct_kernel<1, 4, FP8>), g3, bd, 0, stream, a); break;
+      case 2: hipLaunchKernelGGL((paged_decode_direct_kernel<2, 4, FP8>), g3, bd, 0, stream, a); break;
+      case 4: hipLaunchKernelGGL((paged_decode_direct_kernel<4, 4, FP8>), g3, bd, 0, stream, a); break;
+      default: hipLaunchKernelGGL((paged_decode_direct_kernel<8, 4, FP8>), g3, bd, 0, stream, a); break;
     }
   } else if (pi.block_threads == 16 * 64) {
     if (pi.group_tile == 1)
-      hipLaunchKernelGGL((paged_decode_direct_kernel<1, 16, KV>), g3, bd, 0, stream, a);
+      hipLaunchKernelGGL((paged_decode_direct_kernel<1, 16, FP8>), g3, bd, 0, stream, a);
     else
-      hipLaunchKernelGGL((paged_decode_direct_kernel<2, 16, KV>), g3, bd, 0, stream, a);
+      hipLaunchKernelGGL((paged_decode_direct_kernel<2, 16, FP8>), g3, bd, 0, stream, a);
   } else {
     switch (pi.group_tile) {
-      case 1: hipLaunchKernelGGL((paged_decode_direct_kernel<1, 8, KV>), g3, bd, 0, stream, a); break;
-      case 2: hipLaunchKernelGGL((paged_decode_direct_kernel<2, 8, KV>), g3, bd, 0, stream, a); break;
-      case 4: hipLaunchKernelGGL((paged_decode_direct_kernel<4, 8, KV>), g3, bd, 0, stream, a); break;
-      default: hipLaunchKernelGGL((paged_decode_direct_kernel<8, 8, KV>), g3, bd, 0, stream, a); break;
+      case 1: hipLaunchKernelGGL((paged_decode_direct_kernel<1, 8, FP8>), g3, bd, 0, stream, a); break;
+      case 2: hipLaunchKernelGGL((paged_decode_direct_kernel<2, 8, FP8>), g3, bd, 0, stream, a); break;
+      case 4: hipLaunchKernelGGL((paged_decode_direct_kernel<4, 8, FP8>), g3, bd, 0, stream, a); break;
+      default: hipLaunchKernelGGL((paged_decode_direct_kernel<8, 8, FP8>), g3, bd, 0, stream, a); break;
     }
   }
 }
 
-template <int KV>
+template <bool FP8>
 void launch_split(const loom_paged_decode_plan_info_t &pi, dim3 g3, dim3 b3, hipStream_t stream,
                   const DecodeArgs &a) {
   switch (pi.group_tile) {
-    case 1: hipLaunchKernelGGL((paged_decode_split_kv_kernel<1, KV>), g3, b3, 0, stream, a); break;
-    case 2: hipLaunchKernelGGL((paged_decode_split_kv_kernel<2, KV>), g3, b3, 0, stream, a); break;
-    case 4: hipLaunchKernelGGL((paged_decode_split_kv_kernel<4, KV>), g3, b3, 0, stream, a); break;
-    default: hipLaunchKernelGGL((paged_decode_split_kv_kernel<8, KV>), g3, b3, 0, stream, a); break;
+    case 1: hipLaunchKernelGGL((paged_decode_split_kv_kernel<1, FP8>), g3, b3, 0, stream, a); break;
+    case 2: hipLaunchKernelGGL((paged_decode_split_kv_kernel<2, FP8>), g3, b3, 0, stream, a); break;
+    case 4: hipLaunchKernelGGL((paged_decode_split_kv_kernel<4, FP8>), g3, b3, 0, stream, a); break;
+    default: hipLaunchKernelGGL((paged_decode_split_kv_kernel<8, FP8>), g3, b3, 0, stream, a); break;
   }
 }
 }  // namespace
@@ -1512,6 +1431,19 @@ loom_status_t loom_decode_provider_plan_bf16_paged_batch(
 
   if (B > (uint64_t)kMaxScanBlocks * kThreads)
     return fail(err, LOOM_PLAN_STATE_COUNT_OUT_OF_RANGE, "batch_size", B);
+  if (spec->kv_dtype == LOOM_KV_DTYPE_MXFP4) {  // kernels and rules of their own
+    loom_paged_decode_plan_info_t info{};
+    info.spec = *spec;
+    info.max_total_pages = max_pages;
+    info.flags = opt.flags;
+    const loom_status_t rc = loom::plan_mx4_decode(&info, opt.teams, provider->dev.cus, err);
+    if (rc) return rc;
+    auto *p = new loom_paged_decode_plan;
+    p->device = provider->dev.device;
+    p->info = info;
+    *out = p;
+    return loom::ok(err);
+  }
 
   if (opt.teams == 0 && max_pages <= LOOM_DECODE_DIRECT_MAX_PAGES) {
     // More waves per request when a request may hold more pages; 16-wave
@@ -1561,9 +1493,8 @@ loom_status_t loom_decode_provider_plan_bf16_paged_batch(
   const uint64_t members = hkv * gtiles;
   const uint64_t slots =
       (uint64_t)provider->dev.cus *
-      (spec->kv_dtype == LOOM_KV_DTYPE_MXFP4      ? LOOM_DECODE_SPLIT_WAVES_PER_4CU_MX4
-       : spec->kv_dtype == LOOM_KV_DTYPE_FP8_E4M3 ? LOOM_DECODE_SPLIT_WAVES_PER_4CU_FP8
-                                                  : LOOM_DECODE_SPLIT_WAVES_PER_4CU) / 4;
+      (spec->kv_dtype == LOOM_KV_DTYPE_FP8_E4M3 ? LOOM_DECODE_SPLIT_WAVES_PER_4CU_FP8
+                                                : LOOM_DECODE_SPLIT_WAVES_PER_4CU) / 4;
   uint64_t teams = opt.teams ? opt.teams : std::max<uint64_t>(1, slots / members);
   // Each XCD (every 8th workgroup) holds ceil(teams / 8) whole teams.
   const uint64_t xcd_waves = (teams + 7) / 8 * members;
@@ -1753,10 +1684,41 @@ loom_status_t paged_decode_enqueue_impl(const loom_paged_decode_plan_t *plan,
     if (!ws)  // no decode provider was loaded on this device
       return fail(err, LOOM_PLAN_UNSUPPORTED_DEVICE, "static scratch", dev);
   }
+  if (mx4) {
+    loom::Mx4DecodeArgs m{};
+    m.q = (const uint16_t *)l(0)->ptr;
+    m.k = (const uint8_t *)l(1)->ptr;
+    m.v = (const uint8_t *)l(2)->ptr;
+    m.k_mx = (const uint8_t *)l(10)->ptr;
+    m.v_mx = (const uint8_t *)l(11)->ptr;
+    m.indptr = (const int32_t *)l(3)->ptr;
+    m.indices = (const int32_t *)l(4)->ptr;
+    m.last = (const int32_t *)l(5)->ptr;
+    m.out = (uint16_t *)l(6)->ptr;
+    m.lse = (float *)l(7)->ptr;
+    m.header = (int64_t *)ws;
+    m.states = (float *)(ws + pi.header_bytes);
+    m.pool = (int64_t)s.max_num_pages;
+    m.n_indices = (int64_t)l(4)->numel;
+    m.indices_capacity = (pi.flags & LOOM_PLAN_PAGE_INDICES_CAPACITY) ? 1 : 0;
+    m.batch = (int32_t)s.batch_size;
+    m.hq = (int32_t)s.num_query_heads;
+    m.hkv = (int32_t)s.num_kv_heads;
+    m.group = m.hq / m.hkv;
+    m.tile = (int32_t)pi.group_tile;
+    m.tiles = (int32_t)pi.group_tiles;
+    m.teams = (int32_t)pi.teams;
+    m.splits = pi.algorithm == LOOM_PAGED_DECODE_DIRECT && pi.teams > 1 ? (int32_t)pi.teams : 1;
+    m.page_rows = (int32_t)page_rows;
+    const bool head_major = s.kv_layout == LOOM_KV_LAYOUT_HND;
+    m.head_bytes = head_major ? m.page_rows * 64 : 64;
+    m.row_bytes = head_major ? 64 : m.hkv * 64;
+    m.page_bytes = (int64_t)m.page_rows * m.hkv * 64;
+    m.scale_log2 = s.softmax_scale * 1.44269504088896340736f;
+    return loom::record_launch(scope, loom::launch_mx4_decode(pi, m, scope->queue->stream), err);
+  }
   DecodeArgs a{};
   a.kv_scales = fp8 ? (const float *)l(9)->ptr : nullptr;
-  a.k_mx = mx4 ? (const uint8_t *)l(10)->ptr : nullptr;
-  a.v_mx = mx4 ? (const uint8_t *)l(11)->ptr : nullptr;
   a.q = (const uint16_t *)l(0)->ptr;
   a.k = (const uint16_t *)l(1)->ptr;
   a.v = (const uint16_t *)l(2)->ptr;
@@ -1793,12 +1755,10 @@ loom_status_t paged_decode_enqueue_impl(const loom_paged_decode_plan_t *plan,
   const dim3 g3((unsigned)grid), b3(kThreads);
   if (direct) {
     const dim3 bd(pi.block_threads);
-    if (mx4)
-      launch_direct<kKvMx4>(pi, g3, bd, stream, a);
-    else if (fp8)
-      launch_direct<kKvFp8>(pi, g3, bd, stream, a);
+    if (fp8)
+      launch_direct<true>(pi, g3, bd, stream, a);
     else
-      launch_direct<kKvBf16>(pi, g3, bd, stream, a);
+      launch_direct<false>(pi, g3, bd, stream, a);
     hipError_t e = hipGetLastError();
     if (e == hipSuccess && a.splits > 1) {
       hipLaunchKernelGGL(paged_decode_direct_merge_kernel,
@@ -1807,12 +1767,10 @@ loom_status_t paged_decode_enqueue_impl(const loom_paged_decode_plan_t *plan,
     }
     return loom::record_launch(scope, e, err);
   }
-  if (mx4)
-    launch_split<kKvMx4>(pi, g3, b3, stream, a);
-  else if (fp8)
-    launch_split<kKvFp8>(pi, g3, b3, stream, a);
+  if (fp8)
+    launch_split<true>(pi, g3, b3, stream, a);
   else
-    launch_split<kKvBf16>(pi, g3, b3, stream, a);
+    launch_split<false>(pi, g3, b3, stream, a);
   hipError_t e = hipGetLastError();
   if (e == hipSuccess) {
     // One command: the partial kernel, then the merge of split requests.

@@ -1,0 +1,951 @@
+// Paged decode attention over MXFP4 pages for gfx950 (MI355X), D128, 16-64 rows per
+// page, NHD or HND (no reference counterpart).
+//
+// Per query head: S = q.k / sqrt(128), O = softmax(S).V, LSE in log2, over the values
+// code * 2^(scale - 127) of the request's tokens.  A token costs 136 bytes per kv-head
+// where BF16 pages cost 512, so the arithmetic per byte is four times as dense and the
+// instructions of a step, not its bytes, come close to binding.  The step is built
+// for few of them:
+//   * 32 tokens at a time.  K codes are loaded as the MFMA fragment wants them: lane
+//     (col, quad) takes the 16 bytes of dims 32 quad + [0, 32) of row col, one scale
+//     block, and v_cvt_scalef32_pk_bf16_fp4 widens two codes and applies the block's
+//     scale in one instruction, exactly.  No LDS.  (v_mfma_scale_f32_16x16x128_f8f6f4
+//     takes FP4 itself, but sums its 128 products with errors up to 2^-12 of the
+//     largest, which LSE does not bear.)
+//   * V codes come as 8 dims from 8 col on of rows 4 quad + j; one byte permute per
+//     two tokens turns the widened pairs into the V^T fragment.
+//   * The running bound of the scores is set kLazy above a new maximum and moves only
+//     when a score passes it: the common step has no reduction across lanes and no
+//     rescale, and no weight is above 1 (large V do not overflow).
+//   * P keeps 16 bits, a BF16 high part and a BF16 residual, in one MFMA: a tile is at
+//     most 8 query heads, which fill columns 0-7 and again 8-15; the first eight take
+//     the high parts, the others the residuals, and the two columns' O are added at the
+//     end.
+//
+// Two decompositions, both independent of the page table's contents:
+//   balanced  the 32-token blocks of all valid requests form one virtual list, cut
+//             into `teams` equal ranges; a team is one wave per (kv-head, tile), all
+//             walking the same blocks.  Requests that cross a range leave states, which
+//             a second kernel merges.
+//   direct    one workgroup per (request, kv-head, tile[, split]): its waves take the
+//             blocks in turn and merge in LDS.  One launch, or a merge of the splits.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cfloat>
+#include <cmath>
+
+#include "attn_device.hpp"
+#include "mx4_decode.hpp"
+
+using loom::fail;
+using loom::kMx4StateStride;
+using loom::Mx4DecodeArgs;
+using namespace loom_dev;
+
+namespace {
+
+constexpr int kBlock = 32;  // tokens per step
+constexpr int kThreads = 256;
+constexpr int kWaves = 4;
+constexpr int kMaxTile = 8;  // query heads of a tile
+// Entries of the balanced kernel's prefix table in LDS; a batch beyond it has one
+// entry per 2, 4, ... requests.
+constexpr int kPrefix = 512;
+constexpr int kMaxBatch = 65536;
+// log2 of how far the bound of the scores lies above the maximum that set it.  Weights
+// are 2^-8 and less then, which costs no precision in FP32 or in their two BF16 parts.
+constexpr float kLazy = 8.0f;
+// Normalizer written into a state whose pages failed the guard.
+constexpr float kPoisonNormalizer = -1.0f;
+#ifndef LOOM_MX4_DEPTH
+#define LOOM_MX4_DEPTH 2
+#endif
+#ifndef LOOM_MX4_WAVES_PER_EU
+#define LOOM_MX4_WAVES_PER_EU 2
+#endif
+#ifndef LOOM_MX4_WAVES_PER_4CU
+#define LOOM_MX4_WAVES_PER_4CU 16
+#endif
+#ifndef LOOM_MX4_MIN_TEAM_BLOCKS
+#define LOOM_MX4_MIN_TEAM_BLOCKS 4
+#endif
+constexpr int kDepth = LOOM_MX4_DEPTH;  // blocks in flight per wave
+
+// decode.rs:233-246: indptr[B] is the page_indices length (at most that length for
+// capacity plans).
+__device__ __forceinline__ bool batch_ok(const Mx4DecodeArgs &a, int32_t ip0, int32_t ipB) {
+  return ip0 == 0 && ipB >= 0 &&
+         (a.indices_capacity ? (int64_t)ipB <= a.n_indices : (int64_t)ipB == a.n_indices);
+}
+// Tokens of a request (0 if it fails the per-request guard of decode.rs:430-478).
+__device__ __forceinline__ int64_t request_tokens(const Mx4DecodeArgs &a, int32_t st, int32_t en,
+                                                  int32_t tl, int32_t ipB) {
+  const bool valid = st >= 0 && en > st && en <= ipB && tl >= 1 && tl <= a.page_rows;
+  return valid ? ((int64_t)en - st - 1) * a.page_rows + tl : 0;
+}
+
+// floor(n / d) for 0 <= n < 2^53, d > 0: a double-precision estimate, corrected.
+__device__ __forceinline__ int64_t floor_div(int64_t n, int64_t d) {
+  int64_t q = (int64_t)((double)n / (double)d);
+  while (q * d > n) --q;
+  while ((q + 1) * d <= n) ++q;
+  return q;
+}
+// Team t owns virtual blocks [team_start(t), team_start(t + 1)).
+__device__ __forceinline__ int64_t team_start(int64_t total, int64_t t, int teams) {
+  return floor_div(total * t, teams);
+}
+__device__ __forceinline__ int64_t team_of(int64_t total, int64_t v, int teams) {
+  return floor_div((v + 1) * teams + total - 1, total) - 1;
+}
+// Teams in use: at most the planned count, at least LOOM_MX4_MIN_TEAM_BLOCKS each.
+__device__ __forceinline__ int active_teams(int64_t total, int teams) {
+  return (int)max<int64_t>(1, min<int64_t>(teams, total / LOOM_MX4_MIN_TEAM_BLOCKS));
+}
+
+// One 32-token block as a wave stages it in LDS: K and V codes of one or two kv-heads
+// and the rows' scale words.  Loads go straight to LDS (nothing is held in registers
+// in flight), lane l's 16 bytes to 16 l, so the order within a slot is chosen by the
+// addresses the lanes load from.  Two arrangements:
+//   kSplit  per head 64-byte rows: HND pages, and single heads.  Lane l takes piece
+//           (l & 3) ^ (l >> 4) of row l >> 2 of a half (16 rows).
+//   kPair   128-byte rows of two neighbouring heads: NHD pages, whose rows hold them side
+//           by side; 64-byte loads of half a cache line each ran at 4.5 TB/s where these
+//           reach 5.7 (8 requests of 32768 tokens).  Lane l takes piece
+//           (l & 7) ^ pair_swizzle(row) of row l >> 3 of eight rows.
+// Either way the reads below, which take one 16-byte piece of all rows of a half or 64
+// bytes of every fourth row, meet each LDS bank once.  Scale word c of a half belongs to
+// its row token_of(c).
+enum Arrangement : int { kSplit = 0, kPair = 1 };
+constexpr int kHalfBytes = 16 * 64;
+constexpr int kHeadBytes = 2 * kHalfBytes;  // K (or V) codes of one head's block
+// Row of a half that row c of the MFMA tile S = K.Q^T stands for: S leaves lane (col,
+// quad) rows 4 quad + i, which are tokens 4 i + quad, and the V reads of the four quads
+// then lie in four neighbouring rows.
+__host__ __device__ constexpr int token_of(int c) { return 4 * (c & 3) + (c >> 2); }
+__host__ __device__ constexpr int pair_swizzle(int row) { return (row & 2) * 2 + (row >> 2); }
+
+// Byte offsets in a slot: K of all heads, V of all heads, then the scales (per half and
+// head 16 words).
+template <int NH>
+struct Slot {
+  static constexpr int v = NH * kHeadBytes, ks = 2 * NH * kHeadBytes, vs = ks + NH * 128,
+                       bytes = vs + NH * 128;
+  // scale words of (head, half): pages of 16 rows load a half of all heads at a time,
+  // others both halves of a head
+  template <bool P16>
+  static __host__ __device__ constexpr int scales(int head, int half) {
+    return P16 ? half * NH * 64 + head * 64 : head * 128 + half * 64;
+  }
+};
+
+// Where a block lies: the pages of its two halves (the same one unless pages have 16
+// rows), its first row in the page, and its valid rows (0: none, nothing is read).  All
+// wave-uniform.
+struct Place {
+  int p0, p1, row, rows;
+};
+
+// Vector memory instructions that load_block issues, always.
+template <bool P16, int NH>
+constexpr int kBlockLoads = 4 * NH + (P16 ? 4 : 2);
+// Issues the loads of a block of heads kvh .. kvh + NH - 1 into LDS at byte address
+// `slot`.  Rows past the valid ones arrive as zeros and move no bytes.
+// NT: nontemporal loads of the codes.
+template <bool P16, int NH, int ARR, bool NT>
+__device__ __forceinline__ void load_block(const Mx4DecodeArgs &a, const Place &p, uint32_t slot,
+                                           int lane, int kvh) {
+  using S = Slot<NH>;
+  auto rsrc = [](const uint8_t *base, int bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(base), 0, bytes, 0x00020000);
+  };
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    // rows [0, n) of this half (of the whole block where it lies in one page) exist
+    const int n = !P16 ? p.rows : h == 0 ? min(p.rows, 16) : max(p.rows - 16, 0);
+    const int64_t page = P16 && h == 1 ? p.p1 : p.p0;
+    const int64_t at = page * a.page_bytes + (int64_t)kvh * a.head_bytes + (int64_t)p.row * a.row_bytes;
+    const int skip = P16 ? 0 : 16 * h * a.row_bytes;
+    if constexpr (ARR == kPair) {
+      const int bytes = n > 0 ? (n - 1) * a.row_bytes + 128 : 0;
+      const __amdgpu_buffer_rsrc_t rk = rsrc(a.k + at, bytes), rv = rsrc(a.v + at, bytes);
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const int row = 8 * t + (lane >> 3);
+        const int off = row * a.row_bytes + (((lane & 7) ^ pair_swizzle(row)) << 4) + skip;
+        lds_load16_at<NT>(rk, slot + (2 * h + t) * 1024, off);
+        lds_load16_at<NT>(rv, slot + S::v + (2 * h + t) * 1024, off);
+      }
+    } else {
+      const int bytes = n > 0 ? (n - 1) * a.row_bytes + 64 : 0;
+      const int off = (lane >> 2) * a.row_bytes + (((lane & 3) ^ (lane >> 4)) << 4) + skip;
+#pragma unroll
+      for (int g = 0; g < NH; ++g) {
+        const int64_t head = at + (int64_t)g * a.head_bytes;
+        lds_load16_at<NT>(rsrc(a.k + head, bytes), slot + g * kHeadBytes + h * kHalfBytes, off);
+        lds_load16_at<NT>(rsrc(a.v + head, bytes), slot + S::v + g * kHeadBytes + h * kHalfBytes, off);
+      }
+    }
+    // scale words: one lane each, 16 rows (P16) or 32 of every head
+    if (P16 || h == 0) {
+      constexpr int kRows = P16 ? 16 : 32;
+      if (lane < kRows * NH) {
+        const int row = token_of(lane & 15) + (P16 ? 0 : lane & 16);
+        const int64_t sc = ((page * a.hkv + kvh) * a.page_rows + p.row) * 4;
+        const int off = row < n ? (lane / kRows) * a.page_rows * 4 + row * 4 : INT32_MAX;
+        const int bytes = n > 0 ? ((NH - 1) * a.page_rows + n) * 4 : 0;
+        lds_load4_at(rsrc(a.k_mx + sc, bytes), slot + S::ks + h * NH * 64, off);
+        lds_load4_at(rsrc(a.v_mx + sc, bytes), slot + S::vs + h * NH * 64, off);
+      }
+    }
+  }
+}
+// Until at most N of this wave's vector memory operations are outstanding; LDS reads
+// stay behind it.
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+// Until this wave's LDS reads have returned: before loads into a slot that it read.
+__device__ __forceinline__ void wait_reads() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
+// One wave's decode of a request for NH neighbouring kv-heads and a tile of each one's
+// query heads: the online-softmax states.  acc[e][i] holds O[column col][dim 32 quad +
+// 8 i + e], unnormalized.
+struct HeadState {
+  float m_run, l_run;  // bound of the scores (log2); sum of this lane's weights
+  f32x4 acc[8];
+  u32x4 q[4];  // MFMA c contracts dims 32 quad + 8 c + [0, 8)
+
+  // From the lowest finite maximum, tokens that score -inf weigh nothing.
+  __device__ __forceinline__ void reset() {
+    m_run = -FLT_MAX;
+    l_run = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) acc[e] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  __device__ __forceinline__ void load_q(const uint16_t *row, bool mine, int quad) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      q[c] = mine ? load16(row + quad * 32 + c * 8) : u32x4{0, 0, 0, 0};
+  }
+  // Ends load_q's loads here: left in flight, they would make every block's first
+  // MFMA wait for all loads before it, the pipeline's next blocks among them.
+  __device__ __forceinline__ void settle_q() {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) asm volatile("" : "+v"(q[c]));
+  }
+  __device__ __forceinline__ float normalizer() const { return quad_sum(l_run); }
+  // O of this lane's column (dims 32 quad + [0, 32)) and, by quad 0, LSE.
+  __device__ __forceinline__ void store(uint16_t *o, float *lse, float l, int quad) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      u32x4 w;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = bf16x2_pack(acc[2 * e][i] / l, acc[2 * e + 1][i] / l);
+      *reinterpret_cast<u32x4 *>(o + quad * 32 + i * 8) = w;
+    }
+    if (quad == 0) *lse = m_run + __log2f(l);
+  }
+  // The same column's unnormalized O.
+  __device__ __forceinline__ void stash(float *dst, int quad) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float *o = dst + quad * 32 + i * 8;
+      *reinterpret_cast<f32x4 *>(o) = f32x4{acc[0][i], acc[1][i], acc[2][i], acc[3][i]};
+      *reinterpret_cast<f32x4 *>(o + 4) = f32x4{acc[4][i], acc[5][i], acc[6][i], acc[7][i]};
+    }
+  }
+
+  // Adds the residuals' columns to the high parts' (lane col ^ 8 of the 16).
+  __device__ __forceinline__ void join_columns() {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        acc[e][i] += __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(
+            0, (int)__float_as_uint(acc[e][i]), 0x128, 0xf, 0xf, false));
+  }
+
+  // Dims e = 2 W and 2 W + 1 of O^T += V^T.P^T: V^T's row col of fragment e is dim
+  // 8 col + e, and byte W of the lane's codes holds both dims.
+  template <int W>
+  __device__ __forceinline__ void add_pv(const uint32_t (&v)[2][4], const float (&vs)[2][4],
+                                         bf16x8 p) {
+    uint32_t x[2][4];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        x[h][j] = __builtin_bit_cast(
+            uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v[h][j], vs[h][j], W));
+    const bf16x8 even =
+        as_bf16x8(pack_lo16(x[0][0], x[0][1]), pack_lo16(x[0][2], x[0][3]),
+                  pack_lo16(x[1][0], x[1][1]), pack_lo16(x[1][2], x[1][3]));
+    const bf16x8 odd =
+        as_bf16x8(pack_hi16(x[0][0], x[0][1]), pack_hi16(x[0][2], x[0][3]),
+                  pack_hi16(x[1][0], x[1][1]), pack_hi16(x[1][2], x[1][3]));
+    acc[2 * W] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(even, p, acc[2 * W], 0, 0, 0);
+    acc[2 * W + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(odd, p, acc[2 * W + 1], 0, 0, 0);
+  }
+};
+
+// The block at `slot` (LDS) of which the first `rows` tokens are valid (wave-uniform).
+template <bool P16, int NH, int ARR>
+__device__ __forceinline__ void process_block(HeadState (&st)[NH], const uint8_t *slot, int rows,
+                                              int col, int quad, float scale_log2) {
+  using S = Slot<NH>;
+  f32x4 s[NH][2];
+#pragma unroll
+  for (int g = 0; g < NH; ++g)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      // row token_of(col): its low two bits are col >> 2, its high two col & 3
+      const uint8_t *kp =
+          ARR == kPair ? slot + (16 * h + token_of(col)) * 128 +
+                             (((4 * g + quad) ^ pair_swizzle(token_of(col))) << 4)
+                       : slot + g * kHeadBytes + h * kHalfBytes + token_of(col) * 64 +
+                             ((quad ^ (col & 3)) << 4);
+      const u32x4 k = *reinterpret_cast<const u32x4 *>(kp);
+      const uint32_t ks = mx_scale(*reinterpret_cast<const uint32_t *>(
+                                       slot + S::ks + S::template scales<P16>(g, h) + col * 4),
+                                   quad);
+      s[g][h] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        s[g][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(mx4x8_to_bf16x8(k[c], ks)),
+                                                          as_bf16x8(st[g].q[c]), s[g][h], 0, 0, 0);
+    }
+  // s[g][h][i] = S[token 16 h + 4 i + quad][column col]
+  if (rows < kBlock) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (16 * h + 4 * i + quad >= rows) {
+#pragma unroll
+          for (int g = 0; g < NH; ++g) s[g][h][i] = -INFINITY;
+        }
+  }
+  // (a NaN score makes the maximum NaN, and with it the whole column)
+  float mx[NH];
+  bool passed = false;
+#pragma unroll
+  for (int g = 0; g < NH; ++g) {
+    mx[g] = fmax_nan(fmax_nan(fmax_nan(s[g][0][0], s[g][0][1]), fmax_nan(s[g][0][2], s[g][0][3])),
+                     fmax_nan(fmax_nan(s[g][1][0], s[g][1][1]), fmax_nan(s[g][1][2], s[g][1][3]))) *
+            scale_log2;
+    passed |= mx[g] > st[g].m_run;
+  }
+  if (__builtin_amdgcn_ballot_w64(passed)) {
+#pragma unroll
+    for (int g = 0; g < NH; ++g) {
+      const float top = quad_max_nan(mx[g]);
+      const float m_new = top > st[g].m_run ? top + kLazy : top == top ? st[g].m_run : top;
+      const float al = fast_exp2(st[g].m_run - m_new);
+      st[g].m_run = m_new;
+      st[g].l_run *= al;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) st[g].acc[e] *= al;
+    }
+  }
+#pragma unroll
+  for (int g = 0; g < NH; ++g) {
+    // P^T as the B fragment (k = 8 quad + i: token 4 i + quad of half 0, then of half
+    // 1): columns 0-7 the high halves of the weights, 8-15 what those leave of them.
+    const uint32_t taken = col < 8 ? 0u : 0xffff0000u;
+    uint32_t pw[4];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < 4; i += 2) {
+        const float p0 = fast_exp2(fmaf(s[g][h][i], scale_log2, -st[g].m_run));
+        const float p1 = fast_exp2(fmaf(s[g][h][i + 1], scale_log2, -st[g].m_run));
+        st[g].l_run += p0 + p1;
+        pw[2 * h + i / 2] = pack_hi16(
+            __float_as_uint(p0 - __uint_as_float(__float_as_uint(p0) & taken)),
+            __float_as_uint(p1 - __uint_as_float(__float_as_uint(p1) & taken)));
+      }
+    const bf16x8 p = as_bf16x8(pw[0], pw[1], pw[2], pw[3]);
+    // V codes of rows 4 j + quad.  Rows past the valid ones are zeros and weigh nothing.
+    uint32_t v[2][4];
+    float vs[2][4];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const u32x4 w = *reinterpret_cast<const u32x4 *>(
+          slot + S::vs + S::template scales<P16>(g, h) + quad * 16);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        vs[h][j] = __uint_as_float(mx_scale(w[j], col >> 2));
+        const uint8_t *vp =
+            ARR == kPair ? slot + S::v + (16 * h + 4 * j + quad) * 128 +
+                               (((4 * g + (col >> 2)) ^ pair_swizzle(4 * j + quad)) << 4)
+                         : slot + S::v + g * kHeadBytes + h * kHalfBytes + (4 * j + quad) * 64 +
+                               (((col >> 2) ^ j) << 4);
+        v[h][j] = *reinterpret_cast<const uint32_t *>(vp + (col & 3) * 4);
+      }
+    }
+    st[g].template add_pv<0>(v, vs, p);
+    st[g].template add_pv<1>(v, vs, p);
+    st[g].template add_pv<2>(v, vs, p);
+    st[g].template add_pv<3>(v, vs, p);
+  }
+}
+
+// ---- balanced ---------------------------------------------------------------------
+template <int NH>
+struct BalancedSmem {
+  uint8_t slots[kWaves][kDepth][Slot<NH>::bytes];
+  int64_t prefix[kPrefix];  // blocks before request i * stride
+  int32_t st[kPrefix];      // with stride 1: indptr[i], and the tokens of its last block
+  uint8_t tail[kPrefix];
+  int64_t wave_tot[kWaves];
+};
+
+// Blocks [v0, v0 + 64) of the virtual list, one per lane.
+struct Blocks {
+  int p0, p1;
+  int meta;  // valid rows | first block of its request << 8 | last << 9 | row in page << 16
+  int req;
+};
+
+template <bool P16, class Smem>
+__device__ __forceinline__ Blocks find_blocks(const Mx4DecodeArgs &a, const Smem &sm, int entries, int stride,
+                                              int32_t ipB, int64_t total, int64_t v0, int64_t v_end,
+                                              int lane) {
+  Blocks d = {0, 0, 0, -1};
+  const int64_t v = v0 + lane;
+  if (v >= v_end) return d;
+  int lo = 0, n = entries;  // the last entry with prefix <= v
+  while (n > 1) {
+    const int half = n >> 1;
+    if (sm.prefix[lo + half] <= v) {
+      lo += half;
+      n -= half;
+    } else {
+      n = half;
+    }
+  }
+  int r = lo;
+  int64_t pre = sm.prefix[lo], cnt;
+  int32_t st, tail;
+  if (stride == 1) {
+    cnt = (lo + 1 < entries ? sm.prefix[lo + 1] : total) - pre;
+    st = sm.st[lo];
+    tail = sm.tail[lo];
+  } else {
+    r = lo * stride;
+    while (true) {
+      st = a.indptr[r];
+      const int64_t t = request_tokens(a, st, a.indptr[r + 1], a.last[r], ipB);
+      cnt = (t + kBlock - 1) / kBlock;
+      tail = (int)(t - (cnt - 1) * kBlock);
+      if (v < pre + cnt || r + 1 >= a.batch) break;
+      pre += cnt;
+      ++r;
+    }
+  }
+  const int64_t b = v - pre;
+  const bool last = b == cnt - 1;
+  int rows = last ? tail : kBlock;
+  // token 32 b lies in the request's page 32 b / P, row 32 b % P
+  const int64_t pos = st + (P16 ? 2 * b : a.page_rows == 64 ? b >> 1 : b);
+  const int row = !P16 && a.page_rows == 64 ? (int)(b & 1) * kBlock : 0;
+  d.p0 = a.indices[pos];
+  d.p1 = P16 && rows > 16 ? a.indices[pos + 1] : d.p0;
+  if (d.p0 < 0 || (int64_t)d.p0 >= a.pool || d.p1 < 0 || (int64_t)d.p1 >= a.pool) rows = 0;
+  d.meta = rows | (b == 0 ? 256 : 0) | (last ? 512 : 0) | row << 16;
+  d.req = r;
+  return d;
+}
+
+// NH: kv-heads per wave; they divide Hkv.
+template <bool P16, int NH, int ARR>
+__global__ __launch_bounds__(kThreads, LOOM_MX4_WAVES_PER_EU) void mx4_decode_split_kernel(
+    Mx4DecodeArgs a) {
+  __shared__ BalancedSmem<NH> sm;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = uni(tid >> 6);
+  const int32_t ip0 = a.indptr[0], ipB = a.indptr[a.batch];
+  // ---- the virtual list: prefix of the valid requests' blocks ----------------------
+  int stride = 1;
+  while (a.batch > kPrefix * stride) stride <<= 1;
+  const int entries = (a.batch + stride - 1) / stride;
+  int64_t carry = 0;
+  for (int base = 0; base < a.batch; base += kThreads) {
+    const int r = base + tid;
+    int64_t cnt = 0;
+    int32_t st = 0;
+    int tail = 0;
+    if (r < a.batch) {
+      st = a.indptr[r];
+      const int64_t t = request_tokens(a, st, a.indptr[r + 1], a.last[r], ipB);
+      cnt = (t + kBlock - 1) / kBlock;
+      tail = (int)(t - (cnt - 1) * kBlock);
+    }
+    const int64_t x = wave_incl_scan64(cnt, lane);
+    if (lane == 63) sm.wave_tot[wave] = x;
+    __syncthreads();
+    int64_t before = carry, tot = 0;
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) {
+      const int64_t t = sm.wave_tot[i];
+      before += i < wave ? t : 0;
+      tot += t;
+    }
+    if (r < a.batch) {
+      const int64_t pre = before + x - cnt;
+      if (r % stride == 0) sm.prefix[r / stride] = pre;
+      if (stride == 1) {
+        sm.st[r] = st;
+        sm.tail[r] = (uint8_t)tail;
+      }
+      if (blockIdx.x == 0) a.header[1 + r] = pre;
+    }
+    carry += tot;
+    __syncthreads();
+  }
+  const int64_t total = uni64(carry);
+  const bool ok = batch_ok(a, ip0, ipB);
+  if (blockIdx.x == 0 && tid == 0) {
+    a.header[0] = ok ? total : -1;
+    a.header[1 + a.batch] = total;
+  }
+  if (!ok) return;
+
+  // ---- this wave's team and member --------------------------------------------------
+  // Workgroup b runs on XCD b % 8; a team's members are consecutive waves of one XCD
+  // (one L2, the same blocks at the same time), team t on XCD t % 8.
+  const int members = a.hkv / NH * a.tiles;
+  const int xcd_wave = (int)(blockIdx.x >> 3) * kWaves + wave;
+  const int teams = active_teams(total, a.teams);
+  const int team = (xcd_wave / members) * 8 + (int)(blockIdx.x & 7);
+  const int member = xcd_wave % members;
+  if (team >= teams) return;  // no workgroup barrier follows
+  const int kvh = member % (a.hkv / NH) * NH;
+  const int g0 = member / (a.hkv / NH) * a.tile;
+  const int heads = min(a.tile, a.group - g0);
+  const int64_t v_begin = uni64(team_start(total, team, teams));
+  const int64_t v_end = uni64(team_start(total, team + 1, teams));
+  if (v_begin >= v_end) return;
+  const int n = (int)(v_end - v_begin);
+
+  HeadState w[NH];
+  const int col = lane & 15, quad = lane >> 4;
+  const bool mine = col < heads, loads_q = (col & 7) < heads;
+  const int qh = kvh * a.group + g0 + (col & 7);  // of the first kv-head
+
+  // ---- one continuous stream of blocks ----------------------------------------------
+  // Block i + kDepth - 1 is issued before block i is consumed, across request
+  // boundaries.  Blocks are located 64 at a time, one per lane.
+  Blocks cur = {0, 0, 0, -1}, next = cur;
+  const uint32_t slots = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void *)sm.slots[wave];
+  // Block i into slot i % kDepth; its Blocks::meta and ::req.
+  auto issue = [&](int i, int slot, int &meta, int &req) {
+    const int j = i & 63;
+    if (j == 0) {
+      cur = next;  // located 64 blocks ago
+      if (i + 64 < n)
+        next = find_blocks<P16>(a, sm, entries, stride, ipB, total, v_begin + i + 64, v_end, lane);
+    }
+    meta = i < n ? __builtin_amdgcn_readlane(cur.meta, j) : 0;  // past the range: no rows
+    req = __builtin_amdgcn_readlane(cur.req, j);
+    Place p;
+    p.rows = meta & 255;
+    p.row = meta >> 16;
+    p.p0 = p.rows ? __builtin_amdgcn_readlane(cur.p0, j) : 0;
+    p.p1 = P16 && p.rows ? __builtin_amdgcn_readlane(cur.p1, j) : 0;
+    load_block<P16, NH, ARR, true>(a, p, slots + slot * Slot<NH>::bytes, lane, kvh);
+  };
+
+  int r = -1;
+  bool first = false, last = false, bad = false;
+  auto finish = [&]() {
+#pragma unroll
+    for (int g = 0; g < NH; ++g) {
+      const float l = w[g].normalizer();
+      w[g].join_columns();
+      if (!mine) continue;
+      const int64_t head = qh + g * a.group;
+      if (first && last) {  // the whole request; an invalid page index keeps its sentinels
+        const int64_t row = (int64_t)r * a.hq + head;
+        if (!bad) w[g].store(a.out + row * 128, a.lse + row, l, quad);
+        continue;
+      }
+      // One state per (team, request): slot team + r (along the virtual list the team
+      // or the request advances at every piece).
+      float *st = a.states + ((int64_t)(team + r) * a.hq + head) * kMx4StateStride;
+      if (!bad) w[g].stash(st + 4, quad);
+      if (quad == 0) {
+        st[0] = bad ? 0.0f : w[g].m_run;
+        st[1] = bad ? kPoisonNormalizer : l;
+      }
+    }
+  };
+
+  int meta[kDepth], req[kDepth];  // of blocks i, i + 1, ..., the last being issued
+  next = find_blocks<P16>(a, sm, entries, stride, ipB, total, v_begin, v_end, lane);
+#pragma unroll
+  for (int j = 0; j < kDepth - 1; ++j) issue(j, j, meta[j], req[j]);
+  int slot = 0;
+  for (int i = 0; i < n; ++i) {
+    const int ahead = slot == 0 ? kDepth - 1 : slot - 1;  // (slot + kDepth - 1) % kDepth
+    wait_reads();
+    issue(i + kDepth - 1, ahead, meta[kDepth - 1], req[kDepth - 1]);
+    if (req[0] != r) {
+      if (r >= 0) finish();
+      r = req[0];
+#pragma unroll
+      for (int g = 0; g < NH; ++g)
+        w[g].load_q(a.q + ((int64_t)r * a.hq + qh + g * a.group) * 128, loads_q, quad);
+#pragma unroll
+      for (int g = 0; g < NH; ++g) {
+        w[g].reset();
+        w[g].settle_q();
+      }
+      first = (meta[0] & 256) != 0;
+      bad = false;
+    }
+    last = (meta[0] & 512) != 0;
+    const int rows = meta[0] & 255;
+    bad |= rows == 0;
+    // Block i has arrived once at most the loads issued after it are outstanding
+    // (others in between only make the wait longer).
+    wait_loads<(kDepth - 1) * kBlockLoads<P16, NH>>();
+    process_block<P16, NH, ARR>(w, sm.slots[wave][slot], rows, col, quad, a.scale_log2);
+#pragma unroll
+    for (int j = 0; j + 1 < kDepth; ++j) {
+      meta[j] = meta[j + 1];
+      req[j] = req[j + 1];
+    }
+    if (++slot == kDepth) slot = 0;
+  }
+  finish();
+  // loads past the range still write this wave's slots
+  wait_loads<0>();
+}
+
+// ---- merge ---------------------------------------------------------------------------
+// O and LSE of one (request, query head) from `count` states of consecutive slots, by one
+// workgroup: wave w takes states w, w + 4, ..., a lane two of the 128 dims, eight states
+// in flight; the waves' sums are combined in LDS in wave order.  A poisoned state leaves
+// the request's sentinels.
+constexpr int kMergeBatch = 8;
+__device__ __forceinline__ void merge_states(const Mx4DecodeArgs &a, int r, int qh, int64_t slot0,
+                                             int count) {
+  __shared__ float s_m[kWaves], s_l[kWaves];
+  __shared__ f32x2 s_o[kWaves][64];
+  const int tid = threadIdx.x, lane = tid & 63, wave = uni(tid >> 6);
+  float M = -FLT_MAX, l = 0.f;
+  f32x2 o = {0.f, 0.f};
+  bool poisoned = false;
+  const int64_t step = (int64_t)a.hq * kMx4StateStride;
+  const float *base = a.states + slot0 * step + (int64_t)qh * kMx4StateStride;
+  for (int t = wave; t < count; t += kWaves * kMergeBatch) {
+    float ms[kMergeBatch], ls[kMergeBatch];
+    f32x2 xs[kMergeBatch];
+#pragma unroll
+    for (int u = 0; u < kMergeBatch; ++u) {
+      // past the last state: its values again, with no weight
+      const float *ss = base + min(t + u * kWaves, count - 1) * step;
+      ms[u] = ss[0];
+      ls[u] = ss[1];
+      xs[u] = *reinterpret_cast<const f32x2 *>(ss + 4 + 2 * lane);
+    }
+    float mb = M;
+#pragma unroll
+    for (int u = 0; u < kMergeBatch; ++u) {
+      mb = fmaxf(mb, ms[u]);
+      poisoned |= ls[u] < 0.0f;
+    }
+    const float sc = fast_exp2(M - mb);
+    l *= sc;
+    o *= sc;
+#pragma unroll
+    for (int u = 0; u < kMergeBatch; ++u) {
+      const float f = t + u * kWaves < count ? fast_exp2(ms[u] - mb) : 0.f;
+      l = fmaf(ls[u], f, l);
+      o[0] = fmaf(xs[u][0], f, o[0]);
+      o[1] = fmaf(xs[u][1], f, o[1]);
+    }
+    M = mb;
+  }
+  s_o[wave][lane] = o;
+  if (lane == 0) {
+    s_m[wave] = M;
+    s_l[wave] = poisoned ? kPoisonNormalizer : l;
+  }
+  __syncthreads();
+  if (wave != 0) return;
+  M = s_m[0];
+  poisoned = s_l[0] < 0.0f;
+#pragma unroll
+  for (int i = 1; i < kWaves; ++i) {
+    M = fmaxf(M, s_m[i]);
+    poisoned |= s_l[i] < 0.0f;
+  }
+  if (poisoned) return;
+  l = 0.f;
+  o = f32x2{0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i) {
+    const float f = fast_exp2(s_m[i] - M);
+    l = fmaf(s_l[i], f, l);
+    o[0] = fmaf(s_o[i][lane][0], f, o[0]);
+    o[1] = fmaf(s_o[i][lane][1], f, o[1]);
+  }
+  const int64_t row = (int64_t)r * a.hq + qh;
+  *reinterpret_cast<uint32_t *>(a.out + row * 128 + 2 * lane) = bf16x2_pack(o[0] / l, o[1] / l);
+  if (lane == 0) a.lse[row] = M + __log2f(l);
+}
+
+// The requests that span several teams.  (With fewer blocks than teams no team is
+// empty: active_teams leaves each at least one.)
+__global__ __launch_bounds__(kThreads) void mx4_decode_merge_kernel(Mx4DecodeArgs a) {
+  const int r = (int)(blockIdx.x / a.hq), qh = (int)(blockIdx.x % a.hq);
+  const int64_t total = a.header[0], pre = a.header[1 + r], end = a.header[2 + r];
+  if (total <= 0 || end <= pre) return;
+  const int teams = active_teams(total, a.teams);
+  const int64_t t0 = team_of(total, pre, teams), t1 = team_of(total, end - 1, teams);
+  if (t0 == t1) return;
+  merge_states(a, r, qh, t0 + r, (int)(t1 - t0) + 1);
+}
+
+__global__ __launch_bounds__(kThreads) void mx4_decode_direct_merge_kernel(Mx4DecodeArgs a) {
+  const int r = (int)(blockIdx.x / a.hq), qh = (int)(blockIdx.x % a.hq);
+  merge_states(a, r, qh, (int64_t)r * a.splits, a.splits);
+}
+
+// ---- direct --------------------------------------------------------------------------
+// Wave w of the workgroup takes blocks w, w + W, ... of its split's share of the request,
+// two in flight; the wave states merge in LDS (dynamic: [W][tile] columns of 128 + 2
+// floats).
+#ifndef LOOM_MX4_DIRECT_WAVES
+#define LOOM_MX4_DIRECT_WAVES 16
+#endif
+constexpr int kDirectWaves = LOOM_MX4_DIRECT_WAVES;
+
+template <bool P16>
+__global__ __launch_bounds__(kDirectWaves * 64) void mx4_decode_direct_kernel(Mx4DecodeArgs a) {
+  // Two slots per wave; after the walk the wave states' O, [wave][column][128] floats.
+  extern __shared__ __align__(16) uint8_t s_dyn[];
+  float *const s_acc = reinterpret_cast<float *>(s_dyn);
+  __shared__ float s_m[kDirectWaves][kMaxTile], s_l[kDirectWaves][kMaxTile];
+  __shared__ uint32_t s_bad[kDirectWaves];
+  constexpr int W = kDirectWaves;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = uni(tid >> 6);
+  const int split = (int)(blockIdx.x % a.splits);
+  const int head = (int)(blockIdx.x / a.splits);
+  const int kvh = head % a.hkv;
+  const int rest = head / a.hkv;
+  const int g0 = (rest % a.tiles) * a.tile;
+  const int r = rest / a.tiles;
+  const int heads = min(a.tile, a.group - g0);
+  HeadState st1[1];
+  HeadState &w = st1[0];
+  const int col = lane & 15, quad = lane >> 4;
+  const bool mine = col < heads;
+  const int qh0 = kvh * a.group + g0;
+  // A split always writes its state (a poisoned one where a guard fails), so the
+  // merge never reads a stale one.
+  auto state_of = [&](int g) {
+    return a.states + (((int64_t)r * a.splits + split) * a.hq + qh0 + g) * kMx4StateStride;
+  };
+  auto poison = [&]() {
+    if (a.splits > 1 && tid < heads) {
+      float *ss = state_of(tid);
+      ss[0] = 0.0f;
+      ss[1] = kPoisonNormalizer;
+    }
+  };
+  w.load_q(a.q + ((int64_t)r * a.hq + qh0 + (col & 7)) * 128, (col & 7) < heads, quad);
+  const int32_t ip0 = a.indptr[0], ipB = a.indptr[a.batch];
+  const int32_t st = uni(a.indptr[r]), en = uni(a.indptr[r + 1]), tl = uni(a.last[r]);
+  const int64_t tokens = request_tokens(a, st, en, tl, ipB);
+  if (!batch_ok(a, ip0, ipB) || tokens == 0) return poison();
+  // this split's blocks [lo, hi), this wave's lo + wave + W i
+  const int64_t cnt = (tokens + kBlock - 1) / kBlock;
+  const int64_t lo = cnt * split / a.splits, hi = cnt * (split + 1) / a.splits;
+  const int64_t n = hi - lo > wave ? (hi - lo - wave + W - 1) / W : 0;
+  bool bad = false;
+  w.reset();
+  Blocks cur = {0, 0, 0, 0};
+  auto locate = [&](int64_t i0) {  // the wave's blocks i0 + [0, 64), one per lane
+    cur = Blocks{0, 0, 0, 0};
+    if (i0 + lane >= n) return;
+    const int64_t b = lo + wave + W * (i0 + lane);
+    int rows = (int)min<int64_t>(kBlock, tokens - b * kBlock);
+    const int64_t pos = st + (P16 ? 2 * b : a.page_rows == 64 ? b >> 1 : b);
+    cur.p0 = a.indices[pos];
+    cur.p1 = P16 && rows > 16 ? a.indices[pos + 1] : cur.p0;
+    if (cur.p0 < 0 || (int64_t)cur.p0 >= a.pool || cur.p1 < 0 || (int64_t)cur.p1 >= a.pool) {
+      rows = 0;
+      bad = true;
+    }
+    cur.meta = rows | (!P16 && a.page_rows == 64 ? (int)(b & 1) * kBlock : 0) << 16;
+  };
+  for (int64_t i0 = 0; i0 < n; i0 += 64) {
+    locate(i0);
+    const int m = (int)min<int64_t>(64, n - i0);
+    int rows[2];
+    uint8_t *const slots = s_dyn + wave * 2 * Slot<1>::bytes;
+    const uint32_t slots_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void *)slots;
+    auto issue = [&](int slot, int i, int &rows_out) {
+      const int meta = i < m ? __builtin_amdgcn_readlane(cur.meta, i & 63) : 0;
+      Place p;
+      p.rows = meta & 255;
+      p.row = meta >> 16;
+      p.p0 = p.rows ? __builtin_amdgcn_readlane(cur.p0, i & 63) : 0;
+      p.p1 = P16 && p.rows ? __builtin_amdgcn_readlane(cur.p1, i & 63) : 0;
+      load_block<P16, 1, kSplit, false>(a, p, slots_at + slot * Slot<1>::bytes, lane, kvh);
+      rows_out = p.rows;
+    };
+    wait_reads();
+    issue(0, 0, rows[0]);
+    int i = 0;
+    while (true) {
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        wait_reads();
+        issue(s ^ 1, i + 1, rows[s ^ 1]);
+        if (i == 0) w.settle_q();
+        wait_loads<kBlockLoads<P16, 1>>();
+        process_block<P16, 1, kSplit>(st1, slots + s * Slot<1>::bytes, rows[s], col, quad,
+                                      a.scale_log2);
+        if (++i >= m) goto walked;
+      }
+    }
+  walked:;
+  }
+  const float l = w.normalizer();
+  w.join_columns();
+  // The slots become the states' place; loads past the last block may still write.
+  wait_loads<0>();
+  __syncthreads();
+  if (mine) {
+    w.stash(s_acc + ((int64_t)wave * a.tile + col) * 128, quad);
+    if (quad == 0) {
+      s_m[wave][col] = w.m_run;
+      s_l[wave][col] = l;
+    }
+  }
+  // An invalid page index anywhere in the request keeps its sentinels.
+  if (block_or(bad, s_bad)) return poison();
+  for (int x = tid; x < heads * 128; x += W * 64) {
+    const int g = x >> 7, d = x & 127;
+    float M = -FLT_MAX;
+#pragma unroll
+    for (int i = 0; i < W; ++i) M = fmaxf(M, s_m[i][g]);
+    float L = 0.f, O = 0.f;
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      const float f = fast_exp2(s_m[i][g] - M);
+      L = fmaf(s_l[i][g], f, L);
+      O = fmaf(s_acc[(i * a.tile + g) * 128 + d], f, O);
+    }
+    if (a.splits > 1) {
+      float *ss = state_of(g);
+      ss[4 + d] = O;
+      if (d == 0) {
+        ss[0] = M;
+        ss[1] = L;
+      }
+      continue;
+    }
+    const int64_t row = (int64_t)r * a.hq + qh0 + g;
+    a.out[row * 128 + d] = f32_to_bf16(O / L);
+    if (d == 0) a.lse[row] = M + __log2f(L);
+  }
+}
+
+// kv-heads per wave of the balanced kernel: two neighbours where Hkv is even.
+uint64_t heads_per_wave(uint64_t hkv) { return hkv % 2 == 0 ? 2 : 1; }
+
+size_t direct_lds(uint32_t tile) {
+  return (size_t)kDirectWaves * std::max<size_t>(tile * 128 * 4, 2 * Slot<1>::bytes);
+}
+
+}  // namespace
+
+namespace loom {
+
+#ifndef LOOM_MX4_DIRECT_TOKENS
+#define LOOM_MX4_DIRECT_TOKENS 16384
+#endif
+
+loom_status_t plan_mx4_decode(loom_paged_decode_plan_info_t *info, uint32_t teams_option, int cus,
+                              loom_error_t *err) {
+  const loom_paged_decode_spec_t &s = info->spec;
+  const uint64_t B = s.batch_size, hq = s.num_query_heads, hkv = s.num_kv_heads;
+  const uint64_t group = hq / hkv;
+  const uint32_t tile = (uint32_t)std::min<uint64_t>(group, kMaxTile);
+  const uint64_t tiles = (group + tile - 1) / tile;
+  const uint64_t page_rows = s.page_size ? s.page_size : kPageSize;
+  if (B > (uint64_t)kMaxBatch)
+    return fail(err, LOOM_PLAN_STATE_COUNT_OUT_OF_RANGE, "batch_size", B);
+  info->group_tile = tile;
+  info->group_tiles = (uint32_t)tiles;
+  info->device_cus = (uint32_t)cus;
+  info->header_bytes = 0;
+  const uint64_t heads = B * hkv * tiles;
+  if (teams_option == 0 && info->max_total_pages * page_rows <= LOOM_MX4_DIRECT_TOKENS) {
+    const uint64_t splits = 1;
+    const uint64_t grid = heads * splits;
+    if (grid > (uint64_t)INT32_MAX || B * hq > (uint64_t)INT32_MAX)
+      return fail(err, LOOM_PLAN_STATE_COUNT_OUT_OF_RANGE, "paged batch-decode", grid);
+    info->algorithm = LOOM_PAGED_DECODE_DIRECT;
+    info->teams = (uint32_t)(splits > 1 ? splits : 0);
+    info->state_slots = splits > 1 ? splits * B : 0;
+    info->workspace_bytes = splits > 1 ? splits * B * hq * kMx4StateStride * 4 : 256;
+    info->block_threads = kDirectWaves * 64;
+    info->grid_blocks = (uint32_t)grid;
+    return LOOM_OK;
+  }
+  const uint64_t members = hkv / heads_per_wave(hkv) * tiles;
+  const uint64_t slots = (uint64_t)cus * LOOM_MX4_WAVES_PER_4CU / 4;
+  const uint64_t teams = teams_option ? teams_option : std::max<uint64_t>(1, slots / members);
+  // Each XCD (every 8th workgroup) holds ceil(teams / 8) whole teams.
+  const uint64_t xcd_waves = (teams + 7) / 8 * members;
+  const uint64_t grid = (xcd_waves + kWaves - 1) / kWaves * 8;
+  if (grid > (uint64_t)INT32_MAX || teams > (uint64_t)INT32_MAX || B * hq > (uint64_t)INT32_MAX)
+    return fail(err, LOOM_PLAN_STATE_COUNT_OUT_OF_RANGE, "paged batch-decode", grid);
+  info->algorithm = LOOM_PAGED_DECODE_BALANCED_SPLIT_KV;
+  info->teams = (uint32_t)teams;
+  info->header_bytes = ((B + 2) * 8 + 255) / 256 * 256;
+  info->state_slots = teams + B;
+  info->workspace_bytes = info->header_bytes + info->state_slots * hq * kMx4StateStride * 4;
+  info->block_threads = kThreads;
+  info->grid_blocks = (uint32_t)grid;
+  return LOOM_OK;
+}
+
+hipError_t launch_mx4_decode(const loom_paged_decode_plan_info_t &info, const Mx4DecodeArgs &a,
+                             hipStream_t stream) {
+  const bool p16 = a.page_rows == 16;
+  const dim3 grid(info.grid_blocks), heads((unsigned)((int64_t)a.batch * a.hq));
+  if (info.algorithm == LOOM_PAGED_DECODE_DIRECT) {
+    hipLaunchKernelGGL(p16 ? mx4_decode_direct_kernel<true> : mx4_decode_direct_kernel<false>, grid,
+                       dim3(kDirectWaves * 64), direct_lds(info.group_tile), stream, a);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess || a.splits == 1) return e;
+    hipLaunchKernelGGL(mx4_decode_direct_merge_kernel, heads, dim3(kThreads), 0, stream, a);
+    return hipGetLastError();
+  }
+  const bool nhd = a.row_bytes != 64;  // (with one kv-head the layouts are the same)
+  auto kernel = heads_per_wave(a.hkv) == 1
+                    ? (p16 ? mx4_decode_split_kernel<true, 1, kSplit>
+                           : mx4_decode_split_kernel<false, 1, kSplit>)
+                : nhd ? (p16 ? mx4_decode_split_kernel<true, 2, kPair>
+                             : mx4_decode_split_kernel<false, 2, kPair>)
+                      : (p16 ? mx4_decode_split_kernel<true, 2, kSplit>
+                             : mx4_decode_split_kernel<false, 2, kSplit>);
+  hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, stream, a);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL(mx4_decode_merge_kernel, heads, dim3(kThreads), 0, stream, a);
+  return hipGetLastError();
+}
+
+}  // namespace loom
