@@ -68,8 +68,9 @@ constexpr float kPoisonNormalizer = -1.0f;
 #define LOOM_MX4_WAVES_PER_4CU 16
 #endif
 #ifndef LOOM_MX4_MIN_TEAM_BLOCKS
-#define LOOM_MX4_MIN_TEAM_BLOCKS 4
+#define LOOM_MX4_MIN_TEAM_BLOCKS 2
 #endif
+constexpr int kMinTeamBlocks = LOOM_MX4_MIN_TEAM_BLOCKS;
 constexpr int kDepth = LOOM_MX4_DEPTH;  // blocks in flight per wave
 
 // decode.rs:233-246: indptr[B] is the page_indices length (at most that length for
@@ -92,17 +93,26 @@ __device__ __forceinline__ int64_t floor_div(int64_t n, int64_t d) {
   while ((q + 1) * d <= n) ++q;
   return q;
 }
-// Team t owns virtual blocks [team_start(t), team_start(t + 1)).
-__device__ __forceinline__ int64_t team_start(int64_t total, int64_t t, int teams) {
-  return floor_div(total * t, teams);
-}
-__device__ __forceinline__ int64_t team_of(int64_t total, int64_t v, int teams) {
-  return floor_div((v + 1) * teams + total - 1, total) - 1;
-}
-// Teams in use: at most the planned count, at least LOOM_MX4_MIN_TEAM_BLOCKS each.
-__device__ __forceinline__ int active_teams(int64_t total, int teams) {
-  return (int)max<int64_t>(1, min<int64_t>(teams, total / LOOM_MX4_MIN_TEAM_BLOCKS));
-}
+// The virtual list of `total` blocks in equal ranges: each team in use has `each`
+// blocks, the first `more` of them one more.  At most the planned teams are in use, and
+// (unless that leaves one) each has at least kMinTeamBlocks.
+struct Ranges {
+  int64_t each, more;
+  int teams;
+  __device__ __forceinline__ Ranges(int64_t total, int planned) {
+    teams = (int)max<int64_t>(1, min<int64_t>(planned, total / kMinTeamBlocks));
+    if (total < INT32_MAX)
+      each = (uint32_t)total / (uint32_t)teams;
+    else
+      each = floor_div(total, teams);
+    more = total - each * teams;
+  }
+  __device__ __forceinline__ int64_t start(int64_t t) const { return t * each + min(t, more); }
+  __device__ __forceinline__ int64_t team_of(int64_t v) const {
+    const int64_t longer = more * (each + 1);
+    return v < longer ? floor_div(v, each + 1) : more + floor_div(v - longer, each);
+  }
+};
 
 // One 32-token block as a wave stages it in LDS: K and V codes of one or two kv-heads
 // and the rows' scale words.  Loads go straight to LDS (nothing is held in registers
@@ -239,11 +249,12 @@ struct HeadState {
   __device__ __forceinline__ float normalizer() const { return quad_sum(l_run); }
   // O of this lane's column (dims 32 quad + [0, 32)) and, by quad 0, LSE.
   __device__ __forceinline__ void store(uint16_t *o, float *lse, float l, int quad) const {
+    const float inv = 1.0f / l;  // (its rounding and the product's are 2^-23 of O)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       u32x4 w;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) w[e] = bf16x2_pack(acc[2 * e][i] / l, acc[2 * e + 1][i] / l);
+      for (int e = 0; e < 4; ++e) w[e] = bf16x2_pack(acc[2 * e][i] * inv, acc[2 * e + 1][i] * inv);
       *reinterpret_cast<u32x4 *>(o + quad * 32 + i * 8) = w;
     }
     if (quad == 0) *lse = m_run + __log2f(l);
@@ -410,43 +421,75 @@ struct Blocks {
   int req;
 };
 
+// The virtual list as a wave knows it.  Up to 64 requests: lane r holds request r's
+// inclusive prefix, first page position and tokens of its last block (`in_lanes`).  More:
+// the LDS table.
+struct List {
+  bool in_lanes;
+  uint32_t incl, cnt;  // this lane's request
+  int32_t st, tail;
+  int entries, stride;
+  int32_t ipB;
+  int64_t total;
+};
+
 template <bool P16, class Smem>
-__device__ __forceinline__ Blocks find_blocks(const Mx4DecodeArgs &a, const Smem &sm, int entries, int stride,
-                                              int32_t ipB, int64_t total, int64_t v0, int64_t v_end,
-                                              int lane) {
+__device__ __forceinline__ Blocks find_blocks(const Mx4DecodeArgs &a, const Smem &sm,
+                                              const List &list, int64_t v0, int64_t v_end, int lane) {
   Blocks d = {0, 0, 0, -1};
   const int64_t v = v0 + lane;
-  if (v >= v_end) return d;
-  int lo = 0, n = entries;  // the last entry with prefix <= v
-  while (n > 1) {
-    const int half = n >> 1;
-    if (sm.prefix[lo + half] <= v) {
-      lo += half;
-      n -= half;
-    } else {
-      n = half;
-    }
-  }
-  int r = lo;
-  int64_t pre = sm.prefix[lo], cnt;
-  int32_t st, tail;
-  if (stride == 1) {
-    cnt = (lo + 1 < entries ? sm.prefix[lo + 1] : total) - pre;
-    st = sm.st[lo];
-    tail = sm.tail[lo];
-  } else {
-    r = lo * stride;
+  const bool in = v < v_end;
+  int r = 0;
+  int64_t b = 0, cnt = 1;  // block of its request, and that one's blocks
+  int32_t st = 0, tail = 0;
+  if (list.in_lanes) {
+    // the request of v0, then on while later requests begin at or before v
+    const uint32_t x = (uint32_t)v, end = (uint32_t)min<int64_t>(v0 + 64, v_end);
+    int next = __builtin_ctzll(__builtin_amdgcn_ballot_w64(list.incl > (uint32_t)v0));
+    r = next;
     while (true) {
-      st = a.indptr[r];
-      const int64_t t = request_tokens(a, st, a.indptr[r + 1], a.last[r], ipB);
-      cnt = (t + kBlock - 1) / kBlock;
-      tail = (int)(t - (cnt - 1) * kBlock);
-      if (v < pre + cnt || r + 1 >= a.batch) break;
-      pre += cnt;
-      ++r;
+      const uint32_t e = (uint32_t)__builtin_amdgcn_readlane((int)list.incl, next);
+      if (e >= end) break;
+      ++next;
+      if (x >= e) r = next;
     }
+    st = __shfl(list.st, r, 64);
+    tail = __shfl(list.tail, r, 64);
+    const uint32_t c = (uint32_t)__shfl((int)list.cnt, r, 64);
+    cnt = c;
+    b = x - ((uint32_t)__shfl((int)list.incl, r, 64) - c);
+  } else if (in) {
+    int lo = 0, n = list.entries;  // the last entry with prefix <= v
+    while (n > 1) {
+      const int half = n >> 1;
+      if (sm.prefix[lo + half] <= v) {
+        lo += half;
+        n -= half;
+      } else {
+        n = half;
+      }
+    }
+    r = lo;
+    int64_t pre = sm.prefix[lo];
+    if (list.stride == 1) {
+      cnt = (lo + 1 < list.entries ? sm.prefix[lo + 1] : list.total) - pre;
+      st = sm.st[lo];
+      tail = sm.tail[lo];
+    } else {
+      r = lo * list.stride;
+      while (true) {
+        st = a.indptr[r];
+        const int64_t t = request_tokens(a, st, a.indptr[r + 1], a.last[r], list.ipB);
+        cnt = (t + kBlock - 1) / kBlock;
+        tail = (int)(t - (cnt - 1) * kBlock);
+        if (v < pre + cnt || r + 1 >= a.batch) break;
+        pre += cnt;
+        ++r;
+      }
+    }
+    b = v - pre;
   }
-  const int64_t b = v - pre;
+  if (!in) return d;
   const bool last = b == cnt - 1;
   int rows = last ? tail : kBlock;
   // token 32 b lies in the request's page 32 b / P, row 32 b % P
@@ -469,44 +512,69 @@ __global__ __launch_bounds__(kThreads, LOOM_MX4_WAVES_PER_EU) void mx4_decode_sp
   const int wave = uni(tid >> 6);
   const int32_t ip0 = a.indptr[0], ipB = a.indptr[a.batch];
   // ---- the virtual list: prefix of the valid requests' blocks ----------------------
-  int stride = 1;
-  while (a.batch > kPrefix * stride) stride <<= 1;
-  const int entries = (a.batch + stride - 1) / stride;
-  int64_t carry = 0;
-  for (int base = 0; base < a.batch; base += kThreads) {
-    const int r = base + tid;
-    int64_t cnt = 0;
-    int32_t st = 0;
-    int tail = 0;
-    if (r < a.batch) {
-      st = a.indptr[r];
-      const int64_t t = request_tokens(a, st, a.indptr[r + 1], a.last[r], ipB);
-      cnt = (t + kBlock - 1) / kBlock;
-      tail = (int)(t - (cnt - 1) * kBlock);
+  List list;
+  list.ipB = ipB;
+  list.in_lanes = false;
+  if (a.batch <= 64) {
+    // every wave on its own, in registers: no barrier, no LDS round trip
+    int64_t t = 0;
+    list.st = 0;
+    if (lane < a.batch) {
+      list.st = a.indptr[lane];
+      t = request_tokens(a, list.st, a.indptr[lane + 1], a.last[lane], ipB);
     }
-    const int64_t x = wave_incl_scan64(cnt, lane);
-    if (lane == 63) sm.wave_tot[wave] = x;
-    __syncthreads();
-    int64_t before = carry, tot = 0;
-#pragma unroll
-    for (int i = 0; i < kWaves; ++i) {
-      const int64_t t = sm.wave_tot[i];
-      before += i < wave ? t : 0;
-      tot += t;
-    }
-    if (r < a.batch) {
-      const int64_t pre = before + x - cnt;
-      if (r % stride == 0) sm.prefix[r / stride] = pre;
-      if (stride == 1) {
-        sm.st[r] = st;
-        sm.tail[r] = (uint8_t)tail;
-      }
-      if (blockIdx.x == 0) a.header[1 + r] = pre;
-    }
-    carry += tot;
-    __syncthreads();
+    const int64_t cnt = (t + kBlock - 1) / kBlock;
+    list.cnt = (uint32_t)min<int64_t>(cnt, UINT32_MAX);
+    list.tail = (int)(t - (cnt - 1) * kBlock);
+    list.incl = wave_incl_add_sat_u32(list.cnt);
+    const uint32_t total = (uint32_t)__builtin_amdgcn_readlane((int)list.incl, 63);
+    list.total = total;
+    list.in_lanes = total < (uint32_t)INT32_MAX;  // (else the 64-bit table)
+    if (list.in_lanes && blockIdx.x == 0 && wave == 0 && lane < a.batch)
+      a.header[1 + lane] = list.incl - list.cnt;
   }
-  const int64_t total = uni64(carry);
+  if (!list.in_lanes) {
+    int stride = 1;
+    while (a.batch > kPrefix * stride) stride <<= 1;
+    list.stride = stride;
+    list.entries = (a.batch + stride - 1) / stride;
+    int64_t carry = 0;
+    for (int base = 0; base < a.batch; base += kThreads) {
+      const int r = base + tid;
+      int64_t cnt = 0;
+      int32_t st = 0;
+      int tail = 0;
+      if (r < a.batch) {
+        st = a.indptr[r];
+        const int64_t t = request_tokens(a, st, a.indptr[r + 1], a.last[r], ipB);
+        cnt = (t + kBlock - 1) / kBlock;
+        tail = (int)(t - (cnt - 1) * kBlock);
+      }
+      const int64_t x = wave_incl_scan64(cnt, lane);
+      if (lane == 63) sm.wave_tot[wave] = x;
+      __syncthreads();
+      int64_t before = carry, tot = 0;
+#pragma unroll
+      for (int i = 0; i < kWaves; ++i) {
+        const int64_t t = sm.wave_tot[i];
+        before += i < wave ? t : 0;
+        tot += t;
+      }
+      if (r < a.batch) {
+        const int64_t pre = before + x - cnt;
+        if (r % stride == 0) sm.prefix[r / stride] = pre;
+        if (stride == 1) {
+          sm.st[r] = st;
+          sm.tail[r] = (uint8_t)tail;
+        }
+        if (blockIdx.x == 0) a.header[1 + r] = pre;
+      }
+      carry += tot;
+      __syncthreads();
+    }
+    list.total = uni64(carry);
+  }
+  const int64_t total = list.total;
   const bool ok = batch_ok(a, ip0, ipB);
   if (blockIdx.x == 0 && tid == 0) {
     a.header[0] = ok ? total : -1;
@@ -519,17 +587,16 @@ __global__ __launch_bounds__(kThreads, LOOM_MX4_WAVES_PER_EU) void mx4_decode_sp
   // (one L2, the same blocks at the same time), team t on XCD t % 8.
   const int members = a.hkv / NH * a.tiles;
   const int xcd_wave = (int)(blockIdx.x >> 3) * kWaves + wave;
-  const int teams = active_teams(total, a.teams);
+  const Ranges ranges(total, a.teams);
   const int team = (xcd_wave / members) * 8 + (int)(blockIdx.x & 7);
   const int member = xcd_wave % members;
-  if (team >= teams) return;  // no workgroup barrier follows
+  if (team >= ranges.teams) return;  // no workgroup barrier follows
   const int kvh = member % (a.hkv / NH) * NH;
   const int g0 = member / (a.hkv / NH) * a.tile;
   const int heads = min(a.tile, a.group - g0);
-  const int64_t v_begin = uni64(team_start(total, team, teams));
-  const int64_t v_end = uni64(team_start(total, team + 1, teams));
-  if (v_begin >= v_end) return;
-  const int n = (int)(v_end - v_begin);
+  const int64_t v_begin = ranges.start(team), v_end = ranges.start(team + 1);
+  const int n = (int)min<int64_t>(v_end - v_begin, INT32_MAX - 64);
+  if (n <= 0) return;
 
   HeadState w[NH];
   const int col = lane & 15, quad = lane >> 4;
@@ -547,7 +614,7 @@ __global__ __launch_bounds__(kThreads, LOOM_MX4_WAVES_PER_EU) void mx4_decode_sp
     if (j == 0) {
       cur = next;  // located 64 blocks ago
       if (i + 64 < n)
-        next = find_blocks<P16>(a, sm, entries, stride, ipB, total, v_begin + i + 64, v_end, lane);
+        next = find_blocks<P16>(a, sm, list, v_begin + i + 64, v_end, lane);
     }
     meta = i < n ? __builtin_amdgcn_readlane(cur.meta, j) : 0;  // past the range: no rows
     req = __builtin_amdgcn_readlane(cur.req, j);
@@ -585,7 +652,7 @@ __global__ __launch_bounds__(kThreads, LOOM_MX4_WAVES_PER_EU) void mx4_decode_sp
   };
 
   int meta[kDepth], req[kDepth];  // of blocks i, i + 1, ..., the last being issued
-  next = find_blocks<P16>(a, sm, entries, stride, ipB, total, v_begin, v_end, lane);
+  next = find_blocks<P16>(a, sm, list, v_begin, v_end, lane);
 #pragma unroll
   for (int j = 0; j < kDepth - 1; ++j) issue(j, j, meta[j], req[j]);
   int slot = 0;
@@ -700,14 +767,13 @@ __device__ __forceinline__ void merge_states(const Mx4DecodeArgs &a, int r, int 
   if (lane == 0) a.lse[row] = M + __log2f(l);
 }
 
-// The requests that span several teams.  (With fewer blocks than teams no team is
-// empty: active_teams leaves each at least one.)
+// The requests that span several teams.
 __global__ __launch_bounds__(kThreads) void mx4_decode_merge_kernel(Mx4DecodeArgs a) {
   const int r = (int)(blockIdx.x / a.hq), qh = (int)(blockIdx.x % a.hq);
   const int64_t total = a.header[0], pre = a.header[1 + r], end = a.header[2 + r];
   if (total <= 0 || end <= pre) return;
-  const int teams = active_teams(total, a.teams);
-  const int64_t t0 = team_of(total, pre, teams), t1 = team_of(total, end - 1, teams);
+  const Ranges ranges(total, a.teams);
+  const int64_t t0 = ranges.team_of(pre), t1 = ranges.team_of(end - 1);
   if (t0 == t1) return;
   merge_states(a, r, qh, t0 + r, (int)(t1 - t0) + 1);
 }
@@ -719,161 +785,205 @@ __global__ __launch_bounds__(kThreads) void mx4_decode_direct_merge_kernel(Mx4De
 
 // ---- direct --------------------------------------------------------------------------
 // Wave w of the workgroup takes blocks w, w + W, ... of its split's share of the request,
-// two in flight; the wave states merge in LDS (dynamic: [W][tile] columns of 128 + 2
-// floats).
-#ifndef LOOM_MX4_DIRECT_WAVES
-#define LOOM_MX4_DIRECT_WAVES 16
-#endif
-constexpr int kDirectWaves = LOOM_MX4_DIRECT_WAVES;
+// two in flight; the wave states merge in LDS.
+constexpr int kDirectWaves = 8;
+constexpr int kStash = 132;  // floats between two columns' O in LDS
 
-template <bool P16>
+template <bool P16, int NH, int ARR>
 __global__ __launch_bounds__(kDirectWaves * 64) void mx4_decode_direct_kernel(Mx4DecodeArgs a) {
-  // Two slots per wave; after the walk the wave states' O, [wave][column][128] floats.
-  extern __shared__ __align__(16) uint8_t s_dyn[];
-  float *const s_acc = reinterpret_cast<float *>(s_dyn);
-  __shared__ float s_m[kDirectWaves][kMaxTile], s_l[kDirectWaves][kMaxTile];
-  __shared__ uint32_t s_bad[kDirectWaves];
   constexpr int W = kDirectWaves;
+  constexpr int kCols = NH * kMaxTile;
+  // Each wave's two slots; after its walk its columns' O, kStash floats apart.
+  constexpr int kWaveBytes = 2 * Slot<NH>::bytes;
+  static_assert(kCols * kStash * 4 <= kWaveBytes, "a wave's columns in its slots");
+  __shared__ __align__(16) uint8_t s_wave[W][kWaveBytes];
+  __shared__ float s_m[W][kCols], s_l[W][kCols];
+  __shared__ uint32_t s_bad[W];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = uni(tid >> 6);
-  const int split = (int)(blockIdx.x % a.splits);
-  const int head = (int)(blockIdx.x / a.splits);
-  const int kvh = head % a.hkv;
-  const int rest = head / a.hkv;
-  const int g0 = (rest % a.tiles) * a.tile;
-  const int r = rest / a.tiles;
+  const uint32_t head = blockIdx.x / (uint32_t)a.splits;
+  const int split = (int)(blockIdx.x % (uint32_t)a.splits);
+  const int kvh = (int)(head % (uint32_t)(a.hkv / NH)) * NH;
+  const uint32_t rest = head / (uint32_t)(a.hkv / NH);
+  const int g0 = (int)(rest % (uint32_t)a.tiles) * a.tile;
+  const int r = (int)(rest / (uint32_t)a.tiles);
   const int heads = min(a.tile, a.group - g0);
-  HeadState st1[1];
-  HeadState &w = st1[0];
+  HeadState w[NH];
   const int col = lane & 15, quad = lane >> 4;
-  const bool mine = col < heads;
-  const int qh0 = kvh * a.group + g0;
+  // query head of column c of the workgroup's NH * heads
+  auto query_head = [&](int c) {
+    const int g = NH == 2 && c >= heads ? 1 : 0;
+    return (kvh + g) * a.group + g0 + c - g * heads;
+  };
   // A split always writes its state (a poisoned one where a guard fails), so the
   // merge never reads a stale one.
-  auto state_of = [&](int g) {
-    return a.states + (((int64_t)r * a.splits + split) * a.hq + qh0 + g) * kMx4StateStride;
+  auto state_of = [&](int c) {
+    return a.states + (((int64_t)r * a.splits + split) * a.hq + query_head(c)) * kMx4StateStride;
   };
   auto poison = [&]() {
-    if (a.splits > 1 && tid < heads) {
+    if (a.splits > 1 && tid < NH * heads) {
       float *ss = state_of(tid);
       ss[0] = 0.0f;
       ss[1] = kPoisonNormalizer;
     }
   };
-  w.load_q(a.q + ((int64_t)r * a.hq + qh0 + (col & 7)) * 128, (col & 7) < heads, quad);
+  // One round trip for the guard words, the queries and, when the page-index array is
+  // short, all of it.
+#pragma unroll
+  for (int g = 0; g < NH; ++g)
+    w[g].load_q(a.q + ((int64_t)r * a.hq + (kvh + g) * a.group + g0 + (col & 7)) * 128,
+                (col & 7) < heads, quad);
+  const bool whole_table = a.n_indices <= 128;
+  int tbl0 = 0, tbl1 = 0;
+  if (whole_table) {
+    if (lane < a.n_indices) tbl0 = a.indices[lane];
+    if (lane + 64 < a.n_indices) tbl1 = a.indices[lane + 64];
+  }
   const int32_t ip0 = a.indptr[0], ipB = a.indptr[a.batch];
   const int32_t st = uni(a.indptr[r]), en = uni(a.indptr[r + 1]), tl = uni(a.last[r]);
   const int64_t tokens = request_tokens(a, st, en, tl, ipB);
   if (!batch_ok(a, ip0, ipB) || tokens == 0) return poison();
   // this split's blocks [lo, hi), this wave's lo + wave + W i
   const int64_t cnt = (tokens + kBlock - 1) / kBlock;
-  const int64_t lo = cnt * split / a.splits, hi = cnt * (split + 1) / a.splits;
+  int64_t lo = 0, hi = cnt;
+  if (a.splits > 1) {
+    lo = floor_div(cnt * split, a.splits);
+    hi = floor_div(cnt * (split + 1), a.splits);
+  }
   const int64_t n = hi - lo > wave ? (hi - lo - wave + W - 1) / W : 0;
   bool bad = false;
-  w.reset();
-  Blocks cur = {0, 0, 0, 0};
+#pragma unroll
+  for (int g = 0; g < NH; ++g) w[g].reset();
+  Blocks cur;
   auto locate = [&](int64_t i0) {  // the wave's blocks i0 + [0, 64), one per lane
-    cur = Blocks{0, 0, 0, 0};
-    if (i0 + lane >= n) return;
+    const bool in = i0 + lane < n;
     const int64_t b = lo + wave + W * (i0 + lane);
-    int rows = (int)min<int64_t>(kBlock, tokens - b * kBlock);
+    int rows = in ? (int)min<int64_t>(kBlock, tokens - b * kBlock) : 0;
     const int64_t pos = st + (P16 ? 2 * b : a.page_rows == 64 ? b >> 1 : b);
-    cur.p0 = a.indices[pos];
-    cur.p1 = P16 && rows > 16 ? a.indices[pos + 1] : cur.p0;
-    if (cur.p0 < 0 || (int64_t)cur.p0 >= a.pool || cur.p1 < 0 || (int64_t)cur.p1 >= a.pool) {
+    const bool two = P16 && rows > 16;
+    if (whole_table) {  // pos < 128 for blocks that exist
+      const int j = (int)pos, lo0 = __shfl(tbl0, j & 63, 64), hi0 = __shfl(tbl1, j & 63, 64);
+      const int lo1 = __shfl(tbl0, (j + 1) & 63, 64), hi1 = __shfl(tbl1, (j + 1) & 63, 64);
+      cur.p0 = j < 64 ? lo0 : hi0;
+      cur.p1 = !two ? cur.p0 : j + 1 < 64 ? lo1 : hi1;
+    } else if (in) {
+      cur.p0 = a.indices[pos];
+      cur.p1 = two ? a.indices[pos + 1] : cur.p0;
+    }
+    if (in && (cur.p0 < 0 || (int64_t)cur.p0 >= a.pool || cur.p1 < 0 || (int64_t)cur.p1 >= a.pool)) {
       rows = 0;
       bad = true;
     }
     cur.meta = rows | (!P16 && a.page_rows == 64 ? (int)(b & 1) * kBlock : 0) << 16;
   };
+  uint8_t *const slots = s_wave[wave];
+  const uint32_t slots_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void *)slots;
   for (int64_t i0 = 0; i0 < n; i0 += 64) {
     locate(i0);
     const int m = (int)min<int64_t>(64, n - i0);
-    int rows[2];
-    uint8_t *const slots = s_dyn + wave * 2 * Slot<1>::bytes;
-    const uint32_t slots_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void *)slots;
-    auto issue = [&](int slot, int i, int &rows_out) {
-      const int meta = i < m ? __builtin_amdgcn_readlane(cur.meta, i & 63) : 0;
+    auto issue = [&](int i, int slot) {
+      const int meta = i < m ? __builtin_amdgcn_readlane(cur.meta, i) : 0;
       Place p;
       p.rows = meta & 255;
       p.row = meta >> 16;
-      p.p0 = p.rows ? __builtin_amdgcn_readlane(cur.p0, i & 63) : 0;
-      p.p1 = P16 && p.rows ? __builtin_amdgcn_readlane(cur.p1, i & 63) : 0;
-      load_block<P16, 1, kSplit, false>(a, p, slots_at + slot * Slot<1>::bytes, lane, kvh);
-      rows_out = p.rows;
+      p.p0 = p.rows ? __builtin_amdgcn_readlane(cur.p0, i) : 0;
+      p.p1 = P16 && p.rows ? __builtin_amdgcn_readlane(cur.p1, i) : 0;
+      load_block<P16, NH, ARR, false>(a, p, slots_at + slot * Slot<NH>::bytes, lane, kvh);
+      return p.rows;
     };
     wait_reads();
-    issue(0, 0, rows[0]);
-    int i = 0;
-    while (true) {
+    int rows = issue(0, 0);
+    if (i0 == 0) {
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        wait_reads();
-        issue(s ^ 1, i + 1, rows[s ^ 1]);
-        if (i == 0) w.settle_q();
-        wait_loads<kBlockLoads<P16, 1>>();
-        process_block<P16, 1, kSplit>(st1, slots + s * Slot<1>::bytes, rows[s], col, quad,
-                                      a.scale_log2);
-        if (++i >= m) goto walked;
+      for (int g = 0; g < NH; ++g) w[g].settle_q();
+    }
+    for (int i = 0; i < m; ++i) {
+      wait_reads();
+      const int rows_next = issue(i + 1, (i + 1) & 1);
+      wait_loads<kBlockLoads<P16, NH>>();
+      process_block<P16, NH, ARR>(w, slots + (i & 1) * Slot<NH>::bytes, rows, col, quad,
+                                  a.scale_log2);
+      rows = rows_next;
+    }
+  }
+  float l[NH];
+#pragma unroll
+  for (int g = 0; g < NH; ++g) {
+    l[g] = w[g].normalizer();
+    w[g].join_columns();
+  }
+  // The wave's slots become its columns' place; loads past its last block may still
+  // write them.
+  wait_loads<0>();
+  wait_reads();
+#pragma unroll
+  for (int g = 0; g < NH; ++g)
+    if (col < heads) {
+      const int c = g * heads + col;
+      w[g].stash(reinterpret_cast<float *>(slots) + c * kStash, quad);
+      if (quad == 0) {
+        s_m[wave][c] = w[g].m_run;
+        s_l[wave][c] = l[g];
       }
     }
-  walked:;
-  }
-  const float l = w.normalizer();
-  w.join_columns();
-  // The slots become the states' place; loads past the last block may still write.
-  wait_loads<0>();
-  __syncthreads();
-  if (mine) {
-    w.stash(s_acc + ((int64_t)wave * a.tile + col) * 128, quad);
-    if (quad == 0) {
-      s_m[wave][col] = w.m_run;
-      s_l[wave][col] = l;
-    }
-  }
   // An invalid page index anywhere in the request keeps its sentinels.
   if (block_or(bad, s_bad)) return poison();
-  for (int x = tid; x < heads * 128; x += W * 64) {
-    const int g = x >> 7, d = x & 127;
+  // Four dims of one column per thread.
+  for (int x = tid; x < NH * heads * 32; x += W * 64) {
+    const int g = x >> 5, d = (x & 31) * 4;
     float M = -FLT_MAX;
 #pragma unroll
-    for (int i = 0; i < W; ++i) M = fmaxf(M, s_m[i][g]);
-    float L = 0.f, O = 0.f;
+    for (int i = 0; i < W; ++i) M = fmax_nan(M, s_m[i][g]);
+    float L = 0.f;
+    f32x4 O = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < W; ++i) {
       const float f = fast_exp2(s_m[i][g] - M);
+      const f32x4 o = *reinterpret_cast<const f32x4 *>(
+          reinterpret_cast<const float *>(s_wave[i]) + g * kStash + d);
       L = fmaf(s_l[i][g], f, L);
-      O = fmaf(s_acc[(i * a.tile + g) * 128 + d], f, O);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) O[e] = fmaf(o[e], f, O[e]);
     }
     if (a.splits > 1) {
       float *ss = state_of(g);
-      ss[4 + d] = O;
+      *reinterpret_cast<f32x4 *>(ss + 4 + d) = O;
       if (d == 0) {
         ss[0] = M;
         ss[1] = L;
       }
       continue;
     }
-    const int64_t row = (int64_t)r * a.hq + qh0 + g;
-    a.out[row * 128 + d] = f32_to_bf16(O / L);
+    const int64_t row = (int64_t)r * a.hq + query_head(g);
+    const float inv = 1.0f / L;
+    *reinterpret_cast<u32x2 *>(a.out + row * 128 + d) =
+        u32x2{bf16x2_pack(O[0] * inv, O[1] * inv), bf16x2_pack(O[2] * inv, O[3] * inv)};
     if (d == 0) a.lse[row] = M + __log2f(L);
   }
 }
 
-// kv-heads per wave of the balanced kernel: two neighbours where Hkv is even.
+// kv-heads per wave: two neighbours where Hkv is even, in the balanced kernel always.
 uint64_t heads_per_wave(uint64_t hkv) { return hkv % 2 == 0 ? 2 : 1; }
-
-size_t direct_lds(uint32_t tile) {
-  return (size_t)kDirectWaves * std::max<size_t>(tile * 128 * 4, 2 * Slot<1>::bytes);
-}
 
 }  // namespace
 
 namespace loom {
 
-#ifndef LOOM_MX4_DIRECT_TOKENS
-#define LOOM_MX4_DIRECT_TOKENS 16384
-#endif
+// The algorithm goes by the tokens a plan covers times Hkv (the rows of K to read).
+// Microseconds, direct / balanced, 32x8 heads unless said: 1 x 1000 tokens 8.7 / 11.6;
+// 1 x 32000 14.6 / 24.6; 16 x 256-1536 13.7 / 15.5; 64 x 256-1024 17.6 / 25.1; 16 x 4096
+// 22.7 / 25.7; 64 x 1024-4096 (1.3 M rows) 49.8 / 46.6; 8 x 1000-32000 (1.1 M) 51.4 /
+// 36.3: a direct workgroup has one request's share, so unlike lengths cost it more.
+constexpr uint64_t kDirectRows = 1u << 20;
+// Direct workgroups over NHD pages take two kv-heads from this many rows on, where whole
+// cache lines outweigh the halved parallelism (one / two): 16 x 1024 13.9 / 13.1; 16 x
+// 2048 19.0 / 17.0; 64 x 256-1024 20.3 / 17.6; 1 x 32000 14.6 / 17.4; 4 x 8000 14.7 /
+// 16.7.
+constexpr uint64_t kDirectPairRows = 5u << 16;
+// Workgroups per (request, kv-heads, tile): doubled while they fit the CUs and each keeps
+// kSplitBlocks blocks on average (1 x 1000: 8.7 us with 4, 9.3 with 8; two per CU: no
+// faster).
+constexpr uint64_t kMaxSplits = 64, kSplitBlocks = 4;
 
 loom_status_t plan_mx4_decode(loom_paged_decode_plan_info_t *info, uint32_t teams_option, int cus,
                               loom_error_t *err) {
@@ -889,9 +999,18 @@ loom_status_t plan_mx4_decode(loom_paged_decode_plan_info_t *info, uint32_t team
   info->group_tiles = (uint32_t)tiles;
   info->device_cus = (uint32_t)cus;
   info->header_bytes = 0;
-  const uint64_t heads = B * hkv * tiles;
-  if (teams_option == 0 && info->max_total_pages * page_rows <= LOOM_MX4_DIRECT_TOKENS) {
-    const uint64_t splits = 1;
+  // blocks of 32 tokens that the plan covers
+  const uint64_t blocks = info->max_total_pages * page_rows / kBlock + B;
+  if (blocks > (uint64_t)INT32_MAX)
+    return fail(err, LOOM_PLAN_STATE_COUNT_OUT_OF_RANGE, "paged batch-decode blocks", blocks);
+  const uint64_t rows = info->max_total_pages * page_rows * hkv;
+  if (teams_option == 0 && rows <= kDirectRows) {
+    const bool pair = s.kv_layout != LOOM_KV_LAYOUT_HND && hkv % 2 == 0 && rows >= kDirectPairRows;
+    const uint64_t heads = B * (hkv / (pair ? 2 : 1)) * tiles;
+    uint64_t splits = 1;
+    while (splits < kMaxSplits && heads * splits * 2 <= (uint64_t)cus &&
+           blocks / B >= splits * 2 * kSplitBlocks)
+      splits *= 2;
     const uint64_t grid = heads * splits;
     if (grid > (uint64_t)INT32_MAX || B * hq > (uint64_t)INT32_MAX)
       return fail(err, LOOM_PLAN_STATE_COUNT_OUT_OF_RANGE, "paged batch-decode", grid);
@@ -926,18 +1045,25 @@ hipError_t launch_mx4_decode(const loom_paged_decode_plan_info_t &info, const Mx
   const bool p16 = a.page_rows == 16;
   const dim3 grid(info.grid_blocks), heads((unsigned)((int64_t)a.batch * a.hq));
   if (info.algorithm == LOOM_PAGED_DECODE_DIRECT) {
-    hipLaunchKernelGGL(p16 ? mx4_decode_direct_kernel<true> : mx4_decode_direct_kernel<false>, grid,
-                       dim3(kDirectWaves * 64), direct_lds(info.group_tile), stream, a);
+    // the plan's grid says how many kv-heads its workgroups take
+    const bool pair = (uint64_t)info.grid_blocks * 2 ==
+                      (uint64_t)a.batch * a.hkv * a.tiles * (uint64_t)a.splits;
+    auto kernel = pair
+                      ? (p16 ? mx4_decode_direct_kernel<true, 2, kPair>
+                             : mx4_decode_direct_kernel<false, 2, kPair>)
+                      : (p16 ? mx4_decode_direct_kernel<true, 1, kSplit>
+                             : mx4_decode_direct_kernel<false, 1, kSplit>);
+    hipLaunchKernelGGL(kernel, grid, dim3(info.block_threads), 0, stream, a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || a.splits == 1) return e;
     hipLaunchKernelGGL(mx4_decode_direct_merge_kernel, heads, dim3(kThreads), 0, stream, a);
     return hipGetLastError();
   }
-  const bool nhd = a.row_bytes != 64;  // (with one kv-head the layouts are the same)
   auto kernel = heads_per_wave(a.hkv) == 1
                     ? (p16 ? mx4_decode_split_kernel<true, 1, kSplit>
                            : mx4_decode_split_kernel<false, 1, kSplit>)
-                : nhd ? (p16 ? mx4_decode_split_kernel<true, 2, kPair>
+                : info.spec.kv_layout != LOOM_KV_LAYOUT_HND
+                      ? (p16 ? mx4_decode_split_kernel<true, 2, kPair>
                              : mx4_decode_split_kernel<false, 2, kPair>)
                       : (p16 ? mx4_decode_split_kernel<true, 2, kSplit>
                              : mx4_decode_split_kernel<false, 2, kSplit>);

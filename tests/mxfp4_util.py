@@ -86,15 +86,18 @@ def rows_of(cache, indptr, indices, r, n):
 
 def attend(q, k, v, scale=D ** -0.5):
     """q [hq, 128] over k, v [n, hkv, 128]: (out [hq, 128], lse [hq] in log2)."""
-    group = q.shape[0] // k.shape[1]
+    hkv = k.shape[1]
+    group = q.shape[0] // hkv
     out, lse = np.empty(q.shape), np.empty(q.shape[0])
     with np.errstate(invalid="ignore", over="ignore"):
-        for h in range(q.shape[0]):
-            s = k[:, h // group] @ q[h] * scale
-            m = s.max()
+        for h in range(hkv):
+            heads = slice(h * group, (h + 1) * group)
+            s = np.ascontiguousarray(k[:, h]) @ q[heads].T * scale
+            m = s.max(0)
             p = np.exp(s - m)
-            out[h] = p @ v[:, h // group] / p.sum()
-            lse[h] = (m + math.log(p.sum())) / math.log(2) if np.isfinite(p.sum()) else np.nan
+            total = p.sum(0)
+            out[heads] = (p / total).T @ np.ascontiguousarray(v[:, h])
+            lse[heads] = (m + np.log(total)) / math.log(2)
     return out, lse
 
 

@@ -77,8 +77,9 @@ class Case:
         for r, n in enumerate(self.lens):
             k, v = (mx.rows_of(c, self.indptr, self.indices, r, n) for c in (self.k, self.v))
             g = self.hq // self.hkv
-            for h in range(self.hq):
-                score = max(score, (np.abs(k[:, h // g]) @ np.abs(self.q[r, h])).max())
+            for h in range(self.hkv):
+                heads = np.abs(self.q[r, h * g:(h + 1) * g])
+                score = max(score, (np.abs(np.ascontiguousarray(k[:, h])) @ heads.T).max())
             vmax = max(vmax, np.abs(v).max())
         off = score * mx.D ** -0.5 * LOG2E * 128 * 2.0 ** -24 + 2.0 ** -20
         return (2.0 ** -8 * np.abs(ref_o) + vmax * (2 * off + 2.0 ** -15 + 2.0 ** -20),
@@ -159,6 +160,48 @@ def test_more_requests_than_one_scan_block(env):
     lens = [int(n) for n in rng.integers(1, 40, 600)]
     c = Case(env[0], 6, lens, 4, 2)
     out, lse, _ = run(env, c)
+    check(c, out, lse)
+
+
+@pytest.mark.parametrize("teams", [0, 37, 2000])
+@pytest.mark.parametrize("batch", [64, 65, 300, 600, 1300])
+def test_many_requests(env, batch, teams):
+    """Balanced commands keep the list of up to 64 requests in registers, of up to 512 in
+    LDS, and of more in steps of 2, 4, ... requests; among them requests that no team
+    starts with, and (invalid last-page lengths) some without blocks."""
+    rng = np.random.default_rng(5)
+    lens = [int(n) for n in rng.integers(1, 100, batch)]
+    c = Case(env[0], 6, lens, 4, 2)
+    out, lse, _ = run(env, c, {"teams": teams})
+    check(c, out, lse)
+    x = c.device()
+    broken = sorted(set(int(r) for r in rng.integers(0, batch, 7)) | {0, batch - 1})
+    x[7][env[0].tensor(broken, device="cuda")] = 0
+    got, got_l, _ = run(env, c, {"teams": teams}, operands=x, fill=7.0)
+    for r in range(batch):
+        if r in broken:
+            assert (got[r] == 7.0).all() and (got_l[r] == 7.0).all()
+    whole = [r for r in range(batch) if r not in broken]
+    ref_o, ref_l = c.reference()
+    bo, bl = c.bounds(ref_o, ref_l)
+    assert (np.abs(got - ref_o) <= bo)[whole].all() and (np.abs(got_l - ref_l) <= bl)[whole].all()
+
+
+@pytest.mark.parametrize("shape", [
+    # lens, hq, hkv, page, layout: the planner's three forms at their sizes
+    ([5000], 8, 8, 16, "NHD"),                   # direct, split over many workgroups
+    ([5200, 5100], 32, 32, 16, "NHD"),           # direct, two kv-heads per workgroup
+    ([5200, 5100], 32, 32, 64, "HND"),           # direct, one
+    ([300] * 40, 64, 32, 32, "NHD"),             # direct, two, not split
+    ([17000, 16500], 64, 32, 64, "HND"),         # balanced
+    ([33333], 32, 32, 32, "NHD"),                # balanced, one request in every team
+])
+def test_planned_forms(env, shape):
+    lens, hq, hkv, page, layout = shape
+    c = Case(env[0], 77, lens, hq, hkv, page, layout)
+    out, lse, plan = run(env, c)
+    rows = c.pool * page * hkv
+    assert plan.algorithm == ("direct" if rows <= 1 << 20 else "balanced_split_kv")
     check(c, out, lse)
 
 
