@@ -6,11 +6,17 @@
 //
 // Each head's row is 68 bytes read and 256 written, twice (K and V), with no
 // arithmetic but the conversion, so the kernel is bound by the memory rate, four
-// fifths of it writes.  One workgroup takes 16 output rows: its first wave finds
-// their requests and pages (three dependent round trips, whatever the batch), then
-// 16 lanes per head row load 4 code bytes each and store 16 bytes, K and V
-// together, the heads of a row contiguous.
+// fifths of it writes.  A workgroup takes some output rows (64 head rows, or one
+// output row): its first wave finds their requests and pages, one row per lane,
+// from the table words of 64 requests in its registers (two round trips before the
+// rows' own for batches below 64, else a search first), then 16 lanes per head row
+// load 4 code bytes each and store 16 bytes, K and V together, the heads of a row
+// contiguous.  The stores are streamed past L2: plain ones, whose lines L2 writes
+// back in another order, took 41 us instead of 27.5 (38k rows of 8 kv-heads, HND
+// pages of 64: 5.9 TB/s).
 #include <hip/hip_runtime.h>
+
+#include <algorithm>
 
 #include "attn_device.hpp"
 #include "loom_internal.hpp"
@@ -21,7 +27,15 @@ using namespace loom_dev;
 namespace {
 
 constexpr int kReadThreads = 256;
-constexpr int kReadRows = 16;  // output rows per workgroup
+constexpr int kReadMaxRows = 64;  // output rows per workgroup: at most one per lane
+constexpr uint64_t kReadMaxHeads = 4096;
+// Head rows per workgroup, and how many of them each 16 lanes have in flight.
+// Measured with 16 to 256 head rows and 1 to 4 in flight: 64 are within 4% of the
+// best from 8k rows of 8 kv-heads (8.8 us) to 38k (27.5 us); 256 take 8 us where
+// 64 take 4.5 (300 rows of 32 kv-heads), 16 lose 5% of the large ones.  The number
+// in flight changes less than 3%.
+constexpr int kReadItems = 64;
+constexpr int kReadDepth = 2;
 
 struct ReadArgs {
   const uint8_t *k;
@@ -44,6 +58,8 @@ struct ReadArgs {
   int32_t page_rows;
   int32_t head_bytes;  // NHD: 64; HND pages: page_rows * 64
   int32_t row_bytes;   // NHD: hkv * 64; HND pages: 64
+  int32_t rows;        // output rows per workgroup
+  uint32_t hkv_inv;    // 2^32 / hkv, rounded up
 };
 
 // Largest request r <= batch with kv_indptr[r] <= t, by one wave: 64 entries a
@@ -62,68 +78,96 @@ __device__ __forceinline__ int request_of(const ReadArgs &a, int t, int lane) {
   return lo;
 }
 
+// One head row's part of a lane: 8 codes and their scale byte, of K and of V.
+struct Part {
+  uint32_t k, v, ks, vs;
+};
+
 __global__ __launch_bounds__(kReadThreads) void paged_kv_read_kernel(ReadArgs a) {
-  __shared__ int32_t s_page[kReadRows], s_off[kReadRows];
+  __shared__ int32_t s_page[kReadMaxRows], s_off[kReadMaxRows];
   const int tid = threadIdx.x, lane = tid & 63;
-  const int t0 = (int)blockIdx.x * kReadRows;
-  const int rows = min(kReadRows, a.nnz - t0);
+  const int t0 = (int)blockIdx.x * a.rows;
+  const int rows = min(a.rows, a.nnz - t0);
   if (tid < 64) {
+    // Lane l holds the table words of request r0 + l, and finds the place of row l.
+    const int r0 = a.batch < 64 ? 0 : uni(request_of(a, t0, lane));
+    const int at = min(r0 + lane, a.batch), in = min(at, a.batch - 1);
     const int32_t ip0 = a.indptr[0], ipB = a.indptr[a.batch];
     const int32_t kv0 = a.kv_indptr[0], kvB = a.kv_indptr[a.batch];
+    const int32_t w_kv = a.kv_indptr[at], w_ip = a.indptr[at];
+    const int32_t w_last = a.last[in], w_start = a.kv_start ? a.kv_start[in] : 0;
     const bool ok = ip0 == 0 && ipB >= 0 && kv0 == 0 && kvB >= 0 && kvB <= a.nnz &&
                     (a.indices_capacity ? (int64_t)ipB <= a.n_indices : (int64_t)ipB == a.n_indices);
-    int page = -1, off = 0;
-    if (ok) {
-      const int r0 = uni(request_of(a, t0, lane));
-      // Row j belongs to request r0 + the number of later starts that are <= its
-      // index; more than 64 of those (empty requests): searched again.
-      const int32_t next = r0 + 1 + lane <= a.batch ? a.kv_indptr[r0 + 1 + lane] : INT32_MAX;
-      int r = r0;
+    const int t = t0 + lane;
+    // the last of the 64 requests that starts at or before row t
+    int k = 0;
 #pragma unroll
-      for (int j = 0; j < kReadRows; ++j) {
-        const int more = __builtin_popcountll(__builtin_amdgcn_ballot_w64(next <= t0 + j));
-        const int rj = more < 64 ? r0 + more : request_of(a, t0 + j, lane);
-        if (lane == j) r = rj;
+    for (int step = 32; step; step >>= 1)
+      if (__shfl(w_kv, k + step, 64) <= t) k += step;
+    const int k1 = min(k + 1, 63);
+    int32_t st = __shfl(w_ip, k, 64), en = __shfl(w_ip, k1, 64), tl = __shfl(w_last, k, 64);
+    int32_t b = __shfl(w_kv, k, 64), e = __shfl(w_kv, k1, 64), start = __shfl(w_start, k, 64);
+    int r = min(r0 + k, a.batch);
+    int page = -1, off = 0;
+    if (ok && lane < rows && r < a.batch) {
+      if (k == 63) {  // past 62 short requests: searched, and read, from the table
+        int n = a.batch + 1 - r;  // the answer is one of [r, r + n)
+        while (n > 1) {
+          const int half = n / 2;
+          const bool le = a.kv_indptr[r + half] <= t;
+          r += le ? half : 0;
+          n = le ? n - half : half;
+        }
+        const int rr = min(r, a.batch - 1);
+        st = a.indptr[rr], en = a.indptr[rr + 1], tl = a.last[rr];
+        b = a.kv_indptr[rr], e = a.kv_indptr[rr + 1];
+        start = a.kv_start ? a.kv_start[rr] : 0;
       }
-      if (lane < rows && r < a.batch) {
-        const int t = t0 + lane;
-        const int32_t st = a.indptr[r], en = a.indptr[r + 1], tl = a.last[r];
-        const int32_t b = a.kv_indptr[r], e = a.kv_indptr[r + 1];
-        const int32_t start = a.kv_start ? a.kv_start[r] : 0;
-        const int64_t kv_len = ((int64_t)en - st - 1) * a.page_rows + tl;
-        if (st >= 0 && en > st && en <= ipB && tl >= 1 && tl <= a.page_rows && b >= 0 && b <= t &&
-            t < e && start >= 0 && (int64_t)start + (e - b) <= kv_len) {
-          const int p = start + (t - b);
-          const int32_t idx = a.indices[st + p / a.page_rows];
-          if (idx >= 0 && (int64_t)idx < a.pool) {
-            page = idx;
-            off = p % a.page_rows;
-          }
+      const int64_t kv_len = ((int64_t)en - st - 1) * a.page_rows + tl;
+      if (st >= 0 && en > st && en <= ipB && tl >= 1 && tl <= a.page_rows && b >= 0 && b <= t &&
+          t < e && start >= 0 && (int64_t)start + (e - b) <= kv_len) {
+        const uint32_t p = (uint32_t)start + (uint32_t)(t - b);
+        const int32_t idx = a.indices[st + (int)(p / (uint32_t)a.page_rows)];
+        if (idx >= 0 && (int64_t)idx < a.pool) {
+          page = idx;
+          off = (int)(p % (uint32_t)a.page_rows);
         }
       }
     }
-    if (lane < kReadRows) {
-      s_page[lane] = page;
-      s_off[lane] = off;
-    }
+    s_page[lane] = page;
+    s_off[lane] = off;
   }
   __syncthreads();
   const int c = tid & 15;
   const int64_t page_bytes = (int64_t)a.page_rows * a.hkv * 64;
-#pragma unroll 2
-  for (int i = tid >> 4; i < rows * a.hkv; i += kReadThreads / 16) {
-    const int j = i / a.hkv, h = i - j * a.hkv;
-    const int page = s_page[j], off = s_off[j];
-    if (page < 0) continue;
-    const int64_t at =
-        page * page_bytes + (int64_t)h * a.head_bytes + (int64_t)off * a.row_bytes + c * 4;
-    const int64_t sc = ((((int64_t)page * a.hkv + h) * a.page_rows + off) << 2) + (c >> 2);
-    const uint32_t kc = *reinterpret_cast<const uint32_t *>(a.k + at);
-    const uint32_t vc = *reinterpret_cast<const uint32_t *>(a.v + at);
-    const uint32_t ks = a.k_mx[sc], vs = a.v_mx[sc];
-    const int64_t out = ((int64_t)(t0 + j) * a.hkv + h) * 128 + c * 8;
-    *reinterpret_cast<u32x4 *>(a.k_out + out) = mx4x8_to_bf16x8(kc, ks << 23);
-    *reinterpret_cast<u32x4 *>(a.v_out + out) = mx4x8_to_bf16x8(vc, vs << 23);
+  const int items = rows * a.hkv;
+  constexpr int kStep = kReadThreads / 16;
+  for (int i0 = tid >> 4; i0 < items; i0 += kStep * kReadDepth) {
+    Part part[kReadDepth];
+    int64_t out[kReadDepth];
+#pragma unroll
+    for (int u = 0; u < kReadDepth; ++u) {
+      const int i = i0 + u * kStep;
+      const int j = min(a.hkv == 1 ? i : (int)__umulhi((uint32_t)i, a.hkv_inv), kReadMaxRows - 1);
+      const int page = i < items ? s_page[j] : -1, off = s_off[j];
+      const int h = i - j * a.hkv;
+      out[u] = page < 0 ? -1 : ((int64_t)(t0 + j) * a.hkv + h) * 128 + c * 8;
+      if (page >= 0) {
+        const int64_t at =
+            page * page_bytes + (int64_t)h * a.head_bytes + (int64_t)off * a.row_bytes + c * 4;
+        const int64_t sc = ((((int64_t)page * a.hkv + h) * a.page_rows + off) << 2) + (c >> 2);
+        part[u] = {*reinterpret_cast<const uint32_t *>(a.k + at),
+                   *reinterpret_cast<const uint32_t *>(a.v + at), a.k_mx[sc], a.v_mx[sc]};
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kReadDepth; ++u)
+      if (out[u] >= 0) {
+        __builtin_nontemporal_store(mx4x8_to_bf16x8(part[u].k, part[u].ks << 23),
+                                    reinterpret_cast<u32x4 *>(a.k_out + out[u]));
+        __builtin_nontemporal_store(mx4x8_to_bf16x8(part[u].v, part[u].vs << 23),
+                                    reinterpret_cast<u32x4 *>(a.v_out + out[u]));
+      }
   }
 }
 
@@ -150,7 +194,8 @@ loom_status_t loom_prefill_provider_plan_paged_kv_read(const loom_prefill_provid
   // requests and heads are indexed in 32 bits
   if (s.paged.batch_size >= (uint64_t)INT32_MAX)
     return fail(err, LOOM_PLAN_STATE_COUNT_OUT_OF_RANGE, "K/V read batch", s.paged.batch_size);
-  if (s.paged.num_kv_heads > (uint64_t)INT32_MAX / (64 * 64))
+  // (head rows of a workgroup are divided by the heads by a 32-bit reciprocal)
+  if (s.paged.num_kv_heads > kReadMaxHeads)
     return fail(err, LOOM_PLAN_STATE_COUNT_OUT_OF_RANGE, "K/V read heads", s.paged.num_kv_heads);
   auto *p = new loom_paged_kv_read_plan;
   p->spec = s;
@@ -232,7 +277,9 @@ loom_status_t loom_paged_kv_read_enqueue(const loom_paged_kv_read_plan_t *plan,
   const bool hnd = s.kv_layout == LOOM_KV_LAYOUT_HND;
   a.head_bytes = hnd ? a.page_rows * 64 : 64;
   a.row_bytes = hnd ? 64 : a.hkv * 64;
-  const unsigned grid = (unsigned)((plan->spec.nnz_kv + kReadRows - 1) / kReadRows);
+  a.rows = std::min(std::max(kReadItems / a.hkv, 1), kReadMaxRows);
+  a.hkv_inv = (uint32_t)(((1ull << 32) + a.hkv - 1) / a.hkv);  // (hkv = 1: not used)
+  const unsigned grid = (unsigned)((plan->spec.nnz_kv + a.rows - 1) / a.rows);
   hipLaunchKernelGGL(paged_kv_read_kernel, dim3(grid), dim3(kReadThreads), 0, scope->queue->stream,
                      a);
   return loom::record_launch(scope, hipGetLastError(), err);

@@ -329,6 +329,22 @@ def test_read_back_of_many_requests(env):
         assert same_bits(got, want)
 
 
+@pytest.mark.parametrize("hkv", [1, 5, 70])
+@pytest.mark.parametrize("batch", [1, 62, 63, 64, 65, 127, 200])
+def test_read_back_over_batches(env, batch, hkv):
+    """Around the 64 requests whose table words one wave holds, with empty ones between;
+    1 to 64 output rows per workgroup."""
+    rng = np.random.default_rng(batch)
+    lens = [int(n) for n in rng.integers(1, 24, batch)]
+    c = Case(env[0], batch, lens, hkv, hkv, 16, "HND")
+    counts = [int(rng.integers(0, n + 1)) * int(rng.random() < 0.6) for n in lens]
+    counts[-1] = 1
+    starts = [int(rng.integers(0, n - k + 1)) for n, k in zip(lens, counts)]
+    nnz = sum(counts)
+    for got, want in zip(read(env, c, starts, counts), rows_wanted(c, starts, counts, nnz)):
+        assert same_bits(got, want)
+
+
 def test_read_back_from_the_first_token_without_starts(env):
     c = Case(env[0], 4, [40, 20], 2, 2)
     for got, want in zip(read(env, c, [], [9, 20], give_start=False),
