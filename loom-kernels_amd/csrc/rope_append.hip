@@ -27,6 +27,7 @@
 #include <hip/hip_runtime.h>
 
 #include <cmath>
+#include <type_traits>
 
 #include "attn_device.hpp"
 #include "loom_internal.hpp"
@@ -403,10 +404,13 @@ struct RowSlices {
 
 __device__ __forceinline__ RowSlice load_slice(const AppendArgs &a, int t, int row, int c) {
   RowSlice f = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+  // Both pointers before any branch: a load whose address is a choice between two
+  // fields of the arguments makes the compiler copy them all to scratch memory.
+  const uint16_t *q = a.q, *k = a.k;
   if (row < a.hq + a.hkv) {
     const bool is_kv = row >= a.hq;
-    const uint16_t *src = is_kv ? a.k + ((int64_t)t * a.hkv + row - a.hq) * 128
-                                : a.q + ((int64_t)t * a.hq + row) * 128;
+    const uint16_t *src = is_kv ? k + ((int64_t)t * a.hkv + row - a.hq) * 128
+                                : q + ((int64_t)t * a.hq + row) * 128;
     f.x = *reinterpret_cast<const u32x4 *>(src + c * 8);
     if (is_kv)
       f.v = *reinterpret_cast<const u32x4 *>(a.v + ((int64_t)t * a.hkv + row - a.hq) * 128 + c * 8);
@@ -542,6 +546,13 @@ __device__ __forceinline__ double row_sum(double x) {
 __device__ __forceinline__ uint32_t block_max(uint32_t x) {  // over lanes 4i .. 4i + 3
   x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0xB1, 0xf, 0xf, false));
   return max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x4E, 0xf, 0xf, false));
+}
+
+// In lane 0 of 16: the bytes of lanes 0, 4, 8 and 12, lowest first.
+__device__ __forceinline__ uint32_t row_bytes4(uint32_t x) {
+  const uint32_t two =
+      x | (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x12C, 0xf, 0xf, false) << 8;
+  return two | dpp_other_half(two) << 16;
 }
 
 __device__ __forceinline__ float bf16_at(const u32x4 &x, int i) {
@@ -689,18 +700,25 @@ struct NormForm {
   static __device__ __forceinline__ void row(const Args &a, const Weights &w, int t, int64_t page,
                                              int off, int row, int c, const Angles &s,
                                              const RowSlice &sl) {
-    const bool norm = a.q_norm != nullptr;
-    if (row < a.hq) {
-      float y[8];
-      norm_rotate<float>(sl.x, w.q, norm, a.eps, c, s.sin, s.cos, y);
-      u32x4 o;
+    if (row < a.hq)
+      q_row(a, w, t, row, c, s, sl.x);
+    else
+      kv_row(a, w, page, off, row - a.hq, c, s, sl);
+  }
+  static __device__ __forceinline__ void q_row(const Args &a, const Weights &w, int t, int row,
+                                               int c, const Angles &s, const u32x4 &x) {
+    float y[8];
+    norm_rotate<float>(x, w.q, a.q_norm != nullptr, a.eps, c, s.sin, s.cos, y);
+    u32x4 o;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[e] = loom_dev::bf16x2_pack(y[2 * e], y[2 * e + 1]);
-      __builtin_nontemporal_store(
-          o, reinterpret_cast<u32x4 *>(a.q_out + ((int64_t)t * a.hq + row) * 128 + c * 8));
-      return;
-    }
-    const int kh = row - a.hq;
+    for (int e = 0; e < 4; ++e) o[e] = loom_dev::bf16x2_pack(y[2 * e], y[2 * e + 1]);
+    __builtin_nontemporal_store(
+        o, reinterpret_cast<u32x4 *>(a.q_out + ((int64_t)t * a.hq + row) * 128 + c * 8));
+  }
+  static __device__ __forceinline__ void kv_row(const Args &a, const Weights &w, int64_t page,
+                                                int off, int kh, int c, const Angles &s,
+                                                const RowSlice &sl) {
+    const bool norm = a.q_norm != nullptr;
     const int64_t at =
         page * a.page_rows * a.hkv * 128 + (int64_t)kh * a.head_elems + (int64_t)off * a.row_elems;
     if constexpr (KV == kKvMx4) {
@@ -712,10 +730,12 @@ struct NormForm {
       uint8_t *vp = reinterpret_cast<uint8_t *>(a.v_pages) + at / 2 + c * 4;
       *reinterpret_cast<uint32_t *>(kp) = k4;
       *reinterpret_cast<uint32_t *>(vp) = v4;
-      if ((c & 3) == 0) {
-        const int64_t sc = (((page * a.hkv + kh) * a.page_rows + off) << 2) + (c >> 2);
-        a.k_mx[sc] = (uint8_t)kb;
-        a.v_mx[sc] = (uint8_t)vb;
+      // the row's 4 scale bytes, from lanes 0, 4, 8 and 12, as one word
+      const uint32_t kw = row_bytes4(kb), vw = row_bytes4(vb);
+      const int64_t sc = ((page * a.hkv + kh) * a.page_rows + off) << 2;
+      if (c == 0) {
+        *reinterpret_cast<uint32_t *>(a.k_mx + sc) = kw;
+        *reinterpret_cast<uint32_t *>(a.v_mx + sc) = vw;
       }
     } else {
       float y[8];
@@ -768,6 +788,50 @@ __device__ __forceinline__ void apply_token(const typename Form::Args &a, int t,
   }
 }
 
+// The same by one wave, 4 rows at a time: the Q rows with the next kWaveRows
+// loads in flight, then the K/V rows.
+constexpr int kWaveRows = 4;
+struct WaveSlices {
+  u32x4 q[kWaveRows];
+  RowSlice kv;
+};
+__device__ __forceinline__ u32x4 load_q(const AppendArgs &a, int t, int row, int c) {
+  const u32x4 none = {0, 0, 0, 0};
+  return row < a.hq
+             ? *reinterpret_cast<const u32x4 *>(a.q + ((int64_t)t * a.hq + row) * 128 + c * 8)
+             : none;
+}
+__device__ __forceinline__ WaveSlices load_wave_slices(const AppendArgs &a, int t, int lane) {
+  WaveSlices f;
+#pragma unroll
+  for (int i = 0; i < kWaveRows; ++i) f.q[i] = load_q(a, t, (lane >> 4) + 4 * i, lane & 15);
+  f.kv = load_slice(a, t, a.hq + (lane >> 4), lane & 15);
+  return f;
+}
+template <class Form>
+__device__ __forceinline__ void apply_token_wave(const typename Form::Args &a, int t, int64_t page,
+                                                 int off, int lane, const typename Form::Angles &s,
+                                                 const typename Form::Weights &w, WaveSlices pre) {
+  const int c = lane & 15;
+#pragma unroll 1
+  for (int row = lane >> 4; row < a.hq; row += 4 * kWaveRows)
+#pragma unroll
+    for (int i = 0; i < kWaveRows; ++i) {
+      const int at = row + 4 * i;
+      if (at < a.hq) {
+        const u32x4 x = pre.q[i];
+        pre.q[i] = load_q(a, t, at + 4 * kWaveRows, c);
+        Form::q_row(a, w, t, at, c, s, x);
+      }
+    }
+#pragma unroll 1
+  for (int row = a.hq + (lane >> 4); row < a.hq + a.hkv; row += 4) {
+    const RowSlice now = pre.kv;
+    pre.kv = load_slice(a, t, row + 4, c);
+    Form::kv_row(a, w, page, off, row - a.hq, c, s, now);
+  }
+}
+
 // One launch per command.  Workgroups 0..V-1 each validate one chunk of the
 // command (validate_chunk) and publish the chunk's verdict, tagged with the
 // command's epoch, to every signal copy, then empty their share of the hash
@@ -802,12 +866,12 @@ __device__ __forceinline__ void apply_token(const typename Form::Args &a, int t,
 // Same-address atomics of many workgroups serialize (about 0.1 us each here),
 // so there is no shared counter: every polled word has a few readers and one
 // writer.
-template <class Form>
+template <class Form, bool kPerWave>
 __global__ __launch_bounds__(kApplyThreads) __attribute__((amdgpu_waves_per_eu(Form::kWavesPerEu)))
 void append_validated_kernel(typename Form::Args a) {
   __shared__ int32_t s_ip[kValidateLdsBatch + 1], s_last[kValidateLdsBatch];
   __shared__ uint32_t s_or[kValidateThreads / 64];
-  __shared__ typename Form::Angles s_angles;
+  __shared__ typename Form::Angles s_angles[kPerWave ? kApplyThreads / 64 : 1];
   __shared__ int s_bad;
   const int tid = threadIdx.x;
   const WsLayout w = ws_layout(a.ws);
@@ -869,8 +933,11 @@ void append_validated_kernel(typename Form::Args a) {
     return;
   }
 
-  // token workgroup t
-  const int t = blockIdx.x - a.validate_blocks;
+  // token workgroup: of one token, or of one per wave (past the last: none)
+  const int wg = blockIdx.x - a.validate_blocks;
+  const int wave = kPerWave ? tid >> 6 : 0, lane = kPerWave ? tid & 63 : tid;
+  const int own = kPerWave ? wg * (kApplyThreads / 64) + wave : wg;
+  const int t = kPerWave ? min(own, a.tokens - 1) : own;
   // The token's own slot and position (the validation chunks check the same
   // walk; nothing is written unless they all pass).
   int r = 0, pos = 0, off = 0;
@@ -885,11 +952,16 @@ void append_validated_kernel(typename Form::Args a) {
   // Row loads after the walk: the validation's dependent loads run while the
   // memory system is not yet flooded with the command's row traffic, and the
   // rows still arrive before the verdicts.
-  const RowSlices first = load_first_slices(a, t, tid);
+  const auto first = [&] {
+    if constexpr (kPerWave)
+      return load_wave_slices(a, t, lane);
+    else
+      return load_first_slices(a, t, tid);
+  }();
   const typename Form::Weights w8 = Form::weights(a, tid & 15);
-  Form::sincos(a, pos, tid, s_angles);
-  if (tid < 64) {  // wave 0 polls copy t % kSignalCopies
-    const uint64_t *copy = w.signals + (t % kSignalCopies) * kMaxValidateBlocks;
+  Form::sincos(a, pos, lane, s_angles[wave]);
+  if (tid < 64) {  // wave 0 polls copy wg % kSignalCopies
+    const uint64_t *copy = w.signals + (wg % kSignalCopies) * kMaxValidateBlocks;
     int polls = 0, ready = 0, valid = 0;
     while (polls < a.poll_limit) {
       int mine_ready = 1, mine_valid = 1;
@@ -910,7 +982,11 @@ void append_validated_kernel(typename Form::Args a) {
     }
   }
   __syncthreads();
-  if (!s_bad) apply_token<Form>(a, t, page, off, tid, s_angles, w8, first);
+  if (s_bad || own >= a.tokens) return;
+  if constexpr (kPerWave)
+    apply_token_wave<Form>(a, t, page, off, lane, s_angles[wave], w8, first);
+  else
+    apply_token<Form>(a, t, page, off, tid, s_angles[0], w8, first);
 }
 
 // Two-launch form (plan flag LOOM_PLAN_APPEND_TWO_LAUNCH), for callers that
@@ -1059,6 +1135,7 @@ struct loom_rope_append_plan {
   bool normed = false;  // a plan of loom_rope_provider_plan_norm_paged_append
   float norm_eps = 0;   // 0: no norms
   double inv_freq64[64];
+  int cus = 0;  // of the device (normed plans)
 };
 
 extern "C" {
@@ -1171,11 +1248,13 @@ loom_status_t loom_rope_provider_plan_norm_paged_append(const loom_rope_provider
                                                         loom_error_t *err) {
   if (!provider || !spec || !out) return fail(err, LOOM_NULL_ARGUMENT, "provider");
   loom_norm_rope_append_spec_t s;  // a spec that spec_new would refuse is refused here too
-  const loom_status_t rc =
+  loom_status_t rc =
       loom_norm_rope_append_spec_new(&spec->paged, spec->tokens, spec->explicit_tokens,
                                      spec->rope_theta, spec->norm_eps, &s, err);
   if (rc) return rc;
-  return make_plan(s.paged, s.tokens, s.explicit_tokens != 0, flags, out, err, &s);
+  rc = make_plan(s.paged, s.tokens, s.explicit_tokens != 0, flags, out, err, &s);
+  if (!rc) (*out)->cus = provider->dev.cus;
+  return rc;
 }
 
 void loom_rope_append_plan_free(loom_rope_append_plan_t *p) { delete p; }
@@ -1196,7 +1275,14 @@ constexpr int kAppendOperands = 17;
 // The kernels of one form.  Commands of at most kFusedMaxTokens tokens and
 // kFusedMaxIndices page indices: one launch in which every workgroup validates.
 // Others: the validation workgroups first, then one per token (the plan's bounds
-// keep both within the workspace layout), or the two-launch form.
+// keep both within the workspace layout), or the two-launch form.  A normed
+// command of more tokens than the chip holds workgroups gives each wave a token
+// instead: with one per workgroup the metadata walk, the angles (one wave of four)
+// and the wait for the verdicts are paid once per round of workgroups (8192 tokens
+// of 64 + 8 heads, MXFP4 pages, with their read-back: 101 us, here 81; 2048 of
+// 32 + 8: 23.2 and 18.7; BF16 pages 14.8 and 12.4), while below it a wave alone has
+// more rows to go through (500 tokens of 32 + 8: 14.4 us, 12.2 with a workgroup
+// each).
 template <class Form>
 loom_status_t launch_append(const loom_rope_append_plan_t *plan, loom_command_scope_t *scope,
                             const typename Form::Args &a, loom_error_t *err) {
@@ -1220,7 +1306,17 @@ loom_status_t launch_append(const loom_rope_append_plan_t *plan, loom_command_sc
     }
     return loom::record_launch(scope, e, err);
   }
-  hipLaunchKernelGGL(append_validated_kernel<Form>, dim3((unsigned)grid), threads, 0, stream, a);
+  if constexpr (std::is_same_v<typename Form::Args, NormAppendArgs>) {
+    if (a.tokens >= Form::kWavesPerEu * plan->cus) {
+      const int waves = kApplyThreads / 64;
+      hipLaunchKernelGGL((append_validated_kernel<Form, true>),
+                         dim3((unsigned)(a.validate_blocks + (a.tokens + waves - 1) / waves)),
+                         threads, 0, stream, a);
+      return loom::record_launch(scope, hipGetLastError(), err);
+    }
+  }
+  hipLaunchKernelGGL((append_validated_kernel<Form, false>), dim3((unsigned)grid), threads, 0,
+                     stream, a);
   return loom::record_launch(scope, hipGetLastError(), err);
 }
 

@@ -186,6 +186,42 @@ def test_append_matches_64_bits(env, shape, dtype, norm):
     a.check(a.run(workspace=shape % 2 == 0))
 
 
+@pytest.mark.parametrize("norm", [True, False])
+@pytest.mark.parametrize("dtype", ["mxfp4", "bf16", "fp8_e4m3"])
+@pytest.mark.parametrize("heads", [(1, 1), (6, 3), (28, 4), (40, 10)])
+def test_commands_of_many_tokens(env, heads, dtype, norm):
+    """A token per wave: heads that do not fill a wave's 4 rows, a last workgroup that is
+    not full, the one-launch and the two-launch form alike."""
+    rows = [700, 1, 699, 33]
+    a = Append(env, 60, [711, 5, 699, 90], rows, *heads, dtype=dtype, norm=norm)
+    got = a.run()
+    a.check(got)
+    if heads == (6, 3):
+        two = a.run(flags=env[1].PLAN_APPEND_TWO_LAUNCH)
+        assert all(np.array_equal(got[k], two[k]) for k in got)
+
+
+@pytest.mark.parametrize("dtype", ["mxfp4", "bf16"])
+def test_many_tokens_of_many_requests(env, dtype):
+    rng = np.random.default_rng(61)
+    lens = [int(n) for n in rng.integers(1, 40, 1501)]
+    a = Append(env, 62, lens, [1] * 1501, 4, 1, dtype=dtype, explicit=False)
+    a.check(a.run())
+
+
+@pytest.mark.parametrize("dtype", ["mxfp4", "bf16"])
+def test_many_tokens_with_one_slot_twice_write_nothing(env, dtype):
+    a = Append(env, 63, [800, 700], [800, 700], 4, 2, 32, dtype=dtype)
+
+    def twice(x):
+        x["positions"][1499] = x["positions"][802]
+    for change in (twice, lambda x: x["positions"].__setitem__(3, 800)):
+        got = a.run(change=change)
+        assert (mx.bf16_values(got["query_output"]) == 7.0).all()
+        assert np.array_equal(got["key_pages"], a.pages[0])
+        assert np.array_equal(got["value_pages"], a.pages[1])
+
+
 @pytest.mark.parametrize("dtype", ["mxfp4", "bf16"])
 @pytest.mark.parametrize("batch", [1, 6, 100])
 def test_one_token_per_request(env, batch, dtype):
