@@ -83,6 +83,9 @@ struct loom_command_queue {
   bool shares_used = false;  // by some command of this queue
   uint8_t *zeroed = nullptr;
   uint64_t zeroed_bytes = 0;
+  // Arrival words of direct MXFP4 decode's splits (kMx4Joins), behind `zeroed`, zero
+  // between commands: the last workgroup to arrive clears its word.
+  uint32_t *joins = nullptr;
   std::vector<void *> retired;
   // Device-written status words in pinned, mapped host memory (kStatusWords).
   // A kernel that could not finish a command as specified (see DeviceStatus)
@@ -158,6 +161,9 @@ enum DeviceStatus : int {
   kStatusAppendRefused = 2,
   kStatusWords = 4
 };
+// Arrival words of a queue.
+constexpr uint64_t kMx4Joins = 256;
+
 // Bytes of the append validation workspace (one size for every plan).
 uint64_t append_workspace_bytes();
 // Reads and reports the queue's device status words (0 when all are clear);

@@ -21,7 +21,10 @@ struct Mx4DecodeArgs {
   // (-1: batch rejected) and header[1 + r] = virtual block prefix of request r
   // (r = 0..B); then the split states [slot][Hq][kMx4StateStride].
   int64_t *__restrict__ header;
-  float *__restrict__ states;
+  float *states;
+  // direct with splits: the queue's word of each (request, kv-heads, tile), zero between
+  // commands
+  uint32_t *arrived;
   int64_t pool;
   int64_t n_indices;
   int64_t page_bytes;  // P * Hkv * 64

@@ -1698,6 +1698,7 @@ loom_status_t paged_decode_enqueue_impl(const loom_paged_decode_plan_t *plan,
     m.lse = (float *)l(7)->ptr;
     m.header = (int64_t *)ws;
     m.states = (float *)(ws + pi.header_bytes);
+    m.arrived = scope->queue->joins;
     m.pool = (int64_t)s.max_num_pages;
     m.n_indices = (int64_t)l(4)->numel;
     m.indices_capacity = (pi.flags & LOOM_PLAN_PAGE_INDICES_CAPACITY) ? 1 : 0;

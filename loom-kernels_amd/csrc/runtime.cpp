@@ -203,9 +203,9 @@ int32_t settle(loom_command_completion *c, int32_t *sync_error) {
 
 
 // The queue's device status words (pinned, mapped host memory, zeroed), its
-// share states and its append validation workspace (zero-filled by a kernel on
-// the queue's stream, so every later command on the queue sees it zero), both in
-// one piece of device memory.
+// share states, its append validation workspace and its arrival words (these two
+// zero-filled by a kernel on the queue's stream, so every later command on the queue
+// sees them zero), all in one piece of device memory.
 loom_status_t init_queue_memory(loom_command_queue *q, loom_error_t *err) {
   hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
   hipError_t e = hipStreamIsCapturing(q->stream, &cap);
@@ -224,10 +224,11 @@ loom_status_t init_queue_memory(loom_command_queue *q, loom_error_t *err) {
     e = hipHostGetDevicePointer(&d, h, 0);
   }
   static_assert(loom::kShareBytes % 256 == 0, "the workspace behind it stays aligned");
-  if (e == hipSuccess) e = hipMalloc(&w, loom::kShareBytes + ws_bytes);
+  const uint64_t join_bytes = loom::kMx4Joins * 4;
+  if (e == hipSuccess) e = hipMalloc(&w, loom::kShareBytes + ws_bytes + join_bytes);
   uint8_t *ws = w ? (uint8_t *)w + loom::kShareBytes : nullptr;
   if (e == hipSuccess) {
-    const uint64_t words = ws_bytes / 4;
+    const uint64_t words = (ws_bytes + join_bytes) / 4;
     hipLaunchKernelGGL(loom::zero_words_kernel,
                        dim3((unsigned)std::min<uint64_t>((words + 255) / 256, 1024)), dim3(256), 0,
                        q->stream, (uint32_t *)ws, words);
@@ -239,6 +240,7 @@ loom_status_t init_queue_memory(loom_command_queue *q, loom_error_t *err) {
   q->shares = (uint8_t *)w;
   q->zeroed = ws;
   q->zeroed_bytes = w ? ws_bytes : 0;
+  q->joins = ws ? (uint32_t *)(ws + ws_bytes) : nullptr;
   if (e != hipSuccess) return fail(err, LOOM_CMD_DRIVER, "queue memory", 0, 0, 0, 0, 0.0, e);
   return LOOM_OK;
 }

@@ -298,6 +298,85 @@ def test_invalid_tables_write_nothing(env, teams):
     assert (out[0] == 7.0).all() and np.isfinite(out[1]).all() and (out[1] != 7.0).any()
 
 
+SPLIT = [
+    # lens, hq, hkv, page, layout: plans that split every request over 4 to 64 workgroups
+    ([900], 32, 8, 16, "NHD"),
+    ([1500, 1, 1000], 28, 4, 32, "HND"),
+    ([40000], 4, 1, 64, "NHD"),
+    ([70000], 22, 2, 64, "HND"),
+    ([11000], 32, 32, 16, "NHD"),  # two kv-heads per workgroup
+]
+
+
+@pytest.mark.parametrize("shape", range(len(SPLIT)))
+def test_split_requests_on_one_queue(env, shape):
+    """Commands one after another on one queue, whose arrival words each leaves zero: a
+    valid one, one with an invalid page index in one split, one of another plan, and the
+    first again, in one scope and in a graph that is replayed."""
+    torch, L = env
+    c = Case(torch, 90 + shape, *SPLIT[shape])
+    other = Case(torch, 95, [1000, 950], 8, 2)
+    bad = c.device()
+    bad[6][len(c.indices) // 3] = c.pool
+    commands = [(c, c.device()), (c, bad), (other, other.device()), (c, c.device())]
+    plans = {}
+    for case in (c, other):
+        spec = L.Bf16PagedBatchDecodeSpec(len(case.lens), case.pool, case.hq, case.hkv,
+                                          kv_layout=case.layout, kv_dtype="mxfp4",
+                                          kv_page_size=case.page)
+        plans[case] = L.DecodeProvider.load(0).plan_bf16_paged_batch(spec)
+        assert plans[case].algorithm == "direct" and plans[case].workspace_bytes > 256
+    outs = [(torch.empty(case.q.size, dtype=torch.bfloat16, device="cuda"),
+             torch.empty(case.q.size // mx.D, device="cuda")) for case, _ in commands]
+
+    def enqueue(b, scope, handles):
+        for (case, _), h in zip(commands, handles):
+            plans[case].enqueue_into(scope, L.Mxfp4PagedBatchDecodeArgs(
+                *h[:8], h[8].write(), h[9].write()))
+
+    def bind(b):
+        return [[b.bind_read(t) for t in x] + [b.bind_read_write(t) for t in o]
+                for (_, x), o in zip(commands, outs)]
+
+    def fill():
+        for o in outs:
+            for t in o:
+                t.fill_(7.0)
+        torch.cuda.synchronize()
+
+    def verify(want=[]):
+        got = []
+        for (case, x), (o, l) in zip(commands, outs):
+            shape = (len(case.lens), case.hq)
+            o, l = host_bf16(torch, o).reshape(*shape, mx.D), l.cpu().numpy().reshape(shape)
+            if x is bad:
+                assert (o[0] == 7.0).all() and (l[0] == 7.0).all()
+            elif not want:
+                check(case, o, l)
+            got.append((o, l))
+        want[:] = want or got
+        assert all(np.array_equal(a, b) for g, w in zip(got, want) for a, b in zip(g, w))
+
+    queue = L.CommandQueue(torch.cuda.current_stream(), 8)
+    b = queue.bindings(48)
+    h = bind(b)
+    fill()
+    scope = queue.begin(b)
+    enqueue(b, scope, h)
+    scope.finish().wait()
+    verify()
+    gq = L.GraphQueue(0, 8)
+    gq.reserve_workspace(max(p.workspace_bytes for p in plans.values()))
+    b = gq.bindings(48)
+    h = bind(b)
+    fill()
+    graph = gq.capture(b, lambda s: enqueue(b, s, h)).instantiate()
+    for _ in range(3):
+        graph.launch().wait()
+        verify()
+        fill()
+
+
 def test_capacity_table_in_a_graph(env):
     """One captured command over a capacity table, replayed as the table grows, with
     eager work between the replays."""
