@@ -1027,13 +1027,14 @@ constexpr uint64_t kDirectRows = 1u << 20;
 // 2048 19.0 / 17.0; 64 x 256-1024 20.3 / 17.6; 1 x 32000 14.6 / 17.4; 4 x 8000 14.7 /
 // 16.7.
 constexpr uint64_t kDirectPairRows = 5u << 16;
-// Workgroups per (request, kv-heads, tile).  None are split below kSplitFrom blocks a
-// request: the join costs 2.5 us (one request of 200 tokens 5.8 us, in two 7.9; of 700,
-// 8.3 and in four 8.7; of 1000, 9.1 and in eight 8.3).  From there the walk shrinks with
-// the splits and the join grows, so they are doubled while their square stays within twice
-// the blocks and the CUs hold them (4000 tokens in 8, 16, 32: 10.3, 9.8, 11.4 us; 32000:
-// 28.6, 18.6, 16.7; two per CU: no faster).
-constexpr uint64_t kMaxSplits = 64, kSplitFrom = 28;
+// Workgroups per (request, kv-heads, tile), of 8 waves each (16 were slower at every
+// size).  The walk shrinks with the splits and the join grows, so they are doubled while
+// their square stays within twice a request's blocks and the CUs hold them (4000 tokens in
+// 8, 16, 32: 10.3, 9.8, 11.4 us; 32000: 28.6, 18.6, 16.7; two per CU: no faster).  A join
+// costs 2.5 us, a wave's block about 1: splits that save less than kSplitFrom / 8 blocks a
+// wave are left out (one request of 200 tokens 5.8 us, in two 7.9; of 1000, 9.1 and in
+// eight 8.3; 16 of 1000, 11.4 and in two 14.0).
+constexpr uint64_t kMaxSplits = 64, kSplitFrom = 21;
 
 loom_status_t plan_mx4_decode(loom_paged_decode_plan_info_t *info, uint32_t teams_option, int cus,
                               loom_error_t *err) {
@@ -1060,8 +1061,9 @@ loom_status_t plan_mx4_decode(loom_paged_decode_plan_info_t *info, uint32_t team
     uint64_t splits = 1;
     const uint64_t each = blocks / B;
     while (heads <= kMx4Joins && splits < kMaxSplits && heads * splits * 2 <= (uint64_t)cus &&
-           each >= kSplitFrom && each >= 2 * splits * splits)
+           each >= 2 * splits * splits)
       splits *= 2;
+    if (each * (splits - 1) < kSplitFrom * splits) splits = 1;
     const uint64_t grid = heads * splits;
     if (grid > (uint64_t)INT32_MAX || B * hq > (uint64_t)INT32_MAX)
       return fail(err, LOOM_PLAN_STATE_COUNT_OUT_OF_RANGE, "paged batch-decode", grid);
