@@ -437,7 +437,11 @@ typedef enum loom_paged_decode_algorithm {
    * few such workgroups would stream long requests (max_total_pages / B >=
    * 16 and at most 2 * CUs workgroups after splitting), each request's pages
    * split over 2-8 workgroups of 4 waves (plan info `teams`), whose states a
-   * second kernel merges. */
+   * second kernel merges.
+   * MXFP4 plans (teams option 0) take it for up to 2^20 K rows (max_total_pages *
+   * page size * Hkv): workgroups of 8 waves per (request, one or two kv-heads,
+   * tile), long requests split over up to 64 of them, the last of which to finish
+   * merges their states in the same launch. */
   LOOM_PAGED_DECODE_DIRECT = 2
 } loom_paged_decode_algorithm_t;
 
@@ -453,7 +457,8 @@ typedef enum loom_paged_decode_algorithm {
 typedef struct loom_paged_decode_plan_options {
   uint64_t max_total_pages; /* upper bound of page_indices length; 0 -> max_num_pages */
   uint32_t teams;           /* page ranges; 0 -> chosen for the device (or the direct
-                               algorithm when max_total_pages <= 128) */
+                               algorithm when max_total_pages <= 128; MXFP4: up to
+                               2^20 K rows) */
   uint32_t flags;           /* 0 or LOOM_PLAN_PAGE_INDICES_CAPACITY */
 } loom_paged_decode_plan_options_t;
 
@@ -467,7 +472,8 @@ typedef struct loom_paged_decode_plan_info {
   uint64_t max_total_pages;
   uint64_t state_slots;      /* balanced: teams + batch; split direct: teams * batch */
   uint64_t workspace_bytes;  /* header_bytes + state_slots * Hq * 132 FP32 */
-  uint64_t header_bytes;     /* (batch + 2) int64 page prefixes, 256-byte rounded */
+  uint64_t header_bytes;     /* (batch + 2) int64 page prefixes, 256-byte rounded; split
+                                direct MXFP4 plans: 256 arrival words */
   uint32_t block_threads;
   uint32_t grid_blocks;
   uint32_t device_cus;

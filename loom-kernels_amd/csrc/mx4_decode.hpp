@@ -17,13 +17,14 @@ struct Mx4DecodeArgs {
   const int32_t *__restrict__ last;
   uint16_t *__restrict__ out;
   float *__restrict__ lse;
-  // Workspace: balanced plans first keep header[0] = blocks in the virtual list
+  // Workspace: split direct plans first keep kMx4Joins arrival words (used where the
+  // queue's may not be); balanced plans first keep header[0] = blocks in the virtual list
   // (-1: batch rejected) and header[1 + r] = virtual block prefix of request r
   // (r = 0..B); then the split states [slot][Hq][kMx4StateStride].
   int64_t *__restrict__ header;
   float *states;
-  // direct with splits: the queue's word of each (request, kv-heads, tile), zero between
-  // commands
+  // Direct with splits: the word of each (request, kv-heads, tile) at which its
+  // workgroups count themselves, zero before the launch and after it.
   uint32_t *arrived;
   int64_t pool;
   int64_t n_indices;
@@ -50,8 +51,8 @@ constexpr int kMx4StateStride = 132;
 // max_total_pages and flags are set; `teams_option` as in the plan options.
 loom_status_t plan_mx4_decode(loom_paged_decode_plan_info_t *info, uint32_t teams_option, int cus,
                               loom_error_t *err);
-// Launches the command's kernels.
+// Launches the command's kernels; `clear`: the arrival words first.
 hipError_t launch_mx4_decode(const loom_paged_decode_plan_info_t &info, const Mx4DecodeArgs &args,
-                             hipStream_t stream);
+                             bool clear, hipStream_t stream);
 
 }  // namespace loom

@@ -1698,7 +1698,6 @@ loom_status_t paged_decode_enqueue_impl(const loom_paged_decode_plan_t *plan,
     m.lse = (float *)l(7)->ptr;
     m.header = (int64_t *)ws;
     m.states = (float *)(ws + pi.header_bytes);
-    m.arrived = scope->queue->joins;
     m.pool = (int64_t)s.max_num_pages;
     m.n_indices = (int64_t)l(4)->numel;
     m.indices_capacity = (pi.flags & LOOM_PLAN_PAGE_INDICES_CAPACITY) ? 1 : 0;
@@ -1716,7 +1715,13 @@ loom_status_t paged_decode_enqueue_impl(const loom_paged_decode_plan_t *plan,
     m.row_bytes = head_major ? 64 : m.hkv * 64;
     m.page_bytes = (int64_t)m.page_rows * m.hkv * 64;
     m.scale_log2 = s.softmax_scale * 1.44269504088896340736f;
-    return loom::record_launch(scope, loom::launch_mx4_decode(pi, m, scope->queue->stream), err);
+    // A command that the caller captures into a graph of its own is not in the
+    // queue's order: its arrival words are the workspace's, cleared by every replay.
+    m.arrived = m.splits > 1 ? loom::queue_joins(scope) : nullptr;
+    const bool clear = m.splits > 1 && !m.arrived;
+    if (clear) m.arrived = (uint32_t *)ws;
+    return loom::record_launch(
+        scope, loom::launch_mx4_decode(pi, m, clear, scope->queue->stream), err);
   }
   DecodeArgs a{};
   a.kv_scales = fp8 ? (const float *)l(9)->ptr : nullptr;

@@ -1009,6 +1009,8 @@ __global__ __launch_bounds__(kDirectWaves * 64) void mx4_decode_direct_kernel(Mx
   if (a.splits > 1) arrive();
 }
 
+__global__ void mx4_decode_clear_kernel(uint32_t *arrived) { arrived[threadIdx.x] = 0u; }
+
 // kv-heads per wave: two neighbours where Hkv is even, in the balanced kernel always.
 uint64_t heads_per_wave(uint64_t hkv) { return hkv % 2 == 0 ? 2 : 1; }
 
@@ -1070,7 +1072,9 @@ loom_status_t plan_mx4_decode(loom_paged_decode_plan_info_t *info, uint32_t team
     info->algorithm = LOOM_PAGED_DECODE_DIRECT;
     info->teams = (uint32_t)(splits > 1 ? splits : 0);
     info->state_slots = splits > 1 ? splits * B : 0;
-    info->workspace_bytes = splits > 1 ? splits * B * hq * kMx4StateStride * 4 : 256;
+    info->header_bytes = splits > 1 ? kMx4Joins * 4 : 0;
+    info->workspace_bytes =
+        splits > 1 ? info->header_bytes + splits * B * hq * kMx4StateStride * 4 : 256;
     info->block_threads = kDirectWaves * 64;
     info->grid_blocks = (uint32_t)grid;
     return LOOM_OK;
@@ -1094,7 +1098,7 @@ loom_status_t plan_mx4_decode(loom_paged_decode_plan_info_t *info, uint32_t team
 }
 
 hipError_t launch_mx4_decode(const loom_paged_decode_plan_info_t &info, const Mx4DecodeArgs &a,
-                             hipStream_t stream) {
+                             bool clear, hipStream_t stream) {
   const bool p16 = a.page_rows == 16;
   const dim3 grid(info.grid_blocks);
   if (info.algorithm == LOOM_PAGED_DECODE_DIRECT) {
@@ -1106,6 +1110,11 @@ hipError_t launch_mx4_decode(const loom_paged_decode_plan_info_t &info, const Mx
                              : mx4_decode_direct_kernel<false, 2, kPair>)
                       : (p16 ? mx4_decode_direct_kernel<true, 1, kSplit>
                              : mx4_decode_direct_kernel<false, 1, kSplit>);
+    if (clear) {
+      hipLaunchKernelGGL(mx4_decode_clear_kernel, dim3(1), dim3(kMx4Joins), 0, stream, a.arrived);
+      const hipError_t e = hipGetLastError();
+      if (e != hipSuccess) return e;
+    }
     hipLaunchKernelGGL(kernel, grid, dim3(info.block_threads), 0, stream, a);
     return hipGetLastError();
   }

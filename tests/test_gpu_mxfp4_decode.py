@@ -377,6 +377,50 @@ def test_split_requests_on_one_queue(env, shape):
         fill()
 
 
+def test_split_command_in_a_callers_capture(env):
+    """Captured by the caller into a graph of its own, whose replays the queue does not
+    order, a split command counts its workgroups in its workspace, which may hold
+    anything; the queue's own commands go on between the replays."""
+    torch, L = env
+    c = Case(torch, 96, [900, 1300], 8, 2)
+    x = c.device()
+    spec = L.Bf16PagedBatchDecodeSpec(2, c.pool, 8, 2, kv_dtype="mxfp4")
+    plan = L.DecodeProvider.load(0).plan_bf16_paged_batch(spec)
+    assert plan.algorithm == "direct" and plan.workspace_bytes > 256
+    stream = torch.cuda.Stream()
+    outs = [(torch.empty(c.q.size, dtype=torch.bfloat16, device="cuda"),
+             torch.empty(c.q.size // mx.D, device="cuda")) for _ in range(2)]
+    works = [torch.full((plan.workspace_bytes,), 0xFF, dtype=torch.uint8, device="cuda")
+             for _ in range(2)]
+    queues = [L.CommandQueue(stream, 4) for _ in range(2)]
+    torch.cuda.synchronize()
+
+    def bind(i):
+        b = queues[i].bindings(11)
+        h = [b.bind_read(t) for t in x] + [b.bind_read_write(t).write()
+                                           for t in (*outs[i], works[i])]
+        return b, L.Mxfp4PagedBatchDecodeArgs(*h)
+    b, args = bind(0)
+    scope = queues[0].begin(b)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream, capture_error_mode="thread_local"):
+        plan.enqueue_into(scope, args)
+    scope.finish().wait()
+    for _ in range(3):
+        for t in (*outs[0], *outs[1]):
+            t.fill_(float("nan"))
+        works[0].random_(0, 256)
+        torch.cuda.synchronize()
+        graph.replay()
+        b, args = bind(1)
+        scope = queues[1].begin(b)
+        plan.enqueue_into(scope, args)
+        scope.finish().wait()
+        torch.cuda.synchronize()
+        for o, l in outs:
+            check(c, host_bf16(torch, o).reshape(2, 8, mx.D), l.cpu().numpy().reshape(2, 8))
+
+
 def test_capacity_table_in_a_graph(env):
     """One captured command over a capacity table, replayed as the table grows, with
     eager work between the replays."""
