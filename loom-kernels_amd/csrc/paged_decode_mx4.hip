@@ -3,16 +3,17 @@
 //
 // Per query head: S = q.k / sqrt(128), O = softmax(S).V, LSE in log2, over the values
 // code * 2^(scale - 127) of the request's tokens.  A token costs 136 bytes per kv-head
-// where BF16 pages cost 512, so the arithmetic per byte is four times as dense and the
-// instructions of a step, not its bytes, come close to binding.  The step is built
-// for few of them:
-//   * 32 tokens at a time.  K codes are loaded as the MFMA fragment wants them: lane
-//     (col, quad) takes the 16 bytes of dims 32 quad + [0, 32) of row col, one scale
-//     block, and v_cvt_scalef32_pk_bf16_fp4 widens two codes and applies the block's
-//     scale in one instruction, exactly.  No LDS.  (v_mfma_scale_f32_16x16x128_f8f6f4
-//     takes FP4 itself, but sums its 128 products with errors up to 2^-12 of the
-//     largest, which LSE does not bear.)
-//   * V codes come as 8 dims from 8 col on of rows 4 quad + j; one byte permute per
+// where BF16 pages cost 512, so the arithmetic per byte is four times as dense: a block
+// of 32 tokens and one kv-head takes a wave about 375 ns of instructions (VALU busy half
+// of the balanced kernel's time).  The step is built for few of them:
+//   * 32 tokens at a time, codes and scales loaded straight into LDS, nothing held in
+//     registers in flight.  K is read as the MFMA fragment wants it: lane (col, quad)
+//     takes the 16 bytes of dims 32 quad + [0, 32) of a row, one scale block, and
+//     v_cvt_scalef32_pk_bf16_fp4 widens two codes and applies the block's scale in one
+//     instruction, exactly.  (v_mfma_scale_f32_16x16x128_f8f6f4 takes FP4 itself, but
+//     sums its 128 products with errors up to 2^-12 of the largest, which LSE does not
+//     bear.)
+//   * V codes come as 8 dims from 8 col on of rows 4 j + quad; one byte permute per
 //     two tokens turns the widened pairs into the V^T fragment.
 //   * The running bound of the scores is set kLazy above a new maximum and moves only
 //     when a score passes it: the common step has no reduction across lanes and no
@@ -24,11 +25,15 @@
 //
 // Two decompositions, both independent of the page table's contents:
 //   balanced  the 32-token blocks of all valid requests form one virtual list, cut
-//             into `teams` equal ranges; a team is one wave per (kv-head, tile), all
+//             into `teams` equal ranges; a team is one wave per (kv-heads, tile), all
 //             walking the same blocks.  Requests that cross a range leave states, which
-//             a second kernel merges.
-//   direct    one workgroup per (request, kv-head, tile[, split]): its waves take the
-//             blocks in turn and merge in LDS.  One launch, or a merge of the splits.
+//             a second kernel merges.  Bound by memory: 64 requests of 512-8192 tokens
+//             (32 / 8 heads, 254 MB) 52.0 us, 47.6 without the merge (5.3 TB/s; a large
+//             copy reaches 5.1); 8 of 32768 (64 / 8, 286 MB) 57 us.
+//   direct    one workgroup per (request, kv-heads, tile[, split]): its waves take the
+//             blocks in turn and merge in LDS, the last split of a request the splits.
+//             One launch.  Bound by latency: one request of 200 tokens 5.8 us, 16 of
+//             256-1536 13.4 (32 / 8 heads), 5 of 1-5003 (28 / 4) 10.3.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -58,20 +63,13 @@ constexpr int kMaxBatch = 65536;
 constexpr float kLazy = 8.0f;
 // Normalizer written into a state whose pages failed the guard.
 constexpr float kPoisonNormalizer = -1.0f;
-#ifndef LOOM_MX4_DEPTH
-#define LOOM_MX4_DEPTH 2
-#endif
-#ifndef LOOM_MX4_WAVES_PER_EU
-#define LOOM_MX4_WAVES_PER_EU 2
-#endif
-#ifndef LOOM_MX4_WAVES_PER_4CU
-#define LOOM_MX4_WAVES_PER_4CU 16
-#endif
-#ifndef LOOM_MX4_MIN_TEAM_BLOCKS
-#define LOOM_MX4_MIN_TEAM_BLOCKS 2
-#endif
-constexpr int kMinTeamBlocks = LOOM_MX4_MIN_TEAM_BLOCKS;
-constexpr int kDepth = LOOM_MX4_DEPTH;  // blocks in flight per wave
+// Fewest blocks of a team (a state costs its write and its merge).
+constexpr int kMinTeamBlocks = 2;
+// Balanced kernel: blocks in flight per wave, and waves per four CUs; one wave per SIMD.
+// Three in flight, or more waves, were slower: the pages' order in memory sets the rate,
+// and streams that many in number or that far ahead of each other spoil it.
+constexpr int kDepth = 2;
+constexpr int kWavesPer4Cu = 16;
 
 // decode.rs:233-246: indptr[B] is the page_indices length (at most that length for
 // capacity plans).
@@ -121,8 +119,8 @@ struct Ranges {
 //   kSplit  per head 64-byte rows: HND pages, and single heads.  Lane l takes piece
 //           (l & 3) ^ (l >> 4) of row l >> 2 of a half (16 rows).
 //   kPair   128-byte rows of two neighbouring heads: NHD pages, whose rows hold them side
-//           by side; 64-byte loads of half a cache line each ran at 4.5 TB/s where these
-//           reach 5.7 (8 requests of 32768 tokens).  Lane l takes piece
+//           by side: 64-byte loads take half a cache line each, and every line twice
+//           (8 requests of 32768 tokens at 4.5 TB/s, so 5.7).  Lane l takes piece
 //           (l & 7) ^ pair_swizzle(row) of row l >> 3 of eight rows.
 // Either way the reads below, which take one 16-byte piece of all rows of a half or 64
 // bytes of every fourth row, meet each LDS bank once.  Scale word c of a half belongs to
@@ -505,7 +503,7 @@ __device__ __forceinline__ Blocks find_blocks(const Mx4DecodeArgs &a, const Smem
 
 // NH: kv-heads per wave; they divide Hkv.
 template <bool P16, int NH, int ARR>
-__global__ __launch_bounds__(kThreads, LOOM_MX4_WAVES_PER_EU) void mx4_decode_split_kernel(
+__global__ __launch_bounds__(kThreads, 2) void mx4_decode_split_kernel(
     Mx4DecodeArgs a) {
   __shared__ BalancedSmem<NH> sm;
   const int tid = threadIdx.x, lane = tid & 63;
@@ -814,7 +812,8 @@ __global__ __launch_bounds__(kThreads) void mx4_decode_merge_kernel(Mx4DecodeArg
 
 // ---- direct --------------------------------------------------------------------------
 // Wave w of the workgroup takes blocks w, w + W, ... of its split's share of the request,
-// two in flight; the wave states merge in LDS.
+// two in flight; the wave states merge in LDS.  (One request of 100 tokens: 5.2 us, of
+// 1000 without splits 9.1: a block in each of two waves of a SIMD, about 1 us.)
 constexpr int kDirectWaves = 8;
 constexpr int kStash = 132;  // floats between two columns' O in LDS
 
@@ -1080,7 +1079,7 @@ loom_status_t plan_mx4_decode(loom_paged_decode_plan_info_t *info, uint32_t team
     return LOOM_OK;
   }
   const uint64_t members = hkv / heads_per_wave(hkv) * tiles;
-  const uint64_t slots = (uint64_t)cus * LOOM_MX4_WAVES_PER_4CU / 4;
+  const uint64_t slots = (uint64_t)cus * kWavesPer4Cu / 4;
   const uint64_t teams = teams_option ? teams_option : std::max<uint64_t>(1, slots / members);
   // Each XCD (every 8th workgroup) holds ceil(teams / 8) whole teams.
   const uint64_t xcd_waves = (teams + 7) / 8 * members;

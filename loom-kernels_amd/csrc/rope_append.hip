@@ -510,6 +510,20 @@ __device__ __forceinline__ void apply_row(const AppendArgs &a, int t, int64_t pa
 }
 
 // ---- the normed append ----------------------------------------------------------
+//   y = x w / sqrt(mean(x^2) + eps) per head (optional), rotated by pos * theta^(-2j/128),
+// Q to BF16, K and V to their page slot as BF16, FP8 or MXFP4.  A row of 128 is 16 lanes'
+// 8 values, so its sum, its other half and its blocks' maxima are DPP steps and nothing
+// goes through LDS but the token's sines and cosines.
+//
+// Rounding: Q (and K for BF16 and FP8 pages) in FP32 with one rounding to the output; the
+// angle is a 64-bit product, since pos * inv_freq in FP32 loses the phase of far tokens.
+// K for MXFP4 pages is normed and rotated in 64 bits: a code is an eighth of a power of
+// two wide, and values near the border of two codes would otherwise go either way.
+//
+// Bound by memory in large commands: 8192 tokens of 64 + 8 heads into MXFP4 pages (311 MB)
+// 71 us, 4.4 TB/s, the VALU busy 58% of it (a fifth fewer instructions changed nothing);
+// into BF16 pages (335 MB) 68 us, 4.9 TB/s.  Small ones by the guards' chain: 64 tokens of
+// 32 + 8 heads 7.5 us, about 1000 11.7.
 // Row c ^ 8 of the same 16 lanes (a rotation by 8), and sums over the 16 lanes
 // and maxima over 4 of them (the lanes of one MXFP4 block), on DPP.
 __device__ __forceinline__ uint32_t dpp_other_half(uint32_t x) {

@@ -418,6 +418,48 @@ def test_read_back_guards(env):
     untouched(everything, change=put(4, 3, 10 ** 6))
 
 
+@pytest.mark.parametrize("layout", ["NHD", "HND"])
+def test_pages_past_32_bit_offsets(env, layout):
+    """Codes of 4.6 GB for K and for V: tokens appended to the last page and read back."""
+    torch, L = env
+    pool, page, hkv, lens = 140000, 64, 8, [70, 3]
+    codes = [torch.full((pool * page * hkv * 64,), 0x55, dtype=torch.uint8, device="cuda")
+             for _ in range(2)]
+    scales = [torch.full((pool * page * hkv * 4,), 99, dtype=torch.uint8, device="cuda")
+              for _ in range(2)]
+    rng = np.random.default_rng(64)
+    k, v = (mx.bf16_round(rng.standard_normal((73, hkv, mx.D))) for _ in range(2))
+    q = torch.zeros(73 * hkv * mx.D, dtype=torch.bfloat16, device="cuda")
+    table = [dev(torch, np.array(t, np.int32)) for t in
+             ([0, 2, 3], [pool - 2, pool - 3, pool - 1], [6, 3])]
+    form = dict(kv_layout=layout, kv_page_size=page, kv_dtype="mxfp4")
+    aplan = L.RopeProvider.load(0).plan_norm_paged_append(L.NormRopePagedKvAppendSpec(
+        73, 2, pool, hkv, hkv, rope_theta=THETA, **form))
+    rplan = L.PrefillProvider.load(0).plan_paged_kv_read(L.PagedKvReadSpec(2, 73, pool, hkv, **form))
+    queue = L.CommandQueue(torch.cuda.current_stream(), 4)
+    b = queue.bindings(24)
+    req, pos = np.repeat([0, 1], lens), np.concatenate([np.arange(n) for n in lens])
+    r = b.bind_read
+    hq, hk, hv, hr, hp, *ht, hkv_ = (r(t) for t in (
+        q, dev_bf16(torch, k).flatten(), dev_bf16(torch, v).flatten(),
+        dev(torch, req.astype(np.int32)), dev(torch, pos.astype(np.int32)), *table,
+        dev(torch, np.array([0, 70, 73], np.int32))))
+    pages = [b.bind_read_write(t) for t in (*codes, *scales)]
+    qo, ko, vo = (torch.zeros_like(q) for _ in range(3))
+    hqo, hko, hvo = (b.bind_read_write(t).write() for t in (qo, ko, vo))
+    scope = queue.begin(b)
+    aplan.enqueue_into(scope, L.NormRopePagedKvAppendArgs(
+        hq, hk, hv, *ht, hqo, pages[0].write(), pages[1].write(), hr, hp,
+        key_scales=pages[2].write(), value_scales=pages[3].write()))
+    rplan.enqueue_into(scope, L.PagedKvReadArgs(*(p.read() for p in pages), *ht, hkv_, hko, hvo))
+    scope.finish().wait()
+    for got, rows in ((ko, mx.norm_rotate(k, None, pos, EPS, THETA)), (vo, v)):
+        assert np.array_equal(host_bf16(torch, got).reshape(73, hkv, mx.D),
+                              mx.values(*mx.quantise(rows)))
+    for t in (*codes, *scales):  # nothing before those pages
+        assert (t[:1 << 20] == t[0]).all() and t[0] in (0x55, 99)
+
+
 # ---- together -------------------------------------------------------------------------
 def test_append_decode_and_read_back_in_one_graph(env):
     """A decode step over an MXFP4 cache as a captured graph (normed append, decode), its

@@ -205,6 +205,90 @@ def test_planned_forms(env, shape):
     check(c, out, lse)
 
 
+@pytest.mark.parametrize("teams", [0, 40])
+@pytest.mark.parametrize("shape", [
+    ([50, 3], 128, 1, 16, "NHD"),   # 16 tiles of 8 heads
+    ([70, 33], 17, 17, 32, "NHD"),  # an odd number of kv-heads: one per wave
+    ([41], 27, 3, 64, "HND"),       # 9 heads per kv-head: the second tile of one
+    ([600, 90], 64, 64, 16, "NHD"),
+])
+def test_head_layouts(env, shape, teams):
+    c = Case(env[0], 78, *shape)
+    out, lse, _ = run(env, c, {"teams": teams})
+    check(c, out, lse)
+
+
+def test_the_largest_batch(env):
+    """65536 requests of 1 to 40 tokens; one in 61 compared."""
+    rng = np.random.default_rng(79)
+    lens = [int(n) for n in rng.integers(1, 41, 65536)]
+    c = Case(env[0], 80, lens, 1, 1)
+    for opts in ({}, {"teams": 333}):
+        out, lse, _ = run(env, c, opts)
+        assert np.isfinite(out).all() and np.isfinite(lse).all()
+        part = Case.__new__(Case)
+        part.__dict__.update(c.__dict__)
+        some = list(range(0, 65536, 61)) + [65535]
+        part.lens, part.q = [lens[r] for r in some], c.q[some]
+        pages = [c.indices[c.indptr[r]:c.indptr[r + 1]] for r in some]
+        part.indptr = np.concatenate([[0], np.cumsum([len(p) for p in pages])]).astype(np.int32)
+        part.indices = np.concatenate(pages)
+        check(part, out[some], lse[some])
+
+
+def test_two_queues_at_once(env):
+    """Split commands of two queues on two streams, submitted without waiting."""
+    torch, L = env
+    cases = [Case(torch, 81, [1200, 900], 8, 2), Case(torch, 82, [2500], 32, 8, 32, "HND")]
+    torch.cuda.synchronize()
+    flight = []
+    for c in cases:
+        spec = L.Bf16PagedBatchDecodeSpec(len(c.lens), c.pool, c.hq, c.hkv, kv_layout=c.layout,
+                                          kv_dtype="mxfp4", kv_page_size=c.page)
+        plan = L.DecodeProvider.load(0).plan_bf16_paged_batch(spec)
+        assert plan.workspace_bytes > 256
+        queue = L.CommandQueue(torch.cuda.Stream(), 64)
+        queue.reserve_workspace(plan.workspace_bytes)
+        b = queue.bindings(10)
+        out = torch.full((spec.output_numel,), float("nan"), dtype=torch.bfloat16, device="cuda")
+        lse = torch.full((spec.lse_numel,), float("nan"), device="cuda")
+        torch.cuda.synchronize()
+        h = [b.bind_read(t) for t in c.device()] + [b.bind_read_write(t).write()
+                                                    for t in (out, lse)]
+        flight.append((c, plan, queue, queue.begin(b), L.Mxfp4PagedBatchDecodeArgs(*h), out, lse))
+    torch.cuda.synchronize()
+    for _ in range(50):
+        for _, plan, _, scope, args, _, _ in flight:
+            plan.enqueue_into(scope, args)
+    for _, _, _, scope, _, _, _ in flight:
+        scope.finish().wait()
+    for c, _, _, _, _, out, lse in flight:
+        shape = (len(c.lens), c.hq)
+        check(c, host_bf16(torch, out).reshape(*shape, mx.D), lse.cpu().numpy().reshape(shape))
+
+
+@pytest.mark.parametrize("layout", ["NHD", "HND"])
+def test_pages_past_32_bit_offsets(env, layout):
+    """Codes of 4.6 GB for K and for V, of which the last pages are in use."""
+    torch, L = env
+    c = Case(torch, 83, [100, 1], 16, 8, 64, layout)
+    x = c.device()
+    pool = 140000
+    for i, width in ((1, 64), (2, 64), (3, 4), (4, 4)):
+        size = 64 * 8 * width
+        big = torch.empty(pool * size, dtype=torch.uint8, device="cuda")
+        big[-c.pool * size:] = x[i]
+        x[i] = big
+    x[6] = x[6] + (pool - c.pool)
+    far = Case.__new__(Case)
+    far.__dict__.update(c.__dict__)
+    far.pool = pool
+    for teams in (0, 3):
+        out, lse, _ = run(env, far, {"teams": teams, "max_total_pages": len(c.indices)},
+                          operands=x)
+        check(c, out, lse)
+
+
 def test_results_repeat_bit_for_bit(env):
     c = Case(env[0], 7, [1000, 3, 517], 16, 4, 32, "HND")
     a, b = run(env, c), run(env, c, workspace=True)

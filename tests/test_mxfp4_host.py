@@ -1,6 +1,9 @@
 """CPU tests of the MXFP4 cache's contracts, and of the 64-bit forms that the GPU tests
 compare with."""
 import ctypes as C
+import os
+import re
+import subprocess
 
 import numpy as np
 import pytest
@@ -105,3 +108,23 @@ def test_bf16_rounding_of_the_tests():
     want = torch.from_numpy(x.astype(np.float32)).to(torch.bfloat16).double().numpy()
     assert np.array_equal(mx.bf16_round(x.astype(np.float32).astype(np.float64)), want)
     assert np.array_equal(mx.bf16_values(mx.bf16_bits(want)), want)
+
+
+def test_kernels_keep_out_of_scratch_memory(tmp_path):
+    """An array, or the argument struct, that a kernel indexes with a choice between two
+    fields would live in scratch memory: twice the time of a small append."""
+    from test_kernel_lds import LIB, READELF, code_objects
+    if not os.path.exists(READELF):
+        pytest.skip("no llvm-readelf")
+    seen = 0
+    for i, image in enumerate(code_objects(open(LIB, "rb").read())):
+        path = tmp_path / f"{i}.elf"
+        path.write_bytes(image)
+        notes = subprocess.run([READELF, "--notes", str(path)], check=True, capture_output=True,
+                               text=True).stdout
+        for k in re.split(r"^\s+- \.agpr_count", notes, flags=re.M)[1:]:
+            name = re.search(r"^ {4}\.name:\s+(\S+)", k, flags=re.M).group(1)
+            if re.search("mx4_decode|append|kv_read", name):
+                seen += 1
+                assert re.search(r"\.private_segment_fixed_size:\s+0$", k, flags=re.M), name
+    assert seen > 20
