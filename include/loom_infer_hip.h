@@ -1149,7 +1149,8 @@ loom_status_t loom_paged_kv_read_spec_new(const loom_paged_decode_spec_t *paged,
                                           loom_paged_kv_read_spec_t *out, loom_error_t *err);
 
 typedef struct loom_paged_kv_read_plan loom_paged_kv_read_plan_t;
-/* `flags`: 0 or LOOM_PLAN_PAGE_INDICES_CAPACITY. */
+/* `flags`: 0 or LOOM_PLAN_PAGE_INDICES_CAPACITY.  At most 4096 kv-heads
+ * (LOOM_PLAN_STATE_COUNT_OUT_OF_RANGE). */
 loom_status_t loom_prefill_provider_plan_paged_kv_read(const loom_prefill_provider_t *provider,
                                                        const loom_paged_kv_read_spec_t *spec,
                                                        uint32_t flags,

@@ -1037,6 +1037,19 @@ constexpr uint64_t kDirectPairRows = 5u << 16;
 // eight 8.3; 16 of 1000, 11.4 and in two 14.0).
 constexpr uint64_t kMaxSplits = 64, kSplitFrom = 21;
 
+// The merge kernel's workgroups and their waves per head: one up to 48 states per request
+// on average (64 ragged requests, 5: 52.1 us, with four waves 55.5; 8 of 32k, 33: 56.8 and
+// 57.6).
+struct MergeGrid {
+  uint64_t grid;
+  int parts;
+};
+static MergeGrid merge_grid(uint64_t batch, uint64_t hq, uint64_t teams) {
+  const int parts = teams / batch >= 48 ? kWaves : 1;
+  const uint64_t heads = kWaves / parts;
+  return {batch * ((hq + heads - 1) / heads), parts};
+}
+
 loom_status_t plan_mx4_decode(loom_paged_decode_plan_info_t *info, uint32_t teams_option, int cus,
                               loom_error_t *err) {
   const loom_paged_decode_spec_t &s = info->spec;
@@ -1084,7 +1097,9 @@ loom_status_t plan_mx4_decode(loom_paged_decode_plan_info_t *info, uint32_t team
   // Each XCD (every 8th workgroup) holds ceil(teams / 8) whole teams.
   const uint64_t xcd_waves = (teams + 7) / 8 * members;
   const uint64_t grid = (xcd_waves + kWaves - 1) / kWaves * 8;
-  if (grid > (uint64_t)INT32_MAX || teams > (uint64_t)INT32_MAX || B * hq > (uint64_t)INT32_MAX)
+  // (a launch holds fewer than 2^32 threads)
+  if (grid > UINT32_MAX / kThreads || teams > (uint64_t)INT32_MAX ||
+      B * hq > (uint64_t)INT32_MAX || merge_grid(B, hq, teams).grid > UINT32_MAX / kThreads)
     return fail(err, LOOM_PLAN_STATE_COUNT_OUT_OF_RANGE, "paged batch-decode", grid);
   info->algorithm = LOOM_PAGED_DECODE_BALANCED_SPLIT_KV;
   info->teams = (uint32_t)teams;
@@ -1128,12 +1143,9 @@ hipError_t launch_mx4_decode(const loom_paged_decode_plan_info_t &info, const Mx
   hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, stream, a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
-  // One wave per head up to 48 states per request on average (64 ragged requests, 5:
-  // 52.1 us, with four waves 55.5; 8 of 32k, 33: 56.8 and 57.6).
-  const int parts = a.teams / a.batch >= 48 ? kWaves : 1;
-  const unsigned wg_heads = kWaves / parts, wgs = (a.hq + wg_heads - 1) / wg_heads;
-  hipLaunchKernelGGL(mx4_decode_merge_kernel, dim3((unsigned)a.batch * wgs), dim3(kThreads), 0,
-                     stream, a, parts);
+  const MergeGrid m = merge_grid((uint64_t)a.batch, (uint64_t)a.hq, (uint64_t)a.teams);
+  hipLaunchKernelGGL(mx4_decode_merge_kernel, dim3((unsigned)m.grid), dim3(kThreads), 0, stream, a,
+                     m.parts);
   return hipGetLastError();
 }
 

@@ -204,6 +204,34 @@ def test_other_commands_plans(env):
         assert (x[n] == 7.0).all(), n
 
 
+def test_plans(env):
+    """What only a plan can refuse."""
+    torch, L = env
+    with pytest.raises(L.LoomError) as e:  # the reference-shaped append writes no scales
+        L.RopeProvider.load(0).plan_bf16_paged_append_tokens(
+            L.Bf16RopePagedKvAppendTokensSpec(T, B, POOL, HQ, HKV, kv_dtype="mxfp4"))
+    assert e.value.operand == "kv_dtype"
+    with pytest.raises(L.PlanError):  # more requests than a command takes
+        L.DecodeProvider.load(0).plan_bf16_paged_batch(
+            L.Bf16PagedBatchDecodeSpec(65537, 70000, 1, 1, kv_dtype="mxfp4"))
+    with pytest.raises(L.PlanError):  # a merge of more threads than a launch holds
+        L.DecodeProvider.load(0).plan_bf16_paged_batch(
+            L.Bf16PagedBatchDecodeSpec(65536, 70000, 1024, 1, kv_dtype="mxfp4"), teams=7)
+    with pytest.raises(L.PlanError):
+        L.PrefillProvider.load(0).plan_paged_kv_read(L.PagedKvReadSpec(1, 1, 4, 4097))
+    import ctypes as C
+    out, err = C.c_void_p(), L._ffi.Error()
+    spec = L.PagedKvReadSpec(1, 1, 4, 4)
+    for flags in (2, 1 << 20):
+        assert L.lib().loom_prefill_provider_plan_paged_kv_read(
+            L.PrefillProvider.load(0)._p, C.byref(spec._c), flags, C.byref(out), C.byref(err)) != 0
+        assert err.operand == b"flags" and not out.value
+    with pytest.raises(L.PlanError) as e:
+        L.RopeProvider.load(0).plan_norm_paged_append(
+            L.NormRopePagedKvAppendSpec(T, B, POOL, HQ, HKV), flags=1 << 20)
+    assert e.value.operand == "flags"
+
+
 def test_one_tensor_for_two_operands(env):
     """K and V pages, or an output that is also read, in one buffer."""
     torch, L = env
