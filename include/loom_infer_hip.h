@@ -563,7 +563,8 @@ typedef struct loom_mxfp4_paged_batch_decode_args {
 
 /* Paged decode of a plan whose spec names LOOM_KV_DTYPE_MXFP4: the same command,
  * guards and algorithms over dequantised rows.  The codes become BF16 exactly, so
- * O and LSE are those of the BF16 command over the values the pages hold.  Q, the
+ * O and LSE are those of the BF16 command over the values the pages hold (scales
+ * up to 252, as the append writes them; larger ones may pass BF16's range).  Q, the
  * pages, the scales, O and LSE on 4-byte boundaries.  The other enqueue forms
  * refuse such a plan (LOOM_NULL_ARGUMENT "K_scales"), this one plans over BF16 and
  * FP8 pages (LOOM_NULL_ARGUMENT "args"). */

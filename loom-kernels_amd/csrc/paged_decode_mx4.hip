@@ -13,15 +13,17 @@
 //     instruction, exactly.  (v_mfma_scale_f32_16x16x128_f8f6f4 takes FP4 itself, but
 //     sums its 128 products with errors up to 2^-12 of the largest, which LSE does not
 //     bear.)
-//   * V codes come as 8 dims from 8 col on of rows 4 j + quad; one byte permute per
-//     two tokens turns the widened pairs into the V^T fragment.
+//   * V codes come as 8 dims from 8 col on of rows 4 j + quad.  With up to 4 query heads
+//     in a tile the widened pairs are the V^T fragment as they are: an even and an odd
+//     dim in neighbouring places of the contraction, where P^T has its weight for the one
+//     and a zero for the other, in columns of their own.  With 5 to 8, one byte permute
+//     per two tokens turns the pairs into a fragment of one dim.
 //   * The running bound of the scores is set kLazy above a new maximum and moves only
 //     when a score passes it: the common step has no reduction across lanes and no
 //     rescale, and no weight is above 1 (large V do not overflow).
 //   * P keeps 16 bits, a BF16 high part and a BF16 residual, in one MFMA: a tile is at
-//     most 8 query heads, which fill columns 0-7 and again 8-15; the first eight take
-//     the high parts, the others the residuals, and the two columns' O are added at the
-//     end.
+//     most 8 query heads; columns 0-7 take the high parts, 8-15 the residuals, and the
+//     two columns' O are added at the end.
 //
 // Two decompositions, both independent of the page table's contents:
 //   balanced  the 32-token blocks of all valid requests form one virtual list, cut
@@ -218,12 +220,19 @@ __device__ __forceinline__ void wait_loads() {
 // Until this wave's LDS reads have returned: before loads into a slot that it read.
 __device__ __forceinline__ void wait_reads() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
 
-// One wave's decode of a request for NH neighbouring kv-heads and a tile of each one's
-// query heads: the online-softmax states.  acc[e][i] holds O[column col][dim 32 quad +
-// 8 i + e], unnormalized.
+// One wave's decode of a request for one kv-head and a tile of its query heads: the
+// online-softmax states.
+// Columns 0-7 of the tiles take P's high parts, 8-15 its residuals.  Tiles of 5 to 8
+// heads have a head per column, and acc[e][i] holds O[column col][dim 32 quad + 8 i + e],
+// unnormalized.  Tiles of up to 4 (QUADS) have column c & 3, and columns with bit 2 set
+// take the odd dims, the others the even ones: acc[e][i] holds dim 32 quad + 8 i + 2 e,
+// or + 1.
+template <bool QUADS>
 struct HeadState {
   float m_run, l_run;  // bound of the scores (log2); sum of this lane's weights
-  f32x4 acc[8];
+  static constexpr int kAcc = QUADS ? 4 : 8;
+  static constexpr int kHeadMask = QUADS ? 3 : 7;  // the head of column c: c & kHeadMask
+  f32x4 acc[kAcc];
   u32x4 q[4];  // MFMA c contracts dims 32 quad + 8 c + [0, 8)
 
   // From the lowest finite maximum, tokens that score -inf weigh nothing.
@@ -231,7 +240,7 @@ struct HeadState {
     m_run = -FLT_MAX;
     l_run = 0.0f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) acc[e] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int e = 0; e < kAcc; ++e) acc[e] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
   __device__ __forceinline__ void load_q(const uint16_t *row, bool mine, int quad) {
 #pragma unroll
@@ -245,43 +254,75 @@ struct HeadState {
     for (int c = 0; c < 4; ++c) asm volatile("" : "+v"(q[c]));
   }
   __device__ __forceinline__ float normalizer() const { return quad_sum(l_run); }
-  // O of this lane's column (dims 32 quad + [0, 32)) and, by quad 0, LSE.
-  __device__ __forceinline__ void store(uint16_t *o, float *lse, float l, int quad) const {
+  // The 32 dims 32 quad + 8 i + e of this lane's column (a head of the tile), high parts
+  // and residuals (lane col ^ 8 of the 16) added.
+  __device__ __forceinline__ void columns(f32x4 (&o)[8]) const {
+#pragma unroll
+    for (int e = 0; e < kAcc; ++e)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float x = acc[e][i] + __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(
+                                        0, (int)__float_as_uint(acc[e][i]), 0x128, 0xf, 0xf, false));
+        if constexpr (QUADS) {  // odd dims from lane col + 4
+          o[2 * e][i] = x;
+          o[2 * e + 1][i] = __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(
+              0, (int)__float_as_uint(x), 0x12C, 0xf, 0xf, false));
+        } else {
+          o[e][i] = x;
+        }
+      }
+  }
+  // A column of columns() as O and, by quad 0, LSE.
+  __device__ __forceinline__ void store(const f32x4 (&x)[8], uint16_t *o, float *lse, float l,
+                                        int quad) const {
     const float inv = 1.0f / l;  // (its rounding and the product's are 2^-23 of O)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       u32x4 w;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) w[e] = bf16x2_pack(acc[2 * e][i] * inv, acc[2 * e + 1][i] * inv);
+      for (int e = 0; e < 4; ++e) w[e] = bf16x2_pack(x[2 * e][i] * inv, x[2 * e + 1][i] * inv);
       *reinterpret_cast<u32x4 *>(o + quad * 32 + i * 8) = w;
     }
     if (quad == 0) *lse = m_run + __log2f(l);
   }
-  // The same column's unnormalized O.
-  __device__ __forceinline__ void stash(float *dst, int quad) const {
+  // The same column unnormalized.
+  static __device__ __forceinline__ void stash(const f32x4 (&x)[8], float *dst, int quad) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       float *o = dst + quad * 32 + i * 8;
-      *reinterpret_cast<f32x4 *>(o) = f32x4{acc[0][i], acc[1][i], acc[2][i], acc[3][i]};
-      *reinterpret_cast<f32x4 *>(o + 4) = f32x4{acc[4][i], acc[5][i], acc[6][i], acc[7][i]};
+      *reinterpret_cast<f32x4 *>(o) = f32x4{x[0][i], x[1][i], x[2][i], x[3][i]};
+      *reinterpret_cast<f32x4 *>(o + 4) = f32x4{x[4][i], x[5][i], x[6][i], x[7][i]};
     }
   }
 
-  // Adds the residuals' columns to the high parts' (lane col ^ 8 of the 16).
-  __device__ __forceinline__ void join_columns() {
+  // P^T as B fragments, from a lane's weights p[h][i] of tokens 16 h + 4 i + quad.
+  // One fragment: k = 8 quad + 4 h + i is that token.  QUADS, one per half h: k = 8 quad +
+  // 2 i is the token for even-dim columns and nothing for the others, + 1 the reverse.
+  __device__ __forceinline__ void pack_p(const float (&p)[2][4], int col, bf16x8 (&b)[2]) const {
+    const uint32_t taken = col < 8 ? 0u : 0xffff0000u;
+    uint32_t x[2][4];
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        acc[e][i] += __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(
-            0, (int)__float_as_uint(acc[e][i]), 0x128, 0xf, 0xf, false));
+        x[h][i] = __float_as_uint(p[h][i] - __uint_as_float(__float_as_uint(p[h][i]) & taken));
+    if constexpr (QUADS) {
+      // bytes 3 and 2 of x to the high or the low half, zeros (byte 12: 0) to the other
+      const uint32_t sel = col & 4 ? 0x03020c0cu : 0x0c0c0302u;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        b[h] = as_bf16x8(__builtin_amdgcn_perm(0u, x[h][0], sel), __builtin_amdgcn_perm(0u, x[h][1], sel),
+                         __builtin_amdgcn_perm(0u, x[h][2], sel), __builtin_amdgcn_perm(0u, x[h][3], sel));
+    } else {
+      b[0] = as_bf16x8(pack_hi16(x[0][0], x[0][1]), pack_hi16(x[0][2], x[0][3]),
+                       pack_hi16(x[1][0], x[1][1]), pack_hi16(x[1][2], x[1][3]));
+    }
   }
-
-  // Dims e = 2 W and 2 W + 1 of O^T += V^T.P^T: V^T's row col of fragment e is dim
-  // 8 col + e, and byte W of the lane's codes holds both dims.
+  // Dims 2 W and 2 W + 1 of O^T += V^T.P^T: V^T's row col is dims 8 col + 2 W and its
+  // neighbour, and byte W of the lane's codes holds both.
   template <int W>
   __device__ __forceinline__ void add_pv(const uint32_t (&v)[2][4], const float (&vs)[2][4],
-                                         bf16x8 p) {
+                                         const bf16x8 (&p)[2]) {
     uint32_t x[2][4];
 #pragma unroll
     for (int h = 0; h < 2; ++h)
@@ -289,20 +330,27 @@ struct HeadState {
       for (int j = 0; j < 4; ++j)
         x[h][j] = __builtin_bit_cast(
             uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(v[h][j], vs[h][j], W));
-    const bf16x8 even =
-        as_bf16x8(pack_lo16(x[0][0], x[0][1]), pack_lo16(x[0][2], x[0][3]),
-                  pack_lo16(x[1][0], x[1][1]), pack_lo16(x[1][2], x[1][3]));
-    const bf16x8 odd =
-        as_bf16x8(pack_hi16(x[0][0], x[0][1]), pack_hi16(x[0][2], x[0][3]),
-                  pack_hi16(x[1][0], x[1][1]), pack_hi16(x[1][2], x[1][3]));
-    acc[2 * W] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(even, p, acc[2 * W], 0, 0, 0);
-    acc[2 * W + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(odd, p, acc[2 * W + 1], 0, 0, 0);
+    if constexpr (QUADS) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        acc[W] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+            as_bf16x8(x[h][0], x[h][1], x[h][2], x[h][3]), p[h], acc[W], 0, 0, 0);
+    } else {
+      const bf16x8 even =
+          as_bf16x8(pack_lo16(x[0][0], x[0][1]), pack_lo16(x[0][2], x[0][3]),
+                    pack_lo16(x[1][0], x[1][1]), pack_lo16(x[1][2], x[1][3]));
+      const bf16x8 odd =
+          as_bf16x8(pack_hi16(x[0][0], x[0][1]), pack_hi16(x[0][2], x[0][3]),
+                    pack_hi16(x[1][0], x[1][1]), pack_hi16(x[1][2], x[1][3]));
+      acc[2 * W] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(even, p[0], acc[2 * W], 0, 0, 0);
+      acc[2 * W + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(odd, p[0], acc[2 * W + 1], 0, 0, 0);
+    }
   }
 };
 
 // The block at `slot` (LDS) of which the first `rows` tokens are valid (wave-uniform).
-template <bool P16, int NH, int ARR>
-__device__ __forceinline__ void process_block(HeadState (&st)[NH], const uint8_t *slot, int rows,
+template <bool P16, int NH, int ARR, bool QUADS>
+__device__ __forceinline__ void process_block(HeadState<QUADS> (&st)[NH], const uint8_t *slot, int rows,
                                               int col, int quad, float scale_log2) {
   using S = Slot<NH>;
   f32x4 s[NH][2];
@@ -356,27 +404,22 @@ __device__ __forceinline__ void process_block(HeadState (&st)[NH], const uint8_t
       st[g].m_run = m_new;
       st[g].l_run *= al;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) st[g].acc[e] *= al;
+      for (int e = 0; e < HeadState<QUADS>::kAcc; ++e) st[g].acc[e] *= al;
     }
   }
 #pragma unroll
   for (int g = 0; g < NH; ++g) {
-    // P^T as the B fragment (k = 8 quad + i: token 4 i + quad of half 0, then of half
-    // 1): columns 0-7 the high halves of the weights, 8-15 what those leave of them.
-    const uint32_t taken = col < 8 ? 0u : 0xffff0000u;
-    uint32_t pw[4];
+    float pf[2][4];
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int i = 0; i < 4; i += 2) {
-        const float p0 = fast_exp2(fmaf(s[g][h][i], scale_log2, -st[g].m_run));
-        const float p1 = fast_exp2(fmaf(s[g][h][i + 1], scale_log2, -st[g].m_run));
-        st[g].l_run += p0 + p1;
-        pw[2 * h + i / 2] = pack_hi16(
-            __float_as_uint(p0 - __uint_as_float(__float_as_uint(p0) & taken)),
-            __float_as_uint(p1 - __uint_as_float(__float_as_uint(p1) & taken)));
+        pf[h][i] = fast_exp2(fmaf(s[g][h][i], scale_log2, -st[g].m_run));
+        pf[h][i + 1] = fast_exp2(fmaf(s[g][h][i + 1], scale_log2, -st[g].m_run));
+        st[g].l_run += pf[h][i] + pf[h][i + 1];
       }
-    const bf16x8 p = as_bf16x8(pw[0], pw[1], pw[2], pw[3]);
+    bf16x8 p[2];
+    st[g].pack_p(pf, col, p);
     // V codes of rows 4 j + quad.  Rows past the valid ones are zeros and weigh nothing.
     uint32_t v[2][4];
     float vs[2][4];
@@ -502,7 +545,7 @@ __device__ __forceinline__ Blocks find_blocks(const Mx4DecodeArgs &a, const Smem
 }
 
 // NH: kv-heads per wave; they divide Hkv.
-template <bool P16, int NH, int ARR>
+template <bool P16, int NH, int ARR, bool QUADS>
 __global__ __launch_bounds__(kThreads, 2) void mx4_decode_split_kernel(
     Mx4DecodeArgs a) {
   __shared__ BalancedSmem<NH> sm;
@@ -596,10 +639,11 @@ __global__ __launch_bounds__(kThreads, 2) void mx4_decode_split_kernel(
   const int n = (int)min<int64_t>(v_end - v_begin, INT32_MAX - 64);
   if (n <= 0) return;
 
-  HeadState w[NH];
+  HeadState<QUADS> w[NH];
+  constexpr int kHeadMask = HeadState<QUADS>::kHeadMask;
   const int col = lane & 15, quad = lane >> 4;
-  const bool mine = col < heads, loads_q = (col & 7) < heads;
-  const int qh = kvh * a.group + g0 + (col & 7);  // of the first kv-head
+  const bool mine = col < heads, loads_q = (col & kHeadMask) < heads;
+  const int qh = kvh * a.group + g0 + (col & kHeadMask);  // of the first kv-head
 
   // ---- one continuous stream of blocks ----------------------------------------------
   // Block i + kDepth - 1 is issued before block i is consumed, across request
@@ -630,18 +674,19 @@ __global__ __launch_bounds__(kThreads, 2) void mx4_decode_split_kernel(
 #pragma unroll
     for (int g = 0; g < NH; ++g) {
       const float l = w[g].normalizer();
-      w[g].join_columns();
+      f32x4 o[8];
+      w[g].columns(o);
       if (!mine) continue;
       const int64_t head = qh + g * a.group;
       if (first && last) {  // the whole request; an invalid page index keeps its sentinels
         const int64_t row = (int64_t)r * a.hq + head;
-        if (!bad) w[g].store(a.out + row * 128, a.lse + row, l, quad);
+        if (!bad) w[g].store(o, a.out + row * 128, a.lse + row, l, quad);
         continue;
       }
       // One state per (team, request): slot team + r (along the virtual list the team
       // or the request advances at every piece).
       float *st = a.states + ((int64_t)(team + r) * a.hq + head) * kMx4StateStride;
-      if (!bad) w[g].stash(st + 4, quad);
+      if (!bad) w[g].stash(o, st + 4, quad);
       if (quad == 0) {
         st[0] = bad ? 0.0f : w[g].m_run;
         st[1] = bad ? kPoisonNormalizer : l;
@@ -678,7 +723,7 @@ __global__ __launch_bounds__(kThreads, 2) void mx4_decode_split_kernel(
     // Block i has arrived once at most the loads issued after it are outstanding
     // (others in between only make the wait longer).
     wait_loads<(kDepth - 1) * kBlockLoads<P16, NH>>();
-    process_block<P16, NH, ARR>(w, sm.slots[wave][slot], rows, col, quad, a.scale_log2);
+    process_block<P16, NH, ARR, QUADS>(w, sm.slots[wave][slot], rows, col, quad, a.scale_log2);
 #pragma unroll
     for (int j = 0; j + 1 < kDepth; ++j) {
       meta[j] = meta[j + 1];
@@ -817,7 +862,7 @@ __global__ __launch_bounds__(kThreads) void mx4_decode_merge_kernel(Mx4DecodeArg
 constexpr int kDirectWaves = 8;
 constexpr int kStash = 132;  // floats between two columns' O in LDS
 
-template <bool P16, int NH, int ARR>
+template <bool P16, int NH, int ARR, bool QUADS>
 __global__ __launch_bounds__(kDirectWaves * 64) void mx4_decode_direct_kernel(Mx4DecodeArgs a) {
   constexpr int W = kDirectWaves;
   constexpr int kCols = NH * kMaxTile;
@@ -837,7 +882,8 @@ __global__ __launch_bounds__(kDirectWaves * 64) void mx4_decode_direct_kernel(Mx
   const int g0 = (int)(rest % (uint32_t)a.tiles) * a.tile;
   const int r = (int)(rest / (uint32_t)a.tiles);
   const int heads = min(a.tile, a.group - g0);
-  HeadState w[NH];
+  HeadState<QUADS> w[NH];
+  constexpr int kHeadMask = HeadState<QUADS>::kHeadMask;
   const int col = lane & 15, quad = lane >> 4;
   // query head of column c of the workgroup's NH * heads
   auto query_head = [&](int c) {
@@ -878,8 +924,8 @@ __global__ __launch_bounds__(kDirectWaves * 64) void mx4_decode_direct_kernel(Mx
   // short, all of it.
 #pragma unroll
   for (int g = 0; g < NH; ++g)
-    w[g].load_q(a.q + ((int64_t)r * a.hq + (kvh + g) * a.group + g0 + (col & 7)) * 128,
-                (col & 7) < heads, quad);
+    w[g].load_q(a.q + ((int64_t)r * a.hq + (kvh + g) * a.group + g0 + (col & kHeadMask)) * 128,
+                (col & kHeadMask) < heads, quad);
   const bool whole_table = a.n_indices <= 128;
   int tbl0 = 0, tbl1 = 0;
   if (whole_table) {
@@ -948,31 +994,29 @@ __global__ __launch_bounds__(kDirectWaves * 64) void mx4_decode_direct_kernel(Mx
       wait_reads();
       const int rows_next = issue(i + 1, (i + 1) & 1);
       wait_loads<kBlockLoads<P16, NH>>();
-      process_block<P16, NH, ARR>(w, slots + (i & 1) * Slot<NH>::bytes, rows, col, quad,
+      process_block<P16, NH, ARR, QUADS>(w, slots + (i & 1) * Slot<NH>::bytes, rows, col, quad,
                                   a.scale_log2);
       rows = rows_next;
     }
-  }
-  float l[NH];
-#pragma unroll
-  for (int g = 0; g < NH; ++g) {
-    l[g] = w[g].normalizer();
-    w[g].join_columns();
   }
   // The wave's slots become its columns' place; loads past its last block may still
   // write them.
   wait_loads<0>();
   wait_reads();
 #pragma unroll
-  for (int g = 0; g < NH; ++g)
+  for (int g = 0; g < NH; ++g) {
+    const float l = w[g].normalizer();
+    f32x4 o[8];
+    w[g].columns(o);
     if (col < heads) {
       const int c = g * heads + col;
-      w[g].stash(reinterpret_cast<float *>(slots) + c * kStash, quad);
+      w[g].stash(o, reinterpret_cast<float *>(slots) + c * kStash, quad);
       if (quad == 0) {
         s_m[wave][c] = w[g].m_run;
-        s_l[wave][c] = l[g];
+        s_l[wave][c] = l;
       }
     }
+  }
   // An invalid page index anywhere in the request keeps its sentinels.
   if (block_or(bad, s_bad)) return poison();
   // Four dims of one column per thread.
@@ -1111,19 +1155,34 @@ loom_status_t plan_mx4_decode(loom_paged_decode_plan_info_t *info, uint32_t team
   return LOOM_OK;
 }
 
+using Mx4Kernel = void (*)(Mx4DecodeArgs);
+template <int NH, int ARR, bool QUADS>
+static Mx4Kernel direct_kernel(bool p16) {
+  return p16 ? mx4_decode_direct_kernel<true, NH, ARR, QUADS>
+             : mx4_decode_direct_kernel<false, NH, ARR, QUADS>;
+}
+template <int NH, int ARR, bool QUADS>
+static Mx4Kernel split_kernel(bool p16) {
+  return p16 ? mx4_decode_split_kernel<true, NH, ARR, QUADS>
+             : mx4_decode_split_kernel<false, NH, ARR, QUADS>;
+}
+
 hipError_t launch_mx4_decode(const loom_paged_decode_plan_info_t &info, const Mx4DecodeArgs &a,
                              bool clear, hipStream_t stream) {
-  const bool p16 = a.page_rows == 16;
+  // Tiles of up to 4 heads leave columns for both dims of a code byte: 32 of a block's
+  // 200 vector instructions less (16 requests of 256-1536 tokens, 32 / 8 heads: 12.6 us,
+  // in the other form 13.7; 64 of 2000-4000, 16 / 4: 30.0 and 33.0; 64 of 512-8192: 52.1
+  // and 51.7).
+  const bool p16 = a.page_rows == 16, quads = a.tile <= 4;
   const dim3 grid(info.grid_blocks);
   if (info.algorithm == LOOM_PAGED_DECODE_DIRECT) {
     // the plan's grid says how many kv-heads its workgroups take
     const bool pair = (uint64_t)info.grid_blocks * 2 ==
                       (uint64_t)a.batch * a.hkv * a.tiles * (uint64_t)a.splits;
-    auto kernel = pair
-                      ? (p16 ? mx4_decode_direct_kernel<true, 2, kPair>
-                             : mx4_decode_direct_kernel<false, 2, kPair>)
-                      : (p16 ? mx4_decode_direct_kernel<true, 1, kSplit>
-                             : mx4_decode_direct_kernel<false, 1, kSplit>);
+    auto kernel = quads ? (pair ? direct_kernel<2, kPair, true>(p16)
+                                : direct_kernel<1, kSplit, true>(p16))
+                  : pair ? direct_kernel<2, kPair, false>(p16)
+                         : direct_kernel<1, kSplit, false>(p16);
     if (clear) {
       hipLaunchKernelGGL(mx4_decode_clear_kernel, dim3(1), dim3(kMx4Joins), 0, stream, a.arrived);
       const hipError_t e = hipGetLastError();
@@ -1132,14 +1191,13 @@ hipError_t launch_mx4_decode(const loom_paged_decode_plan_info_t &info, const Mx
     hipLaunchKernelGGL(kernel, grid, dim3(info.block_threads), 0, stream, a);
     return hipGetLastError();
   }
-  auto kernel = heads_per_wave(a.hkv) == 1
-                    ? (p16 ? mx4_decode_split_kernel<true, 1, kSplit>
-                           : mx4_decode_split_kernel<false, 1, kSplit>)
-                : info.spec.kv_layout != LOOM_KV_LAYOUT_HND
-                      ? (p16 ? mx4_decode_split_kernel<true, 2, kPair>
-                             : mx4_decode_split_kernel<false, 2, kPair>)
-                      : (p16 ? mx4_decode_split_kernel<true, 2, kSplit>
-                             : mx4_decode_split_kernel<false, 2, kSplit>);
+  const bool nhd = info.spec.kv_layout != LOOM_KV_LAYOUT_HND, one = heads_per_wave(a.hkv) == 1;
+  auto kernel = quads ? (one   ? split_kernel<1, kSplit, true>(p16)
+                         : nhd ? split_kernel<2, kPair, true>(p16)
+                               : split_kernel<2, kSplit, true>(p16))
+                : one ? split_kernel<1, kSplit, false>(p16)
+                : nhd ? split_kernel<2, kPair, false>(p16)
+                      : split_kernel<2, kSplit, false>(p16);
   hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, stream, a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
