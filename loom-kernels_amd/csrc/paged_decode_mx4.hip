@@ -460,6 +460,10 @@ struct Blocks {
   int p0, p1;
   int meta;  // valid rows | first block of its request << 8 | last << 9 | row in page << 16
   int req;
+  // Ends the loads behind them here, as HeadState::settle_q does and for its reason.
+  __device__ __forceinline__ void settle() {
+    asm volatile("" : "+v"(p0), "+v"(p1), "+v"(meta), "+v"(req));
+  }
 };
 
 // The virtual list as a wave knows it.  Up to 64 requests: lane r holds request r's
@@ -655,8 +659,8 @@ __global__ __launch_bounds__(kThreads, 2) void mx4_decode_split_kernel(
     const int j = i & 63;
     if (j == 0) {
       cur = next;  // located 64 blocks ago
-      if (i + 64 < n)
-        next = find_blocks<P16>(a, sm, list, v_begin + i + 64, v_end, lane);
+      if (i + 64 < n) next = find_blocks<P16>(a, sm, list, v_begin + i + 64, v_end, lane);
+      next.settle();
     }
     meta = i < n ? __builtin_amdgcn_readlane(cur.meta, j) : 0;  // past the range: no rows
     req = __builtin_amdgcn_readlane(cur.req, j);
@@ -696,6 +700,7 @@ __global__ __launch_bounds__(kThreads, 2) void mx4_decode_split_kernel(
 
   int meta[kDepth], req[kDepth];  // of blocks i, i + 1, ..., the last being issued
   next = find_blocks<P16>(a, sm, list, v_begin, v_end, lane);
+  next.settle();
 #pragma unroll
   for (int j = 0; j < kDepth - 1; ++j) issue(j, j, meta[j], req[j]);
   int slot = 0;
@@ -947,7 +952,7 @@ __global__ __launch_bounds__(kDirectWaves * 64) void mx4_decode_direct_kernel(Mx
   bool bad = false;
 #pragma unroll
   for (int g = 0; g < NH; ++g) w[g].reset();
-  Blocks cur;
+  Blocks cur = {0, 0, 0, 0};
   auto locate = [&](int64_t i0) {  // the wave's blocks i0 + [0, 64), one per lane
     const bool in = i0 + lane < n;
     const int64_t b = lo + wave + W * (i0 + lane);
@@ -984,12 +989,11 @@ __global__ __launch_bounds__(kDirectWaves * 64) void mx4_decode_direct_kernel(Mx
       load_block<P16, NH, ARR, false>(a, p, slots_at + slot * Slot<NH>::bytes, lane, kvh);
       return p.rows;
     };
+    cur.settle();
+#pragma unroll
+    for (int g = 0; g < NH; ++g) w[g].settle_q();
     wait_reads();
     int rows = issue(0, 0);
-    if (i0 == 0) {
-#pragma unroll
-      for (int g = 0; g < NH; ++g) w[g].settle_q();
-    }
     for (int i = 0; i < m; ++i) {
       wait_reads();
       const int rows_next = issue(i + 1, (i + 1) & 1);
