@@ -28,7 +28,6 @@ struct Mx4DecodeArgs {
   uint32_t *arrived;
   int64_t pool;
   int64_t n_indices;
-  int64_t page_bytes;  // P * Hkv * 64
   int32_t indices_capacity;
   int32_t batch;
   int32_t hq;

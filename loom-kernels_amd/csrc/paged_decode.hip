@@ -1713,7 +1713,6 @@ loom_status_t paged_decode_enqueue_impl(const loom_paged_decode_plan_t *plan,
     const bool head_major = s.kv_layout == LOOM_KV_LAYOUT_HND;
     m.head_bytes = head_major ? m.page_rows * 64 : 64;
     m.row_bytes = head_major ? 64 : m.hkv * 64;
-    m.page_bytes = (int64_t)m.page_rows * m.hkv * 64;
     m.scale_log2 = s.softmax_scale * 1.44269504088896340736f;
     // A command that the caller captures into a graph of its own is not in the
     // queue's order: its arrival words are the workspace's, cleared by every replay.

@@ -150,22 +150,42 @@ struct Slot {
   }
 };
 
-// Where a block lies: the pages of its two halves (the same one unless pages have 16
-// rows), its first row in the page, and its valid rows (0: none, nothing is read).  All
-// wave-uniform.
+// Where a block lies: the cache row (of 64 code bytes; plans hold below 2^32 of them) and
+// the scale row (of 4 bytes) of its first token and the wave's first kv-head, for pages of
+// 16 rows those of its second half too; and its valid rows (0: none, nothing is read).
+// All wave-uniform: found per lane, 64 blocks at a time, since the 64-bit products of
+// page, head and row for every block took a fifth of a walk's instructions.
 struct Place {
-  int p0, p1, row, rows;
+  uint32_t c0, s0, c1, s1;
+  int rows;
 };
+// The two rows of row `row` of `page`, head kvh.
+__device__ __forceinline__ void cache_rows(const Mx4DecodeArgs &a, int page, int row, int kvh,
+                                           uint32_t &c, uint32_t &s) {
+  const uint32_t pg = (uint32_t)page;
+  s = (pg * (uint32_t)a.hkv + (uint32_t)kvh) * (uint32_t)a.page_rows + (uint32_t)row;
+  c = a.row_bytes == 64 ? s  // HND (and one kv-head): as the scales lie
+                        : (pg * (uint32_t)a.page_rows + (uint32_t)row) * (uint32_t)a.hkv + (uint32_t)kvh;
+}
+
+// row << N of a wave-uniform row, in scalar registers (the compiler fuses the shift into
+// a vector multiply-add of the address otherwise).
+template <int N>
+__device__ __forceinline__ uint64_t row_bytes(uint32_t row) {
+  uint64_t r;
+  asm("s_lshl_b64 %0, %1, %2" : "=s"(r) : "s"((uint64_t)row), "n"(N) : "scc");
+  return r;
+}
 
 // Vector memory instructions that load_block issues, always.
 template <bool P16, int NH>
 constexpr int kBlockLoads = 4 * NH + (P16 ? 4 : 2);
-// Issues the loads of a block of heads kvh .. kvh + NH - 1 into LDS at byte address
+// Issues the loads of a block of NH neighbouring kv-heads into LDS at byte address
 // `slot`.  Rows past the valid ones arrive as zeros and move no bytes.
 // NT: nontemporal loads of the codes.
 template <bool P16, int NH, int ARR, bool NT>
 __device__ __forceinline__ void load_block(const Mx4DecodeArgs &a, const Place &p, uint32_t slot,
-                                           int lane, int kvh) {
+                                           int lane) {
   using S = Slot<NH>;
   auto rsrc = [](const uint8_t *base, int bytes) {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(base), 0, bytes, 0x00020000);
@@ -174,11 +194,11 @@ __device__ __forceinline__ void load_block(const Mx4DecodeArgs &a, const Place &
   for (int h = 0; h < 2; ++h) {
     // rows [0, n) of this half (of the whole block where it lies in one page) exist
     const int n = !P16 ? p.rows : h == 0 ? min(p.rows, 16) : max(p.rows - 16, 0);
-    const int64_t page = P16 && h == 1 ? p.p1 : p.p0;
-    const int64_t at = page * a.page_bytes + (int64_t)kvh * a.head_bytes + (int64_t)p.row * a.row_bytes;
+    const uint32_t c = P16 && h == 1 ? p.c1 : p.c0;
     const int skip = P16 ? 0 : 16 * h * a.row_bytes;
     if constexpr (ARR == kPair) {
-      const int bytes = n > 0 ? (n - 1) * a.row_bytes + 128 : 0;
+      const int bytes = max((n - 1) * a.row_bytes + 128, 0);  // (rows of 128 bytes and more)
+      const uint64_t at = row_bytes<6>(c);
       const __amdgpu_buffer_rsrc_t rk = rsrc(a.k + at, bytes), rv = rsrc(a.v + at, bytes);
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
@@ -188,11 +208,11 @@ __device__ __forceinline__ void load_block(const Mx4DecodeArgs &a, const Place &
         lds_load16_at<NT>(rv, slot + S::v + (2 * h + t) * 1024, off);
       }
     } else {
-      const int bytes = n > 0 ? (n - 1) * a.row_bytes + 64 : 0;
+      const int bytes = max((n - 1) * a.row_bytes + 64, 0);
       const int off = (lane >> 2) * a.row_bytes + (((lane & 3) ^ (lane >> 4)) << 4) + skip;
 #pragma unroll
       for (int g = 0; g < NH; ++g) {
-        const int64_t head = at + (int64_t)g * a.head_bytes;
+        const uint64_t head = row_bytes<6>(c + (uint32_t)g * ((uint32_t)a.head_bytes >> 6));
         lds_load16_at<NT>(rsrc(a.k + head, bytes), slot + g * kHeadBytes + h * kHalfBytes, off);
         lds_load16_at<NT>(rsrc(a.v + head, bytes), slot + S::v + g * kHeadBytes + h * kHalfBytes, off);
       }
@@ -202,9 +222,9 @@ __device__ __forceinline__ void load_block(const Mx4DecodeArgs &a, const Place &
       constexpr int kRows = P16 ? 16 : 32;
       if (lane < kRows * NH) {
         const int row = token_of(lane & 15) + (P16 ? 0 : lane & 16);
-        const int64_t sc = ((page * a.hkv + kvh) * a.page_rows + p.row) * 4;
+        const uint64_t sc = row_bytes<2>(P16 && h == 1 ? p.s1 : p.s0);
         const int off = row < n ? (lane / kRows) * a.page_rows * 4 + row * 4 : INT32_MAX;
-        const int bytes = n > 0 ? ((NH - 1) * a.page_rows + n) * 4 : 0;
+        const int bytes = ((NH - 1) * a.page_rows + n) * 4;
         lds_load4_at(rsrc(a.k_mx + sc, bytes), slot + S::ks + h * NH * 64, off);
         lds_load4_at(rsrc(a.v_mx + sc, bytes), slot + S::vs + h * NH * 64, off);
       }
@@ -457,12 +477,33 @@ struct BalancedSmem {
 
 // Blocks [v0, v0 + 64) of the virtual list, one per lane.
 struct Blocks {
-  int p0, p1;
-  int meta;  // valid rows | first block of its request << 8 | last << 9 | row in page << 16
+  uint32_t c0, s0, c1, s1;  // as in Place
+  int meta;  // valid rows | first block of its request << 8 | last << 9
   int req;
+  // Lane i's rows; `meta`: its meta.
+  template <bool P16>
+  __device__ __forceinline__ Place place(int i, int meta) const {
+    Place p;
+    p.rows = meta & 255;
+    p.c0 = (uint32_t)__builtin_amdgcn_readlane((int)c0, i);
+    p.s0 = (uint32_t)__builtin_amdgcn_readlane((int)s0, i);
+    p.c1 = P16 ? (uint32_t)__builtin_amdgcn_readlane((int)c1, i) : 0;
+    p.s1 = P16 ? (uint32_t)__builtin_amdgcn_readlane((int)s1, i) : 0;
+    return p;
+  }
+  // This lane's rows, from the pages p0 and p1 of its halves; false: an index is invalid.
+  template <bool P16>
+  __device__ __forceinline__ bool set(const Mx4DecodeArgs &a, int p0, int p1, int row, int kvh) {
+    const bool ok = p0 >= 0 && (int64_t)p0 < a.pool && p1 >= 0 && (int64_t)p1 < a.pool;
+    if (ok) {
+      cache_rows(a, p0, row, kvh, c0, s0);
+      if (P16) cache_rows(a, p1, row, kvh, c1, s1);
+    }
+    return ok;
+  }
   // Ends the loads behind them here, as HeadState::settle_q does and for its reason.
   __device__ __forceinline__ void settle() {
-    asm volatile("" : "+v"(p0), "+v"(p1), "+v"(meta), "+v"(req));
+    asm volatile("" : "+v"(c0), "+v"(s0), "+v"(c1), "+v"(s1), "+v"(meta), "+v"(req));
   }
 };
 
@@ -480,8 +521,9 @@ struct List {
 
 template <bool P16, class Smem>
 __device__ __forceinline__ Blocks find_blocks(const Mx4DecodeArgs &a, const Smem &sm,
-                                              const List &list, int64_t v0, int64_t v_end, int lane) {
-  Blocks d = {0, 0, 0, -1};
+                                              const List &list, int64_t v0, int64_t v_end, int lane,
+                                              int kvh) {
+  Blocks d = {0, 0, 0, 0, 0, -1};
   const int64_t v = v0 + lane;
   const bool in = v < v_end;
   int r = 0;
@@ -540,10 +582,9 @@ __device__ __forceinline__ Blocks find_blocks(const Mx4DecodeArgs &a, const Smem
   // token 32 b lies in the request's page 32 b / P, row 32 b % P
   const int64_t pos = st + (P16 ? 2 * b : a.page_rows == 64 ? b >> 1 : b);
   const int row = !P16 && a.page_rows == 64 ? (int)(b & 1) * kBlock : 0;
-  d.p0 = a.indices[pos];
-  d.p1 = P16 && rows > 16 ? a.indices[pos + 1] : d.p0;
-  if (d.p0 < 0 || (int64_t)d.p0 >= a.pool || d.p1 < 0 || (int64_t)d.p1 >= a.pool) rows = 0;
-  d.meta = rows | (b == 0 ? 256 : 0) | (last ? 512 : 0) | row << 16;
+  const int p0 = a.indices[pos], p1 = P16 && rows > 16 ? a.indices[pos + 1] : p0;
+  if (!d.set<P16>(a, p0, p1, row, kvh)) rows = 0;
+  d.meta = rows | (b == 0 ? 256 : 0) | (last ? 512 : 0);
   d.req = r;
   return d;
 }
@@ -640,7 +681,7 @@ __global__ __launch_bounds__(kThreads, 2) void mx4_decode_split_kernel(
   const int g0 = member / (a.hkv / NH) * a.tile;
   const int heads = min(a.tile, a.group - g0);
   const int64_t v_begin = ranges.start(team), v_end = ranges.start(team + 1);
-  const int n = (int)min<int64_t>(v_end - v_begin, INT32_MAX - 64);
+  const int n = uni((int)min<int64_t>(v_end - v_begin, INT32_MAX - 64));
   if (n <= 0) return;
 
   HeadState<QUADS> w[NH];
@@ -652,24 +693,20 @@ __global__ __launch_bounds__(kThreads, 2) void mx4_decode_split_kernel(
   // ---- one continuous stream of blocks ----------------------------------------------
   // Block i + kDepth - 1 is issued before block i is consumed, across request
   // boundaries.  Blocks are located 64 at a time, one per lane.
-  Blocks cur = {0, 0, 0, -1}, next = cur;
+  Blocks cur = {0, 0, 0, 0, 0, -1}, next = cur;
   const uint32_t slots = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void *)sm.slots[wave];
   // Block i into slot i % kDepth; its Blocks::meta and ::req.
   auto issue = [&](int i, int slot, int &meta, int &req) {
     const int j = i & 63;
     if (j == 0) {
       cur = next;  // located 64 blocks ago
-      if (i + 64 < n) next = find_blocks<P16>(a, sm, list, v_begin + i + 64, v_end, lane);
+      if (i + 64 < n) next = find_blocks<P16>(a, sm, list, v_begin + i + 64, v_end, lane, kvh);
       next.settle();
     }
-    meta = i < n ? __builtin_amdgcn_readlane(cur.meta, j) : 0;  // past the range: no rows
+    meta = uni(i < n ? __builtin_amdgcn_readlane(cur.meta, j) : 0);  // past the range: no rows
     req = __builtin_amdgcn_readlane(cur.req, j);
-    Place p;
-    p.rows = meta & 255;
-    p.row = meta >> 16;
-    p.p0 = p.rows ? __builtin_amdgcn_readlane(cur.p0, j) : 0;
-    p.p1 = P16 && p.rows ? __builtin_amdgcn_readlane(cur.p1, j) : 0;
-    load_block<P16, NH, ARR, true>(a, p, slots + slot * Slot<NH>::bytes, lane, kvh);
+    load_block<P16, NH, ARR, true>(a, cur.place<P16>(j, meta),
+                                   slots + slot * Slot<NH>::bytes, lane);
   };
 
   int r = -1;
@@ -699,7 +736,7 @@ __global__ __launch_bounds__(kThreads, 2) void mx4_decode_split_kernel(
   };
 
   int meta[kDepth], req[kDepth];  // of blocks i, i + 1, ..., the last being issued
-  next = find_blocks<P16>(a, sm, list, v_begin, v_end, lane);
+  next = find_blocks<P16>(a, sm, list, v_begin, v_end, lane, kvh);
   next.settle();
 #pragma unroll
   for (int j = 0; j < kDepth - 1; ++j) issue(j, j, meta[j], req[j]);
@@ -952,60 +989,61 @@ __global__ __launch_bounds__(kDirectWaves * 64) void mx4_decode_direct_kernel(Mx
   bool bad = false;
 #pragma unroll
   for (int g = 0; g < NH; ++g) w[g].reset();
-  Blocks cur = {0, 0, 0, 0};
+  Blocks cur = {0, 0, 0, 0, 0, 0};
   auto locate = [&](int64_t i0) {  // the wave's blocks i0 + [0, 64), one per lane
     const bool in = i0 + lane < n;
     const int64_t b = lo + wave + W * (i0 + lane);
     int rows = in ? (int)min<int64_t>(kBlock, tokens - b * kBlock) : 0;
     const int64_t pos = st + (P16 ? 2 * b : a.page_rows == 64 ? b >> 1 : b);
     const bool two = P16 && rows > 16;
+    int p0 = 0, p1 = 0;
     if (whole_table) {  // pos < 128 for blocks that exist
       const int j = (int)pos, lo0 = __shfl(tbl0, j & 63, 64), hi0 = __shfl(tbl1, j & 63, 64);
       const int lo1 = __shfl(tbl0, (j + 1) & 63, 64), hi1 = __shfl(tbl1, (j + 1) & 63, 64);
-      cur.p0 = j < 64 ? lo0 : hi0;
-      cur.p1 = !two ? cur.p0 : j + 1 < 64 ? lo1 : hi1;
+      p0 = j < 64 ? lo0 : hi0;
+      p1 = !two ? p0 : j + 1 < 64 ? lo1 : hi1;
     } else if (in) {
-      cur.p0 = a.indices[pos];
-      cur.p1 = two ? a.indices[pos + 1] : cur.p0;
+      p0 = a.indices[pos];
+      p1 = two ? a.indices[pos + 1] : p0;
     }
-    if (in && (cur.p0 < 0 || (int64_t)cur.p0 >= a.pool || cur.p1 < 0 || (int64_t)cur.p1 >= a.pool)) {
+    const int row = !P16 && a.page_rows == 64 ? (int)(b & 1) * kBlock : 0;
+    if (in && !cur.set<P16>(a, p0, p1, row, kvh)) {
       rows = 0;
       bad = true;
     }
-    cur.meta = rows | (!P16 && a.page_rows == 64 ? (int)(b & 1) * kBlock : 0) << 16;
+    cur.meta = rows;
   };
   uint8_t *const slots = s_wave[wave];
   const uint32_t slots_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void *)slots;
   for (int64_t i0 = 0; i0 < n; i0 += 64) {
     locate(i0);
-    const int m = (int)min<int64_t>(64, n - i0);
-    auto issue = [&](int i, int slot) {
-      const int meta = i < m ? __builtin_amdgcn_readlane(cur.meta, i) : 0;
-      Place p;
-      p.rows = meta & 255;
-      p.row = meta >> 16;
-      p.p0 = p.rows ? __builtin_amdgcn_readlane(cur.p0, i) : 0;
-      p.p1 = P16 && p.rows ? __builtin_amdgcn_readlane(cur.p1, i) : 0;
-      load_block<P16, NH, ARR, false>(a, p, slots_at + slot * Slot<NH>::bytes, lane, kvh);
-      return p.rows;
+    const int m = uni((int)min<int64_t>(64, n - i0));
+    auto issue = [&](int i) {
+      const int rows = __builtin_amdgcn_readlane(cur.meta, i);
+      load_block<P16, NH, ARR, false>(a, cur.place<P16>(i, rows),
+                                      slots_at + (i & 1) * Slot<NH>::bytes, lane);
+      return rows;
     };
     cur.settle();
 #pragma unroll
     for (int g = 0; g < NH; ++g) w[g].settle_q();
     wait_reads();
-    int rows = issue(0, 0);
+    int rows = issue(0);
     for (int i = 0; i < m; ++i) {
-      wait_reads();
-      const int rows_next = issue(i + 1, (i + 1) & 1);
-      wait_loads<kBlockLoads<P16, NH>>();
+      int rows_next = 0;
+      if (i + 1 < m) {
+        wait_reads();
+        rows_next = issue(i + 1);
+        wait_loads<kBlockLoads<P16, NH>>();
+      } else {
+        wait_loads<0>();
+      }
       process_block<P16, NH, ARR, QUADS>(w, slots + (i & 1) * Slot<NH>::bytes, rows, col, quad,
-                                  a.scale_log2);
+                                         a.scale_log2);
       rows = rows_next;
     }
   }
-  // The wave's slots become its columns' place; loads past its last block may still
-  // write them.
-  wait_loads<0>();
+  // The wave's slots become its columns' place.
   wait_reads();
 #pragma unroll
   for (int g = 0; g < NH; ++g) {
@@ -1108,6 +1146,10 @@ loom_status_t plan_mx4_decode(loom_paged_decode_plan_info_t *info, uint32_t team
   const uint64_t page_rows = s.page_size ? s.page_size : kPageSize;
   if (B > (uint64_t)kMaxBatch)
     return fail(err, LOOM_PLAN_STATE_COUNT_OUT_OF_RANGE, "batch_size", B);
+  uint64_t pool_rows;
+  if (__builtin_mul_overflow(s.max_num_pages * page_rows, hkv, &pool_rows) ||
+      pool_rows > UINT32_MAX)
+    return fail(err, LOOM_PLAN_STATE_COUNT_OUT_OF_RANGE, "paged batch-decode cache rows", pool_rows);
   info->group_tile = tile;
   info->group_tiles = (uint32_t)tiles;
   info->device_cus = (uint32_t)cus;
