@@ -164,8 +164,9 @@ enum DeviceStatus : int {
   kStatusAppendRefused = 2,
   kStatusWords = 4
 };
-// Arrival words of a queue.
-constexpr uint64_t kMx4Joins = 256;
+// Arrival words of a queue, and the bytes from one to the next: atomics on one
+// memory line wait for each other.
+constexpr uint64_t kMx4Joins = 256, kMx4JoinBytes = 256;
 
 // Bytes of the append validation workspace (one size for every plan).
 uint64_t append_workspace_bytes();

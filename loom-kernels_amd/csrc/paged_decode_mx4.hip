@@ -942,15 +942,16 @@ __global__ __launch_bounds__(kDirectWaves * 64) void mx4_decode_direct_kernel(Mx
   // for its own to arrive before the barrier behind which one thread counts the
   // workgroup.  A release fence instead writes the XCD's whole L2 back: 40 us here.
   auto arrive = [&]() {
+    uint32_t *const arrived = a.arrived + (uint64_t)head * (loom::kMx4JoinBytes / 4);
     wait_loads<0>();  // and stores
     __syncthreads();
     if (tid == 0)
-      s_arrived = __hip_atomic_fetch_add(&a.arrived[head], 1u, __ATOMIC_RELAXED,
+      s_arrived = __hip_atomic_fetch_add(arrived, 1u, __ATOMIC_RELAXED,
                                          __HIP_MEMORY_SCOPE_AGENT);
     __syncthreads();
     if (s_arrived != (uint32_t)a.splits - 1u) return;
     if (tid == 0)
-      __hip_atomic_store(&a.arrived[head], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      __hip_atomic_store(arrived, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     const int cols = NH * heads;
     const int parts = cols <= 1 ? 8 : cols <= 2 ? 4 : cols <= 4 ? 2 : 1;
     static_assert(W == 8, "parts");
@@ -1094,7 +1095,9 @@ __global__ __launch_bounds__(kDirectWaves * 64) void mx4_decode_direct_kernel(Mx
   if (a.splits > 1) arrive();
 }
 
-__global__ void mx4_decode_clear_kernel(uint32_t *arrived) { arrived[threadIdx.x] = 0u; }
+__global__ void mx4_decode_clear_kernel(uint32_t *arrived) {
+  arrived[threadIdx.x * (loom::kMx4JoinBytes / 4)] = 0u;
+}
 
 // kv-heads per wave: two neighbours where Hkv is even, in the balanced kernel always.
 uint64_t heads_per_wave(uint64_t hkv) { return hkv % 2 == 0 ? 2 : 1; }
@@ -1104,8 +1107,8 @@ uint64_t heads_per_wave(uint64_t hkv) { return hkv % 2 == 0 ? 2 : 1; }
 namespace loom {
 
 // The algorithm goes by the tokens a plan covers times Hkv (the rows of K to read).
-// Microseconds, direct / balanced, 32x8 heads unless said: 1 x 1000 tokens 8.3 / 11.6;
-// 1 x 32000 16.7 / 24.6; 16 x 256-1536 13.7 / 15.5; 64 x 256-1024 17.6 / 25.1; 16 x 4096
+// Microseconds, direct / balanced, 32x8 heads unless said: 1 x 1000 tokens 7.4 / 11.6;
+// 1 x 32000 14.4 / 24.6; 16 x 256-1536 13.7 / 15.5; 64 x 256-1024 17.6 / 25.1; 16 x 4096
 // 22.7 / 25.7; 64 x 1024-4096 (1.3 M rows) 49.8 / 46.6; 8 x 1000-32000 (1.1 M) 51.4 /
 // 36.3: a direct workgroup has one request's share, so unlike lengths cost it more.
 constexpr uint64_t kDirectRows = 1u << 20;
@@ -1114,14 +1117,15 @@ constexpr uint64_t kDirectRows = 1u << 20;
 // 2048 19.0 / 17.0; 64 x 256-1024 20.3 / 17.6; 1 x 32000 14.6 / 17.4; 4 x 8000 14.7 /
 // 16.7.
 constexpr uint64_t kDirectPairRows = 5u << 16;
-// Workgroups per (request, kv-heads, tile), of 8 waves each (16 were slower at every
-// size).  The walk shrinks with the splits and the join grows, so they are doubled while
-// their square stays within twice a request's blocks and the CUs hold them (4000 tokens in
-// 8, 16, 32: 10.3, 9.8, 11.4 us; 32000: 28.6, 18.6, 16.7; two per CU: no faster).  A join
-// costs 2.5 us, a wave's block about 1: splits that save less than kSplitFrom / 8 blocks a
-// wave are left out (one request of 200 tokens 5.8 us, in two 7.9; of 1000, 9.1 and in
-// eight 8.3; 16 of 1000, 11.4 and in two 14.0).
-constexpr uint64_t kMaxSplits = 64, kSplitFrom = 21;
+// Workgroups per (request, kv-heads, tile), of 8 waves each (4 and 16 were slower).  The
+// walk shrinks with the splits and the join grows, so they are doubled while their square
+// stays within twice a request's blocks and the CUs hold them (4000 tokens in 8, 16, 32:
+// 10.3, 9.8, 11.4 us; two per CU: no faster).  A join costs about 2 us, and 4 where every
+// CU joins at once; a wave's block costs 1.  Splits that save fewer than kSplitFrom / 8
+// blocks a wave are left out (one request of 200 tokens: 4.9 us, in two 7; of 1000, 7.9
+// and in eight 7.4), kSplitFromMany / 8 where the requests' own workgroups are more than
+// an eighth of the CUs (8 of 1000: 8.8, in four each 10.2; 16 of 2000: 12.6 and 13.1).
+constexpr uint64_t kMaxSplits = 64, kSplitFrom = 21, kSplitFromMany = 40;
 
 // The merge kernel's workgroups and their waves per head: one up to 48 states per request
 // on average (64 ragged requests, 5: 52.1 us, with four waves 55.5; 8 of 32k, 33: 56.8 and
@@ -1167,14 +1171,15 @@ loom_status_t plan_mx4_decode(loom_paged_decode_plan_info_t *info, uint32_t team
     while (heads <= kMx4Joins && splits < kMaxSplits && heads * splits * 2 <= (uint64_t)cus &&
            each >= 2 * splits * splits)
       splits *= 2;
-    if (each * (splits - 1) < kSplitFrom * splits) splits = 1;
+    const uint64_t from = heads * 8 <= (uint64_t)cus ? kSplitFrom : kSplitFromMany;
+    if (each * (splits - 1) < from * splits) splits = 1;
     const uint64_t grid = heads * splits;
     if (grid > (uint64_t)INT32_MAX || B * hq > (uint64_t)INT32_MAX)
       return fail(err, LOOM_PLAN_STATE_COUNT_OUT_OF_RANGE, "paged batch-decode", grid);
     info->algorithm = LOOM_PAGED_DECODE_DIRECT;
     info->teams = (uint32_t)(splits > 1 ? splits : 0);
     info->state_slots = splits > 1 ? splits * B : 0;
-    info->header_bytes = splits > 1 ? kMx4Joins * 4 : 0;
+    info->header_bytes = splits > 1 ? kMx4Joins * kMx4JoinBytes : 0;
     info->workspace_bytes =
         splits > 1 ? info->header_bytes + splits * B * hq * kMx4StateStride * 4 : 256;
     info->block_threads = kDirectWaves * 64;

@@ -232,7 +232,7 @@ loom_status_t init_queue_memory(loom_command_queue *q, loom_error_t *err) {
     e = hipHostGetDevicePointer(&d, h, 0);
   }
   static_assert(loom::kShareBytes % 256 == 0, "the workspace behind it stays aligned");
-  const uint64_t join_bytes = loom::kMx4Joins * 4;
+  const uint64_t join_bytes = loom::kMx4Joins * loom::kMx4JoinBytes;
   if (e == hipSuccess) e = hipMalloc(&w, loom::kShareBytes + ws_bytes + join_bytes);
   uint8_t *ws = w ? (uint8_t *)w + loom::kShareBytes : nullptr;
   if (e == hipSuccess) {
