@@ -715,19 +715,20 @@ struct NormForm {
                                              int off, int row, int c, const Angles &s,
                                              const RowSlice &sl) {
     if (row < a.hq)
-      q_row(a, w, t, row, c, s, sl.x);
+      __builtin_nontemporal_store(
+          q_row(a, w, c, s, sl.x),
+          reinterpret_cast<u32x4 *>(a.q_out + ((int64_t)t * a.hq + row) * 128 + c * 8));
     else
       kv_row(a, w, page, off, row - a.hq, c, s, sl);
   }
-  static __device__ __forceinline__ void q_row(const Args &a, const Weights &w, int t, int row,
-                                               int c, const Angles &s, const u32x4 &x) {
+  static __device__ __forceinline__ u32x4 q_row(const Args &a, const Weights &w, int c,
+                                                const Angles &s, const u32x4 &x) {
     float y[8];
     norm_rotate<float>(x, w.q, a.q_norm != nullptr, a.eps, c, s.sin, s.cos, y);
     u32x4 o;
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[e] = loom_dev::bf16x2_pack(y[2 * e], y[2 * e + 1]);
-    __builtin_nontemporal_store(
-        o, reinterpret_cast<u32x4 *>(a.q_out + ((int64_t)t * a.hq + row) * 128 + c * 8));
+    return o;
   }
   static __device__ __forceinline__ void kv_row(const Args &a, const Weights &w, int64_t page,
                                                 int off, int kh, int c, const Angles &s,
@@ -809,40 +810,57 @@ struct WaveSlices {
   u32x4 q[kWaveRows];
   RowSlice kv;
 };
-__device__ __forceinline__ u32x4 load_q(const AppendArgs &a, int t, int row, int c) {
-  const u32x4 none = {0, 0, 0, 0};
-  return row < a.hq
-             ? *reinterpret_cast<const u32x4 *>(a.q + ((int64_t)t * a.hq + row) * 128 + c * 8)
-             : none;
-}
-__device__ __forceinline__ WaveSlices load_wave_slices(const AppendArgs &a, int t, int lane) {
+// A token's rows: range-limited loads and stores, zeros past the last row.  (With
+// branches instead, the compiler can no longer tell which of a turn's loads have to have
+// arrived, and waits for all.)
+struct TokenRows {
+  __amdgpu_buffer_rsrc_t q, k, v, out;
+  __device__ __forceinline__ TokenRows(const AppendArgs &a, int t)
+      : q(rows(a.q, t, a.hq)), k(rows(a.k, t, a.hkv)), v(rows(a.v, t, a.hkv)),
+        out(rows(a.q_out, t, a.hq)) {}
+  static __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows(const uint16_t *base, int t,
+                                                                int heads) {
+    return __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<uint16_t *>(base + (int64_t)t * heads * 128), 0, heads * 256, 0x00020000);
+  }
+  __device__ __forceinline__ u32x4 load_q(int row, int c) const {
+    return loom_dev::load16_rows<false>(q, row * 256 + c * 16);
+  }
+  __device__ __forceinline__ void store_q(int row, int c, const u32x4 &x) const {
+    __builtin_amdgcn_raw_buffer_store_b128(x, out, row * 256 + c * 16, 0, 2);  // nontemporal
+  }
+  __device__ __forceinline__ RowSlice load_kv(int row, int c) const {
+    return {loom_dev::load16_rows<false>(k, row * 256 + c * 16),
+            loom_dev::load16_rows<false>(v, row * 256 + c * 16)};
+  }
+};
+__device__ __forceinline__ WaveSlices load_wave_slices(const TokenRows &rows, int lane) {
   WaveSlices f;
+  f.kv = rows.load_kv(lane >> 4, lane & 15);
 #pragma unroll
-  for (int i = 0; i < kWaveRows; ++i) f.q[i] = load_q(a, t, (lane >> 4) + 4 * i, lane & 15);
-  f.kv = load_slice(a, t, a.hq + (lane >> 4), lane & 15);
+  for (int i = 0; i < kWaveRows; ++i) f.q[i] = rows.load_q((lane >> 4) + 4 * i, lane & 15);
   return f;
 }
 template <class Form>
-__device__ __forceinline__ void apply_token_wave(const typename Form::Args &a, int t, int64_t page,
-                                                 int off, int lane, const typename Form::Angles &s,
-                                                 const typename Form::Weights &w, WaveSlices pre) {
-  const int c = lane & 15;
+__device__ __forceinline__ void apply_token_wave(const typename Form::Args &a, const TokenRows &rows,
+                                                 int64_t page, int off, int lane,
+                                                 const typename Form::Angles &s,
+                                                 typename Form::Weights w, WaveSlices pre) {
+  const int c = lane & 15, r = lane >> 4;
+  // Ends these loads here (they have long arrived), for the same reason.
+  asm volatile("" : "+v"(w.q), "+v"(w.k), "+v"(pre.kv.x), "+v"(pre.kv.v));
 #pragma unroll 1
-  for (int row = lane >> 4; row < a.hq; row += 4 * kWaveRows)
+  for (int row = 0; row < a.hq; row += 4 * kWaveRows)
 #pragma unroll
     for (int i = 0; i < kWaveRows; ++i) {
-      const int at = row + 4 * i;
-      if (at < a.hq) {
-        const u32x4 x = pre.q[i];
-        pre.q[i] = load_q(a, t, at + 4 * kWaveRows, c);
-        Form::q_row(a, w, t, at, c, s, x);
-      }
+      const int at = row + 4 * i + r;
+      rows.store_q(at, c, Form::q_row(a, w, c, s, pre.q[i]));
+      pre.q[i] = rows.load_q(at + 4 * kWaveRows, c);  // into the registers just read
     }
 #pragma unroll 1
-  for (int row = a.hq + (lane >> 4); row < a.hq + a.hkv; row += 4) {
-    const RowSlice now = pre.kv;
-    pre.kv = load_slice(a, t, row + 4, c);
-    Form::kv_row(a, w, page, off, row - a.hq, c, s, now);
+  for (int row = r; row - r < a.hkv; row += 4) {
+    if (row < a.hkv) Form::kv_row(a, w, page, off, row, c, s, pre.kv);
+    pre.kv = rows.load_kv(row + 4, c);
   }
 }
 
@@ -950,7 +968,7 @@ void append_validated_kernel(typename Form::Args a) {
   // token workgroup: of one token, or of one per wave (past the last: none)
   const int wg = blockIdx.x - a.validate_blocks;
   const int wave = kPerWave ? tid >> 6 : 0, lane = kPerWave ? tid & 63 : tid;
-  const int own = kPerWave ? wg * (kApplyThreads / 64) + wave : wg;
+  const int own = kPerWave ? wg * (kApplyThreads / 64) + loom_dev::uni(wave) : wg;
   const int t = kPerWave ? min(own, a.tokens - 1) : own;
   // The token's own slot and position (the validation chunks check the same
   // walk; nothing is written unless they all pass).
@@ -966,9 +984,10 @@ void append_validated_kernel(typename Form::Args a) {
   // Row loads after the walk: the validation's dependent loads run while the
   // memory system is not yet flooded with the command's row traffic, and the
   // rows still arrive before the verdicts.
+  const TokenRows rows(a, t);
   const auto first = [&] {
     if constexpr (kPerWave)
-      return load_wave_slices(a, t, lane);
+      return load_wave_slices(rows, lane);
     else
       return load_first_slices(a, t, tid);
   }();
@@ -998,7 +1017,7 @@ void append_validated_kernel(typename Form::Args a) {
   __syncthreads();
   if (s_bad || own >= a.tokens) return;
   if constexpr (kPerWave)
-    apply_token_wave<Form>(a, t, page, off, lane, s_angles[wave], w8, first);
+    apply_token_wave<Form>(a, rows, page, off, lane, s_angles[wave], w8, first);
   else
     apply_token<Form>(a, t, page, off, tid, s_angles[0], w8, first);
 }

@@ -81,13 +81,16 @@ class Append:
                 y[name] = dev(t, p)
         return x, y
 
-    def run(self, flags=0, workspace=False, change=None):
+    def run(self, flags=0, workspace=False, change=None, odd_output=False):
         t = self.torch
         plan = self.L.RopeProvider.load(0).plan_norm_paged_append(self.spec(), flags=flags)
         queue = self.L.CommandQueue(t.cuda.current_stream(), 4)
         x, y = self.operands()
         if change:
             change(x)
+        if odd_output:  # the rotated queries one element past an aligned start
+            y["query_output"] = t.full((y["query_output"].numel() + 1,), 7.0, dtype=t.bfloat16,
+                                       device="cuda")[1:]
         if workspace:
             y["workspace"] = t.zeros(plan.workspace_bytes, dtype=t.uint8, device="cuda")
         b = queue.bindings(20)
@@ -199,6 +202,23 @@ def test_commands_of_many_tokens(env, heads, dtype, norm):
     if heads == (6, 3):
         two = a.run(flags=env[1].PLAN_APPEND_TWO_LAUNCH)
         assert all(np.array_equal(got[k], two[k]) for k in got)
+
+
+@pytest.mark.parametrize("rows", [3, 90, 1300])
+def test_rows_on_two_byte_boundaries(env, rows):
+    """The append's operands need no alignment beyond their elements'."""
+    torch = env[0]
+    a = Append(env, 65, [rows + 9], [rows], 6, 3)
+    plain = a.run()
+
+    def shift(x):
+        for n in ("query", "key", "value", "query_norm", "key_norm"):
+            b = torch.empty(x[n].numel() + 9, dtype=torch.bfloat16, device="cuda")
+            b[1:1 + x[n].numel()] = x[n].flatten()
+            x[n] = b[1:1 + x[n].numel()]
+    a.check(plain)
+    got = a.run(change=shift, odd_output=True)
+    assert all(np.array_equal(got[k], plain[k]) for k in got)
 
 
 @pytest.mark.parametrize("dtype", ["mxfp4", "bf16"])
