@@ -12,8 +12,8 @@
 // rows' own for batches below 64, else a search first), then 16 lanes per head row
 // load 4 code bytes each and store 16 bytes, K and V together, the heads of a row
 // contiguous.  The stores are streamed past L2: plain ones, whose lines L2 writes
-// back in another order, took 41 us instead of 27.5 (38k rows of 8 kv-heads, HND
-// pages of 64: 5.9 TB/s).
+// back in another order, took 41 us instead of 27.1 (38k rows of 8 kv-heads, HND
+// pages of 64: 6.0 TB/s).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -31,11 +31,12 @@ constexpr int kReadMaxRows = 64;  // output rows per workgroup: at most one per 
 constexpr uint64_t kReadMaxHeads = 4096;
 // Head rows per workgroup, and how many of them each 16 lanes have in flight.
 // Measured with 16 to 256 head rows and 1 to 4 in flight: 64 are within 4% of the
-// best from 8k rows of 8 kv-heads (8.8 us) to 38k (27.5 us); 256 take 8 us where
-// 64 take 4.5 (300 rows of 32 kv-heads), 16 lose 5% of the large ones.  The number
-// in flight changes less than 3%.
+// best from 8k rows of 8 kv-heads (8.3 us) to 38k (27.1 us); 256 take 8 us where
+// 64 take 4.5 (300 rows of 32 kv-heads), 16 lose 5% of the large ones.  Four in
+// flight against one: 64 scattered rows of 8 kv-heads and their append 11.6 and
+// 11.8 us, about 1000 14.4 and 14.8.
 constexpr int kReadItems = 64;
-constexpr int kReadDepth = 2;
+constexpr int kReadDepth = 4;
 
 struct ReadArgs {
   const uint8_t *k;
@@ -142,23 +143,26 @@ __global__ __launch_bounds__(kReadThreads) void paged_kv_read_kernel(ReadArgs a)
   const int64_t page_bytes = (int64_t)a.page_rows * a.hkv * 64;
   const int items = rows * a.hkv;
   constexpr int kStep = kReadThreads / 16;
+#pragma unroll 1
   for (int i0 = tid >> 4; i0 < items; i0 += kStep * kReadDepth) {
     Part part[kReadDepth];
     int64_t out[kReadDepth];
+    // Loads without branches: rows that are not written read some row of the pool.  (A
+    // branch round them makes the compiler wait for one turn's before the next.)
 #pragma unroll
     for (int u = 0; u < kReadDepth; ++u) {
-      const int i = i0 + u * kStep;
-      const int j = min(a.hkv == 1 ? i : (int)__umulhi((uint32_t)i, a.hkv_inv), kReadMaxRows - 1);
-      const int page = i < items ? s_page[j] : -1, off = s_off[j];
-      const int h = i - j * a.hkv;
-      out[u] = page < 0 ? -1 : ((int64_t)(t0 + j) * a.hkv + h) * 128 + c * 8;
-      if (page >= 0) {
-        const int64_t at =
-            page * page_bytes + (int64_t)h * a.head_bytes + (int64_t)off * a.row_bytes + c * 4;
-        const int64_t sc = ((((int64_t)page * a.hkv + h) * a.page_rows + off) << 2) + (c >> 2);
-        part[u] = {*reinterpret_cast<const uint32_t *>(a.k + at),
-                   *reinterpret_cast<const uint32_t *>(a.v + at), a.k_mx[sc], a.v_mx[sc]};
-      }
+      const int i = min(i0 + u * kStep, items - 1);
+      const int j = a.hkv == 1 ? i : (int)__umulhi((uint32_t)i, a.hkv_inv);
+      const int page = s_page[j], off = s_off[j], h = i - j * a.hkv;
+      const int64_t pg = max(page, 0);
+      out[u] = page < 0 || i0 + u * kStep >= items
+                   ? -1
+                   : ((int64_t)(t0 + j) * a.hkv + h) * 128 + c * 8;
+      const int64_t at =
+          pg * page_bytes + (int64_t)h * a.head_bytes + (int64_t)off * a.row_bytes + c * 4;
+      const int64_t sc = (((pg * a.hkv + h) * a.page_rows + off) << 2) + (c >> 2);
+      part[u] = {*reinterpret_cast<const uint32_t *>(a.k + at),
+                 *reinterpret_cast<const uint32_t *>(a.v + at), a.k_mx[sc], a.v_mx[sc]};
     }
 #pragma unroll
     for (int u = 0; u < kReadDepth; ++u)

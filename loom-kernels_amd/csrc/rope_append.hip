@@ -1312,10 +1312,10 @@ constexpr int kAppendOperands = 17;
 // command of more tokens than the chip holds workgroups gives each wave a token
 // instead: with one per workgroup the metadata walk, the angles (one wave of four)
 // and the wait for the verdicts are paid once per round of workgroups (8192 tokens
-// of 64 + 8 heads, MXFP4 pages, with their read-back: 101 us, here 81; 2048 of
-// 32 + 8: 23.2 and 18.7; BF16 pages 14.8 and 12.4), while below it a wave alone has
-// more rows to go through (500 tokens of 32 + 8: 14.4 us, 12.2 with a workgroup
-// each).
+// of 64 + 8 heads, MXFP4 pages, with their read-back: 97 us, here 75; 4096 of
+// 32 + 8: 35.1 and 26.9; 2048 into BF16 pages 14.6 and 12.4), while below it a
+// wave alone has more rows to go through (500 tokens of 32 + 8: 13.9 us, 12.2 with
+// a workgroup each).
 template <class Form>
 loom_status_t launch_append(const loom_rope_append_plan_t *plan, loom_command_scope_t *scope,
                             const typename Form::Args &a, loom_error_t *err) {
