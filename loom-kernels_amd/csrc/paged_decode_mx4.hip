@@ -30,12 +30,12 @@
 //             into `teams` equal ranges; a team is one wave per (kv-heads, tile), all
 //             walking the same blocks.  Requests that cross a range leave states, which
 //             a second kernel merges.  Bound by memory: 64 requests of 512-8192 tokens
-//             (32 / 8 heads, 254 MB) 52.0 us, 47.6 without the merge (5.3 TB/s; a large
-//             copy reaches 5.1); 8 of 32768 (64 / 8, 286 MB) 57 us.
+//             (32 / 8 heads, 254 MB) 52.3 us, 47.6 without the merge (5.3 TB/s; a large
+//             copy reaches 5.1); 8 of 32768 (64 / 8, 286 MB) 56 us.
 //   direct    one workgroup per (request, kv-heads, tile[, split]): its waves take the
 //             blocks in turn and merge in LDS, the last split of a request the splits.
-//             One launch.  Bound by latency: one request of 200 tokens 5.8 us, 16 of
-//             256-1536 13.4 (32 / 8 heads), 5 of 1-5003 (28 / 4) 10.3.
+//             One launch.  Bound by latency: one request of 200 tokens 4.9 us, 16 of
+//             256-1536 11.3 (32 / 8 heads), 5 of 1-5003 (28 / 4) 9.5.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -899,8 +899,8 @@ __global__ __launch_bounds__(kThreads) void mx4_decode_merge_kernel(Mx4DecodeArg
 
 // ---- direct --------------------------------------------------------------------------
 // Wave w of the workgroup takes blocks w, w + W, ... of its split's share of the request,
-// two in flight; the wave states merge in LDS.  (One request of 100 tokens: 5.2 us, of
-// 1000 without splits 9.1: a block in each of two waves of a SIMD, about 1 us.)
+// two in flight; the wave states merge in LDS.  (One request of 200 tokens: 4.9 us, of
+// 1000 without splits 7.9: a block in each of two waves of a SIMD, about 1 us.)
 constexpr int kDirectWaves = 8;
 constexpr int kStash = 132;  // floats between two columns' O in LDS
 

@@ -521,9 +521,9 @@ __device__ __forceinline__ void apply_row(const AppendArgs &a, int t, int64_t pa
 // two wide, and values near the border of two codes would otherwise go either way.
 //
 // Bound by memory in large commands: 8192 tokens of 64 + 8 heads into MXFP4 pages (311 MB)
-// 71 us, 4.4 TB/s, the VALU busy for more than half of it (a fifth fewer instructions
-// changed nothing); into BF16 pages (335 MB) 68 us, 4.9 TB/s.  Small ones by the guards'
-// chain: 64 tokens of 32 + 8 heads 7.5 us, about 1000 11.7.
+// 65 us, 4.8 TB/s, the VALU busy for more than half of it (a fifth fewer instructions
+// changed nothing); into BF16 pages (335 MB) 67 us, 5.0 TB/s.  Small ones by the guards'
+// chain: 64 tokens of 32 + 8 heads 7.5 us, about 1000 10.4.
 // Row c ^ 8 of the same 16 lanes (a rotation by 8), and sums over the 16 lanes
 // and maxima over 4 of them (the lanes of one MXFP4 block), on DPP.
 __device__ __forceinline__ uint32_t dpp_other_half(uint32_t x) {
