@@ -1108,19 +1108,20 @@ namespace loom {
 
 // The algorithm goes by the tokens a plan covers times Hkv (the rows of K to read).
 // Microseconds, direct / balanced, 32x8 heads unless said: 1 x 1000 tokens 7.4 / 11.6;
-// 1 x 32000 14.4 / 24.6; 16 x 256-1536 13.7 / 15.5; 64 x 256-1024 17.6 / 25.1; 16 x 4096
-// 22.7 / 25.7; 64 x 1024-4096 (1.3 M rows) 49.8 / 46.6; 8 x 1000-32000 (1.1 M) 51.4 /
-// 36.3: a direct workgroup has one request's share, so unlike lengths cost it more.
+// 1 x 32000 14.4 / 23.5; 16 x 256-1536 11.5 / 15.5; 64 x 256-1024 15.8 / 21.9; 16 x 4096
+// 20.8 / 22.7; 64 x 1024-4096 (1.3 M rows) 45.4 / 40.4; 8 x 1000-32000 (1.1 M) 44.7 /
+// 38.4: a direct workgroup has one request's share, so unlike lengths cost it more.
 constexpr uint64_t kDirectRows = 1u << 20;
 // Direct workgroups over NHD pages take two kv-heads from this many rows on, where whole
-// cache lines outweigh the halved parallelism (one / two): 16 x 1024 13.9 / 13.1; 16 x
-// 2048 19.0 / 17.0; 64 x 256-1024 20.3 / 17.6; 1 x 32000 14.6 / 17.4; 4 x 8000 14.7 /
-// 16.7.
+// cache lines outweigh the halved parallelism (one / two): 16 x 256-1536 (below it) 11.5 /
+// 15.9; 64 x 256-1024 19.1 / 15.8; 16 x 4096 28.3 / 20.8, of 64 / 8 heads 27.8 / 22.2;
+// but 32 x 512-4096 of 64 / 8 28.7 / 34.4.
 constexpr uint64_t kDirectPairRows = 5u << 16;
 // Workgroups per (request, kv-heads, tile), of 8 waves each (4 and 16 were slower).  The
 // walk shrinks with the splits and the join grows, so they are doubled while their square
-// stays within twice a request's blocks and the CUs hold them (4000 tokens in 8, 16, 32:
-// 10.3, 9.8, 11.4 us; two per CU: no faster).  A join costs about 2 us, and 4 where every
+// stays within twice a request's blocks and the CUs hold them (1000 tokens in 8, 16, 32:
+// 7.4, 7.4, 8.3 us; 8000: 11.3, 9.4, 9.5; 32000: 23.0, 15.8, 14.4; two per CU: no faster).
+// A join costs about 2 us, and 4 where every
 // CU joins at once; a wave's block costs 1.  Splits that save fewer than kSplitFrom / 8
 // blocks a wave are left out (one request of 200 tokens: 4.9 us, in two 7; of 1000, 7.9
 // and in eight 7.4), kSplitFromMany / 8 where the requests' own workgroups are more than
