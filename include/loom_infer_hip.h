@@ -473,7 +473,7 @@ typedef struct loom_paged_decode_plan_info {
   uint64_t state_slots;      /* balanced: teams + batch; split direct: teams * batch */
   uint64_t workspace_bytes;  /* header_bytes + state_slots * Hq * 132 FP32 */
   uint64_t header_bytes;     /* (batch + 2) int64 page prefixes, 256-byte rounded; split
-                                direct MXFP4 plans: 256 arrival words */
+                                direct MXFP4 plans: 256 arrival words, 256 bytes each */
   uint32_t block_threads;
   uint32_t grid_blocks;
   uint32_t device_cus;

@@ -1121,11 +1121,11 @@ constexpr uint64_t kDirectPairRows = 5u << 16;
 // walk shrinks with the splits and the join grows, so they are doubled while their square
 // stays within twice a request's blocks and the CUs hold them (1000 tokens in 8, 16, 32:
 // 7.4, 7.4, 8.3 us; 8000: 11.3, 9.4, 9.5; 32000: 23.0, 15.8, 14.4; two per CU: no faster).
-// A join costs about 2 us, and 4 where every
-// CU joins at once; a wave's block costs 1.  Splits that save fewer than kSplitFrom / 8
-// blocks a wave are left out (one request of 200 tokens: 4.9 us, in two 7; of 1000, 7.9
-// and in eight 7.4), kSplitFromMany / 8 where the requests' own workgroups are more than
-// an eighth of the CUs (8 of 1000: 8.8, in four each 10.2; 16 of 2000: 12.6 and 13.1).
+// A join costs about 2 us, and 4 where every CU joins at once; a wave's block costs 1.
+// Splits that save fewer than kSplitFrom / 8 blocks a wave are left out (one request of
+// 700 tokens: 6.9 us, split 8.1; of 1000, 8.1 and in eight 7.4), kSplitFromMany / 8 where
+// the requests' own workgroups are more than an eighth of the CUs (8 of 1000: 8.8, in
+// four each 10.2; 16 of 2000: 12.6 and 13.1).
 constexpr uint64_t kMaxSplits = 64, kSplitFrom = 21, kSplitFromMany = 40;
 
 // The merge kernel's workgroups and their waves per head: one up to 48 states per request
