@@ -25,7 +25,8 @@ FLAGS=(--offload-arch=gfx950 -O1 -g -std=c++17 -fPIC -Wall -Wno-unused-function 
        -Wno-unused-result -Xclang -target-feature -Xclang -packed-fp32-ops
        -I"$root/include" -I"$csrc")
 pids=()
-for s in contract.cpp runtime.cpp paged_decode.hip paged_prefill.hip rope_append.hip; do
+for s in contract.cpp runtime.cpp paged_decode.hip paged_decode_mx4.hip paged_prefill.hip kv_read.hip \
+         rope_append.hip; do
   "$HIPCC" -x hip "${FLAGS[@]}" "${HOSTSAN[@]}" -c "$csrc/$s" -o "$out/obj/${s%.*}.o" \
       2> >(grep -v "packed-fp32-ops' is not a recognized feature" >&2) &
   pids+=($!)
