@@ -1175,7 +1175,8 @@ loom_status_t plan_mx4_decode(loom_paged_decode_plan_info_t *info, uint32_t team
     const uint64_t from = heads * 8 <= (uint64_t)cus ? kSplitFrom : kSplitFromMany;
     if (each * (splits - 1) < from * splits) splits = 1;
     const uint64_t grid = heads * splits;
-    if (grid > (uint64_t)INT32_MAX || B * hq > (uint64_t)INT32_MAX)
+    // (a launch holds fewer than 2^32 threads)
+    if (grid > UINT32_MAX / (kDirectWaves * 64) || B * hq > (uint64_t)INT32_MAX)
       return fail(err, LOOM_PLAN_STATE_COUNT_OUT_OF_RANGE, "paged batch-decode", grid);
     info->algorithm = LOOM_PAGED_DECODE_DIRECT;
     info->teams = (uint32_t)(splits > 1 ? splits : 0);
