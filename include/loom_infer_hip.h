@@ -558,7 +558,11 @@ typedef struct loom_mxfp4_paged_batch_decode_args {
   loom_handle_t lse;           /* Write<f32>  [B, Hq], log2 domain */
   loom_handle_t workspace;     /* Write<u8>   [plan workspace_bytes], or {0, 0}: the states lie
                                   in the queue's workspace, as for
-                                  loom_paged_decode_enqueue_bf16 */
+                                  loom_paged_decode_enqueue_bf16 (none are kept by plans
+                                  with state_slots 0).  Captured by the caller into a graph
+                                  of its own, a command without this operand uses no
+                                  memory of the queue and runs in the direct form unsplit,
+                                  slower over long requests */
 } loom_mxfp4_paged_batch_decode_args_t;
 
 /* Paged decode of a plan whose spec names LOOM_KV_DTYPE_MXFP4: the same command,

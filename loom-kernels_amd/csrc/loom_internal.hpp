@@ -147,9 +147,9 @@ static_assert(1024 * 8 * kStateWidth * 4 <= kShareBytes, "single decode's partit
 // the queue's other commands, nor bound to its lifetime.  (A graph queue's
 // capture has the buffer of its private queue, which the graph owns.)
 uint8_t *queue_shares(loom_command_scope *scope, uint64_t bytes);
-// The queue's arrival words for a command of the scope, or null under the same
-// capture by the caller.
-uint32_t *queue_joins(loom_command_scope *scope);
+// Whether the scope's commands run in the queue's order: not under that capture by
+// the caller.
+bool in_queue_order(const loom_command_scope *scope);
 
 // Device status words of a command queue (loom_command_queue::status_*).
 enum DeviceStatus : int {

@@ -1670,8 +1670,16 @@ loom_status_t paged_decode_enqueue_impl(const loom_paged_decode_plan_t *plan,
     return fail(err, LOOM_ENQ_MISALIGNED_BUFFER, "kv_scales", (int64_t)l(9)->ptr, 4);
 
   uint8_t *ws = nullptr;
+  // A command that the caller captures into a graph of its own is not in the queue's
+  // order: replayed beside the queue's own commands it would share their scratch, header,
+  // states and arrival words.  MXFP4 commands without a workspace operand run there in the
+  // direct form, unsplit, which needs none; nor do plans without states anywhere.
+  const bool in_order = !mx4 || pi.state_slots == 0 || loom::in_queue_order(scope);
   if (where == DecodeWorkspace::kOperand) {
     ws = (uint8_t *)l(8)->ptr;
+  } else if (mx4 && (pi.state_slots == 0 || !in_order)) {
+    if (loom::mx4_direct_grid(pi, 1) == 0)
+      return fail(err, LOOM_ENQ_WORKSPACE_NOT_RESERVED, "workspace", 0, pi.workspace_bytes);
   } else if (where == DecodeWorkspace::kQueue) {
     rc = loom::queue_workspace(scope->queue, pi.workspace_bytes, false, &ws, err);
     if (rc) return rc;
@@ -1696,8 +1704,10 @@ loom_status_t paged_decode_enqueue_impl(const loom_paged_decode_plan_t *plan,
     m.last = (const int32_t *)l(5)->ptr;
     m.out = (uint16_t *)l(6)->ptr;
     m.lse = (float *)l(7)->ptr;
-    m.header = (int64_t *)ws;
-    m.states = (float *)(ws + pi.header_bytes);
+    if (ws) {
+      m.header = (int64_t *)ws;
+      m.states = (float *)(ws + pi.header_bytes);
+    }
     m.pool = (int64_t)s.max_num_pages;
     m.n_indices = (int64_t)l(4)->numel;
     m.indices_capacity = (pi.flags & LOOM_PLAN_PAGE_INDICES_CAPACITY) ? 1 : 0;
@@ -1708,17 +1718,16 @@ loom_status_t paged_decode_enqueue_impl(const loom_paged_decode_plan_t *plan,
     m.tile = (int32_t)pi.group_tile;
     m.tiles = (int32_t)pi.group_tiles;
     m.teams = (int32_t)pi.teams;
-    m.splits = pi.algorithm == LOOM_PAGED_DECODE_DIRECT && pi.teams > 1 ? (int32_t)pi.teams : 1;
+    m.splits =
+        ws && pi.algorithm == LOOM_PAGED_DECODE_DIRECT && pi.teams > 1 ? (int32_t)pi.teams : 1;
     m.page_rows = (int32_t)page_rows;
     const bool head_major = s.kv_layout == LOOM_KV_LAYOUT_HND;
     m.head_bytes = head_major ? m.page_rows * 64 : 64;
     m.row_bytes = head_major ? 64 : m.hkv * 64;
     m.scale_log2 = s.softmax_scale * 1.44269504088896340736f;
-    // A command that the caller captures into a graph of its own is not in the
-    // queue's order: its arrival words are the workspace's, cleared by every replay.
-    m.arrived = m.splits > 1 ? loom::queue_joins(scope) : nullptr;
-    const bool clear = m.splits > 1 && !m.arrived;
-    if (clear) m.arrived = (uint32_t *)ws;
+    // out of order the arrival words are the operand's, cleared by every replay
+    const bool clear = m.splits > 1 && !in_order;
+    if (m.splits > 1) m.arrived = clear ? (uint32_t *)ws : scope->queue->joins;
     return loom::record_launch(
         scope, loom::launch_mx4_decode(pi, m, clear, scope->queue->stream), err);
   }

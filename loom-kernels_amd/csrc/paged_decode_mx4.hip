@@ -1128,6 +1128,21 @@ constexpr uint64_t kDirectPairRows = 5u << 16;
 // four each 10.2; 16 of 2000: 12.6 and 13.1).
 constexpr uint64_t kMaxSplits = 64, kSplitFrom = 21, kSplitFromMany = 40;
 
+// kv-heads per direct workgroup.
+static uint64_t direct_heads(const loom_paged_decode_plan_info_t &info) {
+  const loom_paged_decode_spec_t &s = info.spec;
+  const uint64_t page_rows = s.page_size ? s.page_size : kPageSize;
+  return s.kv_layout != LOOM_KV_LAYOUT_HND && s.num_kv_heads % 2 == 0 &&
+                 info.max_total_pages * page_rows * s.num_kv_heads >= kDirectPairRows
+             ? 2
+             : 1;
+}
+uint64_t mx4_direct_grid(const loom_paged_decode_plan_info_t &info, uint64_t splits) {
+  const uint64_t grid = info.spec.batch_size * (info.spec.num_kv_heads / direct_heads(info)) *
+                        info.group_tiles * splits;
+  return grid <= UINT32_MAX / (kDirectWaves * 64) ? grid : 0;
+}
+
 // The merge kernel's workgroups and their waves per head: one up to 48 states per request
 // on average (64 ragged requests, 5: 52.1 us, with four waves 55.5; 8 of 32k, 33: 56.8 and
 // 57.6).
@@ -1165,8 +1180,9 @@ loom_status_t plan_mx4_decode(loom_paged_decode_plan_info_t *info, uint32_t team
     return fail(err, LOOM_PLAN_STATE_COUNT_OUT_OF_RANGE, "paged batch-decode blocks", blocks);
   const uint64_t rows = info->max_total_pages * page_rows * hkv;
   if (teams_option == 0 && rows <= kDirectRows) {
-    const bool pair = s.kv_layout != LOOM_KV_LAYOUT_HND && hkv % 2 == 0 && rows >= kDirectPairRows;
-    const uint64_t heads = B * (hkv / (pair ? 2 : 1)) * tiles;
+    const uint64_t heads = mx4_direct_grid(*info, 1);
+    if (heads == 0 || B * hq > (uint64_t)INT32_MAX)
+      return fail(err, LOOM_PLAN_STATE_COUNT_OUT_OF_RANGE, "paged batch-decode", B * hq);
     uint64_t splits = 1;
     const uint64_t each = blocks / B;
     while (heads <= kMx4Joins && splits < kMaxSplits && heads * splits * 2 <= (uint64_t)cus &&
@@ -1174,10 +1190,7 @@ loom_status_t plan_mx4_decode(loom_paged_decode_plan_info_t *info, uint32_t team
       splits *= 2;
     const uint64_t from = heads * 8 <= (uint64_t)cus ? kSplitFrom : kSplitFromMany;
     if (each * (splits - 1) < from * splits) splits = 1;
-    const uint64_t grid = heads * splits;
-    // (a launch holds fewer than 2^32 threads)
-    if (grid > UINT32_MAX / (kDirectWaves * 64) || B * hq > (uint64_t)INT32_MAX)
-      return fail(err, LOOM_PLAN_STATE_COUNT_OUT_OF_RANGE, "paged batch-decode", grid);
+    const uint64_t grid = heads * splits;  // (split ones are at most the CUs)
     info->algorithm = LOOM_PAGED_DECODE_DIRECT;
     info->teams = (uint32_t)(splits > 1 ? splits : 0);
     info->state_slots = splits > 1 ? splits * B : 0;
@@ -1227,11 +1240,9 @@ hipError_t launch_mx4_decode(const loom_paged_decode_plan_info_t &info, const Mx
   // in the other form 13.7; 64 of 2000-4000, 16 / 4: 30.0 and 33.0; 64 of 512-8192: 52.1
   // and 51.7).
   const bool p16 = a.page_rows == 16, quads = a.tile <= 4;
-  const dim3 grid(info.grid_blocks);
-  if (info.algorithm == LOOM_PAGED_DECODE_DIRECT) {
-    // the plan's grid says how many kv-heads its workgroups take
-    const bool pair = (uint64_t)info.grid_blocks * 2 ==
-                      (uint64_t)a.batch * a.hkv * a.tiles * (uint64_t)a.splits;
+  if (info.algorithm == LOOM_PAGED_DECODE_DIRECT || !a.states) {
+    const dim3 grid((unsigned)mx4_direct_grid(info, (uint64_t)a.splits));
+    const bool pair = direct_heads(info) == 2;
     auto kernel = quads ? (pair ? direct_kernel<2, kPair, true>(p16)
                                 : direct_kernel<1, kSplit, true>(p16))
                   : pair ? direct_kernel<2, kPair, false>(p16)
@@ -1241,7 +1252,7 @@ hipError_t launch_mx4_decode(const loom_paged_decode_plan_info_t &info, const Mx
       const hipError_t e = hipGetLastError();
       if (e != hipSuccess) return e;
     }
-    hipLaunchKernelGGL(kernel, grid, dim3(info.block_threads), 0, stream, a);
+    hipLaunchKernelGGL(kernel, grid, dim3(kDirectWaves * 64), 0, stream, a);
     return hipGetLastError();
   }
   const bool nhd = info.spec.kv_layout != LOOM_KV_LAYOUT_HND, one = heads_per_wave(a.hkv) == 1;
@@ -1251,7 +1262,7 @@ hipError_t launch_mx4_decode(const loom_paged_decode_plan_info_t &info, const Mx
                 : one ? split_kernel<1, kSplit, false>(p16)
                 : nhd ? split_kernel<2, kPair, false>(p16)
                       : split_kernel<2, kSplit, false>(p16);
-  hipLaunchKernelGGL(kernel, grid, dim3(kThreads), 0, stream, a);
+  hipLaunchKernelGGL(kernel, dim3(info.grid_blocks), dim3(kThreads), 0, stream, a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;
   const MergeGrid m = merge_grid((uint64_t)a.batch, (uint64_t)a.hq, (uint64_t)a.teams);

@@ -143,9 +143,7 @@ loom_status_t queue_workspace(loom_command_queue *q, uint64_t bytes, bool zeroed
   return LOOM_OK;
 }
 
-// Whether the scope's commands run in the queue's order: not if the caller captures
-// its stream into a graph of its own.
-static bool in_queue_order(const loom_command_scope *scope) {
+bool in_queue_order(const loom_command_scope *scope) {
   if (scope->capturing) return true;
   hipStreamCaptureStatus cap = hipStreamCaptureStatusNone;
   if (hipStreamIsCapturing(scope->queue->stream, &cap) != hipSuccess) {
@@ -160,10 +158,6 @@ uint8_t *queue_shares(loom_command_scope *scope, uint64_t bytes) {
   if (bytes > kShareBytes || !in_queue_order(scope)) return nullptr;
   q->shares_used = true;
   return q->shares;
-}
-
-uint32_t *queue_joins(loom_command_scope *scope) {
-  return in_queue_order(scope) ? scope->queue->joins : nullptr;
 }
 
 uint32_t read_device_status(const loom_command_queue *q) {
