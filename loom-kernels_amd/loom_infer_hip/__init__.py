@@ -377,7 +377,8 @@ class NormRopePagedKvAppendSpec:
     def __init__(self, tokens, batch_size, max_num_pages, num_query_heads, num_kv_heads,
                  head_dim=HEAD_DIM, page_size=PAGE_SIZE, kv_layout="NHD", kv_dtype="bf16",
                  kv_page_size=None, rope_theta=10000.0, norm_eps=None, explicit_tokens=True):
-        if norm_eps is not None and not norm_eps > 0:  # 0 means "no norms" in the C spec
+        # 0 means "no norms" in the C spec, whose epsilon is FP32
+        if norm_eps is not None and not C.c_float(norm_eps).value > 0:
             raise ContractError(3, "InvalidEpsilon",
                                 f"RMSNorm epsilon must be finite and positive, got {norm_eps:g}",
                                 None, (0, 0, 0, 0), float(norm_eps), 0)
