@@ -568,10 +568,13 @@ typedef struct loom_mxfp4_paged_batch_decode_args {
 /* Paged decode of a plan whose spec names LOOM_KV_DTYPE_MXFP4: the same command,
  * guards and algorithms over dequantised rows.  The codes become BF16 exactly, so
  * O and LSE are those of the BF16 command over the values the pages hold (scales
- * up to 252, as the append writes them; larger ones may pass BF16's range).  Q, the
- * pages, the scales, O and LSE on 4-byte boundaries.  The other enqueue forms
- * refuse such a plan (LOOM_NULL_ARGUMENT "K_scales"), this one plans over BF16 and
- * FP8 pages (LOOM_NULL_ARGUMENT "args"). */
+ * up to 252, as the append writes them; larger ones may pass BF16's range).  Sums are
+ * FP32: V up to 2^128 over the request's tokens cannot overflow them.  A token that
+ * scores -inf weighs nothing; a head all of whose tokens do has LSE -inf and O NaN,
+ * one with a score of +inf or NaN has both NaN.  Q, the pages, the scales, O and LSE
+ * on 4-byte boundaries.  The other enqueue forms refuse such a plan
+ * (LOOM_NULL_ARGUMENT "K_scales"), this one plans over BF16 and FP8 pages
+ * (LOOM_NULL_ARGUMENT "args"). */
 loom_status_t loom_paged_decode_enqueue_mxfp4(const loom_paged_decode_plan_t *plan,
                                               loom_command_scope_t *scope,
                                               const loom_mxfp4_paged_batch_decode_args_t *args,

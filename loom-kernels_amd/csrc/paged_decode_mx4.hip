@@ -20,7 +20,9 @@
 //     per two tokens turns the pairs into a fragment of one dim.
 //   * The running bound of the scores is set kLazy above a new maximum and moves only
 //     when a score passes it: the common step has no reduction across lanes and no
-//     rescale, and no weight is above 1 (large V do not overflow).
+//     rescale.  No weight is above 1, so the FP32 sum of weights times V, divided at
+//     the end, stays in range for V below 2^128 over the request's tokens; larger V
+//     (up to 6 * 2^125) may overflow it although their mean does not.
 //   * P keeps 16 bits, a BF16 high part and a BF16 residual, in one MFMA: a tile is at
 //     most 8 query heads; columns 0-7 take the high parts, 8-15 the residuals, and the
 //     two columns' O are added at the end.
