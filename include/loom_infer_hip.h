@@ -574,7 +574,8 @@ typedef struct loom_mxfp4_paged_batch_decode_args {
  * one with a score of +inf or NaN has both NaN.  Q, the pages, the scales, O and LSE
  * on 4-byte boundaries.  The other enqueue forms refuse such a plan
  * (LOOM_NULL_ARGUMENT "K_scales"), this one plans over BF16 and FP8 pages
- * (LOOM_NULL_ARGUMENT "args"). */
+ * (LOOM_NULL_ARGUMENT "args").  A spec whose softmax_scale was set to anything but a
+ * finite positive number is refused by the plan (LOOM_PLAN_INVALID_OPTION). */
 loom_status_t loom_paged_decode_enqueue_mxfp4(const loom_paged_decode_plan_t *plan,
                                               loom_command_scope_t *scope,
                                               const loom_mxfp4_paged_batch_decode_args_t *args,

@@ -1168,6 +1168,9 @@ loom_status_t plan_mx4_decode(loom_paged_decode_plan_info_t *info, uint32_t team
   const uint64_t page_rows = s.page_size ? s.page_size : kPageSize;
   if (B > (uint64_t)kMaxBatch)
     return fail(err, LOOM_PLAN_STATE_COUNT_OUT_OF_RANGE, "batch_size", B);
+  // the bound of a step is its largest product times the scale, and masked ones are -inf
+  if (!(s.softmax_scale > 0.0f) || !std::isfinite(s.softmax_scale))
+    return fail(err, LOOM_PLAN_INVALID_OPTION, "softmax_scale");
   uint64_t pool_rows;
   if (__builtin_mul_overflow(s.max_num_pages * page_rows, hkv, &pool_rows) ||
       pool_rows > UINT32_MAX)
