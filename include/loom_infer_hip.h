@@ -455,7 +455,9 @@ typedef enum loom_paged_decode_algorithm {
 
 /* Planner inputs.  Zero means "choose for this device". */
 typedef struct loom_paged_decode_plan_options {
-  uint64_t max_total_pages; /* upper bound of page_indices length; 0 -> max_num_pages */
+  uint64_t max_total_pages; /* upper bound of page_indices length; 0 -> max_num_pages.  The
+                               algorithm and its splits go by it: give what the commands
+                               will hold where the pool is much larger */
   uint32_t teams;           /* page ranges; 0 -> chosen for the device (or the direct
                                algorithm when max_total_pages <= 128; MXFP4: up to
                                2^20 K rows) */

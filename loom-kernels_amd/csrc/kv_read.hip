@@ -12,7 +12,7 @@
 // rows' own for batches below 64, else a search first), then 16 lanes per head row
 // load 4 code bytes each and store 16 bytes, K and V together, the heads of a row
 // contiguous.  The stores are streamed past L2: plain ones, whose lines L2 writes
-// back in another order, took 41 us instead of 27.1 (38k rows of 8 kv-heads, HND
+// back in another order, took 41 us instead of 27.1 (31.5k rows of 8 kv-heads, HND
 // pages of 64: 6.0 TB/s).
 #include <hip/hip_runtime.h>
 
@@ -31,7 +31,7 @@ constexpr int kReadMaxRows = 64;  // output rows per workgroup: at most one per 
 constexpr uint64_t kReadMaxHeads = 4096;
 // Head rows per workgroup, and how many of them each 16 lanes have in flight.
 // Measured with 16 to 256 head rows and 1 to 4 in flight: 64 are within 4% of the
-// best from 8k rows of 8 kv-heads (8.3 us) to 38k (27.1 us); 256 take 8 us where
+// best from 8k rows of 8 kv-heads (8.3 us) to 31.5k (27.1 us); 256 take 8 us where
 // 64 take 4.5 (300 rows of 32 kv-heads), 16 lose 5% of the large ones.  Four in
 // flight against one: 64 scattered rows of 8 kv-heads and their append 11.6 and
 // 11.8 us, about 1000 14.4 and 14.8.

@@ -522,8 +522,11 @@ __device__ __forceinline__ void apply_row(const AppendArgs &a, int t, int64_t pa
 //
 // Bound by memory in large commands: 8192 tokens of 64 + 8 heads into MXFP4 pages (311 MB)
 // 65 us, 4.8 TB/s, the VALU busy for more than half of it (a fifth fewer instructions
-// changed nothing); into BF16 pages (335 MB) 67 us, 5.0 TB/s.  Small ones by the guards'
-// chain: 64 tokens of 32 + 8 heads 7.5 us, about 1000 10.4.
+// changed nothing); into BF16 pages (336 MB) 66 us, 5.1 TB/s.  Into FP8 pages (319 MB) 68
+// us, 4.7 TB/s: 17 MB less than BF16, but sixteen quotients and encodings a lane and row
+// in vector instructions.  Small ones by the guards' chain: 64 tokens of 32 + 8 heads
+// 7.5 us (BF16 6.8, FP8 9.0), about 1000 10.4 (9.0, 11.3).
+
 // Row c ^ 8 of the same 16 lanes (a rotation by 8), and sums over the 16 lanes
 // and maxima over 4 of them (the lanes of one MXFP4 block), on DPP.
 __device__ __forceinline__ uint32_t dpp_other_half(uint32_t x) {
