@@ -546,8 +546,8 @@ __device__ __forceinline__ double dpp_f64(double x) {
       (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, 0xf, 0xf, false);
   return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
 }
-__device__ __forceinline__ float dpp_value(float x, int) { return dpp_f32<0x128>(x); }
-__device__ __forceinline__ double dpp_value(double x, int) { return dpp_f64<0x128>(x); }
+__device__ __forceinline__ float dpp_value(float x) { return dpp_f32<0x128>(x); }
+__device__ __forceinline__ double dpp_value(double x) { return dpp_f64<0x128>(x); }
 __device__ __forceinline__ float row_sum(float x) {
   x += dpp_f32<0x128>(x);
   x += dpp_f32<0x124>(x);
@@ -595,7 +595,7 @@ __device__ __forceinline__ void norm_rotate(const u32x4 &x, const u32x4 &w, bool
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int pair = (c * 8 + i) & 63;
-    const F other = dpp_value(y[i], 0);
+    const F other = dpp_value(y[i]);
     // first half: first*cos - second*sin; second half: second*cos + first*sin
     y[i] = y[i] * cs[pair] + (c < 8 ? -other : other) * sn[pair];
   }
