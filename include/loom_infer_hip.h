@@ -357,7 +357,10 @@ void loom_command_queue_free(loom_command_queue_t *queue);
  * when they are captured.  `zeroed_bytes` (an append plan's workspace_bytes)
  * is already held from queue creation; asking for more than that fails with
  * LOOM_ENQ_WORKSPACE_NOT_RESERVED.  Buffers only grow; they are freed with the
- * queue (or with the graph that captured its commands).
+ * queue (or with the graph that captured its commands).  Commands share them in the
+ * queue's order: a graph of the caller's own that captured such commands on the
+ * queue's stream may not be replayed beside the queue's other commands, nor after
+ * it is freed.  (MXFP4 decode takes nothing of the queue's there.)
  *
  * Direct single decode of 640 tokens or more and row-tile prefill of few rows
  * over long contexts keep states in a third buffer of the queue, 4.1 MiB from
