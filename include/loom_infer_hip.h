@@ -205,9 +205,10 @@ typedef enum loom_kv_dtype {
    * code * 2^(scale - 127), and a scale of 255 makes its block NaN.  Pages are
    * u8 [pool, P, Hkv, 64] (NHD) or [pool, Hkv, P, 64] (HND); the scales lie apart,
    * u8 [pool, Hkv, P, 4] for both layouts.  68 bytes per row against 256 in BF16.
-   * Paged decode (loom_paged_decode_enqueue_mxfp4), the normed append
-   * (loom_norm_rope_append_*) and the read back (loom_paged_kv_read_*) take
-   * them; paged prefill and the reference-shaped append do not. */
+   * Paged decode (loom_paged_decode_enqueue_mxfp4), window attention
+   * (loom_window_attention_*), the normed append (loom_norm_rope_append_*) and the
+   * read back (loom_paged_kv_read_*) take them; paged prefill and the
+   * reference-shaped append do not. */
   LOOM_KV_DTYPE_MXFP4 = 2
 } loom_kv_dtype_t;
 #define LOOM_MXFP4_ROW_BYTES 64u  /* code bytes of a row of 128 values */
@@ -1198,6 +1199,94 @@ loom_status_t loom_paged_kv_read_enqueue(const loom_paged_kv_read_plan_t *plan,
                                          loom_command_scope_t *scope,
                                          const loom_paged_kv_read_args_t *args,
                                          loom_error_t *err);
+
+/* ------------------------------------------------------------------------ */
+/* Attention with a sliding window and sinks over a paged cache (no reference   */
+/* counterpart): one new token per request, or a chunk of new rows.              */
+/*   Row i of a request of L tokens and n new rows stands at p = L - n + i and   */
+/*   sees token t where t <= p and (t > p - window or t < sinks or window = 0).   */
+/*   O = softmax(scale q.k) V over the tokens that it sees, LSE their log2 sum.   */
+/* A token that a row does not see has no part in it, whatever its K and V hold.  */
+typedef struct loom_window_attention_spec {
+  loom_paged_decode_spec_t paged; /* heads, pool, layout, page size and element type (BF16, FP8
+                                     E4M3 or MXFP4) of the pages */
+  uint64_t rows;                  /* query rows of a command; the batch for the one-row form */
+  uint64_t window;                /* tokens up to a row's own that it sees; 0: all of them */
+  uint64_t sinks;                 /* first tokens of a request that every row sees besides */
+  int32_t explicit_rows;          /* 0: one row per request, at kv_len - 1 */
+} loom_window_attention_spec_t;
+
+/* `paged` as from loom_paged_decode_spec_new and its setters.  explicit_rows = 0 takes
+ * rows = batch_size (LOOM_LENGTH_MISMATCH otherwise). */
+loom_status_t loom_window_attention_spec_new(const loom_paged_decode_spec_t *paged, uint64_t rows,
+                                             int32_t explicit_rows, uint64_t window, uint64_t sinks,
+                                             loom_window_attention_spec_t *out, loom_error_t *err);
+
+typedef struct loom_window_attention_plan loom_window_attention_plan_t;
+
+typedef struct loom_window_attention_plan_info {
+  loom_window_attention_spec_t spec;
+  int32_t algorithm;      /* LOOM_PAGED_PREFILL_ROW_TILE or LOOM_PAGED_PREFILL_LONG_TILE */
+  uint32_t tile_cols;     /* flattened (row, head of the group) columns per workgroup */
+  uint64_t row_tiles;     /* upper bound of the tiles over any valid qo_indptr */
+  uint64_t grid_blocks;   /* row_tiles * Hkv (times the workgroups that share a tile, see
+                             loom_window_attention_enqueue) */
+  uint32_t block_threads;
+  uint32_t flags;
+} loom_window_attention_plan_info_t;
+
+/* The one-row form (explicit_rows = 0) of a decode provider and the ragged form of a
+ * prefill provider (LOOM_PLAN_INVALID_OPTION "explicit_rows" for the other).  `flags`:
+ * LOOM_PLAN_PAGE_INDICES_CAPACITY and, ragged, at most one of LOOM_PLAN_PREFILL_TILE_16
+ * and LOOM_PLAN_PREFILL_TILE_LONG; none: chosen from the spec.  At most 4096 kv-heads,
+ * rows * Hq within 31 bits and a grid of less than 2^32 threads
+ * (LOOM_PLAN_STATE_COUNT_OUT_OF_RANGE); a softmax_scale set by hand is finite and positive
+ * (LOOM_PLAN_INVALID_OPTION). */
+loom_status_t loom_decode_provider_plan_window_paged_batch(
+    const loom_decode_provider_t *provider, const loom_window_attention_spec_t *spec, uint32_t flags,
+    loom_window_attention_plan_t **out, loom_error_t *err);
+loom_status_t loom_prefill_provider_plan_window_paged(const loom_prefill_provider_t *provider,
+                                                      const loom_window_attention_spec_t *spec,
+                                                      uint32_t flags,
+                                                      loom_window_attention_plan_t **out,
+                                                      loom_error_t *err);
+void loom_window_attention_plan_free(loom_window_attention_plan_t *plan);
+void loom_window_attention_plan_get_info(const loom_window_attention_plan_t *plan,
+                                         loom_window_attention_plan_info_t *info);
+
+typedef struct loom_window_attention_args {
+  loom_handle_t query;         /* Read<bf16> [rows, Hq, 128] */
+  loom_handle_t key_pages;     /* Read<bf16 or u8>, as the spec's element type has them */
+  loom_handle_t value_pages;
+  loom_handle_t qo_indptr;     /* Read<i32>  [B+1] (ragged form; {0, 0} for the one-row form): a
+                                  request may have no rows */
+  loom_handle_t page_indptr;   /* Read<i32>  [B+1] */
+  loom_handle_t page_indices;  /* Read<i32>  [>= B] */
+  loom_handle_t last_page_len; /* Read<i32>  [B] */
+  loom_handle_t output;        /* Write<bf16> [rows, Hq, 128] */
+  loom_handle_t lse;           /* Write<f32>  [rows, Hq], log2 domain */
+  loom_handle_t kv_scales;     /* Read<f32> [2] for FP8 pages, else {0, 0} */
+  loom_handle_t key_scales;    /* Read<u8> [pool, Hkv, P, 4] for MXFP4 pages, else {0, 0} */
+  loom_handle_t value_scales;
+} loom_window_attention_args_t;
+
+/* One command, one kernel.  Only the page indices of tokens that some row of the request
+ * sees are read: the others, of pages that the caller has given away, may hold anything.
+ * Device guards: page_indptr or qo_indptr with wrong ends leaves every output untouched; a
+ * request with an invalid page range or last-page length, a visible page index out of range
+ * or more rows than tokens leaves its rows untouched, and so does every request from the
+ * first decreasing qo_indptr range on.  Few rows over long contexts are shared by several
+ * workgroups per tile, whose states lie in a buffer of the queue
+ * (loom_command_queue_reserve_workspace); captured by the caller into a graph of its own the
+ * command runs without it, slower.  A token that scores -inf, or whose weight is below
+ * FP32's range, weighs nothing; a row whose tokens all score -inf has LSE -inf and O NaN,
+ * one with a score of +inf or NaN has both NaN.  Q, the pages, the MXFP4 scales and O on
+ * 4-byte boundaries.  page_indices * P holds at most 2^31 - 1 tokens
+ * (LOOM_ENQ_PAGE_INDICES_TOO_LONG). */
+loom_status_t loom_window_attention_enqueue(const loom_window_attention_plan_t *plan,
+                                            loom_command_scope_t *scope,
+                                            const loom_window_attention_args_t *args,
+                                            loom_error_t *err);
 
 /* ------------------------------------------------------------------------ */
 /* Graph capture and replay, crates/loom-infer-cuda/src/graph/mod.rs           */

@@ -853,7 +853,7 @@ loom_status_t loom_ragged_prefill_causal_kv_end(const loom_ragged_prefill_spec_t
   return LOOM_OK;
 }
 
-// ---- normed append and read back (no reference counterpart) ------------------------
+// ---- normed append, read back, window attention (no reference counterpart) ---------
 // The geometry of an embedded paged spec: what spec_new and its setters let through.
 static loom_status_t check_paged(const loom_paged_decode_spec_t *p, loom_error_t *err) {
   loom_paged_decode_spec_t t;
@@ -906,6 +906,26 @@ loom_status_t loom_paged_kv_read_spec_new(const loom_paged_decode_spec_t *paged,
     return fail(err, LOOM_ELEMENT_COUNT_OVERFLOW);
   out->paged = *paged;
   out->nnz_kv = nnz_kv;
+  return loom::ok(err);
+}
+
+loom_status_t loom_window_attention_spec_new(const loom_paged_decode_spec_t *paged, uint64_t rows,
+                                             int32_t explicit_rows, uint64_t window, uint64_t sinks,
+                                             loom_window_attention_spec_t *out, loom_error_t *err) {
+  if (!paged || !out) return fail(err, LOOM_NULL_ARGUMENT, "paged");
+  const loom_status_t rc = check_paged(paged, err);
+  if (rc) return rc;
+  uint64_t t;
+  if (rows == 0) return fail(err, LOOM_ZERO_DIMENSION);
+  if (!explicit_rows && rows != paged->batch_size)
+    return fail(err, LOOM_LENGTH_MISMATCH, "rows", paged->batch_size, rows);
+  if (mul_ovf(rows, paged->num_query_heads, &t) || mul_ovf(t, loom::kHeadDim, &t))
+    return fail(err, LOOM_ELEMENT_COUNT_OVERFLOW);
+  out->paged = *paged;
+  out->rows = rows;
+  out->window = window;
+  out->sinks = sinks;
+  out->explicit_rows = explicit_rows ? 1 : 0;
   return loom::ok(err);
 }
 

@@ -193,3 +193,10 @@ struct DeviceInfo {
 loom_status_t query_device(int device, DeviceInfo *out, loom_error_t *err);
 
 }  // namespace loom
+
+struct loom_decode_provider {
+  loom::DeviceInfo dev;
+};
+struct loom_prefill_provider {
+  loom::DeviceInfo dev;
+};

@@ -1288,10 +1288,6 @@ __global__ __launch_bounds__(kMergeWaves * 64) void single_decode_split_k_merge_
 }  // namespace
 
 // ---- provider / plan / enqueue -----------------------------------------------
-struct loom_decode_provider {
-  loom::DeviceInfo dev;
-};
-
 struct loom_paged_decode_plan {
   loom_paged_decode_plan_info_t info{};
   int device = 0;

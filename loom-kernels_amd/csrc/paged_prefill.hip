@@ -1384,10 +1384,6 @@ __global__ __launch_bounds__(W * 64, 2) void ragged_prefill_pipe_kernel(PrefillA
 }  // namespace
 
 // ---- provider / plan / enqueue -----------------------------------------------
-struct loom_prefill_provider {
-  loom::DeviceInfo dev;
-};
-
 struct loom_paged_prefill_plan {
   loom_paged_prefill_plan_info_t info{};
   uint32_t tile_cols = 16;  // flattened columns per workgroup

@@ -1,0 +1,810 @@
+// Attention with a sliding window and sinks over paged K/V for gfx950 (MI355X), D128,
+// BF16, FP8 E4M3 or MXFP4 pages of 16-64 rows, NHD or HND (no reference counterpart):
+// one new token per request (decode) or ragged rows of new tokens (a chunk).
+//
+// A row at position p of its request sees token t <= p where t > p - window or t < sinks;
+//   O = sum_t softmax(scale q.k_t)_t v_t,   LSE = log2 sum_t 2^(scale log2(e) q.k_t).
+// The query rows of a request and the heads of one kv-head's group are flattened, (row, group
+// head) -> row * group + head, and cut into tiles of columns, as for paged prefill.  A tile
+// walks the 16-row blocks that some column of it sees: the sinks' blocks, then those from
+// the first row's window start to the last row's own token.  Blocks in between are never
+// touched, nor are their page indices.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "attn_device.hpp"
+#include "loom_internal.hpp"
+#include "prefill_device.hpp"
+
+using loom::fail;
+using namespace loom_dev;
+
+namespace {
+
+enum Kv : int { kBf16, kFp8, kMx4 };
+template <Kv KV>
+constexpr int kRowBytes = KV == kBf16 ? 256 : KV == kFp8 ? 128 : 64;  // of one head's K or V
+
+struct WindowArgs : PrefillArgs {
+  const uint8_t *k_mx;  // MXFP4 scales
+  const uint8_t *v_mx;
+  int32_t window;       // INT32_MAX: none
+  int32_t sinks;
+  int32_t head_bytes;   // from one kv-head's rows of a page to the next
+  int32_t row_bytes;    // from one token's row to the next
+  int32_t head_tiles;   // one-row form: tiles per request
+  uint32_t *arrived;    // splits: arrival words, loom::kMx4JoinBytes apart
+};
+
+// A tile's place and what its columns see (wave-uniform).
+struct Tile {
+  TileLoc loc;
+  int kv_len;
+  int group_rows;     // the request's query rows
+  int fcols, col0;    // its columns, and the tile's first
+  int p_lo, p_hi;     // positions of the tile's first and last row
+  int sink_blocks, first_block, blocks;  // the walk, in 16-row blocks
+  // 16-row block of the request at place x of the walk
+  __device__ __forceinline__ int block(int x) const {
+    return x < sink_blocks ? x : x - sink_blocks + first_block;
+  }
+  // tokens of it that some column may see, from its first row on
+  __device__ __forceinline__ int rows(const WindowArgs &a, int x) const {
+    const int b = block(x);
+    return min(16, (x < sink_blocks ? min(a.sinks, p_hi + 1) : p_hi + 1) - 16 * b);
+  }
+};
+
+// Finds the workgroup's tile of TC columns; false: none, or a failed guard.
+template <int W, int TC>
+__device__ __forceinline__ bool find_tile(const WindowArgs &a, LocateSmem<W> &sm, Tile &t, int split) {
+  TileLoc &l = t.loc;
+  if (a.qo) {
+    if (!locate_tile<W, false, TC, true, true>(a, sm, l, split)) return false;
+  } else {
+    l.kvh = (int)(blockIdx.x % (uint32_t)a.hkv);
+    l.rank = (int)(blockIdx.x / (uint32_t)a.hkv) - split * a.row_tiles;
+    const int r = (int)((uint32_t)l.rank / (uint32_t)a.head_tiles);
+    l.tile0 = l.rank - r * a.head_tiles;
+    l.qs = r;
+    l.qe = r + 1;
+    l.fbeg = 0;
+    const int32_t ip0 = a.indptr[0];
+    l.ipB = uni(a.indptr[a.batch]);
+    l.ps = uni(a.indptr[r]);
+    l.pe = uni(a.indptr[r + 1]);
+    l.tl = uni(a.last[r]);
+    if (ip0 != 0 || l.ipB < 0 ||
+        (a.indices_capacity ? (int64_t)l.ipB > a.n_indices : (int64_t)l.ipB != a.n_indices))
+      return false;
+  }
+  if (l.ps < 0 || l.pe <= l.ps || l.pe > l.ipB || l.tl < 1 || l.tl > a.page_rows) return false;
+  // (the enqueue bounds page_indices * page_rows by 2^31 - 1)
+  t.kv_len = (l.pe - l.ps - 1) * a.page_rows + l.tl;
+  t.group_rows = l.qe - l.qs;
+  if (t.group_rows > t.kv_len) return false;
+  t.fcols = t.group_rows * a.group;
+  t.col0 = l.tile0 * TC;
+  const int p0 = t.kv_len - t.group_rows;
+  t.p_lo = p0 + (int)((uint32_t)t.col0 / (uint32_t)a.group);
+  t.p_hi = p0 + (int)((uint32_t)min(t.col0 + TC - 1, t.fcols - 1) / (uint32_t)a.group);
+  t.first_block = max(0, t.p_lo + 1 - a.window) >> 4;
+  t.sink_blocks = min((int)(((uint32_t)a.sinks + 15) >> 4), t.first_block);
+  t.blocks = t.sink_blocks + (t.p_hi >> 4) + 1 - t.first_block;
+  return true;
+}
+
+// Whether a page index of a token that some row of the request sees is out of range: this
+// thread's share of `threads`.  (The same for every tile of the request.)
+__device__ __forceinline__ bool bad_pages(const WindowArgs &a, const Tile &t, int tid, int threads) {
+  const int lg = a.blocks_lg + 4;
+  const int first = max(0, t.kv_len - t.group_rows + 1 - a.window) >> lg;
+  const int sinks = min((int)(((uint32_t)a.sinks + (1u << lg) - 1) >> lg), first);
+  const int n = sinks + (t.loc.pe - t.loc.ps) - first;
+  bool bad = false;
+  for (int i = tid; i < n; i += threads) {
+    const int32_t x = a.indices[t.loc.ps + (i < sinks ? i : i - sinks + first)];
+    bad |= x < 0 || (int64_t)x >= a.pool;
+  }
+  return bad;
+}
+
+// Byte offset of row `row` of `page` for kv-head kvh, in K and V alike.
+template <Kv KV>
+__device__ __forceinline__ uint64_t row_at(const WindowArgs &a, int page, int row, int kvh) {
+  return (uint64_t)(uint32_t)page * (uint32_t)(a.page_rows * kRowBytes<KV>) * (uint32_t)a.hkv +
+         (uint64_t)(uint32_t)kvh * (uint32_t)a.head_bytes + (uint32_t)row * (uint32_t)a.row_bytes;
+}
+// The same in the MXFP4 scales.
+__device__ __forceinline__ uint64_t scale_at(const WindowArgs &a, int page, int row, int kvh) {
+  return (((uint64_t)(uint32_t)page * (uint32_t)a.hkv + (uint32_t)kvh) * (uint32_t)a.page_rows +
+          (uint32_t)row) * 4;
+}
+
+// One column's O and LSE token by token, by one wave: for columns whose O is not finite.
+// The tiles' products multiply a hidden token's V with a weight of zero, which is not
+// zero where V is infinite or NaN; here hidden tokens, and weights of zero, have no part.
+// (Not made to be fast: about 0.15 us per token.)
+template <Kv KV>
+__device__ __forceinline__ void exact_column(const WindowArgs &a, const Tile &t, int f, int lane,
+                                             float v_scale) {
+  const int qi = (int)((uint32_t)f / (uint32_t)a.group);
+  const int64_t row = (int64_t)(t.loc.qs + qi) * a.hq + (int64_t)t.loc.kvh * a.group + (f - qi * a.group);
+  const int end = t.kv_len - t.group_rows + qi + 1, beg = max(0, end - a.window);
+  const int sinks = min(a.sinks, beg), n = sinks + end - beg;
+  const uint32_t qw = *reinterpret_cast<const uint32_t *>(a.q + row * 128 + 2 * lane);
+  const float q0 = bf16_lo(qw), q1 = bf16_hi(qw);
+  float m = -INFINITY, l = 0.0f, o0 = 0.0f, o1 = 0.0f;
+  auto pair = [&](const uint16_t *base, const uint8_t *mx, uint64_t at, uint64_t sc, float &x, float &y) {
+    const uint8_t *b = reinterpret_cast<const uint8_t *>(base) + at;
+    if constexpr (KV == kBf16) {
+      const uint32_t w = *reinterpret_cast<const uint32_t *>(b + 4 * lane);
+      x = bf16_lo(w);
+      y = bf16_hi(w);
+    } else if constexpr (KV == kFp8) {
+      const f32x2 w = __builtin_amdgcn_cvt_pk_f32_fp8(
+          *reinterpret_cast<const uint16_t *>(b + 2 * lane), false);
+      x = w[0];
+      y = w[1];
+    } else {
+      const uint32_t w = mx4x8_to_bf16x8(b[lane], (uint32_t)mx[sc + (lane >> 4)] << 23)[0];
+      x = bf16_lo(w);
+      y = bf16_hi(w);
+    }
+  };
+  for (int i0 = 0; i0 < n; i0 += 64) {
+    const int i = min(i0 + lane, n - 1), tok = i < sinks ? i : i - sinks + beg;
+    const int pages = a.indices[t.loc.ps + (tok >> (a.blocks_lg + 4))];
+    const int in_page = tok & (a.page_rows - 1);
+    const int c = min(64, n - i0);
+    for (int j = 0; j < c; ++j) {
+      const int page = __builtin_amdgcn_readlane(pages, j), r = __builtin_amdgcn_readlane(in_page, j);
+      const uint64_t at = row_at<KV>(a, page, r, t.loc.kvh), sc = scale_at(a, page, r, t.loc.kvh);
+      float k0, k1, v0, v1;
+      pair(a.k, a.k_mx, at, sc, k0, k1);
+      pair(a.v, a.v_mx, at, sc, v0, v1);
+      float s = fmaf(q0, k0, q1 * k1);
+#pragma unroll
+      for (int x = 32; x >= 1; x >>= 1) s += __shfl_xor(s, x, 64);
+      s *= a.scale_log2;
+      if (s == -INFINITY) continue;
+      const float mn = fmax_nan(m, s), old = m == -INFINITY ? 0.0f : fast_exp2(m - mn);
+      const float p = fast_exp2(s - mn);  // (NaN at +inf)
+      l = fmaf(l, old, p);
+      // (where a sum is infinite and its weight vanishes, it has no part either)
+      o0 = old == 0.0f ? 0.0f : o0 * old;
+      o1 = old == 0.0f ? 0.0f : o1 * old;
+      if (p != 0.0f) {
+        o0 = fmaf(p, v0, o0);
+        o1 = fmaf(p, v1, o1);
+      }
+      m = mn;
+    }
+  }
+  const float inv = 1.0f / l;
+  *reinterpret_cast<uint32_t *>(a.out + row * 128 + 2 * lane) =
+      bf16x2_pack(l == 0.0f ? NAN : o0 * inv * v_scale, l == 0.0f ? NAN : o1 * inv * v_scale);
+  if (lane == 0) a.lse[row] = m + __log2f(l);
+}
+
+// ---- row tiles ---------------------------------------------------------------------
+// One workgroup of W waves per (16 columns, kv-head[, split]).  Wave w takes 32-token steps
+// w, w + W, ... of the walk (of its split's share of it), each through LDS of its own
+// (PipeWave's slot: whole rows, so a load instruction covers whole lines, in an order that
+// spreads the fragment reads over the banks), and the wave states merge in LDS.  Per step:
+// S = K.Q^T in 8 MFMAs of 16x16x32, the softmax with a running maximum that moves only when
+// a score passes it by 2^8, and O^T += V^T.P^T in 16, P as a BF16 high part and a BF16
+// residual (16 bits: few tokens carry a short window, whose errors do not average out).
+// BF16 and FP8 rows go straight to LDS; MXFP4 codes are loaded into registers, one block of
+// 32 values and its scale per lane, and written to LDS as BF16, which serves K and V alike.
+constexpr int kRowWaves = 4;
+constexpr int kStash = 132;  // floats between two columns' O in LDS, and of a split's state
+
+template <Kv KV>
+using RowPipe = PipeWave<4, KV == kFp8, true, 1>;
+template <Kv KV>
+constexpr int kRowSlots = KV == kMx4 ? 1 : 2;
+
+template <Kv KV>
+struct RowsSmem {
+  __align__(16) uint8_t slots[kRowWaves][kRowSlots<KV> * RowPipe<KV>::kSlotBytes];
+  LocateSmem<kRowWaves> loc;
+  float m[kRowWaves][16], l[kRowWaves][16];
+  uint32_t bad[kRowWaves];
+  uint32_t arrived;
+  uint32_t redo;  // columns whose O is not finite
+};
+
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+// Until this wave's LDS reads have returned: before loads into a slot that it read.
+__device__ __forceinline__ void wait_reads() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
+// Split states go past L2, which the XCDs do not share.
+__device__ __forceinline__ void store_state(float *p, float x, float y) {
+  __hip_atomic_store(reinterpret_cast<uint64_t *>(p), __builtin_bit_cast(uint64_t, f32x2{x, y}),
+                     __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ f32x2 load_state(const float *p) {
+  return __builtin_bit_cast(f32x2, __hip_atomic_load(reinterpret_cast<const uint64_t *>(p),
+                                                     __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+}
+
+// MXFP4 rows of a step in registers: lane l holds 32 values, codes (l & 3) of row l >> 2 of
+// each half, and their scale byte.
+struct MxStage {
+  u32x4 k[2], v[2];
+  uint32_t ks[2], vs[2];
+};
+// Codes of row r, block b of 32 values, to a slot as BF16.
+template <class Pipe>
+__device__ __forceinline__ void put_mx(uint8_t *slot, bool is_v, int r, int b, const u32x4 &w,
+                                       uint32_t scale) {
+  uint8_t *dst = slot + (is_v ? Pipe::v_group(r >> 2) : (r >> 2) * Pipe::kKGroup) + (r & 3) * 256 +
+                 ((4 * b) ^ Pipe::swizzle(r)) * 16;
+#pragma unroll
+  for (int u = 0; u < 4; ++u)
+    *reinterpret_cast<u32x4 *>(dst + 16 * u) = mx4x8_to_bf16x8(w[u], scale << 23);
+}
+
+template <Kv KV>
+__global__ __launch_bounds__(kRowWaves * 64) void window_rows_kernel(WindowArgs args) {
+  constexpr int W = kRowWaves, TC = 16;
+  constexpr bool FP8 = KV == kFp8;
+  using Pipe = RowPipe<KV>;
+  constexpr int kSlot = Pipe::kSlotBytes;
+  static_assert(TC * kStash * 4 <= kRowSlots<KV> * kSlot, "a wave's columns in its slots");
+  __shared__ RowsSmem<KV> sm;
+  WindowArgs a = args;
+  float v_scale = 1.0f;
+  if constexpr (FP8) {
+    a.scale_log2 *= a.kv_scales[0];
+    v_scale = a.kv_scales[1];
+  }
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = uni(tid >> 6);
+  const int col = lane & 15, quad = lane >> 4;
+  const int split = a.splits > 1 ? (int)(blockIdx.x / (uint32_t)(a.row_tiles * a.hkv)) : 0;
+  Tile t;
+  if (!find_tile<W, TC>(a, sm.loc, t, split)) return;
+  const int kvh = t.loc.kvh;
+  // this lane's column
+  const int f = t.col0 + col;
+  const bool valid = f < t.fcols;
+  const int qi = valid ? (int)((uint32_t)f / (uint32_t)a.group) : 0;
+  const int end_col = valid ? t.kv_len - t.group_rows + qi + 1 : 0;
+  const int beg_col = max(0, end_col - a.window);
+  // tokens [full_beg, full_end) are seen by every column
+  const int full_beg = max(0, t.p_hi + 1 - a.window), full_end = t.p_lo + 1;
+  Pipe pw{a, lane, col, quad};
+  pw.reset(sm.slots[wave]);
+  {
+    const uint16_t *qp =
+        a.q + ((int64_t)(t.loc.qs + qi) * a.hq + (int64_t)kvh * a.group + (f - qi * a.group)) * 128;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) pw.qf[0][c] = valid ? load16(qp + Pipe::q_dim(c, quad)) : u32x4{0, 0, 0, 0};
+  }
+  // this split's steps [lo, hi), this wave's lo + wave + W i
+  const int steps = (t.blocks + 1) >> 1;
+  int lo = 0, hi = steps;
+  if (a.splits > 1) {
+    lo = (int)((int64_t)steps * split / a.splits);
+    hi = (int)((int64_t)steps * (split + 1) / a.splits);
+  }
+  const int n = hi - lo > wave ? (hi - lo - wave + W - 1) / W : 0;
+
+  // Where the wave's half steps lie, 64 at a time, one per lane: byte offset of the first
+  // row in K and V (and in the MXFP4 scales), and block << 5 | rows.
+  uint32_t at_lo = 0, at_hi = 0, sc_lo = 0, sc_hi = 0;
+  int meta = 0;
+  auto locate = [&](int i0) {
+    const int x = 2 * (lo + wave + W * (i0 + (lane >> 1))) + (lane & 1);
+    const bool in = x < t.blocks;
+    const int b = t.block(x);
+    int rows = in ? t.rows(a, x) : 0;
+    const int page = in ? a.indices[t.loc.ps + (b >> a.blocks_lg)] : 0;
+    if (page < 0 || (int64_t)page >= a.pool) rows = 0;  // (refused below)
+    const int row = (b & ((1 << a.blocks_lg) - 1)) * 16;
+    const uint64_t at = row_at<KV>(a, page, row, kvh);
+    at_lo = (uint32_t)at;
+    at_hi = (uint32_t)(at >> 32);
+    if constexpr (KV == kMx4) {
+      const uint64_t sc = scale_at(a, page, row, kvh);
+      sc_lo = (uint32_t)sc;
+      sc_hi = (uint32_t)(sc >> 32);
+    }
+    meta = b << 5 | rows;
+  };
+  auto lane64 = [&](uint32_t l, uint32_t h, int j) {
+    return ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)h, j) << 32) |
+           (uint32_t)__builtin_amdgcn_readlane((int)l, j);
+  };
+  auto rsrc = [](const void *base, uint64_t at, int bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<uint8_t *>(reinterpret_cast<const uint8_t *>(base) + at), 0, bytes, 0x00020000);
+  };
+  // BF16 and FP8: the loads of step i (of the located 32) into the slot at LDS address `slot`
+  constexpr int kHalf = Pipe::kGroups / 2;
+  constexpr int kStepLoads = 4 * kHalf;
+  int lane_off[kHalf];
+  if constexpr (KV != kMx4) {
+    const int unit = (lane & (Pipe::kUnits - 1)) ^ Pipe::swizzle(lane / Pipe::kUnits);
+#pragma unroll
+    for (int x = 0; x < kHalf; ++x)
+      lane_off[x] = (x * Pipe::kGroupRows + lane / Pipe::kUnits) * a.row_bytes + unit * 16;
+  }
+  auto issue = [&](int i, uint32_t slot) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int j = 2 * i + h;
+      const int rows = __builtin_amdgcn_readlane(meta, j) & 31;
+      const uint64_t at = lane64(at_lo, at_hi, j);
+      const int bytes = rows > 0 ? (rows - 1) * a.row_bytes + kRowBytes<KV> : 0;
+      const __amdgpu_buffer_rsrc_t rk = rsrc(a.k, at, bytes), rv = rsrc(a.v, at, bytes);
+#pragma unroll
+      for (int x = 0; x < kHalf; ++x) {
+        lds_load16_at(rk, slot + (uint32_t)((h * kHalf + x) * Pipe::kKGroup), lane_off[x]);
+        lds_load16_at(rv, slot + (uint32_t)(Pipe::v_group(x) + h * (Pipe::v_group(kHalf) - Pipe::v_group(0))),
+                      lane_off[x]);
+      }
+    }
+  };
+  // MXFP4: the same into registers
+  auto fetch = [&](int i, MxStage &g) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int j = 2 * i + h;
+      const int rows = __builtin_amdgcn_readlane(meta, j) & 31;
+      const uint64_t at = lane64(at_lo, at_hi, j), sc = lane64(sc_lo, sc_hi, j);
+      const int bytes = rows > 0 ? (rows - 1) * a.row_bytes + 64 : 0;
+      const int off = (lane >> 2) * a.row_bytes + (lane & 3) * 16;
+      g.k[h] = load16_rows<false>(rsrc(a.k, at, bytes), off);
+      g.v[h] = load16_rows<false>(rsrc(a.v, at, bytes), off);
+      g.ks[h] = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(rsrc(a.k_mx, sc, 4 * rows), lane, 0, 0);
+      g.vs[h] = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(rsrc(a.v_mx, sc, 4 * rows), lane, 0, 0);
+    }
+  };
+
+  float m_run = -INFINITY, l_run = 0.0f;
+  f32x4(&acc)[8] = pw.acc[0];
+  // The softmax and products of step i, whose rows lie at `slot` bytes of the wave's ring.
+  auto process = [&](int i, int slot) {
+    const auto k = pw.read_k(slot);
+    f32x4 s[2] = {};
+#pragma unroll
+    for (int x = 0; x < 8; ++x) {
+      const int c = x >> 1, h = x & 1;
+      u32x4 w;
+      if constexpr (FP8)
+        w = fp8x8_to_bf16x8(u32x2{k.f[c >> 1][h][2 * (c & 1)], k.f[c >> 1][h][2 * (c & 1) + 1]});
+      else
+        w = k.f[c][h];
+      s[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(w), as_bf16x8(pw.qf[0][c]), s[h], 0, 0, 0);
+    }
+    // s[h][j]: token 16 block(h) + 4 quad + j
+    const int t0 = (__builtin_amdgcn_readlane(meta, 2 * i) >> 5) * 16;
+    const int t1 = (__builtin_amdgcn_readlane(meta, 2 * i + 1) >> 5) * 16;
+    if (t0 < full_beg || t0 + 16 > full_end || t1 < full_beg || t1 + 16 > full_end) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int tok = (h ? t1 : t0) + 4 * quad + j;
+          s[h][j] = tok < end_col && (tok >= beg_col || tok < a.sinks) ? s[h][j] : -INFINITY;
+        }
+    }
+    const float ml = fmax_nan(fmax_nan(fmax_nan(s[0][0], s[0][1]), fmax_nan(s[0][2], s[0][3])),
+                              fmax_nan(fmax_nan(s[1][0], s[1][1]), fmax_nan(s[1][2], s[1][3])));
+    if (__builtin_amdgcn_ballot_w64(ml * a.scale_log2 > m_run + 8.0f)) {
+      const float mx = quad_max_nan(ml) * a.scale_log2;
+      const bool grow = mx > m_run + 8.0f;
+      const float m_ref = grow ? mx : m_run;
+      if (__builtin_amdgcn_ballot_w64(grow && m_run != -INFINITY)) {
+        const float al = fast_exp2(m_run - (m_ref == -INFINITY ? 0.0f : m_ref));
+#pragma unroll
+        for (int e = 0; e < 8; ++e) acc[e] *= al;
+        l_run *= al;
+      }
+      m_run = m_ref;
+    }
+    const float m_use = m_run == -INFINITY ? 0.0f : m_run;  // nothing visible yet
+    u32x4 ph, pl;
+#pragma unroll
+    for (int y = 0; y < 4; ++y) {
+      const float x0 = fast_exp2(fmaf(s[y >> 1][2 * (y & 1)], a.scale_log2, -m_use));
+      const float x1 = fast_exp2(fmaf(s[y >> 1][2 * (y & 1) + 1], a.scale_log2, -m_use));
+      const uint32_t b0 = __float_as_uint(x0), b1 = __float_as_uint(x1);
+      ph[y] = pack_hi16(b0, b1);
+      pl[y] = pack_hi16(__float_as_uint(x0 - __uint_as_float(b0 & 0xffff0000u)),
+                        __float_as_uint(x1 - __uint_as_float(b1 & 0xffff0000u)));
+      l_run += x0 + x1;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const u32x4 b = pw.read_v(slot, e);
+      const bf16x8 w = as_bf16x8(FP8 ? fp8x8_to_bf16x8(u32x2{b[0], b[1]}) : b);
+      acc[e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, as_bf16x8(ph), acc[e], 0, 0, 0);
+      acc[e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, as_bf16x8(pl), acc[e], 0, 0, 0);
+    }
+  };
+
+  const uint32_t ring_at =
+      (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)sm.slots[wave];
+  bool bad = false;
+  for (int i0 = 0; i0 == 0 || i0 < n; i0 += 32) {
+    const int c = min(32, n - i0);
+    if (c > 0) locate(i0);
+    if constexpr (KV == kMx4) {
+      MxStage st;
+      if (c > 0) fetch(0, st);
+      if (i0 == 0) bad = bad_pages(a, t, tid, W * 64);
+      for (int i = 0; i < c; ++i) {
+        const MxStage cur = st;
+        if (i + 1 < c) fetch(i + 1, st);
+        wave_lds_fence();  // the slot's reads of the step before
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          put_mx<Pipe>(sm.slots[wave], false, 16 * h + (lane >> 2), lane & 3, cur.k[h], cur.ks[h]);
+          put_mx<Pipe>(sm.slots[wave], true, 16 * h + (lane >> 2), lane & 3, cur.v[h], cur.vs[h]);
+        }
+        wave_lds_fence();
+        process(i, 0);
+      }
+    } else {
+      // (queries and index words have arrived: no wait of the compiler's in the walk)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) asm volatile("" : "+v"(pw.qf[0][x]));
+      asm volatile("" : "+v"(at_lo), "+v"(at_hi), "+v"(meta));
+      wait_reads();
+      if (c > 0) issue(0, ring_at);
+      if (i0 == 0) {
+        bad = bad_pages(a, t, tid, W * 64);
+        asm volatile("" ::"s"(__builtin_amdgcn_ballot_w64(bad)));
+      }
+      for (int i = 0; i < c; ++i) {
+        if (i + 1 < c) {
+          wait_reads();
+          issue(i + 1, ring_at + (uint32_t)(((i + 1) & 1) * kSlot));
+          wait_loads<kStepLoads>();
+        } else {
+          wait_loads<0>();
+        }
+        process(i, (i & 1) * kSlot);
+      }
+    }
+  }
+
+  // The wave's columns to its slot.  acc[e][j] = O[column][16 e + 4 quad + j]
+  wait_reads();
+  wave_lds_fence();
+  float *const stash = reinterpret_cast<float *>(sm.slots[wave]);
+  const float l_col = quad_sum(l_run);
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    *reinterpret_cast<f32x4 *>(stash + col * kStash + 16 * e + 4 * quad) = acc[e];
+  if (quad == 0) {
+    sm.m[wave][col] = m_run;
+    sm.l[wave][col] = l_col;
+  }
+  if (tid == 0) sm.redo = 0;
+  if (block_or(bad, sm.bad)) return;
+  const int cols = min(TC, t.fcols - t.col0);
+  constexpr int kItems = TC * 32 / (W * 64);  // 4 dims of a column each
+  f32x4 o[kItems];
+  float ms[kItems], ls[kItems];
+#pragma unroll
+  for (int y = 0; y < kItems; ++y) {
+    const int c = (y * W * 64 + tid) >> 5, d = (tid & 31) * 4;
+    float M = -INFINITY, L = 0.0f;
+#pragma unroll
+    for (int i = 0; i < W; ++i) M = fmaxf(M, sm.m[i][c]);
+    f32x4 O = {};
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      const float w = sm.m[i][c] == -INFINITY ? 0.0f : fast_exp2(sm.m[i][c] - M);
+      const f32x4 x = *reinterpret_cast<const f32x4 *>(reinterpret_cast<const float *>(sm.slots[i]) +
+                                                       c * kStash + d);
+      L = fmaf(sm.l[i][c], w, L);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) O[e] = fmaf(x[e], w, O[e]);
+    }
+    o[y] = O;
+    ms[y] = M;
+    ls[y] = L;
+  }
+  if (a.splits > 1) {
+    // Every split writes its columns' states and counts itself at the tile's word; the last
+    // one finds them all, merges them and clears the word for the queue's next command.
+    // Nobody waits.  Each wave waits for its own stores before the barrier behind which
+    // one thread counts the workgroup (a release fence would write the XCD's L2 back).
+    const int64_t step = (int64_t)a.row_tiles * a.hkv * TC * kStash;
+    float *const tile_states = a.states + ((int64_t)t.loc.rank * a.hkv + kvh) * TC * kStash;
+#pragma unroll
+    for (int y = 0; y < kItems; ++y) {
+      const int c = (y * W * 64 + tid) >> 5, d = (tid & 31) * 4;
+      if (c >= cols) continue;
+      float *const st = tile_states + split * step + c * kStash;
+      store_state(st + 4 + d, o[y][0], o[y][1]);
+      store_state(st + 6 + d, o[y][2], o[y][3]);
+      if (d == 0) store_state(st, ms[y], ls[y]);
+    }
+    wait_loads<0>();  // and stores
+    __syncthreads();
+    uint32_t *const word = a.arrived + (uint64_t)(t.loc.rank * a.hkv + kvh) * (loom::kMx4JoinBytes / 4);
+    if (tid == 0)
+      sm.arrived = __hip_atomic_fetch_add(word, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    if (sm.arrived != (uint32_t)a.splits - 1u) return;
+    if (tid == 0) __hip_atomic_store(word, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+#pragma unroll
+    for (int y = 0; y < kItems; ++y) {
+      const int c = min((y * W * 64 + tid) >> 5, cols - 1), d = (tid & 31) * 4;
+      float M = -INFINITY, L = 0.0f;
+      f32x4 O = {};
+      for (int i0 = 0; i0 < a.splits; i0 += 4) {
+        f32x2 ml[4], x[4][2];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          // past the last state: its values again, with no weight
+          const float *st = tile_states + min(i0 + i, a.splits - 1) * step + c * kStash;
+          ml[i] = load_state(st);
+          x[i][0] = load_state(st + 4 + d);
+          x[i][1] = load_state(st + 6 + d);
+        }
+        float mb = M;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mb = fmaxf(mb, ml[i][0]);
+        const float old = M == -INFINITY ? 0.0f : fast_exp2(M - mb);
+        L *= old;
+        O *= old;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float w =
+              i0 + i < a.splits && ml[i][0] != -INFINITY ? fast_exp2(ml[i][0] - mb) : 0.0f;
+          L = fmaf(ml[i][1], w, L);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) O[e] = fmaf(x[i][e >> 1][e & 1], w, O[e]);
+        }
+        M = mb;
+      }
+      o[y] = O;
+      ms[y] = M;
+      ls[y] = L;
+    }
+  }
+  // Columns that are not finite are found token by token.
+#pragma unroll
+  for (int y = 0; y < kItems; ++y) {
+    const int c = (y * W * 64 + tid) >> 5;
+    const float inv = 1.0f / ls[y] * v_scale;
+    o[y] *= inv;
+    bool finite = true;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) finite &= fabsf(o[y][e]) < INFINITY;
+    if (c < cols && !finite) atomicOr(&sm.redo, 1u << c);
+  }
+  __syncthreads();
+  const uint32_t redo = uni((int)sm.redo);
+#pragma unroll
+  for (int y = 0; y < kItems; ++y) {
+    const int c = (y * W * 64 + tid) >> 5, d = (tid & 31) * 4;
+    if (c >= cols || (redo >> c & 1)) continue;
+    const int fc = t.col0 + c, rc = (int)((uint32_t)fc / (uint32_t)a.group);
+    const int64_t row = (int64_t)(t.loc.qs + rc) * a.hq + (int64_t)kvh * a.group + (fc - rc * a.group);
+    *reinterpret_cast<u32x2 *>(a.out + row * 128 + d) =
+        u32x2{bf16x2_pack(o[y][0], o[y][1]), bf16x2_pack(o[y][2], o[y][3])};
+    if (d == 0) a.lse[row] = ms[y] + __log2f(ls[y]);
+  }
+  if (redo)
+    for (int c = wave; c < cols; c += W)
+      if (redo >> c & 1) exact_column<KV>(a, t, t.col0 + c, lane, v_scale);
+}
+
+}  // namespace
+
+// ---- plan / enqueue -------------------------------------------------------------------
+struct loom_window_attention_plan {
+  loom_window_attention_plan_info_t info{};
+  int cus = 0;
+};
+
+namespace {
+
+constexpr uint64_t kMaxHeads = 4096;  // kv-heads: a row of all of them in a 32-bit stride
+constexpr int kMaxSplits = 16;
+
+// Workgroups per (tile, kv-head) of a row-tile command of `grid` unsplit ones, whose walks
+// hold about `tokens` tokens: as many as fill two workgroups per CU and leave every wave two
+// steps.
+int row_splits(uint64_t grid, uint64_t tokens, int cus) {
+  const uint64_t steps = (tokens + 31) / 32;
+  const uint64_t most = std::min<uint64_t>(kMaxSplits, 2 * (uint64_t)cus / std::max<uint64_t>(grid, 1));
+  return (int)std::max<uint64_t>(1, std::min(most, steps / (2 * kRowWaves)));
+}
+
+loom_status_t make_plan(const loom::DeviceInfo &dev, const loom_window_attention_spec_t *spec,
+                        uint32_t flags, loom_window_attention_plan_t **out, loom_error_t *err) {
+  loom_window_attention_spec_t s;
+  const loom_status_t rc =
+      loom_window_attention_spec_new(&spec->paged, spec->rows, spec->explicit_rows, spec->window,
+                                     spec->sinks, &s, err);
+  if (rc) return rc;
+  const float scale = s.paged.softmax_scale;
+  if (!(scale > 0.0f) || !std::isfinite(scale))
+    return fail(err, LOOM_PLAN_INVALID_OPTION, "softmax_scale");
+  const uint64_t hq = s.paged.num_query_heads, hkv = s.paged.num_kv_heads, group = hq / hkv;
+  const uint64_t batch = s.paged.batch_size;
+  if (hkv > kMaxHeads) return fail(err, LOOM_PLAN_STATE_COUNT_OUT_OF_RANGE, "window heads", hkv);
+  if (s.rows > (uint64_t)INT32_MAX / hq || batch >= (uint64_t)INT32_MAX)
+    return fail(err, LOOM_PLAN_STATE_COUNT_OUT_OF_RANGE, "window rows", s.rows);
+  const uint64_t cols = s.rows * group, tc = 16;
+  const uint64_t tiles = s.explicit_rows ? std::min(cols, (cols + (tc - 1) * batch) / tc)
+                                         : batch * ((group + tc - 1) / tc);
+  if (tiles * hkv * (kRowWaves * 64) >= (1ull << 32))
+    return fail(err, LOOM_PLAN_STATE_COUNT_OUT_OF_RANGE, "window rows", s.rows);
+  auto *p = new loom_window_attention_plan;
+  p->info.spec = s;
+  p->info.algorithm = flags & LOOM_PLAN_PREFILL_TILE_LONG ? LOOM_PAGED_PREFILL_LONG_TILE : LOOM_PAGED_PREFILL_ROW_TILE;
+  p->info.tile_cols = (uint32_t)tc;
+  p->info.row_tiles = tiles;
+  p->info.grid_blocks = tiles * hkv;
+  p->info.block_threads = kRowWaves * 64;
+  p->info.flags = flags;
+  p->cus = dev.cus;
+  *out = p;
+  return loom::ok(err);
+}
+
+}  // namespace
+
+extern "C" {
+
+loom_status_t loom_decode_provider_plan_window_paged_batch(
+    const loom_decode_provider_t *provider, const loom_window_attention_spec_t *spec, uint32_t flags,
+    loom_window_attention_plan_t **out, loom_error_t *err) {
+  if (!provider || !spec || !out) return fail(err, LOOM_NULL_ARGUMENT, "provider");
+  if (flags & ~LOOM_PLAN_PAGE_INDICES_CAPACITY)
+    return fail(err, LOOM_PLAN_INVALID_OPTION, "flags", flags);
+  if (spec->explicit_rows) return fail(err, LOOM_PLAN_INVALID_OPTION, "explicit_rows", 1);
+  return make_plan(provider->dev, spec, flags, out, err);
+}
+
+loom_status_t loom_prefill_provider_plan_window_paged(const loom_prefill_provider_t *provider,
+                                                      const loom_window_attention_spec_t *spec,
+                                                      uint32_t flags,
+                                                      loom_window_attention_plan_t **out,
+                                                      loom_error_t *err) {
+  if (!provider || !spec || !out) return fail(err, LOOM_NULL_ARGUMENT, "provider");
+  constexpr uint32_t kTiles = LOOM_PLAN_PREFILL_TILE_16 | LOOM_PLAN_PREFILL_TILE_LONG;
+  if ((flags & ~(LOOM_PLAN_PAGE_INDICES_CAPACITY | kTiles)) || (flags & kTiles) == kTiles)
+    return fail(err, LOOM_PLAN_INVALID_OPTION, "flags", flags);
+  if (!spec->explicit_rows) return fail(err, LOOM_PLAN_INVALID_OPTION, "explicit_rows", 0);
+  return make_plan(provider->dev, spec, flags, out, err);
+}
+
+void loom_window_attention_plan_free(loom_window_attention_plan_t *p) { delete p; }
+
+void loom_window_attention_plan_get_info(const loom_window_attention_plan_t *p,
+                                         loom_window_attention_plan_info_t *info) {
+  if (p && info) *info = p->info;
+}
+
+loom_status_t loom_window_attention_enqueue(const loom_window_attention_plan_t *plan,
+                                            loom_command_scope_t *scope,
+                                            const loom_window_attention_args_t *args,
+                                            loom_error_t *err) {
+  if (!plan || !scope || !args) return fail(err, LOOM_NULL_ARGUMENT, "plan");
+  const loom_window_attention_spec_t &s = plan->info.spec;
+  const loom_paged_decode_spec_t &pg = s.paged;
+  const bool fp8 = pg.kv_dtype == LOOM_KV_DTYPE_FP8_E4M3, mx = pg.kv_dtype == LOOM_KV_DTYPE_MXFP4;
+  const loom_dtype_t kv_t = fp8 || mx ? LOOM_DTYPE_U8 : LOOM_DTYPE_BF16;
+  const uint64_t page_rows = pg.page_size ? pg.page_size : loom::kPageSize;
+  const uint64_t head_rows = pg.max_num_pages * page_rows * pg.num_kv_heads;
+  const uint64_t kvn = head_rows * (mx ? LOOM_MXFP4_ROW_BYTES : loom::kHeadDim);
+  const uint64_t qn = s.rows * pg.num_query_heads * loom::kHeadDim;
+  struct Operand {
+    loom::OperandSpec spec;
+    loom_handle_t handle;
+    uint64_t want;
+    bool aligned;  // 4-byte boundary
+  };
+  // the operands of every form, then those of some
+  const Operand all[12] = {
+      {{"Q", LOOM_DTYPE_BF16, false}, args->query, qn, true},
+      {{"K_pages", kv_t, false}, args->key_pages, kvn, true},
+      {{"V_pages", kv_t, false}, args->value_pages, kvn, true},
+      {{"page_indptr", LOOM_DTYPE_I32, false}, args->page_indptr, pg.batch_size + 1, false},
+      {{"page_indices", LOOM_DTYPE_I32, false}, args->page_indices, 0, false},
+      {{"last_page_len", LOOM_DTYPE_I32, false}, args->last_page_len, pg.batch_size, false},
+      {{"O", LOOM_DTYPE_BF16, true}, args->output, qn, true},
+      {{"LSE", LOOM_DTYPE_F32, true}, args->lse, s.rows * pg.num_query_heads, true},
+      {{"qo_indptr", LOOM_DTYPE_I32, false}, args->qo_indptr, pg.batch_size + 1, false},
+      {{"kv_scales", LOOM_DTYPE_F32, false}, args->kv_scales, 2, true},
+      {{"K_scales", LOOM_DTYPE_U8, false}, args->key_scales, head_rows * LOOM_MXFP4_ROW_SCALES, true},
+      {{"V_scales", LOOM_DTYPE_U8, false}, args->value_scales, head_rows * LOOM_MXFP4_ROW_SCALES, true}};
+  int which[12], n = 0;
+  for (int i = 0; i < 12; ++i)
+    if (i < 8 || (i == 8 && s.explicit_rows) || (i == 9 && fp8) || (i >= 10 && mx)) which[n++] = i;
+  loom::OperandSpec ops[12];
+  loom_handle_t hs[12];
+  for (int j = 0; j < n; ++j) {
+    ops[j] = all[which[j]].spec;
+    hs[j] = all[which[j]].handle;
+  }
+  const loom::Lease *found[12], *l[12] = {};
+  loom_status_t rc = loom::resolve_command(scope, hs, ops, n, found, err);
+  if (rc) return rc;
+  for (int j = 0; j < n; ++j) {
+    const Operand &o = all[which[j]];
+    l[which[j]] = found[j];
+    if (which[j] == 4) {
+      if (found[j]->numel < pg.batch_size)
+        return fail(err, LOOM_ENQ_PAGE_INDICES_TOO_SHORT, o.spec.name, pg.batch_size, found[j]->numel);
+      if (found[j]->numel > (uint64_t)INT32_MAX / page_rows)
+        return fail(err, LOOM_ENQ_PAGE_INDICES_TOO_LONG, o.spec.name,
+                    (int64_t)((uint64_t)INT32_MAX / page_rows), found[j]->numel);
+    } else if (found[j]->numel != o.want) {
+      return fail(err, LOOM_ENQ_LENGTH_MISMATCH, o.spec.name, o.want, found[j]->numel);
+    }
+    if (o.aligned && found[j]->ptr % 4 != 0)
+      return fail(err, LOOM_ENQ_MISALIGNED_BUFFER, o.spec.name, (int64_t)found[j]->ptr, 4);
+  }
+  WindowArgs a{};
+  a.q = (const uint16_t *)l[0]->ptr;
+  a.k = (const uint16_t *)l[1]->ptr;
+  a.v = (const uint16_t *)l[2]->ptr;
+  a.indptr = (const int32_t *)l[3]->ptr;
+  a.indices = (const int32_t *)l[4]->ptr;
+  a.last = (const int32_t *)l[5]->ptr;
+  a.out = (uint16_t *)l[6]->ptr;
+  a.lse = (float *)l[7]->ptr;
+  a.qo = s.explicit_rows ? (const int32_t *)l[8]->ptr : nullptr;
+  a.kv_scales = fp8 ? (const float *)l[9]->ptr : nullptr;
+  a.k_mx = mx ? (const uint8_t *)l[10]->ptr : nullptr;
+  a.v_mx = mx ? (const uint8_t *)l[11]->ptr : nullptr;
+  a.batch = (int32_t)pg.batch_size;
+  a.nnz = (int32_t)s.rows;
+  a.hq = (int32_t)pg.num_query_heads;
+  a.hkv = (int32_t)pg.num_kv_heads;
+  a.group = a.hq / a.hkv;
+  a.pool = (int64_t)pg.max_num_pages;
+  a.n_indices = (int64_t)l[4]->numel;
+  a.scale_log2 = pg.softmax_scale * 1.44269504088896340736f;
+  a.indices_capacity = (plan->info.flags & LOOM_PLAN_PAGE_INDICES_CAPACITY) ? 1 : 0;
+  a.page_rows = (int32_t)page_rows;
+  a.blocks_lg = page_rows == 64 ? 2 : page_rows == 32 ? 1 : 0;
+  const int row = mx ? 64 : fp8 ? 128 : 256;
+  const bool hnd = pg.kv_layout == LOOM_KV_LAYOUT_HND;
+  a.head_bytes = hnd ? a.page_rows * row : row;
+  a.row_bytes = hnd ? row : a.hkv * row;
+  a.window = s.window == 0 || s.window > (uint64_t)INT32_MAX ? INT32_MAX : (int32_t)s.window;
+  a.sinks = (int32_t)std::min<uint64_t>(s.sinks, INT32_MAX - 64);
+  a.row_tiles = (int32_t)plan->info.row_tiles;
+  a.head_tiles = (a.group + 15) / 16;
+  // the tokens that a request's rows see, at most: its window, or the average context
+  const uint64_t tokens =
+      std::min<uint64_t>((uint64_t)a.window + (uint64_t)a.sinks + s.rows / pg.batch_size,
+                         (uint64_t)a.n_indices * page_rows / pg.batch_size);
+  const uint64_t grid = plan->info.grid_blocks;
+  a.splits = row_splits(grid, tokens, plan->cus);
+  if (a.splits > 1) {
+    a.arrived = scope->queue->joins;
+    a.states = (float *)loom::queue_shares(scope, (uint64_t)a.splits * grid * 16 * kStash * 4);
+    if (!a.states || !a.arrived || grid > loom::kMx4Joins) a.splits = 1;
+  }
+  const dim3 blocks((unsigned)(grid * a.splits)), threads(plan->info.block_threads);
+  hipStream_t stream = scope->queue->stream;
+  if (mx)
+    hipLaunchKernelGGL(window_rows_kernel<kMx4>, blocks, threads, 0, stream, a);
+  else if (fp8)
+    hipLaunchKernelGGL(window_rows_kernel<kFp8>, blocks, threads, 0, stream, a);
+  else
+    hipLaunchKernelGGL(window_rows_kernel<kBf16>, blocks, threads, 0, stream, a);
+  return loom::record_launch(scope, hipGetLastError(), err);
+}
+
+}  // extern "C"

@@ -426,6 +426,41 @@ class PagedKvReadSpec:
     mx_scales_numel = property(lambda s: s.paged.mx_scales_numel)
 
 
+class WindowPagedAttentionSpec:
+    """Attention with a sliding window and sinks over a paged cache in BF16, FP8 E4M3 or
+    MXFP4 (no reference counterpart).  A row at position p sees the tokens up to its own
+    that lie in the last `window` (0: all) or are among the request's first `sinks`.
+    `explicit_rows` False: one row per request at kv_len - 1 (rows = batch_size), for a
+    decode provider; else `rows` new rows, ragged by qo_indptr, for a prefill provider."""
+
+    def __init__(self, rows, batch_size, max_num_pages, num_query_heads, num_kv_heads,
+                 head_dim=HEAD_DIM, page_size=PAGE_SIZE, kv_layout="NHD", kv_dtype="bf16",
+                 kv_page_size=None, window=0, sinks=0, explicit_rows=True):
+        for name, n in (("rows", rows), ("window", window), ("sinks", sinks)):
+            if not 0 <= n < 1 << 64:
+                raise ValueError(f"{name} must lie in 0 .. 2^64 - 1, got {n}")
+        self.paged = Bf16PagedBatchDecodeSpec(batch_size, max_num_pages, num_query_heads,
+                                              num_kv_heads, head_dim, page_size, kv_layout,
+                                              kv_dtype, kv_page_size)
+        self._c = _ffi.WindowAttentionSpec()
+        _call(lib().loom_window_attention_spec_new, C.byref(self.paged._c), rows,
+              1 if explicit_rows else 0, window, sinks, C.byref(self._c))
+
+    rows = property(lambda s: s._c.rows)
+    window = property(lambda s: s._c.window)
+    sinks = property(lambda s: s._c.sinks)
+    explicit_rows = property(lambda s: bool(s._c.explicit_rows))
+    batch_size = property(lambda s: s.paged.batch_size)
+    max_num_pages = property(lambda s: s.paged.max_num_pages)
+    num_query_heads = property(lambda s: s.paged.num_query_heads)
+    num_kv_heads = property(lambda s: s.paged.num_kv_heads)
+    query_numel = property(lambda s: s.rows * s.num_query_heads * HEAD_DIM)
+    output_numel = query_numel
+    lse_numel = property(lambda s: s.rows * s.num_query_heads)
+    kv_pages_numel = property(lambda s: s.paged.kv_pages_numel)
+    mx_scales_numel = property(lambda s: s.paged.mx_scales_numel)
+
+
 def _wrap_paged(c_spec) -> Bf16PagedBatchDecodeSpec:
     s = Bf16PagedBatchDecodeSpec.__new__(Bf16PagedBatchDecodeSpec)
     s._c = c_spec
@@ -885,6 +920,56 @@ class Bf16SingleDecodeSplitKPlan:
             pass
 
 
+@dataclass(frozen=True)
+class WindowPagedAttentionArgs:
+    """Operands of window attention: `qo_indptr` [B+1] for the ragged form, `kv_scales`
+    [k_scale, v_scale] for FP8 pages, `key_scales` and `value_scales` for MXFP4 pages."""
+    query: Read
+    key_pages: Read
+    value_pages: Read
+    page_indptr: Read
+    page_indices: Read
+    last_page_len: Read
+    output: Write
+    lse: Write
+    qo_indptr: Optional[Read] = None
+    kv_scales: Optional[Read] = None
+    key_scales: Optional[Read] = None
+    value_scales: Optional[Read] = None
+
+    def __post_init__(self):
+        c = _ffi.WindowAttentionArgs(*[
+            _h(getattr(self, f)) for f, _ in _ffi.WindowAttentionArgs._fields_])
+        object.__setattr__(self, "_struct", c)
+        object.__setattr__(self, "_ref", C.byref(c))
+
+
+class WindowPagedAttentionPlan:
+    def __init__(self, ptr, spec):
+        self._p = ptr
+        self._spec = spec
+        self.info = _ffi.WindowAttentionPlanInfo()
+        lib().loom_window_attention_plan_get_info(self._p, C.byref(self.info))
+
+    def spec(self):
+        return self._spec
+
+    @property
+    def algorithm(self) -> str:
+        return {1: "row_tile", 3: "long_tile"}[self.info.algorithm]
+
+    def enqueue_into(self, scope: CommandScope, args: WindowPagedAttentionArgs):
+        _enqueue(_ffi.load().loom_window_attention_enqueue, self._p, scope._p, args._ref)
+
+    def __del__(self):
+        try:
+            if getattr(self, "_p", None):
+                lib().loom_window_attention_plan_free(self._p)
+                self._p = None
+        except Exception:  # interpreter shutdown: module globals are gone
+            pass
+
+
 class DecodeProvider:
     """decode.rs:1001-1104."""
 
@@ -921,6 +1006,15 @@ class DecodeProvider:
         _call(lib().loom_decode_provider_plan_bf16_paged_batch, self._p, C.byref(spec._c),
               C.byref(opt), C.byref(out))
         return Bf16PagedBatchDecodePlan(out.value, spec)
+
+    def plan_window_paged_batch(self, spec: WindowPagedAttentionSpec,
+                                indices_capacity: bool = False) -> WindowPagedAttentionPlan:
+        """Window attention of one row per request (explicit_rows False; no reference
+        counterpart)."""
+        out = C.c_void_p()
+        _call(lib().loom_decode_provider_plan_window_paged_batch, self._p, C.byref(spec._c),
+              PLAN_PAGE_INDICES_CAPACITY if indices_capacity else 0, C.byref(out))
+        return WindowPagedAttentionPlan(out.value, spec)
 
     def __del__(self):
         try:
@@ -1286,6 +1380,16 @@ class PrefillProvider:
         _call(lib().loom_prefill_provider_plan_paged_kv_read, self._p, C.byref(spec._c),
               PLAN_PAGE_INDICES_CAPACITY if indices_capacity else 0, C.byref(out))
         return PagedKvReadPlan(out.value, spec)
+
+    def plan_window_paged(self, spec: WindowPagedAttentionSpec, indices_capacity: bool = False,
+                          tile_cols=0) -> WindowPagedAttentionPlan:
+        """Window attention of ragged rows (no reference counterpart); `tile_cols`: 0
+        (chosen from the spec), 16 (row tiles) or "long" (long tiles)."""
+        out = C.c_void_p()
+        _call(lib().loom_prefill_provider_plan_window_paged, self._p, C.byref(spec._c),
+              (PLAN_PAGE_INDICES_CAPACITY if indices_capacity else 0)
+              | _prefill_tile_flag(tile_cols), C.byref(out))
+        return WindowPagedAttentionPlan(out.value, spec)
 
     def __del__(self):
         try:

@@ -168,6 +168,22 @@ class PagedKvReadArgs(C.Structure):
                                       "kv_start", "key", "value")]
 
 
+class WindowAttentionSpec(C.Structure):
+    _fields_ = [("paged", PagedDecodeSpec), ("rows", u64), ("window", u64), ("sinks", u64),
+                ("explicit_rows", i32)]
+
+
+class WindowAttentionPlanInfo(C.Structure):
+    _fields_ = [("spec", WindowAttentionSpec), ("algorithm", i32), ("tile_cols", u32),
+                ("row_tiles", u64), ("grid_blocks", u64), ("block_threads", u32), ("flags", u32)]
+
+
+class WindowAttentionArgs(C.Structure):
+    _fields_ = [(n, Handle) for n in ("query", "key_pages", "value_pages", "qo_indptr",
+                                      "page_indptr", "page_indices", "last_page_len", "output",
+                                      "lse", "kv_scales", "key_scales", "value_scales")]
+
+
 P = C.POINTER
 pi32 = P(i32)
 E = P(Error)
@@ -291,6 +307,15 @@ SIGNATURES = {
     "loom_prefill_provider_plan_paged_kv_read": (i32, [vp, P(PagedKvReadSpec), u32, P(vp), E]),
     "loom_paged_kv_read_plan_free": (None, [vp]),
     "loom_paged_kv_read_enqueue": (i32, [vp, vp, P(PagedKvReadArgs), E]),
+    "loom_window_attention_spec_new": (
+        i32, [P(PagedDecodeSpec), u64, i32, u64, u64, P(WindowAttentionSpec), E]),
+    "loom_decode_provider_plan_window_paged_batch": (
+        i32, [vp, P(WindowAttentionSpec), u32, P(vp), E]),
+    "loom_prefill_provider_plan_window_paged": (
+        i32, [vp, P(WindowAttentionSpec), u32, P(vp), E]),
+    "loom_window_attention_plan_free": (None, [vp]),
+    "loom_window_attention_plan_get_info": (None, [vp, P(WindowAttentionPlanInfo)]),
+    "loom_window_attention_enqueue": (i32, [vp, vp, P(WindowAttentionArgs), E]),
     "loom_graph_queue_new": (i32, [C.c_int, u64, P(vp), E]),
     "loom_graph_queue_free": (None, [vp]),
     "loom_graph_queue_bindings": (i32, [vp, u64, P(vp), E]),

@@ -26,7 +26,7 @@ FLAGS=(--offload-arch=gfx950 -O1 -g -std=c++17 -fPIC -Wall -Wno-unused-function 
        -I"$root/include" -I"$csrc")
 pids=()
 for s in contract.cpp runtime.cpp paged_decode.hip paged_decode_mx4.hip paged_prefill.hip kv_read.hip \
-         rope_append.hip; do
+         rope_append.hip window_attention.hip; do
   "$HIPCC" -x hip "${FLAGS[@]}" "${HOSTSAN[@]}" -c "$csrc/$s" -o "$out/obj/${s%.*}.o" \
       2> >(grep -v "packed-fp32-ops' is not a recognized feature" >&2) &
   pids+=($!)
