@@ -604,18 +604,402 @@ __global__ __launch_bounds__(kRowWaves * 64) void window_rows_kernel(WindowArgs 
       if (redo >> c & 1) exact_column<KV>(a, t, t.col0 + c, lane, v_scale);
 }
 
+// ---- long tiles --------------------------------------------------------------------
+// Many rows: the pipelined long tiles of paged prefill (PipeWave: 32 columns per wave, NW
+// waves over 32 * NW columns, G = W / NW groups of them that split the walk) over the
+// blocks of the walk, in 32-token steps of two blocks each.  Two steps at most at either end of
+// the window, and the sinks', hide tokens from some columns and are masked; the steps
+// between take PipeWave's unmasked path.  P is rounded once to BF16, and the normalizer sums
+// the rounded weights: the errors of many tokens average out below O's own rounding.
+//
+// BF16 and FP8 blocks are loaded straight into the ring, NW slots deep.  MXFP4 codes go
+// through registers, 32 values and their scale per lane and block, two steps ahead, and are
+// written to a ring of two slots as BF16: widened once per workgroup instead of once per
+// wave (32 conversions per wave and step, and V's scales, which run along the
+// contraction's other axis, would have to be applied to P).
+template <int W, int NW>
+struct LongSmem {
+  LocateSmem<W> loc;
+  float m[W][32], l[W][32];  // the groups' column states
+  uint32_t bad[W];
+  uint32_t redo[NW];         // columns of a group's wave whose O is not finite
+  int32_t next_idx[W][64];   // page indices of the next 64 blocks
+};
+
+template <Kv KV, int W, int NW>
+__global__ __launch_bounds__(W * 64, 2) void window_long_kernel(WindowArgs args) {
+  constexpr int G = W / NW, TC = 32 * NW;
+  constexpr int kOutRow = 256 + 16;  // bytes of a row of O in LDS
+  constexpr bool FP8 = KV == kFp8, MX = KV == kMx4;
+  using Pipe = PipeWave<NW, FP8, false, G>;
+  constexpr int kSlot = Pipe::kSlotBytes, kSlots = MX ? 2 : Pipe::kSlots;
+  constexpr int kRingBytes = G * kSlots * kSlot;
+  constexpr int kMergeBytes = G > 1 ? W * 64 * 64 * 4 : 0;
+  constexpr int kOutBytes = W * 32 * kOutRow;
+  __shared__ LongSmem<W, NW> sm;
+  __shared__ __align__(16) uint8_t ring[std::max({kRingBytes, kMergeBytes, kOutBytes})];
+  WindowArgs a = args;
+  float v_scale = 1.0f;
+  if constexpr (FP8) {
+    a.scale_log2 *= a.kv_scales[0];
+    v_scale = a.kv_scales[1];
+  }
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = uni(tid >> 6);
+  const int col = lane & 15, quad = lane >> 4;
+  Tile t;
+  if (!find_tile<W, TC>(a, sm.loc, t, 0)) return;
+  const int kvh = t.loc.kvh;
+  auto row_of = [&](int f) { return (int)((uint32_t)f / (uint32_t)a.group); };
+  const int wq = wave % NW, grp = wave / NW;  // the wave's columns and its group
+  const int own0 = t.col0 + 32 * wq;
+  const int p0 = t.kv_len - t.group_rows;
+  Pipe lw{a, lane, col, quad};
+  int beg_col[2], end_col[2], qi_t[2], gh_t[2];
+  bool colv_t[2];
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    const int f = own0 + 16 * c + col;
+    colv_t[c] = f < t.fcols;
+    qi_t[c] = colv_t[c] ? row_of(f) : 0;
+    gh_t[c] = colv_t[c] ? f - qi_t[c] * a.group : 0;
+    end_col[c] = colv_t[c] ? p0 + qi_t[c] + 1 : 0;
+    beg_col[c] = max(0, end_col[c] - a.window);
+  }
+  lw.reset(ring + grp * kSlots * kSlot);
+  // Steps that need no mask, [first_full, last_full): whose tokens every column of the
+  // wave sees; and the steps up to the wave's last column's own token.
+  int first_full = 0, last_full = 0, own_steps = 0;
+  if (own0 < t.fcols) {
+    const int w_lo = p0 + row_of(own0), w_hi = p0 + row_of(min(own0 + 31, t.fcols - 1));
+    const int x0 = t.sink_blocks - t.first_block;  // place of block b of the window: b + x0
+    first_full = (((max(0, w_hi + 1 - a.window) + 15) >> 4) + x0 + 1) >> 1;
+    last_full = (((w_lo + 1) >> 4) + x0) >> 1;
+    own_steps = ((w_hi >> 4) + 1 + x0 + 1) >> 1;
+  }
+  // The first page indices, then the queries: the first K/V loads wait for the former only.
+  const int idx =
+      lane < t.blocks ? a.indices[t.loc.ps + (t.block(lane) >> a.blocks_lg)] : 0;
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    const uint16_t *qp = colv_t[c] ? a.q + ((int64_t)(t.loc.qs + qi_t[c]) * a.hq +
+                                            (int64_t)kvh * a.group + gh_t[c]) * 128
+                                   : a.q;
+#pragma unroll
+    for (int x = 0; x < 4; ++x) lw.qf[c][x] = load16(qp + Pipe::q_dim(x, quad));
+  }
+  // Lane l holds the place of block 64 win + l of the walk in the wave's matrix (K or V):
+  // address of its first row, valid rows' bytes, and (MXFP4) its scales' address.
+  const bool loads_k = wq < NW / 2;
+  const uint64_t kv_base = (uint64_t)(loads_k ? a.k : a.v);
+  const uint64_t mx_base = MX ? (uint64_t)(loads_k ? a.k_mx : a.v_mx) : 0;
+  int win = -1;
+  uint32_t blk_lo = 0, blk_hi = 0, mx_lo = 0, mx_hi = 0;
+  int blk_rows = 0;
+  auto place = [&](int b) {
+    if ((b >> 5) == win) return;
+    win = b >> 5;
+    const int x = 64 * win + lane;
+    const int blk = t.block(x);
+    int rows = x < t.blocks ? t.rows(a, x) : 0;
+    const int pg = win == 0 ? idx : sm.next_idx[wave][lane];
+    if (pg < 0 || (int64_t)pg >= a.pool) rows = 0;  // (the request is refused)
+    const int row = (blk & ((1 << a.blocks_lg) - 1)) * 16;
+    const uint64_t at = kv_base + row_at<KV>(a, pg, row, kvh);
+    blk_lo = (uint32_t)at;
+    blk_hi = (uint32_t)(at >> 32);
+    blk_rows = rows;
+    if constexpr (MX) {
+      const uint64_t sc = mx_base + scale_at(a, pg, row, kvh);
+      mx_lo = (uint32_t)sc;
+      mx_hi = (uint32_t)(sc >> 32);
+    }
+    asm volatile("" ::"v"(blk_lo), "v"(blk_hi), "v"(blk_rows) : "memory");  // next_idx is read
+    // (past the walk's end: past the buffer's, or of no use)
+    lds_load4(__builtin_amdgcn_make_buffer_rsrc(const_cast<int32_t *>(a.indices + t.loc.ps), 0,
+                                                4 * (t.loc.pe - t.loc.ps), 0x00020000),
+              &sm.next_idx[wave][0], (t.block(x + 64) >> a.blocks_lg) * 4);
+  };
+  auto lane64 = [](uint32_t l, uint32_t h, int j) {
+    return ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)h, j) << 32) |
+           (uint32_t)__builtin_amdgcn_readlane((int)l, j);
+  };
+  auto rsrc = [](uint64_t at, int bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void *>(at), 0, bytes, 0x00020000);
+  };
+  // Checked and masked while the first blocks are on their way.
+  bool bad = false;
+  auto first = [&]() {
+    bad = bad_pages(a, t, tid, W * 64);
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) lw.qf[c][x] = colv_t[c] ? lw.qf[c][x] : u32x4{0, 0, 0, 0};
+  };
+  auto mask = [&](typename Pipe::Scores &s, int b) {
+    const int t0 = 16 * t.block(2 * b) + 4 * quad, t1 = 16 * t.block(2 * b + 1) + 4 * quad;
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int tok = (h ? t1 : t0) + i;
+          s.s[c][h][i] =
+              tok < end_col[c] && (tok >= beg_col[c] || tok < a.sinks) ? s.s[c][h][i] : -INFINITY;
+        }
+  };
+  const int nb = (t.blocks + 1) >> 1, steps = (nb + G - 1) / G;
+  const int nbw = uni(max(0, (min(own_steps, nb) - grp + G - 1) / G));
+  first_full = uni(first_full);
+  last_full = uni(last_full);
+  auto slot_of = [](int j) { return (j & (kSlots - 1)) * kSlot; };
+  typename Pipe::Scores sa, sb;
+  typename Pipe::VFrags v = {};
+  typename Pipe::Weights w = {};
+  // The walk: at step j the wave's group takes the weights of its j-th block, the scores of
+  // the next and the products of the one before; `feed(j, s)` (s: j, or its slot) meets the
+  // other waves and refills the ring.
+  auto walk = [&](auto feed) {
+    if (nbw > 0) {
+      const auto k = lw.read_k(0);
+#pragma unroll
+      for (int c = 0; c < 8; ++c) lw.score(k, sa, c);
+    }
+    int j = 0;
+    while (j < nbw) {
+#pragma unroll
+      for (int s = 0; s < kSlots; ++s) {
+        if (s > 0 && j >= nbw) break;
+        feed(j, s);
+        typename Pipe::Scores &cur = s & 1 ? sb : sa, &nxt = s & 1 ? sa : sb;
+        const int b = G * j + grp;
+        if (b < first_full || b >= last_full) mask(cur, b);
+        lw.step(slot_of(s + 1), slot_of(s), cur, nxt, v, w);
+        ++j;
+      }
+    }
+#pragma unroll
+    for (int x = 0; x < 8; ++x) lw.product(v, w, x);
+    for (; j < steps; ++j) {  // (MXFP4: registers are named by j's parity)
+      if (!MX || !(j & 1))
+        feed(j, MX ? 0 : j);
+      else
+        feed(j, 1);
+    }
+  };
+  const uint32_t ring_lds = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)ring +
+                            (uint32_t)(grp * kSlots * kSlot);
+  if constexpr (!MX) {
+    // K runs one block ahead of V, so that one barrier per step publishes K (j + 1) and V (j);
+    // a slot is refilled one step after it was read.
+    int lane_off[16 / Pipe::kGroupRows];
+    {
+      const int sub = (lane & (Pipe::kUnits - 1)) ^ Pipe::swizzle(lane / Pipe::kUnits);
+#pragma unroll
+      for (int x = 0; x < 16 / Pipe::kGroupRows; ++x)
+        lane_off[x] = (x * Pipe::kGroupRows + lane / Pipe::kUnits) * a.row_bytes + sub * 16;
+    }
+    auto load = [&](int b, uint32_t slot) {
+      place(b);
+#pragma unroll
+      for (int y = 0; y < (NW == 4 ? 1 : 2); ++y) {
+        const int h = NW == 4 ? (wq & 1) : y;
+        const int l = (2 * b + h) & 63;
+        const int rows = __builtin_amdgcn_readlane(blk_rows, l);
+        const __amdgpu_buffer_rsrc_t r = rsrc(lane64(blk_lo, blk_hi, l),
+                                              rows > 0 ? (rows - 1) * a.row_bytes + kRowBytes<KV> : 0);
+        constexpr int kHalf = Pipe::kGroups / 2;
+#pragma unroll
+        for (int x = 0; x < kHalf; ++x) {
+          const uint32_t kg = (uint32_t)((h * kHalf + x) * Pipe::kKGroup);
+          const uint32_t vg = (uint32_t)(Pipe::v_group(x) + h * (Pipe::v_group(kHalf) - Pipe::v_group(0)));
+          lds_load16_at(r, slot + (loads_k ? kg : vg), lane_off[x]);
+        }
+      }
+    };
+    const int ahead = uni(kSlots - (loads_k ? 0 : 1));
+    if (loads_k) load(grp, ring_lds);
+#pragma unroll
+    for (int j = 1 - kSlots; j < 0; ++j) load(G * (j + ahead) + grp, ring_lds + slot_of(j + ahead));
+    first();
+    Pipe::template publish<(kSlots - 1) * Pipe::kLoads>();
+    walk([&](int j, int s) {
+      Pipe::template publish<(kSlots - 2) * Pipe::kLoads>();
+      load(G * (j + ahead) + grp, ring_lds + slot_of(s + ahead));
+    });
+  } else {
+    // The wave's share of a block: its 16-row half (NW = 2: both), 32 values per lane.
+    constexpr int kHalves = NW == 4 ? 1 : 2;
+    struct Share {
+      u32x4 w[kHalves];
+      uint32_t s[kHalves];
+    };
+    auto fetch = [&](int b, Share &g) {
+      place(b);
+#pragma unroll
+      for (int y = 0; y < kHalves; ++y) {
+        const int l = (2 * b + (NW == 4 ? (wq & 1) : y)) & 63;
+        const int rows = __builtin_amdgcn_readlane(blk_rows, l);
+        g.w[y] = load16_rows<false>(
+            rsrc(lane64(blk_lo, blk_hi, l), rows > 0 ? (rows - 1) * a.row_bytes + 64 : 0),
+            (lane >> 2) * a.row_bytes + (lane & 3) * 16);
+        g.s[y] = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(rsrc(lane64(mx_lo, mx_hi, l), 4 * rows),
+                                                              lane, 0, 0);
+      }
+    };
+    uint8_t *const group_ring = ring + grp * kSlots * kSlot;
+    auto put = [&](int slot, const Share &g) {
+#pragma unroll
+      for (int y = 0; y < kHalves; ++y)
+        put_mx<Pipe>(group_ring + slot, !loads_k, 16 * (NW == 4 ? (wq & 1) : y) + (lane >> 2), lane & 3,
+                     g.w[y], g.s[y]);
+    };
+    // K (j + 2) and V (j + 1) are written at step j, to slots read at step j - 1.
+    const int ahead = uni(loads_k ? 2 : 1);
+    Share g[2], f0;
+    if (loads_k) fetch(grp, f0);
+    fetch(G * (ahead - 1) + grp, g[0]);
+    fetch(G * ahead + grp, g[1]);
+    first();
+    if (loads_k) put(0, f0);
+    put(slot_of(ahead - 1), g[0]);
+    fetch(G * (ahead + 1) + grp, g[0]);
+    auto meet = [&]() {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+    };
+    meet();
+    // (g[1]: item ahead, g[0]: ahead + 1; item j + ahead sits in g[(j + 1) & 1])
+    walk([&](int j, int s) {
+      meet();  // (every wave has read K (j) and V (j - 1))
+      put(slot_of(s + ahead), g[(s + 1) & 1]);
+      fetch(G * (j + ahead + 2) + grp, g[(s + 1) & 1]);
+    });
+  }
+  wait_loads<0>();
+
+  float L[2], M[2];
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    L[c] = quad_sum(lw.lsum[c]);
+    M[c] = -lw.nmax[c];
+    if (G > 1 && quad == 0) {
+      sm.m[wave][16 * c + col] = M[c];
+      sm.l[wave][16 * c + col] = L[c];
+    }
+  }
+  if (tid < NW) sm.redo[tid] = 0;
+  if (block_or(bad, sm.bad)) return;
+  constexpr int kOwn = 8 / G;  // 16-dim blocks that a group finishes
+  if constexpr (G > 1) {
+    // The groups' states merge: every wave writes the dims that other groups finish, group
+    // g finishes dims 128 g / G .. of its columns.
+    static_assert(W * 2 * 8 * 64 * sizeof(f32x4) <= sizeof(ring), "merge staging");
+    f32x4 *xs = reinterpret_cast<f32x4 *>(ring) + lane;
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (e / kOwn != grp) xs[((wave * 2 + c) * 8 + e) * 64] = lw.acc[c][e];
+    __syncthreads();
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+#pragma unroll
+      for (int g = 0; g < G; ++g) M[c] = fmaxf(M[c], sm.m[g * NW + wq][16 * c + col]);
+      float f[G];
+      L[c] = 0.0f;
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        const float m = sm.m[g * NW + wq][16 * c + col];
+        f[g] = m == -INFINITY ? 0.0f : fast_exp2(m - M[c]);
+        L[c] = fmaf(sm.l[g * NW + wq][16 * c + col], f[g], L[c]);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        if (e / kOwn != grp) continue;
+        f32x4 o = {};
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+          const f32x4 x = g == grp ? lw.acc[c][e] : xs[(((g * NW + wq) * 2 + c) * 8 + e) * 64];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[i] = fmaf(x[i], f[g], o[i]);
+        }
+        lw.acc[c][e] = o;
+      }
+    }
+  }
+  // Columns that are not finite are found token by token.
+  uint32_t redo = 0;
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    const float inv = 1.0f / L[c] * v_scale;
+    float z = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e / kOwn == grp) {
+        lw.acc[c][e] *= inv;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) z = fmaf(lw.acc[c][e][i], 0.0f, z);  // NaN: not finite
+      }
+    const uint64_t b = __builtin_amdgcn_ballot_w64(colv_t[c] && !(z == 0.0f));
+    redo |= (uint32_t)((b | b >> 16 | b >> 32 | b >> 48) & 0xffff) << (16 * c);
+  }
+  if constexpr (G > 1) {
+    if (redo && lane == 0) atomicOr(&sm.redo[wq], redo);
+    __syncthreads();
+    redo = (uint32_t)uni((int)sm.redo[wq]);
+  }
+  // O through LDS, each wave its own 32 rows: whole rows go out 16 bytes per lane.
+  static_assert(W * 32 * kOutRow <= sizeof(ring), "O staging");
+  uint8_t *ot = ring + wave * 32 * kOutRow;
+  int row_head[2];  // output row of each tile's column, -1: none
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    const bool mine = colv_t[c] && !(redo >> (16 * c + col) & 1);
+    row_head[c] = mine ? (t.loc.qs + qi_t[c]) * a.hq + kvh * a.group + gh_t[c] : -1;
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e / kOwn == grp)
+        *reinterpret_cast<u32x2 *>(ot + (16 * c + col) * kOutRow + 32 * e + 8 * quad) =
+            u32x2{bf16x2_pack(lw.acc[c][e][0], lw.acc[c][e][1]),
+                  bf16x2_pack(lw.acc[c][e][2], lw.acc[c][e][3])};
+    if (quad == 0 && grp == 0 && mine) a.lse[row_head[c]] = M[c] + __log2f(L[c]);
+  }
+  wave_lds_fence();
+  constexpr int kOwnUnits = 2 * kOwn, kRowsPer = 64 / kOwnUnits;  // 16-byte units of a row
+  const int unit = grp * kOwnUnits + (lane & (kOwnUnits - 1));
+#pragma unroll
+  for (int x = 0; x < 32 / kRowsPer; ++x) {
+    const int r = x * kRowsPer + lane / kOwnUnits;  // column of the wave
+    const int rh0 = __shfl(row_head[0], r & 15, 64), rh1 = __shfl(row_head[1], r & 15, 64);
+    const int rh = r < 16 ? rh0 : rh1;
+    if (rh >= 0)
+      *reinterpret_cast<u32x4 *>(a.out + (int64_t)rh * 128 + unit * 8) =
+          *reinterpret_cast<const u32x4 *>(ot + r * kOutRow + unit * 16);
+  }
+  if (redo)
+    for (int c = grp; c < 32; c += G)
+      if (redo >> c & 1) exact_column<KV>(a, t, own0 + c, lane, v_scale);
+}
+
 }  // namespace
 
 // ---- plan / enqueue -------------------------------------------------------------------
 struct loom_window_attention_plan {
   loom_window_attention_plan_info_t info{};
   int cus = 0;
+  uint32_t groups = 1;  // long tiles: wave groups that split a walk
 };
 
 namespace {
 
 constexpr uint64_t kMaxHeads = 4096;  // kv-heads: a row of all of them in a 32-bit stride
 constexpr int kMaxSplits = 16;
+
+// Long tiles from this many columns per request on.
+constexpr uint64_t kLongMinCols = 256;
 
 // Workgroups per (tile, kv-head) of a row-tile command of `grid` unsplit ones, whose walks
 // hold about `tokens` tokens: as many as fill two workgroups per CU and leave every wave two
@@ -624,6 +1008,13 @@ int row_splits(uint64_t grid, uint64_t tokens, int cus) {
   const uint64_t steps = (tokens + 31) / 32;
   const uint64_t most = std::min<uint64_t>(kMaxSplits, 2 * (uint64_t)cus / std::max<uint64_t>(grid, 1));
   return (int)std::max<uint64_t>(1, std::min(most, steps / (2 * kRowWaves)));
+}
+
+template <Kv KV>
+auto kernel_of(const loom_window_attention_plan &p) {
+  if (p.info.algorithm != LOOM_PAGED_PREFILL_LONG_TILE) return window_rows_kernel<KV>;
+  if (p.info.tile_cols == 128) return p.groups == 2 ? window_long_kernel<KV, 8, 4> : window_long_kernel<KV, 4, 4>;
+  return p.groups == 4 ? window_long_kernel<KV, 8, 2> : window_long_kernel<KV, 4, 2>;
 }
 
 loom_status_t make_plan(const loom::DeviceInfo &dev, const loom_window_attention_spec_t *spec,
@@ -641,20 +1032,30 @@ loom_status_t make_plan(const loom::DeviceInfo &dev, const loom_window_attention
   if (hkv > kMaxHeads) return fail(err, LOOM_PLAN_STATE_COUNT_OUT_OF_RANGE, "window heads", hkv);
   if (s.rows > (uint64_t)INT32_MAX / hq || batch >= (uint64_t)INT32_MAX)
     return fail(err, LOOM_PLAN_STATE_COUNT_OUT_OF_RANGE, "window rows", s.rows);
-  const uint64_t cols = s.rows * group, tc = 16;
-  const uint64_t tiles = s.explicit_rows ? std::min(cols, (cols + (tc - 1) * batch) / tc)
-                                         : batch * ((group + tc - 1) / tc);
-  if (tiles * hkv * (kRowWaves * 64) >= (1ull << 32))
+  const uint64_t cols = s.rows * group, cus = (uint64_t)dev.cus;
+  auto tiles_of = [&](uint64_t tc) {
+    return s.explicit_rows ? std::min(cols, (cols + (tc - 1) * batch) / tc)
+                           : batch * ((group + tc - 1) / tc);
+  };
+  const bool long_tile =
+      flags & LOOM_PLAN_PREFILL_TILE_LONG ||
+      (!(flags & LOOM_PLAN_PREFILL_TILE_16) && s.explicit_rows && cols >= kLongMinCols * batch);
+  const uint64_t tc = !long_tile ? 16 : (cols / 128) * hkv >= 2 * cus ? 128 : 64;
+  const uint64_t tiles = tiles_of(tc), grid = tiles * hkv;
+  const uint32_t groups = !long_tile ? 1 : tc == 128 ? (grid <= 2 * cus ? 2 : 1) : grid <= cus ? 4 : 2;
+  const uint32_t waves = !long_tile ? kRowWaves : (uint32_t)tc / 32 * groups;
+  if (grid * (waves * 64) >= (1ull << 32))
     return fail(err, LOOM_PLAN_STATE_COUNT_OUT_OF_RANGE, "window rows", s.rows);
   auto *p = new loom_window_attention_plan;
   p->info.spec = s;
-  p->info.algorithm = flags & LOOM_PLAN_PREFILL_TILE_LONG ? LOOM_PAGED_PREFILL_LONG_TILE : LOOM_PAGED_PREFILL_ROW_TILE;
+  p->info.algorithm = long_tile ? LOOM_PAGED_PREFILL_LONG_TILE : LOOM_PAGED_PREFILL_ROW_TILE;
   p->info.tile_cols = (uint32_t)tc;
   p->info.row_tiles = tiles;
-  p->info.grid_blocks = tiles * hkv;
-  p->info.block_threads = kRowWaves * 64;
+  p->info.grid_blocks = grid;
+  p->info.block_threads = waves * 64;
   p->info.flags = flags;
   p->cus = dev.cus;
+  p->groups = groups;
   *out = p;
   return loom::ok(err);
 }
@@ -790,7 +1191,8 @@ loom_status_t loom_window_attention_enqueue(const loom_window_attention_plan_t *
       std::min<uint64_t>((uint64_t)a.window + (uint64_t)a.sinks + s.rows / pg.batch_size,
                          (uint64_t)a.n_indices * page_rows / pg.batch_size);
   const uint64_t grid = plan->info.grid_blocks;
-  a.splits = row_splits(grid, tokens, plan->cus);
+  const bool long_tile = plan->info.algorithm == LOOM_PAGED_PREFILL_LONG_TILE;
+  a.splits = long_tile ? 1 : row_splits(grid, tokens, plan->cus);
   if (a.splits > 1) {
     a.arrived = scope->queue->joins;
     a.states = (float *)loom::queue_shares(scope, (uint64_t)a.splits * grid * 16 * kStash * 4);
@@ -798,12 +1200,10 @@ loom_status_t loom_window_attention_enqueue(const loom_window_attention_plan_t *
   }
   const dim3 blocks((unsigned)(grid * a.splits)), threads(plan->info.block_threads);
   hipStream_t stream = scope->queue->stream;
-  if (mx)
-    hipLaunchKernelGGL(window_rows_kernel<kMx4>, blocks, threads, 0, stream, a);
-  else if (fp8)
-    hipLaunchKernelGGL(window_rows_kernel<kFp8>, blocks, threads, 0, stream, a);
-  else
-    hipLaunchKernelGGL(window_rows_kernel<kBf16>, blocks, threads, 0, stream, a);
+  const auto kernel = mx    ? kernel_of<kMx4>(*plan)
+                      : fp8 ? kernel_of<kFp8>(*plan)
+                            : kernel_of<kBf16>(*plan);
+  hipLaunchKernelGGL(kernel, blocks, threads, 0, stream, a);
   return loom::record_launch(scope, hipGetLastError(), err);
 }
 
