@@ -200,16 +200,28 @@ __device__ __forceinline__ void exact_column(const WindowArgs &a, const Tile &t,
 // BF16 and FP8 rows go straight to LDS; MXFP4 codes are loaded into registers, one block of
 // 32 values and its scale per lane, and written to LDS as BF16, which serves K and V alike.
 constexpr int kRowWaves = 4;
+constexpr int kAhead = 2;    // MXFP4: steps in flight
 constexpr int kStash = 132;  // floats between two columns' O in LDS, and of a split's state
 
 template <Kv KV>
 using RowPipe = PipeWave<4, KV == kFp8, true, 1>;
+// 16-row blocks of a step.
 template <Kv KV>
-constexpr int kRowSlots = KV == kMx4 ? 1 : 2;
+constexpr int kStepBlocks = KV == kFp8 ? 2 : 1;
+// A step's rows in LDS: PipeWave's slot (FP8), or the first half of its K and of its V.
+template <Kv KV>
+struct RowSlot {
+  using Pipe = RowPipe<KV>;
+  static constexpr int kGroups = KV == kFp8 ? Pipe::kGroups : Pipe::kGroups / 2;  // of each of K and V
+  static constexpr int kVShift = KV == kFp8 ? 0 : -kGroups * Pipe::kKGroup;  // of V, against PipeWave's
+  static constexpr int kBytes = KV == kFp8 ? Pipe::kSlotBytes : kGroups * (Pipe::kKGroup + Pipe::kVGroup);
+  static constexpr int kSlots = KV == kMx4 ? 1 : 2;
+  static constexpr int kWaveBytes = (std::max(kSlots * kBytes, 16 * kStash * 4) + 15) & ~15;
+};
 
 template <Kv KV>
 struct RowsSmem {
-  __align__(16) uint8_t slots[kRowWaves][kRowSlots<KV> * RowPipe<KV>::kSlotBytes];
+  __align__(16) uint8_t slots[kRowWaves][RowSlot<KV>::kWaveBytes];
   LocateSmem<kRowWaves> loc;
   float m[kRowWaves][16], l[kRowWaves][16];
   uint32_t bad[kRowWaves];
@@ -234,18 +246,16 @@ __device__ __forceinline__ f32x2 load_state(const float *p) {
                                                      __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
 }
 
-// MXFP4 rows of a step in registers: lane l holds 32 values, codes (l & 3) of row l >> 2 of
-// each half, and their scale byte.
+// MXFP4 rows of a step in registers: lane l holds 32 values, block l & 3 of row l >> 2, and
+// their scale byte.
 struct MxStage {
-  u32x4 k[2], v[2];
-  uint32_t ks[2], vs[2];
+  u32x4 k, v;
+  uint32_t ks, vs;
 };
-// Codes of row r, block b of 32 values, to a slot as BF16.
+// Block b of 32 values of row r to a slot as BF16; `group`: where the row's group lies.
 template <class Pipe>
-__device__ __forceinline__ void put_mx(uint8_t *slot, bool is_v, int r, int b, const u32x4 &w,
-                                       uint32_t scale) {
-  uint8_t *dst = slot + (is_v ? Pipe::v_group(r >> 2) : (r >> 2) * Pipe::kKGroup) + (r & 3) * 256 +
-                 ((4 * b) ^ Pipe::swizzle(r)) * 16;
+__device__ __forceinline__ void put_mx(uint8_t *group, int r, int b, const u32x4 &w, uint32_t scale) {
+  uint8_t *dst = group + (r & 3) * 256 + ((4 * b) ^ Pipe::swizzle(r)) * 16;
 #pragma unroll
   for (int u = 0; u < 4; ++u)
     *reinterpret_cast<u32x4 *>(dst + 16 * u) = mx4x8_to_bf16x8(w[u], scale << 23);
@@ -256,8 +266,8 @@ __global__ __launch_bounds__(kRowWaves * 64) void window_rows_kernel(WindowArgs 
   constexpr int W = kRowWaves, TC = 16;
   constexpr bool FP8 = KV == kFp8;
   using Pipe = RowPipe<KV>;
-  constexpr int kSlot = Pipe::kSlotBytes;
-  static_assert(TC * kStash * 4 <= kRowSlots<KV> * kSlot, "a wave's columns in its slots");
+  using Slot = RowSlot<KV>;
+  constexpr int H = kStepBlocks<KV>, kPlaced = 64 / H;  // steps placed at once
   __shared__ RowsSmem<KV> sm;
   WindowArgs a = args;
   float v_scale = 1.0f;
@@ -289,7 +299,7 @@ __global__ __launch_bounds__(kRowWaves * 64) void window_rows_kernel(WindowArgs 
     for (int c = 0; c < 4; ++c) pw.qf[0][c] = valid ? load16(qp + Pipe::q_dim(c, quad)) : u32x4{0, 0, 0, 0};
   }
   // this split's steps [lo, hi), this wave's lo + wave + W i
-  const int steps = (t.blocks + 1) >> 1;
+  const int steps = (t.blocks + H - 1) / H;
   int lo = 0, hi = steps;
   if (a.splits > 1) {
     lo = (int)((int64_t)steps * split / a.splits);
@@ -297,12 +307,12 @@ __global__ __launch_bounds__(kRowWaves * 64) void window_rows_kernel(WindowArgs 
   }
   const int n = hi - lo > wave ? (hi - lo - wave + W - 1) / W : 0;
 
-  // Where the wave's half steps lie, 64 at a time, one per lane: byte offset of the first
-  // row in K and V (and in the MXFP4 scales), and block << 5 | rows.
+  // Where the blocks of the wave's steps lie, 64 at a time, one per lane: byte offset of the
+  // first row in K and V (and in the MXFP4 scales), and block << 5 | rows.
   uint32_t at_lo = 0, at_hi = 0, sc_lo = 0, sc_hi = 0;
   int meta = 0;
   auto locate = [&](int i0) {
-    const int x = 2 * (lo + wave + W * (i0 + (lane >> 1))) + (lane & 1);
+    const int x = H * (lo + wave + W * (i0 + lane / H)) + lane % H;
     const bool in = x < t.blocks;
     const int b = t.block(x);
     int rows = in ? t.rows(a, x) : 0;
@@ -327,9 +337,9 @@ __global__ __launch_bounds__(kRowWaves * 64) void window_rows_kernel(WindowArgs 
     return __builtin_amdgcn_make_buffer_rsrc(
         const_cast<uint8_t *>(reinterpret_cast<const uint8_t *>(base) + at), 0, bytes, 0x00020000);
   };
-  // BF16 and FP8: the loads of step i (of the located 32) into the slot at LDS address `slot`
-  constexpr int kHalf = Pipe::kGroups / 2;
-  constexpr int kStepLoads = 4 * kHalf;
+  // BF16 and FP8: the loads of step i (of the placed ones) into the slot at LDS address `slot`
+  constexpr int kHalf = Pipe::kGroups / 2;  // groups of a block
+  constexpr int kStepLoads = 2 * H * kHalf;
   int lane_off[kHalf];
   if constexpr (KV != kMx4) {
     const int unit = (lane & (Pipe::kUnits - 1)) ^ Pipe::swizzle(lane / Pipe::kUnits);
@@ -339,8 +349,8 @@ __global__ __launch_bounds__(kRowWaves * 64) void window_rows_kernel(WindowArgs 
   }
   auto issue = [&](int i, uint32_t slot) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int j = 2 * i + h;
+    for (int h = 0; h < H; ++h) {
+      const int j = H * i + h;
       const int rows = __builtin_amdgcn_readlane(meta, j) & 31;
       const uint64_t at = lane64(at_lo, at_hi, j);
       const int bytes = rows > 0 ? (rows - 1) * a.row_bytes + kRowBytes<KV> : 0;
@@ -348,57 +358,63 @@ __global__ __launch_bounds__(kRowWaves * 64) void window_rows_kernel(WindowArgs 
 #pragma unroll
       for (int x = 0; x < kHalf; ++x) {
         lds_load16_at(rk, slot + (uint32_t)((h * kHalf + x) * Pipe::kKGroup), lane_off[x]);
-        lds_load16_at(rv, slot + (uint32_t)(Pipe::v_group(x) + h * (Pipe::v_group(kHalf) - Pipe::v_group(0))),
+        lds_load16_at(rv, slot + (uint32_t)(Slot::kVShift + Pipe::v_group(x) +
+                                            h * (Pipe::v_group(kHalf) - Pipe::v_group(0))),
                       lane_off[x]);
       }
     }
   };
   // MXFP4: the same into registers
   auto fetch = [&](int i, MxStage &g) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int j = 2 * i + h;
-      const int rows = __builtin_amdgcn_readlane(meta, j) & 31;
-      const uint64_t at = lane64(at_lo, at_hi, j), sc = lane64(sc_lo, sc_hi, j);
-      const int bytes = rows > 0 ? (rows - 1) * a.row_bytes + 64 : 0;
-      const int off = (lane >> 2) * a.row_bytes + (lane & 3) * 16;
-      g.k[h] = load16_rows<false>(rsrc(a.k, at, bytes), off);
-      g.v[h] = load16_rows<false>(rsrc(a.v, at, bytes), off);
-      g.ks[h] = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(rsrc(a.k_mx, sc, 4 * rows), lane, 0, 0);
-      g.vs[h] = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(rsrc(a.v_mx, sc, 4 * rows), lane, 0, 0);
-    }
+    const int rows = __builtin_amdgcn_readlane(meta, i) & 31;
+    const uint64_t at = lane64(at_lo, at_hi, i), sc = lane64(sc_lo, sc_hi, i);
+    const int bytes = rows > 0 ? (rows - 1) * a.row_bytes + 64 : 0;
+    const int off = (lane >> 2) * a.row_bytes + (lane & 3) * 16;
+    g.k = load16_rows<false>(rsrc(a.k, at, bytes), off);
+    g.v = load16_rows<false>(rsrc(a.v, at, bytes), off);
+    g.ks = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(rsrc(a.k_mx, sc, 4 * rows), lane, 0, 0);
+    g.vs = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(rsrc(a.v_mx, sc, 4 * rows), lane, 0, 0);
   };
 
   float m_run = -INFINITY, l_run = 0.0f;
   f32x4(&acc)[8] = pw.acc[0];
-  // The softmax and products of step i, whose rows lie at `slot` bytes of the wave's ring.
-  auto process = [&](int i, int slot) {
-    const auto k = pw.read_k(slot);
-    f32x4 s[2] = {};
+  // The softmax and products of step i, whose rows lie at `slot`.
+  auto process = [&](int i, const uint8_t *slot) {
+    f32x4 s[H] = {};  // s[h][j]: token 4 quad + j of block h
+    if constexpr (FP8) {
+      u32x4 k[2][2];
 #pragma unroll
-    for (int x = 0; x < 8; ++x) {
-      const int c = x >> 1, h = x & 1;
-      u32x4 w;
-      if constexpr (FP8)
-        w = fp8x8_to_bf16x8(u32x2{k.f[c >> 1][h][2 * (c & 1)], k.f[c >> 1][h][2 * (c & 1) + 1]});
-      else
-        w = k.f[c][h];
-      s[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(w), as_bf16x8(pw.qf[0][c]), s[h], 0, 0, 0);
+      for (int x = 0; x < 4; ++x)
+        k[x >> 1][x & 1] = *reinterpret_cast<const u32x4 *>(slot + pw.kofs[x >> 1] + (x & 1) * kHalf * Pipe::kKGroup);
+#pragma unroll
+      for (int x = 0; x < 8; ++x) {
+        const u32x4 &w = k[x >> 2][x & 1];
+        const int c = x >> 1;
+        s[x & 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+            as_bf16x8(fp8x8_to_bf16x8(u32x2{w[2 * (c & 1)], w[2 * (c & 1) + 1]})), as_bf16x8(pw.qf[0][c]),
+            s[x & 1], 0, 0, 0);
+      }
+    } else {
+      u32x4 k[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) k[c] = *reinterpret_cast<const u32x4 *>(slot + pw.kofs[c]);
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        s[0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(k[c]), as_bf16x8(pw.qf[0][c]), s[0], 0, 0, 0);
     }
-    // s[h][j]: token 16 block(h) + 4 quad + j
-    const int t0 = (__builtin_amdgcn_readlane(meta, 2 * i) >> 5) * 16;
-    const int t1 = (__builtin_amdgcn_readlane(meta, 2 * i + 1) >> 5) * 16;
-    if (t0 < full_beg || t0 + 16 > full_end || t1 < full_beg || t1 + 16 > full_end) {
+    float ml = -INFINITY;
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+    for (int h = 0; h < H; ++h) {
+      const int t0 = (__builtin_amdgcn_readlane(meta, H * i + h) >> 5) * 16;
+      if (t0 < full_beg || t0 + 16 > full_end) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const int tok = (h ? t1 : t0) + 4 * quad + j;
+          const int tok = t0 + 4 * quad + j;
           s[h][j] = tok < end_col && (tok >= beg_col || tok < a.sinks) ? s[h][j] : -INFINITY;
         }
+      }
+      ml = fmax_nan(ml, fmax_nan(fmax_nan(s[h][0], s[h][1]), fmax_nan(s[h][2], s[h][3])));
     }
-    const float ml = fmax_nan(fmax_nan(fmax_nan(s[0][0], s[0][1]), fmax_nan(s[0][2], s[0][3])),
-                              fmax_nan(fmax_nan(s[1][0], s[1][1]), fmax_nan(s[1][2], s[1][3])));
     if (__builtin_amdgcn_ballot_w64(ml * a.scale_log2 > m_run + 8.0f)) {
       const float mx = quad_max_nan(ml) * a.scale_log2;
       const bool grow = mx > m_run + 8.0f;
@@ -412,9 +428,9 @@ __global__ __launch_bounds__(kRowWaves * 64) void window_rows_kernel(WindowArgs 
       m_run = m_ref;
     }
     const float m_use = m_run == -INFINITY ? 0.0f : m_run;  // nothing visible yet
-    u32x4 ph, pl;
+    uint32_t ph[2 * H], pl[2 * H];
 #pragma unroll
-    for (int y = 0; y < 4; ++y) {
+    for (int y = 0; y < 2 * H; ++y) {
       const float x0 = fast_exp2(fmaf(s[y >> 1][2 * (y & 1)], a.scale_log2, -m_use));
       const float x1 = fast_exp2(fmaf(s[y >> 1][2 * (y & 1) + 1], a.scale_log2, -m_use));
       const uint32_t b0 = __float_as_uint(x0), b1 = __float_as_uint(x1);
@@ -423,36 +439,53 @@ __global__ __launch_bounds__(kRowWaves * 64) void window_rows_kernel(WindowArgs 
                         __float_as_uint(x1 - __uint_as_float(b1 & 0xffff0000u)));
       l_run += x0 + x1;
     }
+    if constexpr (FP8) {
+      bf16x8 w[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const u32x4 b = pw.read_v(slot, e);
-      const bf16x8 w = as_bf16x8(FP8 ? fp8x8_to_bf16x8(u32x2{b[0], b[1]}) : b);
-      acc[e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, as_bf16x8(ph), acc[e], 0, 0, 0);
-      acc[e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w, as_bf16x8(pl), acc[e], 0, 0, 0);
+      for (int e = 0; e < 8; ++e) {
+        const u32x2 b = lds_read_tr8(slot + pw.vofs[e >> 1] + (e & 1) * 16);
+        w[e] = as_bf16x8(fp8x8_to_bf16x8(b));
+        acc[e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[e], as_bf16x8(ph[0], ph[1], ph[2], ph[3]), acc[e], 0, 0, 0);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        acc[e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[e], as_bf16x8(pl[0], pl[1], pl[2], pl[3]), acc[e], 0, 0, 0);
+    } else {
+      // high parts and residuals in the two halves of the contraction
+      const bf16x8 p = as_bf16x8(ph[0], ph[1], pl[0], pl[1]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const u32x2 b = lds_read_tr16(slot + Slot::kVShift + pw.vofs[e >> 1] + (e & 1) * 32);
+        acc[e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(b[0], b[1], b[0], b[1]), p, acc[e], 0, 0, 0);
+      }
     }
   };
 
   const uint32_t ring_at =
       (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)sm.slots[wave];
+  uint8_t *const slots = sm.slots[wave];
   bool bad = false;
-  for (int i0 = 0; i0 == 0 || i0 < n; i0 += 32) {
-    const int c = min(32, n - i0);
+  for (int i0 = 0; i0 == 0 || i0 < n; i0 += kPlaced) {
+    const int c = min(kPlaced, n - i0);
     if (c > 0) locate(i0);
     if constexpr (KV == kMx4) {
-      MxStage st;
-      if (c > 0) fetch(0, st);
-      if (i0 == 0) bad = bad_pages(a, t, tid, W * 64);
-      for (int i = 0; i < c; ++i) {
-        const MxStage cur = st;
-        if (i + 1 < c) fetch(i + 1, st);
-        wave_lds_fence();  // the slot's reads of the step before
+      // registers of kAhead steps in flight
+      MxStage st[kAhead];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          put_mx<Pipe>(sm.slots[wave], false, 16 * h + (lane >> 2), lane & 3, cur.k[h], cur.ks[h]);
-          put_mx<Pipe>(sm.slots[wave], true, 16 * h + (lane >> 2), lane & 3, cur.v[h], cur.vs[h]);
+      for (int u = 0; u < kAhead; ++u)
+        if (c > 0) fetch(min(u, c - 1), st[u]);
+      if (i0 == 0) bad = bad_pages(a, t, tid, W * 64);
+      for (int i = 0; i < c; i += kAhead) {
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+          if (u > 0 && i + u >= c) break;
+          wave_lds_fence();  // the slot's reads of the step before
+          put_mx<Pipe>(slots + (lane >> 4) * Pipe::kKGroup, lane >> 2, lane & 3, st[u].k, st[u].ks);
+          put_mx<Pipe>(slots + Slot::kVShift + Pipe::v_group(lane >> 4), lane >> 2, lane & 3, st[u].v, st[u].vs);
+          fetch(min(i + u + kAhead, c - 1), st[u]);
+          wave_lds_fence();
+          process(i + u, slots);
         }
-        wave_lds_fence();
-        process(i, 0);
       }
     } else {
       // (queries and index words have arrived: no wait of the compiler's in the walk)
@@ -461,19 +494,21 @@ __global__ __launch_bounds__(kRowWaves * 64) void window_rows_kernel(WindowArgs 
       asm volatile("" : "+v"(at_lo), "+v"(at_hi), "+v"(meta));
       wait_reads();
       if (c > 0) issue(0, ring_at);
+      if (c > 1) issue(1, ring_at + (uint32_t)Slot::kBytes);
       if (i0 == 0) {
         bad = bad_pages(a, t, tid, W * 64);
         asm volatile("" ::"s"(__builtin_amdgcn_ballot_w64(bad)));
       }
       for (int i = 0; i < c; ++i) {
-        if (i + 1 < c) {
-          wait_reads();
-          issue(i + 1, ring_at + (uint32_t)(((i + 1) & 1) * kSlot));
+        if (i + 1 < c)
           wait_loads<kStepLoads>();
-        } else {
+        else
           wait_loads<0>();
+        process(i, slots + (i & 1) * Slot::kBytes);
+        if (i + 2 < c) {
+          wait_reads();
+          issue(i + 2, ring_at + (uint32_t)((i & 1) * Slot::kBytes));
         }
-        process(i, (i & 1) * kSlot);
       }
     }
   }
@@ -849,11 +884,14 @@ __global__ __launch_bounds__(W * 64, 2) void window_long_kernel(WindowArgs args)
       }
     };
     uint8_t *const group_ring = ring + grp * kSlots * kSlot;
+    const int half_at = loads_k ? 4 * Pipe::kKGroup : Pipe::v_group(4) - Pipe::v_group(0);
+    const int put_at = (loads_k ? (lane >> 4) * Pipe::kKGroup : Pipe::v_group(lane >> 4)) +
+                       (NW == 4 ? (wq & 1) * half_at : 0);
     auto put = [&](int slot, const Share &g) {
 #pragma unroll
       for (int y = 0; y < kHalves; ++y)
-        put_mx<Pipe>(group_ring + slot, !loads_k, 16 * (NW == 4 ? (wq & 1) : y) + (lane >> 2), lane & 3,
-                     g.w[y], g.s[y]);
+        put_mx<Pipe>(group_ring + slot + put_at + (NW == 4 ? 0 : y * half_at), lane >> 2, lane & 3, g.w[y],
+                     g.s[y]);
     };
     // K (j + 2) and V (j + 1) are written at step j, to slots read at step j - 1.
     const int ahead = uni(loads_k ? 2 : 1);
