@@ -199,7 +199,7 @@ __device__ __forceinline__ void exact_column(const WindowArgs &a, const Tile &t,
 // residual (16 bits: few tokens carry a short window, whose errors do not average out).
 // BF16 and FP8 rows go straight to LDS; MXFP4 codes are loaded into registers, one block of
 // 32 values and its scale per lane, and written to LDS as BF16, which serves K and V alike.
-constexpr int kRowWaves = 4;
+constexpr int kRowWaves = 8;
 constexpr int kAhead = 2;    // MXFP4: steps in flight
 constexpr int kStash = 132;  // floats between two columns' O in LDS, and of a split's state
 
@@ -247,18 +247,18 @@ __device__ __forceinline__ f32x2 load_state(const float *p) {
 }
 
 // MXFP4 rows of a step in registers: lane l holds 32 values, block l & 3 of row l >> 2, and
-// their scale byte.
+// the row's scale word.
 struct MxStage {
   u32x4 k, v;
   uint32_t ks, vs;
 };
 // Block b of 32 values of row r to a slot as BF16; `group`: where the row's group lies.
 template <class Pipe>
-__device__ __forceinline__ void put_mx(uint8_t *group, int r, int b, const u32x4 &w, uint32_t scale) {
+__device__ __forceinline__ void put_mx(uint8_t *group, int r, int b, const u32x4 &w, uint32_t scales) {
   uint8_t *dst = group + (r & 3) * 256 + ((4 * b) ^ Pipe::swizzle(r)) * 16;
+  const uint32_t scale = mx_scale(scales, b);
 #pragma unroll
-  for (int u = 0; u < 4; ++u)
-    *reinterpret_cast<u32x4 *>(dst + 16 * u) = mx4x8_to_bf16x8(w[u], scale << 23);
+  for (int u = 0; u < 4; ++u) *reinterpret_cast<u32x4 *>(dst + 16 * u) = mx4x8_to_bf16x8(w[u], scale);
 }
 
 template <Kv KV>
@@ -372,8 +372,8 @@ __global__ __launch_bounds__(kRowWaves * 64) void window_rows_kernel(WindowArgs 
     const int off = (lane >> 2) * a.row_bytes + (lane & 3) * 16;
     g.k = load16_rows<false>(rsrc(a.k, at, bytes), off);
     g.v = load16_rows<false>(rsrc(a.v, at, bytes), off);
-    g.ks = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(rsrc(a.k_mx, sc, 4 * rows), lane, 0, 0);
-    g.vs = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(rsrc(a.v_mx, sc, 4 * rows), lane, 0, 0);
+    g.ks = __builtin_amdgcn_raw_buffer_load_b32(rsrc(a.k_mx, sc, 4 * rows), lane & ~3, 0, 0);
+    g.vs = __builtin_amdgcn_raw_buffer_load_b32(rsrc(a.v_mx, sc, 4 * rows), lane & ~3, 0, 0);
   };
 
   float m_run = -INFINITY, l_run = 0.0f;
@@ -381,11 +381,14 @@ __global__ __launch_bounds__(kRowWaves * 64) void window_rows_kernel(WindowArgs 
   // The softmax and products of step i, whose rows lie at `slot`.
   auto process = [&](int i, const uint8_t *slot) {
     f32x4 s[H] = {};  // s[h][j]: token 4 quad + j of block h
+    u32x2 v[8];
     if constexpr (FP8) {
       u32x4 k[2][2];
 #pragma unroll
       for (int x = 0; x < 4; ++x)
         k[x >> 1][x & 1] = *reinterpret_cast<const u32x4 *>(slot + pw.kofs[x >> 1] + (x & 1) * kHalf * Pipe::kKGroup);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = lds_read_tr8(slot + pw.vofs[e >> 1] + (e & 1) * 16);
 #pragma unroll
       for (int x = 0; x < 8; ++x) {
         const u32x4 &w = k[x >> 2][x & 1];
@@ -398,6 +401,8 @@ __global__ __launch_bounds__(kRowWaves * 64) void window_rows_kernel(WindowArgs 
       u32x4 k[4];
 #pragma unroll
       for (int c = 0; c < 4; ++c) k[c] = *reinterpret_cast<const u32x4 *>(slot + pw.kofs[c]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = lds_read_tr16(slot + Slot::kVShift + pw.vofs[e >> 1] + (e & 1) * 32);
 #pragma unroll
       for (int c = 0; c < 4; ++c)
         s[0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(k[c]), as_bf16x8(pw.qf[0][c]), s[0], 0, 0, 0);
@@ -443,8 +448,7 @@ __global__ __launch_bounds__(kRowWaves * 64) void window_rows_kernel(WindowArgs 
       bf16x8 w[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const u32x2 b = lds_read_tr8(slot + pw.vofs[e >> 1] + (e & 1) * 16);
-        w[e] = as_bf16x8(fp8x8_to_bf16x8(b));
+        w[e] = as_bf16x8(fp8x8_to_bf16x8(v[e]));
         acc[e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[e], as_bf16x8(ph[0], ph[1], ph[2], ph[3]), acc[e], 0, 0, 0);
       }
 #pragma unroll
@@ -455,8 +459,8 @@ __global__ __launch_bounds__(kRowWaves * 64) void window_rows_kernel(WindowArgs 
       const bf16x8 p = as_bf16x8(ph[0], ph[1], pl[0], pl[1]);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const u32x2 b = lds_read_tr16(slot + Slot::kVShift + pw.vofs[e >> 1] + (e & 1) * 32);
-        acc[e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(b[0], b[1], b[0], b[1]), p, acc[e], 0, 0, 0);
+        acc[e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(v[e][0], v[e][1], v[e][0], v[e][1]), p,
+                                                         acc[e], 0, 0, 0);
       }
     }
   };
@@ -879,8 +883,8 @@ __global__ __launch_bounds__(W * 64, 2) void window_long_kernel(WindowArgs args)
         g.w[y] = load16_rows<false>(
             rsrc(lane64(blk_lo, blk_hi, l), rows > 0 ? (rows - 1) * a.row_bytes + 64 : 0),
             (lane >> 2) * a.row_bytes + (lane & 3) * 16);
-        g.s[y] = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(rsrc(lane64(mx_lo, mx_hi, l), 4 * rows),
-                                                              lane, 0, 0);
+        g.s[y] = __builtin_amdgcn_raw_buffer_load_b32(rsrc(lane64(mx_lo, mx_hi, l), 4 * rows), lane & ~3,
+                                                      0, 0);
       }
     };
     uint8_t *const group_ring = ring + grp * kSlots * kSlot;
@@ -1040,12 +1044,14 @@ constexpr int kMaxSplits = 16;
 constexpr uint64_t kLongMinCols = 256;
 
 // Workgroups per (tile, kv-head) of a row-tile command of `grid` unsplit ones, whose walks
-// hold about `tokens` tokens: as many as fill two workgroups per CU and leave every wave two
-// steps.
-int row_splits(uint64_t grid, uint64_t tokens, int cus) {
-  const uint64_t steps = (tokens + 31) / 32;
-  const uint64_t most = std::min<uint64_t>(kMaxSplits, 2 * (uint64_t)cus / std::max<uint64_t>(grid, 1));
-  return (int)std::max<uint64_t>(1, std::min(most, steps / (2 * kRowWaves)));
+// hold about `tokens` tokens: at most one per CU, and each with work for its join (2 us):
+// the more CUs stream already, the less another one adds.
+int row_splits(uint64_t grid, uint64_t tokens, int cus, bool mx) {
+  const uint64_t blocks = (tokens + 15) / 16;
+  const uint64_t most = std::min<uint64_t>(kMaxSplits, (uint64_t)cus / std::max<uint64_t>(grid, 1));
+  // 16-row blocks per wave
+  const uint64_t least = std::max<uint64_t>(1, grid * (mx ? 8 : 16) / (uint64_t)cus);
+  return (int)std::max<uint64_t>(1, std::min(most, blocks / (least * kRowWaves)));
 }
 
 template <Kv KV>
@@ -1230,7 +1236,7 @@ loom_status_t loom_window_attention_enqueue(const loom_window_attention_plan_t *
                          (uint64_t)a.n_indices * page_rows / pg.batch_size);
   const uint64_t grid = plan->info.grid_blocks;
   const bool long_tile = plan->info.algorithm == LOOM_PAGED_PREFILL_LONG_TILE;
-  a.splits = long_tile ? 1 : row_splits(grid, tokens, plan->cus);
+  a.splits = long_tile ? 1 : row_splits(grid, tokens, plan->cus, mx);
   if (a.splits > 1) {
     a.arrived = scope->queue->joins;
     a.states = (float *)loom::queue_shares(scope, (uint64_t)a.splits * grid * 16 * kStash * 4);
