@@ -57,12 +57,69 @@ struct Tile {
   }
 };
 
+// The tile of this workgroup among those of up to 64 requests, the request of the longest
+// walks first and a request's last rows first: the launch does not end with a few long
+// walks alone (four chunks of 512 rows behind 2048-16384 tokens, the longest listed first
+// and so dispatched last: 481 us without the order).  Every wave holds the table, a request
+// per lane.  Rows belong to the requests before the first falling qo_indptr range.
+template <int TC>
+__device__ __forceinline__ bool locate_longest_first(const WindowArgs &a, TileLoc &l, int split) {
+  const int lane = threadIdx.x & 63;
+  const bool in = lane < a.batch;
+  int32_t s0 = 0, s1 = 0, p0 = 0, p1 = 0, t1 = 0;
+  if (in) {
+    s0 = a.qo[lane];
+    s1 = a.qo[lane + 1];
+    p0 = a.indptr[lane];
+    p1 = a.indptr[lane + 1];
+    t1 = a.last[lane];
+  }
+  l.kvh = (int)(blockIdx.x % (uint32_t)a.hkv);
+  l.rank = (int)(blockIdx.x / (uint32_t)a.hkv) - split * a.row_tiles;
+  const uint64_t falls = __builtin_amdgcn_ballot_w64(in && !(s0 >= 0 && s1 >= s0 && s1 <= a.nnz));
+  const int valid = falls ? __builtin_ctzll(falls) : a.batch;
+  // (columns fit 31 bits: the plan checks it)
+  const uint32_t cnt = lane < valid ? ((uint32_t)(s1 - s0) * (uint32_t)a.group + TC - 1) / TC : 0u;
+  // place among the requests, by tokens that the last row sees (pages, beyond the window)
+  const int64_t key = in ? min((int64_t)p1 - p0, (int64_t)(a.window / a.page_rows) + 1) : -1;
+  const int k32 = (int)max<int64_t>(-1, key);
+  int place = 0;
+  for (int r = 0; r < a.batch; ++r) {
+    const int other = __builtin_amdgcn_readlane(k32, r);
+    place += other > k32 || (other == k32 && r < lane) ? 1 : 0;
+  }
+  // counts in that order, one per lane (lanes past the batch: places past it)
+  const uint32_t ordered = (uint32_t)__builtin_amdgcn_ds_permute((in ? place : lane) * 4, (int)cnt);
+  const uint32_t incl = wave_incl_add_sat_u32(ordered);
+  const uint32_t before = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)incl, 0x138, 0xf, 0xf, false);
+  const uint64_t who = __builtin_amdgcn_ballot_w64((uint32_t)l.rank >= before && (uint32_t)l.rank < incl);
+  if (__builtin_amdgcn_readlane(s0, 0) != 0 || __builtin_amdgcn_readlane(s1, a.batch - 1) != a.nnz ||
+      __builtin_amdgcn_readlane(p0, 0) != 0)
+    return false;
+  l.ipB = __builtin_amdgcn_readlane(p1, a.batch - 1);
+  if (l.ipB < 0 || (a.indices_capacity ? (int64_t)l.ipB > a.n_indices : (int64_t)l.ipB != a.n_indices))
+    return false;
+  if (!who) return false;
+  const int at = __builtin_ctzll(who);
+  const int r = __builtin_ctzll(__builtin_amdgcn_ballot_w64(in && place == at));
+  l.tile0 = (int)(__builtin_amdgcn_readlane((int)incl, at) - 1u - (uint32_t)l.rank);
+  l.qs = __builtin_amdgcn_readlane(s0, r);
+  l.qe = __builtin_amdgcn_readlane(s1, r);
+  l.ps = __builtin_amdgcn_readlane(p0, r);
+  l.pe = __builtin_amdgcn_readlane(p1, r);
+  l.tl = __builtin_amdgcn_readlane(t1, r);
+  l.fbeg = 0;
+  return true;
+}
+
 // Finds the workgroup's tile of TC columns; false: none, or a failed guard.
 template <int W, int TC>
 __device__ __forceinline__ bool find_tile(const WindowArgs &a, LocateSmem<W> &sm, Tile &t, int split) {
   TileLoc &l = t.loc;
   if (a.qo) {
-    if (!locate_tile<W, false, TC, true, true>(a, sm, l, split)) return false;
+    if (a.batch <= 64 ? !locate_longest_first<TC>(a, l, split)
+                      : !locate_tile<W, false, TC, false, true>(a, sm, l, split))
+      return false;
   } else {
     l.kvh = (int)(blockIdx.x % (uint32_t)a.hkv);
     l.rank = (int)(blockIdx.x / (uint32_t)a.hkv) - split * a.row_tiles;
