@@ -116,14 +116,15 @@ struct LocateSmem {
 // the way (16 requests of 256 BF16 rows, GQA4 32/8: 35.0 -> 34.3 us; 1 x 1024
 // 22.3 -> 21.5, 1 x 512 13.8 -> 12.9; a batch of two on row tiles 14.2 -> 13.5).
 //
-// EMPTY (paged): a request may have no rows (equal qo_indptr entries).
+// EMPTY (paged): a request may have no rows (equal qo_indptr entries).  `block`: the
+// workgroup's place, where it is not its number.
 template <int W, bool RAGGED, int TC, bool INTERLEAVE, bool EMPTY = false>
 __device__ __forceinline__ bool locate_tile(const PrefillArgs &a, LocateSmem<W> &sm, TileLoc &t,
-                                            int split = 0) {
+                                            int split = 0, uint32_t block = blockIdx.x) {
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  t.kvh = (int)(blockIdx.x % a.hkv);
-  const int64_t n_tiles = a.row_tiles, m = (int64_t)(blockIdx.x / a.hkv) - split * n_tiles;
+  t.kvh = (int)(block % a.hkv);
+  const int64_t n_tiles = a.row_tiles, m = (int64_t)(block / a.hkv) - split * n_tiles;
   t.rank = (int)m;
   int64_t rank = m;
   if (a.tile_layer > 0) {

@@ -35,8 +35,20 @@ struct WindowArgs : PrefillArgs {
   int32_t head_bytes;   // from one kv-head's rows of a page to the next
   int32_t row_bytes;    // from one token's row to the next
   int32_t head_tiles;   // one-row form: tiles per request
+  uint32_t group_inv;   // 2^32 / group, rounded up, where that divides every column; 0: it does not
   uint32_t *arrived;    // splits: arrival words, loom::kMx4JoinBytes apart
+  // Row tiles over MXFP4 pages with an even number of kv-heads: the workgroups of the command,
+  // and its blocks are dealt so that two neighbouring heads, whose rows or scales share
+  // cache lines, run on one XCD; 0: in order.
+  int32_t pair_heads;
 };
+
+// Row of column f: f / group.  (A division takes about 35 instructions, and a tile has
+// nine of them.)
+__device__ __forceinline__ int row_of(const WindowArgs &a, int f) {
+  if (a.group == 1) return f;
+  return a.group_inv ? (int)__umulhi((uint32_t)f, a.group_inv) : (int)((uint32_t)f / (uint32_t)a.group);
+}
 
 // A tile's place and what its columns see (wave-uniform).
 struct Tile {
@@ -63,7 +75,8 @@ struct Tile {
 // and so dispatched last: 481 us without the order).  Every wave holds the table, a request
 // per lane.  Rows belong to the requests before the first falling qo_indptr range.
 template <int TC>
-__device__ __forceinline__ bool locate_longest_first(const WindowArgs &a, TileLoc &l, int split) {
+__device__ __forceinline__ bool locate_longest_first(const WindowArgs &a, TileLoc &l, int split,
+                                                     uint32_t block) {
   const int lane = threadIdx.x & 63;
   const bool in = lane < a.batch;
   int32_t s0 = 0, s1 = 0, p0 = 0, p1 = 0, t1 = 0;
@@ -74,8 +87,8 @@ __device__ __forceinline__ bool locate_longest_first(const WindowArgs &a, TileLo
     p1 = a.indptr[lane + 1];
     t1 = a.last[lane];
   }
-  l.kvh = (int)(blockIdx.x % (uint32_t)a.hkv);
-  l.rank = (int)(blockIdx.x / (uint32_t)a.hkv) - split * a.row_tiles;
+  l.kvh = (int)(block % (uint32_t)a.hkv);
+  l.rank = (int)(block / (uint32_t)a.hkv) - split * a.row_tiles;
   const uint64_t falls = __builtin_amdgcn_ballot_w64(in && !(s0 >= 0 && s1 >= s0 && s1 <= a.nnz));
   const int valid = falls ? __builtin_ctzll(falls) : a.batch;
   // (columns fit 31 bits: the plan checks it)
@@ -114,15 +127,16 @@ __device__ __forceinline__ bool locate_longest_first(const WindowArgs &a, TileLo
 
 // Finds the workgroup's tile of TC columns; false: none, or a failed guard.
 template <int W, int TC>
-__device__ __forceinline__ bool find_tile(const WindowArgs &a, LocateSmem<W> &sm, Tile &t, int split) {
+__device__ __forceinline__ bool find_tile(const WindowArgs &a, LocateSmem<W> &sm, Tile &t, int split,
+                                          uint32_t block) {
   TileLoc &l = t.loc;
   if (a.qo) {
-    if (a.batch <= 64 ? !locate_longest_first<TC>(a, l, split)
-                      : !locate_tile<W, false, TC, false, true>(a, sm, l, split))
+    if (a.batch <= 64 ? !locate_longest_first<TC>(a, l, split, block)
+                      : !locate_tile<W, false, TC, false, true>(a, sm, l, split, block))
       return false;
   } else {
-    l.kvh = (int)(blockIdx.x % (uint32_t)a.hkv);
-    l.rank = (int)(blockIdx.x / (uint32_t)a.hkv) - split * a.row_tiles;
+    l.kvh = (int)(block % (uint32_t)a.hkv);
+    l.rank = (int)(block / (uint32_t)a.hkv) - split * a.row_tiles;
     const int r = (int)((uint32_t)l.rank / (uint32_t)a.head_tiles);
     l.tile0 = l.rank - r * a.head_tiles;
     l.qs = r;
@@ -145,8 +159,8 @@ __device__ __forceinline__ bool find_tile(const WindowArgs &a, LocateSmem<W> &sm
   t.fcols = t.group_rows * a.group;
   t.col0 = l.tile0 * TC;
   const int p0 = t.kv_len - t.group_rows;
-  t.p_lo = p0 + (int)((uint32_t)t.col0 / (uint32_t)a.group);
-  t.p_hi = p0 + (int)((uint32_t)min(t.col0 + TC - 1, t.fcols - 1) / (uint32_t)a.group);
+  t.p_lo = p0 + row_of(a, t.col0);
+  t.p_hi = p0 + row_of(a, min(t.col0 + TC - 1, t.fcols - 1));
   t.first_block = max(0, t.p_lo + 1 - a.window) >> 4;
   t.sink_blocks = min((int)(((uint32_t)a.sinks + 15) >> 4), t.first_block);
   t.blocks = t.sink_blocks + (t.p_hi >> 4) + 1 - t.first_block;
@@ -187,7 +201,7 @@ __device__ __forceinline__ uint64_t scale_at(const WindowArgs &a, int page, int 
 template <Kv KV>
 __device__ __forceinline__ void exact_column(const WindowArgs &a, const Tile &t, int f, int lane,
                                              float v_scale) {
-  const int qi = (int)((uint32_t)f / (uint32_t)a.group);
+  const int qi = row_of(a, f);
   const int64_t row = (int64_t)(t.loc.qs + qi) * a.hq + (int64_t)t.loc.kvh * a.group + (f - qi * a.group);
   const int end = t.kv_len - t.group_rows + qi + 1, beg = max(0, end - a.window);
   const int sinks = min(a.sinks, beg), n = sinks + end - beg;
@@ -347,14 +361,19 @@ __global__ __launch_bounds__(kRowWaves * 64) void window_rows_kernel(WindowArgs 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = uni(tid >> 6);
   const int col = lane & 15, quad = lane >> 4;
-  const int split = a.splits > 1 ? (int)(blockIdx.x / (uint32_t)(a.row_tiles * a.hkv)) : 0;
+  uint32_t block = blockIdx.x;
+  if (KV == kMx4 && a.pair_heads) {
+    block = ((block >> 4) << 4) + 2 * (block & 7) + ((block >> 3) & 1);
+    if (block >= (uint32_t)a.pair_heads) return;
+  }
+  const int split = a.splits > 1 ? (int)(block / (uint32_t)(a.row_tiles * a.hkv)) : 0;
   Tile t;
-  if (!find_tile<W, TC>(a, sm.loc, t, split)) return;
+  if (!find_tile<W, TC>(a, sm.loc, t, split, block)) return;
   const int kvh = t.loc.kvh;
   // this lane's column
   const int f = t.col0 + col;
   const bool valid = f < t.fcols;
-  const int qi = valid ? (int)((uint32_t)f / (uint32_t)a.group) : 0;
+  const int qi = valid ? row_of(a, f) : 0;
   const int end_col = valid ? t.kv_len - t.group_rows + qi + 1 : 0;
   const int beg_col = max(0, end_col - a.window);
   // tokens [full_beg, full_end) are seen by every column
@@ -702,7 +721,7 @@ __global__ __launch_bounds__(kRowWaves * 64) void window_rows_kernel(WindowArgs 
   for (int y = 0; y < kItems; ++y) {
     const int c = (y * W * 64 + tid) >> 5, d = (tid & 31) * 4;
     if (c >= cols || (redo >> c & 1)) continue;
-    const int fc = t.col0 + c, rc = (int)((uint32_t)fc / (uint32_t)a.group);
+    const int fc = t.col0 + c, rc = row_of(a, fc);
     const int64_t row = (int64_t)(t.loc.qs + rc) * a.hq + (int64_t)kvh * a.group + (fc - rc * a.group);
     *reinterpret_cast<u32x2 *>(a.out + row * 128 + d) =
         u32x2{bf16x2_pack(o[y][0], o[y][1]), bf16x2_pack(o[y][2], o[y][3])};
@@ -757,9 +776,8 @@ __global__ __launch_bounds__(W * 64, 2) void window_long_kernel(WindowArgs args)
   const int wave = uni(tid >> 6);
   const int col = lane & 15, quad = lane >> 4;
   Tile t;
-  if (!find_tile<W, TC>(a, sm.loc, t, 0)) return;
+  if (!find_tile<W, TC>(a, sm.loc, t, 0, blockIdx.x)) return;
   const int kvh = t.loc.kvh;
-  auto row_of = [&](int f) { return (int)((uint32_t)f / (uint32_t)a.group); };
   const int wq = wave % NW, grp = wave / NW;  // the wave's columns and its group
   const int own0 = t.col0 + 32 * wq;
   const int p0 = t.kv_len - t.group_rows;
@@ -770,7 +788,7 @@ __global__ __launch_bounds__(W * 64, 2) void window_long_kernel(WindowArgs args)
   for (int c = 0; c < 2; ++c) {
     const int f = own0 + 16 * c + col;
     colv_t[c] = f < t.fcols;
-    qi_t[c] = colv_t[c] ? row_of(f) : 0;
+    qi_t[c] = colv_t[c] ? row_of(a, f) : 0;
     gh_t[c] = colv_t[c] ? f - qi_t[c] * a.group : 0;
     end_col[c] = colv_t[c] ? p0 + qi_t[c] + 1 : 0;
     beg_col[c] = max(0, end_col[c] - a.window);
@@ -780,7 +798,7 @@ __global__ __launch_bounds__(W * 64, 2) void window_long_kernel(WindowArgs args)
   // wave sees; and the steps up to the wave's last column's own token.
   int first_full = 0, last_full = 0, own_steps = 0;
   if (own0 < t.fcols) {
-    const int w_lo = p0 + row_of(own0), w_hi = p0 + row_of(min(own0 + 31, t.fcols - 1));
+    const int w_lo = p0 + row_of(a, own0), w_hi = p0 + row_of(a, min(own0 + 31, t.fcols - 1));
     const int x0 = t.sink_blocks - t.first_block;  // place of block b of the window: b + x0
     first_full = (((max(0, w_hi + 1 - a.window) + 15) >> 4) + x0 + 1) >> 1;
     last_full = (((w_lo + 1) >> 4) + x0) >> 1;
@@ -1115,8 +1133,21 @@ namespace {
 constexpr uint64_t kMaxHeads = 4096;  // kv-heads: a row of all of them in a 32-bit stride
 constexpr int kMaxSplits = 16;
 
-// Long tiles from this many columns per request on.
-constexpr uint64_t kLongMinCols = 256;
+// Long tiles where row tiles would fill the chip twice.  Microseconds, row / long tiles: 8
+// x 16 rows behind 5000 tokens 32/8 under windows of 1024 13.4 / 20.0, 8 x 32 (512 row
+// tiles) 23.3 / 20.3, 8 x 64 42.8 / 21.6; over the whole prefix 56 / 82, 94 / 80, 166 / 93;
+// FP8 and MXFP4 pages alike.
+bool takes_long(uint64_t cols, uint64_t hkv, uint64_t cus) { return cols * hkv >= 16 * 2 * cus; }
+
+// Wave groups of the long tiles: as many as `tiles` full ones of 128 columns (or a grid of
+// 64-column ones) leave room for.  Walks over the whole prefix differ, so the longest are
+// cut in two while two workgroups per CU hold all: 4 x 512 rows behind 2048-16384 tokens
+// 370 us in one group, 270 in two (MXFP4 442 / 311), but under windows of 4096, all alike, 142
+// / 160, and 8 x 512 528 / 574.
+uint32_t long_groups(uint64_t tile_cols, uint64_t tiles, uint64_t grid, uint64_t cus, bool whole) {
+  if (tile_cols == 128) return whole && 2 * tiles <= 5 * cus ? 2 : 1;
+  return grid <= cus ? 4 : 2;
+}
 
 // Workgroups per (tile, kv-head) of a row-tile command of `grid` unsplit ones, whose walks
 // hold about `tokens` tokens: at most one per CU, and each with work for its join (2 us):
@@ -1158,10 +1189,10 @@ loom_status_t make_plan(const loom::DeviceInfo &dev, const loom_window_attention
   };
   const bool long_tile =
       flags & LOOM_PLAN_PREFILL_TILE_LONG ||
-      (!(flags & LOOM_PLAN_PREFILL_TILE_16) && s.explicit_rows && cols >= kLongMinCols * batch);
+      (!(flags & LOOM_PLAN_PREFILL_TILE_16) && s.explicit_rows && takes_long(cols, hkv, cus));
   const uint64_t tc = !long_tile ? 16 : (cols / 128) * hkv >= 2 * cus ? 128 : 64;
   const uint64_t tiles = tiles_of(tc), grid = tiles * hkv;
-  const uint32_t groups = !long_tile ? 1 : tc == 128 ? (grid <= 2 * cus ? 2 : 1) : grid <= cus ? 4 : 2;
+  const uint32_t groups = long_tile ? long_groups(tc, cols * hkv / 128, grid, cus, s.window == 0) : 1;
   const uint32_t waves = !long_tile ? kRowWaves : (uint32_t)tc / 32 * groups;
   if (grid * (waves * 64) >= (1ull << 32))
     return fail(err, LOOM_PLAN_STATE_COUNT_OUT_OF_RANGE, "window rows", s.rows);
@@ -1305,6 +1336,9 @@ loom_status_t loom_window_attention_enqueue(const loom_window_attention_plan_t *
   a.sinks = (int32_t)std::min<uint64_t>(s.sinks, INT32_MAX - 64);
   a.row_tiles = (int32_t)plan->info.row_tiles;
   a.head_tiles = (a.group + 15) / 16;
+  // (exact while column * group < 2^32)
+  if (a.group > 1 && s.rows * (uint64_t)a.group * (uint64_t)a.group < (1ull << 32))
+    a.group_inv = (uint32_t)(((1ull << 32) + a.group - 1) / a.group);
   // the tokens that a request's rows see, at most: its window, or the average context
   const uint64_t tokens =
       std::min<uint64_t>((uint64_t)a.window + (uint64_t)a.sinks + s.rows / pg.batch_size,
@@ -1317,7 +1351,10 @@ loom_status_t loom_window_attention_enqueue(const loom_window_attention_plan_t *
     a.states = (float *)loom::queue_shares(scope, (uint64_t)a.splits * grid * 16 * kStash * 4);
     if (!a.states || !a.arrived || grid > loom::kMx4Joins) a.splits = 1;
   }
-  const dim3 blocks((unsigned)(grid * a.splits)), threads(plan->info.block_threads);
+  uint64_t workgroups = grid * a.splits;
+  a.pair_heads = mx && !long_tile && a.hkv % 2 == 0 ? (int32_t)workgroups : 0;
+  if (a.pair_heads) workgroups = (workgroups + 15) / 16 * 16;
+  const dim3 blocks((unsigned)workgroups), threads(plan->info.block_threads);
   hipStream_t stream = scope->queue->stream;
   const auto kernel = mx    ? kernel_of<kMx4>(*plan)
                       : fp8 ? kernel_of<kFp8>(*plan)
