@@ -261,7 +261,7 @@ __device__ __forceinline__ void exact_column(const WindowArgs &a, const Tile &t,
 }
 
 // ---- row tiles ---------------------------------------------------------------------
-// One workgroup of W waves per (16 columns, kv-head[, split]).  Wave w takes 32-token steps
+// One workgroup of W waves per (16 or 32 columns, kv-head[, split]).  Wave w takes 32-token steps
 // w, w + W, ... of the walk (of its split's share of it), each through LDS of its own
 // (PipeWave's slot: whole rows, so a load instruction covers whole lines, in an order that
 // spreads the fragment reads over the banks), and the wave states merge in LDS.  Per step:
@@ -287,14 +287,16 @@ struct RowSlot {
   static constexpr int kVShift = KV == kFp8 ? 0 : -kGroups * Pipe::kKGroup;  // of V, against PipeWave's
   static constexpr int kBytes = KV == kFp8 ? Pipe::kSlotBytes : kGroups * (Pipe::kKGroup + Pipe::kVGroup);
   static constexpr int kSlots = KV == kMx4 ? 1 : 2;
-  static constexpr int kWaveBytes = (std::max(kSlots * kBytes, 16 * kStash * 4) + 15) & ~15;
 };
 
-template <Kv KV>
+template <Kv KV, int CT>
 struct RowsSmem {
-  __align__(16) uint8_t slots[kRowWaves][RowSlot<KV>::kWaveBytes];
+  using Slot = RowSlot<KV>;
+  // a wave's slots, and after its walk its columns' O
+  static constexpr int kWaveBytes = (std::max(Slot::kSlots * Slot::kBytes, 16 * CT * kStash * 4) + 15) & ~15;
+  __align__(16) uint8_t slots[kRowWaves][kWaveBytes];
   LocateSmem<kRowWaves> loc;
-  float m[kRowWaves][16], l[kRowWaves][16];
+  float m[kRowWaves][16 * CT], l[kRowWaves][16 * CT];
   uint32_t bad[kRowWaves];
   uint32_t arrived;
   uint32_t redo;  // columns whose O is not finite
@@ -344,14 +346,14 @@ __device__ __forceinline__ void put_mx(uint8_t *group, int lane, const u32x4 &w,
   }
 }
 
-template <Kv KV>
-__global__ __launch_bounds__(kRowWaves * 64) void window_rows_kernel(WindowArgs args) {
-  constexpr int W = kRowWaves, TC = 16;
+template <Kv KV, int CT, bool NT>
+__global__ __launch_bounds__(kRowWaves * 64, 2) void window_rows_kernel(WindowArgs args) {
+  constexpr int W = kRowWaves, TC = 16 * CT;
   constexpr bool FP8 = KV == kFp8;
   using Pipe = RowPipe<KV>;
   using Slot = RowSlot<KV>;
   constexpr int H = kStepBlocks<KV>, kPlaced = 64 / H;  // steps placed at once
-  __shared__ RowsSmem<KV> sm;
+  __shared__ RowsSmem<KV, CT> sm;
   WindowArgs a = args;
   float v_scale = 1.0f;
   if constexpr (FP8) {
@@ -370,21 +372,23 @@ __global__ __launch_bounds__(kRowWaves * 64) void window_rows_kernel(WindowArgs 
   Tile t;
   if (!find_tile<W, TC>(a, sm.loc, t, split, block)) return;
   const int kvh = t.loc.kvh;
-  // this lane's column
-  const int f = t.col0 + col;
-  const bool valid = f < t.fcols;
-  const int qi = valid ? row_of(a, f) : 0;
-  const int end_col = valid ? t.kv_len - t.group_rows + qi + 1 : 0;
-  const int beg_col = max(0, end_col - a.window);
   // tokens [full_beg, full_end) are seen by every column
   const int full_beg = max(0, t.p_hi + 1 - a.window), full_end = t.p_lo + 1;
   Pipe pw{a, lane, col, quad};
   pw.reset(sm.slots[wave]);
-  {
+  // this lane's columns, one of each 16
+  int beg_col[CT], end_col[CT];
+#pragma unroll
+  for (int x = 0; x < CT; ++x) {
+    const int f = t.col0 + 16 * x + col;
+    const bool valid = f < t.fcols;
+    const int qi = valid ? row_of(a, f) : 0;
+    end_col[x] = valid ? t.kv_len - t.group_rows + qi + 1 : 0;
+    beg_col[x] = max(0, end_col[x] - a.window);
     const uint16_t *qp =
         a.q + ((int64_t)(t.loc.qs + qi) * a.hq + (int64_t)kvh * a.group + (f - qi * a.group)) * 128;
 #pragma unroll
-    for (int c = 0; c < 4; ++c) pw.qf[0][c] = valid ? load16(qp + Pipe::q_dim(c, quad)) : u32x4{0, 0, 0, 0};
+    for (int c = 0; c < 4; ++c) pw.qf[x][c] = valid ? load16(qp + Pipe::q_dim(c, quad)) : u32x4{0, 0, 0, 0};
   }
   // this split's steps [lo, hi), this wave's lo + wave + W i
   const int steps = (t.blocks + H - 1) / H;
@@ -445,8 +449,8 @@ __global__ __launch_bounds__(kRowWaves * 64) void window_rows_kernel(WindowArgs 
       const __amdgpu_buffer_rsrc_t rk = rsrc(a.k, at, bytes), rv = rsrc(a.v, at, bytes);
 #pragma unroll
       for (int x = 0; x < kHalf; ++x) {
-        lds_load16_at(rk, slot + (uint32_t)((h * kHalf + x) * Pipe::kKGroup), lane_off[x]);
-        lds_load16_at(rv, slot + (uint32_t)(Slot::kVShift + Pipe::v_group(x) +
+        lds_load16_at<NT>(rk, slot + (uint32_t)((h * kHalf + x) * Pipe::kKGroup), lane_off[x]);
+        lds_load16_at<NT>(rv, slot + (uint32_t)(Slot::kVShift + Pipe::v_group(x) +
                                             h * (Pipe::v_group(kHalf) - Pipe::v_group(0))),
                       lane_off[x]);
       }
@@ -458,32 +462,38 @@ __global__ __launch_bounds__(kRowWaves * 64) void window_rows_kernel(WindowArgs 
     const uint64_t at = lane64(at_lo, at_hi, i), sc = lane64(sc_lo, sc_hi, i);
     const int bytes = rows > 0 ? (rows - 1) * a.row_bytes + 64 : 0;
     const int off = mx_row(lane) * a.row_bytes + (lane & 3) * 16;
-    g.k = load16_rows<false>(rsrc(a.k, at, bytes), off);
-    g.v = load16_rows<false>(rsrc(a.v, at, bytes), off);
+    g.k = load16_rows<NT>(rsrc(a.k, at, bytes), off);
+    g.v = load16_rows<NT>(rsrc(a.v, at, bytes), off);
     g.ks = __builtin_amdgcn_raw_buffer_load_b32(rsrc(a.k_mx, sc, 4 * rows), 4 * mx_row(lane), 0, 0);
     g.vs = __builtin_amdgcn_raw_buffer_load_b32(rsrc(a.v_mx, sc, 4 * rows), 4 * mx_row(lane), 0, 0);
   };
 
-  float m_run = -INFINITY, l_run = 0.0f;
-  f32x4(&acc)[8] = pw.acc[0];
+  float m_run[CT], l_run[CT];
+#pragma unroll
+  for (int x = 0; x < CT; ++x) {
+    m_run[x] = -INFINITY;
+    l_run[x] = 0.0f;
+  }
+  f32x4(&acc)[2][8] = pw.acc;
   // The softmax and products of step i, whose rows lie at `slot`.
   auto process = [&](int i, const uint8_t *slot) {
-    f32x4 s[H] = {};  // s[h][j]: token 4 quad + j of block h
+    f32x4 s[CT][H] = {};  // s[x][h][j]: token 4 quad + j of block h, column of the x-th 16
     u32x2 v[8];
     if constexpr (FP8) {
       u32x4 k[2][2];
 #pragma unroll
-      for (int x = 0; x < 4; ++x)
-        k[x >> 1][x & 1] = *reinterpret_cast<const u32x4 *>(slot + pw.kofs[x >> 1] + (x & 1) * kHalf * Pipe::kKGroup);
+      for (int y = 0; y < 4; ++y)
+        k[y >> 1][y & 1] = *reinterpret_cast<const u32x4 *>(slot + pw.kofs[y >> 1] + (y & 1) * kHalf * Pipe::kKGroup);
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[e] = lds_read_tr8(slot + pw.vofs[e >> 1] + (e & 1) * 16);
 #pragma unroll
-      for (int x = 0; x < 8; ++x) {
-        const u32x4 &w = k[x >> 2][x & 1];
-        const int c = x >> 1;
-        s[x & 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-            as_bf16x8(fp8x8_to_bf16x8(u32x2{w[2 * (c & 1)], w[2 * (c & 1) + 1]})), as_bf16x8(pw.qf[0][c]),
-            s[x & 1], 0, 0, 0);
+      for (int y = 0; y < 8; ++y) {
+        const u32x4 &w = k[y >> 2][y & 1];
+        const int c = y >> 1;
+        const bf16x8 kw = as_bf16x8(fp8x8_to_bf16x8(u32x2{w[2 * (c & 1)], w[2 * (c & 1) + 1]}));
+#pragma unroll
+        for (int x = 0; x < CT; ++x)
+          s[x][y & 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kw, as_bf16x8(pw.qf[x][c]), s[x][y & 1], 0, 0, 0);
       }
     } else {
       u32x4 k[4];
@@ -493,62 +503,94 @@ __global__ __launch_bounds__(kRowWaves * 64) void window_rows_kernel(WindowArgs 
       for (int e = 0; e < 8; ++e) v[e] = lds_read_tr16(slot + Slot::kVShift + pw.vofs[e >> 1] + (e & 1) * 32);
 #pragma unroll
       for (int c = 0; c < 4; ++c)
-        s[0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(k[c]), as_bf16x8(pw.qf[0][c]), s[0], 0, 0, 0);
+#pragma unroll
+        for (int x = 0; x < CT; ++x)
+          s[x][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(k[c]), as_bf16x8(pw.qf[x][c]), s[x][0], 0, 0, 0);
     }
-    float ml = -INFINITY;
+    int t0[H];
+    bool full = true;
 #pragma unroll
     for (int h = 0; h < H; ++h) {
-      const int t0 = (__builtin_amdgcn_readlane(meta, H * i + h) >> 5) * 16;
-      if (t0 < full_beg || t0 + 16 > full_end) {
+      t0[h] = (__builtin_amdgcn_readlane(meta, H * i + h) >> 5) * 16;
+      full &= t0[h] >= full_beg && t0[h] + 16 <= full_end;
+    }
+    if (!full) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int tok = t0 + 4 * quad + j;
-          s[h][j] = tok < end_col && (tok >= beg_col || tok < a.sinks) ? s[h][j] : -INFINITY;
+      for (int x = 0; x < CT; ++x)
+#pragma unroll
+        for (int h = 0; h < H; ++h)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int tok = t0[h] + 4 * quad + j;
+            s[x][h][j] =
+                tok < end_col[x] && (tok >= beg_col[x] || tok < a.sinks) ? s[x][h][j] : -INFINITY;
+          }
+    }
+    float ml[CT];
+    bool above = false;
+#pragma unroll
+    for (int x = 0; x < CT; ++x) {
+      ml[x] = -INFINITY;
+#pragma unroll
+      for (int h = 0; h < H; ++h)
+        ml[x] = fmax_nan(ml[x], fmax_nan(fmax_nan(s[x][h][0], s[x][h][1]), fmax_nan(s[x][h][2], s[x][h][3])));
+      above |= ml[x] * a.scale_log2 > m_run[x] + 8.0f;
+    }
+    if (__builtin_amdgcn_ballot_w64(above)) {
+#pragma unroll
+      for (int x = 0; x < CT; ++x) {
+        const float mx = quad_max_nan(ml[x]) * a.scale_log2;
+        const bool grow = mx > m_run[x] + 8.0f;
+        const float m_ref = grow ? mx : m_run[x];
+        if (__builtin_amdgcn_ballot_w64(grow && m_run[x] != -INFINITY)) {
+          const float al = fast_exp2(m_run[x] - (m_ref == -INFINITY ? 0.0f : m_ref));
+#pragma unroll
+          for (int e = 0; e < 8; ++e) acc[x][e] *= al;
+          l_run[x] *= al;
         }
+        m_run[x] = m_ref;
       }
-      ml = fmax_nan(ml, fmax_nan(fmax_nan(s[h][0], s[h][1]), fmax_nan(s[h][2], s[h][3])));
     }
-    if (__builtin_amdgcn_ballot_w64(ml * a.scale_log2 > m_run + 8.0f)) {
-      const float mx = quad_max_nan(ml) * a.scale_log2;
-      const bool grow = mx > m_run + 8.0f;
-      const float m_ref = grow ? mx : m_run;
-      if (__builtin_amdgcn_ballot_w64(grow && m_run != -INFINITY)) {
-        const float al = fast_exp2(m_run - (m_ref == -INFINITY ? 0.0f : m_ref));
+    uint32_t ph[CT][2 * H], pl[CT][2 * H];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) acc[e] *= al;
-        l_run *= al;
+    for (int x = 0; x < CT; ++x) {
+      const float m_use = m_run[x] == -INFINITY ? 0.0f : m_run[x];  // nothing visible yet
+#pragma unroll
+      for (int y = 0; y < 2 * H; ++y) {
+        const float x0 = fast_exp2(fmaf(s[x][y >> 1][2 * (y & 1)], a.scale_log2, -m_use));
+        const float x1 = fast_exp2(fmaf(s[x][y >> 1][2 * (y & 1) + 1], a.scale_log2, -m_use));
+        const uint32_t b0 = __float_as_uint(x0), b1 = __float_as_uint(x1);
+        ph[x][y] = pack_hi16(b0, b1);
+        pl[x][y] = pack_hi16(__float_as_uint(x0 - __uint_as_float(b0 & 0xffff0000u)),
+                             __float_as_uint(x1 - __uint_as_float(b1 & 0xffff0000u)));
+        l_run[x] += x0 + x1;
       }
-      m_run = m_ref;
-    }
-    const float m_use = m_run == -INFINITY ? 0.0f : m_run;  // nothing visible yet
-    uint32_t ph[2 * H], pl[2 * H];
-#pragma unroll
-    for (int y = 0; y < 2 * H; ++y) {
-      const float x0 = fast_exp2(fmaf(s[y >> 1][2 * (y & 1)], a.scale_log2, -m_use));
-      const float x1 = fast_exp2(fmaf(s[y >> 1][2 * (y & 1) + 1], a.scale_log2, -m_use));
-      const uint32_t b0 = __float_as_uint(x0), b1 = __float_as_uint(x1);
-      ph[y] = pack_hi16(b0, b1);
-      pl[y] = pack_hi16(__float_as_uint(x0 - __uint_as_float(b0 & 0xffff0000u)),
-                        __float_as_uint(x1 - __uint_as_float(b1 & 0xffff0000u)));
-      l_run += x0 + x1;
     }
     if constexpr (FP8) {
       bf16x8 w[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         w[e] = as_bf16x8(fp8x8_to_bf16x8(v[e]));
-        acc[e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[e], as_bf16x8(ph[0], ph[1], ph[2], ph[3]), acc[e], 0, 0, 0);
+#pragma unroll
+        for (int x = 0; x < CT; ++x)
+          acc[x][e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+              w[e], as_bf16x8(ph[x][0], ph[x][1], ph[x][2], ph[x][3]), acc[x][e], 0, 0, 0);
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        acc[e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(w[e], as_bf16x8(pl[0], pl[1], pl[2], pl[3]), acc[e], 0, 0, 0);
+#pragma unroll
+        for (int x = 0; x < CT; ++x)
+          acc[x][e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+              w[e], as_bf16x8(pl[x][0], pl[x][1], pl[x][2], pl[x][3]), acc[x][e], 0, 0, 0);
     } else {
       // high parts and residuals in the two halves of the contraction
-      const bf16x8 p = as_bf16x8(ph[0], ph[1], pl[0], pl[1]);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        acc[e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(v[e][0], v[e][1], v[e][0], v[e][1]), p,
-                                                         acc[e], 0, 0, 0);
+        const bf16x8 w = as_bf16x8(v[e][0], v[e][1], v[e][0], v[e][1]);
+#pragma unroll
+        for (int x = 0; x < CT; ++x)
+          acc[x][e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+              w, as_bf16x8(ph[x][0], ph[x][1], pl[x][0], pl[x][1]), acc[x][e], 0, 0, 0);
       }
     }
   };
@@ -583,7 +625,9 @@ __global__ __launch_bounds__(kRowWaves * 64) void window_rows_kernel(WindowArgs 
     } else {
       // (queries and index words have arrived: no wait of the compiler's in the walk)
 #pragma unroll
-      for (int x = 0; x < 4; ++x) asm volatile("" : "+v"(pw.qf[0][x]));
+      for (int x = 0; x < CT; ++x)
+#pragma unroll
+        for (int c2 = 0; c2 < 4; ++c2) asm volatile("" : "+v"(pw.qf[x][c2]));
       asm volatile("" : "+v"(at_lo), "+v"(at_hi), "+v"(meta));
       wait_reads();
       if (c > 0) issue(0, ring_at);
@@ -606,17 +650,20 @@ __global__ __launch_bounds__(kRowWaves * 64) void window_rows_kernel(WindowArgs 
     }
   }
 
-  // The wave's columns to its slot.  acc[e][j] = O[column][16 e + 4 quad + j]
+  // The wave's columns to its slot.  acc[x][e][j] = O[column of the x-th 16][16 e + 4 quad + j]
   wait_reads();
   wave_lds_fence();
   float *const stash = reinterpret_cast<float *>(sm.slots[wave]);
-  const float l_col = quad_sum(l_run);
 #pragma unroll
-  for (int e = 0; e < 8; ++e)
-    *reinterpret_cast<f32x4 *>(stash + col * kStash + 16 * e + 4 * quad) = acc[e];
-  if (quad == 0) {
-    sm.m[wave][col] = m_run;
-    sm.l[wave][col] = l_col;
+  for (int x = 0; x < CT; ++x) {
+    const float l_col = quad_sum(l_run[x]);
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      *reinterpret_cast<f32x4 *>(stash + (16 * x + col) * kStash + 16 * e + 4 * quad) = acc[x][e];
+    if (quad == 0) {
+      sm.m[wave][16 * x + col] = m_run[x];
+      sm.l[wave][16 * x + col] = l_col;
+    }
   }
   if (tid == 0) sm.redo = 0;
   if (block_or(bad, sm.bad)) return;
@@ -1126,18 +1173,33 @@ struct loom_window_attention_plan {
   loom_window_attention_plan_info_t info{};
   int cus = 0;
   uint32_t groups = 1;  // long tiles: wave groups that split a walk
+  bool once = false;    // row tiles: a request has one tile per kv-head, as a rule
 };
+
+// Bytes of a command's rows from which they are loaded past the caches, where each is
+// read once: 64 requests under windows of 4096 (1.1 GB) 170 -> 151 us, 8 of 8192 on FP8
+// pages (134 MB) 32.5 -> 29.5; but 16 of 1024 (61 MB), which the last-level cache may hold
+// still, 14.4 -> 17.1.
+constexpr uint64_t kPastCaches = 96ull << 20;
 
 namespace {
 
 constexpr uint64_t kMaxHeads = 4096;  // kv-heads: a row of all of them in a 32-bit stride
 constexpr int kMaxSplits = 16;
 
-// Long tiles where row tiles would fill the chip twice.  Microseconds, row / long tiles: 8
-// x 16 rows behind 5000 tokens 32/8 under windows of 1024 13.4 / 20.0, 8 x 32 (512 row
-// tiles) 23.3 / 20.3, 8 x 64 42.8 / 21.6; over the whole prefix 56 / 82, 94 / 80, 166 / 93;
-// FP8 and MXFP4 pages alike.
-bool takes_long(uint64_t cols, uint64_t hkv, uint64_t cus) { return cols * hkv >= 16 * 2 * cus; }
+// Columns per workgroup, from the number of row tiles of 16 that the command holds (a
+// request's last one is about half full).  Microseconds, 16 / 32 / long, rows behind 5000
+// tokens 32/8:
+//  - one per CU: 16 (8 x 16 rows under windows of 1024 13.7 / 15.0 / 20.0, over the whole
+//    prefix 56 / 63 / 82; one request of 8 rows 9.5 / 13.5 / 18.0);
+//  - two: 32, which share a walk's rows (8 x 32 rows 23.4 / 17.3 / 20.5, whole 94 / 59 / 80;
+//    MXFP4 27.2 / 19.1 / 26.3, whole 81 / 55 / 72, but 8 x 1-32, 300 tiles, 39 / 48: two
+//    workgroups of its 16 fit a CU);
+//  - more: long tiles (8 x 64 rows 42.0 / 30.2 / 21.9, whole 164 / 96 / 92).
+uint64_t row_tile_cols(uint64_t tiles, uint64_t cus, bool mx) {
+  if (4 * tiles <= (mx ? 6 : 5) * cus) return 16;
+  return 4 * tiles <= 9 * cus ? 32 : 0;
+}
 
 // Wave groups of the long tiles: as many as `tiles` full ones of 128 columns (or a grid of
 // 64-column ones) leave room for.  Walks over the whole prefix differ, so the longest are
@@ -1161,8 +1223,11 @@ int row_splits(uint64_t grid, uint64_t tokens, int cus, bool mx) {
 }
 
 template <Kv KV>
-auto kernel_of(const loom_window_attention_plan &p) {
-  if (p.info.algorithm != LOOM_PAGED_PREFILL_LONG_TILE) return window_rows_kernel<KV>;
+auto kernel_of(const loom_window_attention_plan &p, uint64_t bytes) {
+  if (p.info.algorithm != LOOM_PAGED_PREFILL_LONG_TILE)
+    return p.info.tile_cols == 32 ? window_rows_kernel<KV, 2, false>
+           : p.once && bytes >= kPastCaches ? window_rows_kernel<KV, 1, true>
+                                   : window_rows_kernel<KV, 1, false>;
   if (p.info.tile_cols == 128) return p.groups == 2 ? window_long_kernel<KV, 8, 4> : window_long_kernel<KV, 4, 4>;
   return p.groups == 4 ? window_long_kernel<KV, 8, 2> : window_long_kernel<KV, 4, 2>;
 }
@@ -1183,14 +1248,21 @@ loom_status_t make_plan(const loom::DeviceInfo &dev, const loom_window_attention
   if (s.rows > (uint64_t)INT32_MAX / hq || batch >= (uint64_t)INT32_MAX)
     return fail(err, LOOM_PLAN_STATE_COUNT_OUT_OF_RANGE, "window rows", s.rows);
   const uint64_t cols = s.rows * group, cus = (uint64_t)dev.cus;
+  // columns of a request, as a rule
+  const uint64_t group_cols = s.explicit_rows ? (cols + batch - 1) / batch : group;
   auto tiles_of = [&](uint64_t tc) {
     return s.explicit_rows ? std::min(cols, (cols + (tc - 1) * batch) / tc)
                            : batch * ((group + tc - 1) / tc);
   };
+  const bool mx = s.paged.kv_dtype == LOOM_KV_DTYPE_MXFP4;
+  const uint64_t row_cols =
+      row_tile_cols((s.explicit_rows ? cols / 16 + (batch + 1) / 2 : tiles_of(16)) * hkv, cus, mx);
   const bool long_tile =
       flags & LOOM_PLAN_PREFILL_TILE_LONG ||
-      (!(flags & LOOM_PLAN_PREFILL_TILE_16) && s.explicit_rows && takes_long(cols, hkv, cus));
-  const uint64_t tc = !long_tile ? 16 : (cols / 128) * hkv >= 2 * cus ? 128 : 64;
+      (!(flags & LOOM_PLAN_PREFILL_TILE_16) && s.explicit_rows && row_cols == 0);
+  const uint64_t tc = !long_tile                      ? (row_cols == 16 || group_cols <= 16 ? 16 : 32)
+                      : (cols / 128) * hkv >= 2 * cus ? 128
+                                                      : 64;
   const uint64_t tiles = tiles_of(tc), grid = tiles * hkv;
   const uint32_t groups = long_tile ? long_groups(tc, cols * hkv / 128, grid, cus, s.window == 0) : 1;
   const uint32_t waves = !long_tile ? kRowWaves : (uint32_t)tc / 32 * groups;
@@ -1206,6 +1278,7 @@ loom_status_t make_plan(const loom::DeviceInfo &dev, const loom_window_attention
   p->info.flags = flags;
   p->cus = dev.cus;
   p->groups = groups;
+  p->once = group_cols <= tc;
   *out = p;
   return loom::ok(err);
 }
@@ -1335,7 +1408,7 @@ loom_status_t loom_window_attention_enqueue(const loom_window_attention_plan_t *
   a.window = s.window == 0 || s.window > (uint64_t)INT32_MAX ? INT32_MAX : (int32_t)s.window;
   a.sinks = (int32_t)std::min<uint64_t>(s.sinks, INT32_MAX - 64);
   a.row_tiles = (int32_t)plan->info.row_tiles;
-  a.head_tiles = (a.group + 15) / 16;
+  a.head_tiles = (a.group + (int32_t)plan->info.tile_cols - 1) / (int32_t)plan->info.tile_cols;
   // (exact while column * group < 2^32)
   if (a.group > 1 && s.rows * (uint64_t)a.group * (uint64_t)a.group < (1ull << 32))
     a.group_inv = (uint32_t)(((1ull << 32) + a.group - 1) / a.group);
@@ -1348,7 +1421,7 @@ loom_status_t loom_window_attention_enqueue(const loom_window_attention_plan_t *
   a.splits = long_tile ? 1 : row_splits(grid, tokens, plan->cus, mx);
   if (a.splits > 1) {
     a.arrived = scope->queue->joins;
-    a.states = (float *)loom::queue_shares(scope, (uint64_t)a.splits * grid * 16 * kStash * 4);
+    a.states = (float *)loom::queue_shares(scope, (uint64_t)a.splits * grid * plan->info.tile_cols * kStash * 4);
     if (!a.states || !a.arrived || grid > loom::kMx4Joins) a.splits = 1;
   }
   uint64_t workgroups = grid * a.splits;
@@ -1356,9 +1429,10 @@ loom_status_t loom_window_attention_enqueue(const loom_window_attention_plan_t *
   if (a.pair_heads) workgroups = (workgroups + 15) / 16 * 16;
   const dim3 blocks((unsigned)workgroups), threads(plan->info.block_threads);
   hipStream_t stream = scope->queue->stream;
-  const auto kernel = mx    ? kernel_of<kMx4>(*plan)
-                      : fp8 ? kernel_of<kFp8>(*plan)
-                            : kernel_of<kBf16>(*plan);
+  const uint64_t bytes = tokens * pg.batch_size * pg.num_kv_heads * 2 * (mx ? 68 : (uint64_t)row);
+  const auto kernel = mx    ? kernel_of<kMx4>(*plan, bytes)
+                      : fp8 ? kernel_of<kFp8>(*plan, bytes)
+                            : kernel_of<kBf16>(*plan, bytes);
   hipLaunchKernelGGL(kernel, blocks, threads, 0, stream, a);
   return loom::record_launch(scope, hipGetLastError(), err);
 }
