@@ -268,26 +268,38 @@ __device__ __forceinline__ void exact_column(const WindowArgs &a, const Tile &t,
 // S = K.Q^T in 8 MFMAs of 16x16x32, the softmax with a running maximum that moves only when
 // a score passes it by 2^8, and O^T += V^T.P^T in 16, P as a BF16 high part and a BF16
 // residual (16 bits: few tokens carry a short window, whose errors do not average out).
-// BF16 and FP8 rows go straight to LDS; MXFP4 codes are loaded into registers, one block of
-// 32 values and its scale per lane, and written to LDS as BF16, which serves K and V alike.
+// Rows, codes and scales go straight to LDS.  Widened to BF16 on the way, as the long tiles
+// have them, MXFP4 rows cost a wave 360 cycles of LDS per 32 tokens, four times what the
+// codes take (64 single tokens under windows of 4096: 75 us).
 constexpr int kRowWaves = 8;
-constexpr int kAhead = 2;    // MXFP4: steps in flight
 constexpr int kStash = 132;  // floats between two columns' O in LDS, and of a split's state
 
 template <Kv KV>
 using RowPipe = PipeWave<4, KV == kFp8, true, 1>;
 // 16-row blocks of a step.
 template <Kv KV>
-constexpr int kStepBlocks = KV == kFp8 ? 2 : 1;
-// A step's rows in LDS: PipeWave's slot (FP8), or the first half of its K and of its V.
+constexpr int kStepBlocks = KV == kBf16 ? 1 : 2;
+// A step's rows in LDS.  FP8: PipeWave's slot; BF16: the first half of its K and of its V.
+// MXFP4: per block 16 rows of 64 code bytes, K then V, whose four 16-byte pieces are
+// permuted by the row (piece c of row r at c ^ (r >> 2)), so that a fragment's read, one
+// piece of all rows, and 64 bytes of four neighbouring rows each meet every bank once; then
+// per block the K scale words, and the V ones, of rows mx_token(0), mx_token(1), ...
 template <Kv KV>
 struct RowSlot {
   using Pipe = RowPipe<KV>;
   static constexpr int kGroups = KV == kFp8 ? Pipe::kGroups : Pipe::kGroups / 2;  // of each of K and V
   static constexpr int kVShift = KV == kFp8 ? 0 : -kGroups * Pipe::kKGroup;  // of V, against PipeWave's
-  static constexpr int kBytes = KV == kFp8 ? Pipe::kSlotBytes : kGroups * (Pipe::kKGroup + Pipe::kVGroup);
-  static constexpr int kSlots = KV == kMx4 ? 1 : 2;
+  static constexpr int kMxV = 2 * 1024, kMxKs = 4 * 1024, kMxVs = kMxKs + 128;
+  static constexpr int kBytes = KV == kMx4   ? kMxVs + 128
+                                : KV == kFp8 ? Pipe::kSlotBytes
+                                             : kGroups * (Pipe::kKGroup + Pipe::kVGroup);
+  static constexpr int kSlots = KV == kMx4 ? 3 : 2;
+  static constexpr int kLoads = KV == kMx4 ? 8 : 2 * kGroups;  // instructions of a step
 };
+// MXFP4: the row of a block that row c of the MFMA tile S = K.Q^T stands for.  S leaves lane
+// (col, quad) rows 4 quad + j, which are tokens 4 j + quad, and the V reads of the four
+// quads then lie in four neighbouring rows.
+__device__ __forceinline__ int mx_token(int c) { return 4 * (c & 3) + (c >> 2); }
 
 template <Kv KV, int CT>
 struct RowsSmem {
@@ -319,33 +331,6 @@ __device__ __forceinline__ f32x2 load_state(const float *p) {
                                                      __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
 }
 
-// MXFP4 rows of a 16-row block in registers: lane l holds 32 values, block l & 3 of row
-// mx_row(l), and the row's scale word.
-struct MxStage {
-  u32x4 k, v;
-  uint32_t ks, vs;
-};
-// In this order of rows the 16 lanes that LDS writes at once meet each bank once: their
-// rows lie in four groups, 16 bytes further each in K, 32 in V (where lanes of the last two
-// groups write neighbouring units in turn).  With rows in order they shared a quarter of
-// the banks, and the writes took 257 cycles of a step's 310 in LDS.
-__device__ __forceinline__ int mx_row(int lane) { return 4 * ((lane >> 2) & 3) + (lane >> 4); }
-// A lane's 32 values to a slot as BF16; `group`: where the row's group (mx_row / 4) lies.
-template <class Pipe, bool V>
-__device__ __forceinline__ void put_mx(uint8_t *group, int lane, const u32x4 &w, uint32_t scales) {
-  const int b = lane & 3, r3 = lane >> 4;
-  const bool turn = V && (lane & 8);
-  uint8_t *const dst = group + r3 * 256 + ((4 * b) ^ Pipe::swizzle(r3)) * 16;
-  uint8_t *const even = dst + (turn ? 16 : 0), *const odd = dst + (turn ? 0 : 16);
-  const uint32_t scale = mx_scale(scales, b);
-#pragma unroll
-  for (int u = 0; u < 4; u += 2) {
-    const uint32_t x = turn ? w[u + 1] : w[u], y = turn ? w[u] : w[u + 1];
-    *reinterpret_cast<u32x4 *>(even + 16 * u) = mx4x8_to_bf16x8(x, scale);
-    *reinterpret_cast<u32x4 *>(odd + 16 * u) = mx4x8_to_bf16x8(y, scale);
-  }
-}
-
 template <Kv KV, int CT, bool NT>
 __global__ __launch_bounds__(kRowWaves * 64, 2) void window_rows_kernel(WindowArgs args) {
   constexpr int W = kRowWaves, TC = 16 * CT;
@@ -375,7 +360,8 @@ __global__ __launch_bounds__(kRowWaves * 64, 2) void window_rows_kernel(WindowAr
   // tokens [full_beg, full_end) are seen by every column
   const int full_beg = max(0, t.p_hi + 1 - a.window), full_end = t.p_lo + 1;
   Pipe pw{a, lane, col, quad};
-  pw.reset(sm.slots[wave]);
+  uint8_t *const slots = sm.slots[wave];
+  pw.reset(slots);
   // this lane's columns, one of each 16
   int beg_col[CT], end_col[CT];
 #pragma unroll
@@ -388,7 +374,10 @@ __global__ __launch_bounds__(kRowWaves * 64, 2) void window_rows_kernel(WindowAr
     const uint16_t *qp =
         a.q + ((int64_t)(t.loc.qs + qi) * a.hq + (int64_t)kvh * a.group + (f - qi * a.group)) * 128;
 #pragma unroll
-    for (int c = 0; c < 4; ++c) pw.qf[x][c] = valid ? load16(qp + Pipe::q_dim(c, quad)) : u32x4{0, 0, 0, 0};
+    for (int c = 0; c < 4; ++c) {
+      const int d = KV == kMx4 ? 32 * quad + 8 * c : Pipe::q_dim(c, quad);
+      pw.qf[x][c] = valid ? load16(qp + d) : u32x4{0, 0, 0, 0};
+    }
   }
   // this split's steps [lo, hi), this wave's lo + wave + W i
   const int steps = (t.blocks + H - 1) / H;
@@ -429,11 +418,13 @@ __global__ __launch_bounds__(kRowWaves * 64, 2) void window_rows_kernel(WindowAr
     return __builtin_amdgcn_make_buffer_rsrc(
         const_cast<uint8_t *>(reinterpret_cast<const uint8_t *>(base) + at), 0, bytes, 0x00020000);
   };
-  // BF16 and FP8: the loads of step i (of the placed ones) into the slot at LDS address `slot`
-  constexpr int kHalf = Pipe::kGroups / 2;  // groups of a block
-  constexpr int kStepLoads = 2 * H * kHalf;
-  int lane_off[kHalf];
-  if constexpr (KV != kMx4) {
+  // The loads of step i (of the placed ones) into the slot at LDS address `slot`
+  constexpr int kHalf = Slot::kGroups / H;  // groups of a block (BF16, FP8)
+  int lane_off[kHalf], mx_off = 0;
+  if constexpr (KV == kMx4) {
+    lane_off[0] = (lane >> 2) * a.row_bytes + (((lane & 3) ^ (lane >> 4)) << 4);
+    mx_off = 4 * mx_token(lane & 15);
+  } else {
     const int unit = (lane & (Pipe::kUnits - 1)) ^ Pipe::swizzle(lane / Pipe::kUnits);
 #pragma unroll
     for (int x = 0; x < kHalf; ++x)
@@ -447,25 +438,24 @@ __global__ __launch_bounds__(kRowWaves * 64, 2) void window_rows_kernel(WindowAr
       const uint64_t at = lane64(at_lo, at_hi, j);
       const int bytes = rows > 0 ? (rows - 1) * a.row_bytes + kRowBytes<KV> : 0;
       const __amdgpu_buffer_rsrc_t rk = rsrc(a.k, at, bytes), rv = rsrc(a.v, at, bytes);
+      if constexpr (KV == kMx4) {
+        const uint64_t sc = lane64(sc_lo, sc_hi, j);
+        lds_load16_at<NT>(rk, slot + 1024 * h, lane_off[0]);
+        lds_load16_at<NT>(rv, slot + Slot::kMxV + 1024 * h, lane_off[0]);
+        if (lane < 16) {
+          lds_load4_at(rsrc(a.k_mx, sc, 4 * rows), slot + Slot::kMxKs + 64 * h, mx_off);
+          lds_load4_at(rsrc(a.v_mx, sc, 4 * rows), slot + Slot::kMxVs + 64 * h, mx_off);
+        }
+      } else {
 #pragma unroll
-      for (int x = 0; x < kHalf; ++x) {
-        lds_load16_at<NT>(rk, slot + (uint32_t)((h * kHalf + x) * Pipe::kKGroup), lane_off[x]);
-        lds_load16_at<NT>(rv, slot + (uint32_t)(Slot::kVShift + Pipe::v_group(x) +
-                                            h * (Pipe::v_group(kHalf) - Pipe::v_group(0))),
-                      lane_off[x]);
+        for (int x = 0; x < kHalf; ++x) {
+          lds_load16_at<NT>(rk, slot + (uint32_t)((h * kHalf + x) * Pipe::kKGroup), lane_off[x]);
+          lds_load16_at<NT>(rv, slot + (uint32_t)(Slot::kVShift + Pipe::v_group(x) +
+                                                  h * (Pipe::v_group(kHalf) - Pipe::v_group(0))),
+                            lane_off[x]);
+        }
       }
     }
-  };
-  // MXFP4: the same into registers
-  auto fetch = [&](int i, MxStage &g) {
-    const int rows = __builtin_amdgcn_readlane(meta, i) & 31;
-    const uint64_t at = lane64(at_lo, at_hi, i), sc = lane64(sc_lo, sc_hi, i);
-    const int bytes = rows > 0 ? (rows - 1) * a.row_bytes + 64 : 0;
-    const int off = mx_row(lane) * a.row_bytes + (lane & 3) * 16;
-    g.k = load16_rows<NT>(rsrc(a.k, at, bytes), off);
-    g.v = load16_rows<NT>(rsrc(a.v, at, bytes), off);
-    g.ks = __builtin_amdgcn_raw_buffer_load_b32(rsrc(a.k_mx, sc, 4 * rows), 4 * mx_row(lane), 0, 0);
-    g.vs = __builtin_amdgcn_raw_buffer_load_b32(rsrc(a.v_mx, sc, 4 * rows), 4 * mx_row(lane), 0, 0);
   };
 
   float m_run[CT], l_run[CT];
@@ -477,35 +467,73 @@ __global__ __launch_bounds__(kRowWaves * 64, 2) void window_rows_kernel(WindowAr
   f32x4(&acc)[2][8] = pw.acc;
   // The softmax and products of step i, whose rows lie at `slot`.
   auto process = [&](int i, const uint8_t *slot) {
-    f32x4 s[CT][H] = {};  // s[x][h][j]: token 4 quad + j of block h, column of the x-th 16
-    u32x2 v[8];
-    if constexpr (FP8) {
-      u32x4 k[2][2];
+    f32x4 s[CT][H] = {};  // s[x][h][j]: token 4 quad + j (MXFP4: 4 j + quad) of block h
+    u32x4 v[8];           // Vᵀ fragments (FP8: still bytes)
+    auto score = [&](const u32x4 &w, int c, int h) {
 #pragma unroll
-      for (int y = 0; y < 4; ++y)
-        k[y >> 1][y & 1] = *reinterpret_cast<const u32x4 *>(slot + pw.kofs[y >> 1] + (y & 1) * kHalf * Pipe::kKGroup);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = lds_read_tr8(slot + pw.vofs[e >> 1] + (e & 1) * 16);
-#pragma unroll
-      for (int y = 0; y < 8; ++y) {
-        const u32x4 &w = k[y >> 2][y & 1];
-        const int c = y >> 1;
-        const bf16x8 kw = as_bf16x8(fp8x8_to_bf16x8(u32x2{w[2 * (c & 1)], w[2 * (c & 1) + 1]}));
-#pragma unroll
-        for (int x = 0; x < CT; ++x)
-          s[x][y & 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kw, as_bf16x8(pw.qf[x][c]), s[x][y & 1], 0, 0, 0);
-      }
-    } else {
+      for (int x = 0; x < CT; ++x)
+        s[x][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(w), as_bf16x8(pw.qf[x][c]), s[x][h],
+                                                          0, 0, 0);
+    };
+    if constexpr (KV == kBf16) {
       u32x4 k[4];
 #pragma unroll
       for (int c = 0; c < 4; ++c) k[c] = *reinterpret_cast<const u32x4 *>(slot + pw.kofs[c]);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = lds_read_tr16(slot + Slot::kVShift + pw.vofs[e >> 1] + (e & 1) * 32);
+      for (int e = 0; e < 8; ++e) {  // the same tokens twice: for the weights' two parts
+        const u32x2 b = lds_read_tr16(slot + Slot::kVShift + pw.vofs[e >> 1] + (e & 1) * 32);
+        v[e] = u32x4{b[0], b[1], b[0], b[1]};
+      }
 #pragma unroll
-      for (int c = 0; c < 4; ++c)
+      for (int c = 0; c < 4; ++c) score(k[c], c, 0);
+    } else if constexpr (FP8) {
+      const auto k = pw.read_k((int)(slot - slots));
 #pragma unroll
-        for (int x = 0; x < CT; ++x)
-          s[x][0] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(k[c]), as_bf16x8(pw.qf[x][c]), s[x][0], 0, 0, 0);
+      for (int e = 0; e < 8; ++e) v[e] = pw.read_v((int)(slot - slots), e);
+#pragma unroll
+      for (int y = 0; y < 8; ++y) {
+        const u32x4 &w = k.f[FP8 ? y >> 2 : 0][y & 1];
+        const int o = 2 * ((y >> 1) & 1);
+        score(fp8x8_to_bf16x8(u32x2{w[o], w[o + 1]}), y >> 1, y & 1);
+      }
+    } else {
+      // K: lane (col, quad) takes dims 32 quad + [0, 32) of row mx_token(col), one scale block.
+      // V: dims 8 col + [0, 8) of tokens 4 j + quad; the widened pairs of two tokens make
+      // two fragments of one dim each, dims 8 col + e of fragment e.
+      u32x4 kw[2], vs[2];
+      uint32_t ks[2], vw[2][4];
+      const uint8_t *const kp = slot + mx_token(col) * 64 + ((quad ^ (col & 3)) << 4);
+      const uint8_t *const vp = slot + Slot::kMxV + quad * 64 + (col & 3) * 4;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        kw[h] = *reinterpret_cast<const u32x4 *>(kp + 1024 * h);
+        ks[h] = *reinterpret_cast<const uint32_t *>(slot + Slot::kMxKs + 64 * h + 4 * col);
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        vs[h] = *reinterpret_cast<const u32x4 *>(slot + Slot::kMxVs + 64 * h + 16 * quad);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          vw[h][j] = *reinterpret_cast<const uint32_t *>(vp + 1024 * h + 256 * j + (((col >> 2) ^ j) << 4));
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t scale = mx_scale(ks[h], quad);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) score(mx4x8_to_bf16x8(kw[h][c], scale), c, h);
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int j = 0; j < 4; j += 2) {
+          const u32x4 b0 = mx4x8_to_bf16x8(vw[h][j], mx_scale(vs[h][j], col >> 2));
+          const u32x4 b1 = mx4x8_to_bf16x8(vw[h][j + 1], mx_scale(vs[h][j + 1], col >> 2));
+#pragma unroll
+          for (int e = 0; e < 8; e += 2) {
+            v[e][2 * h + (j >> 1)] = pack_lo16(b0[e >> 1], b1[e >> 1]);
+            v[e + 1][2 * h + (j >> 1)] = pack_hi16(b0[e >> 1], b1[e >> 1]);
+          }
+        }
     }
     int t0[H];
     bool full = true;
@@ -521,7 +549,7 @@ __global__ __launch_bounds__(kRowWaves * 64, 2) void window_rows_kernel(WindowAr
         for (int h = 0; h < H; ++h)
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const int tok = t0[h] + 4 * quad + j;
+            const int tok = t0[h] + (KV == kMx4 ? 4 * j + quad : 4 * quad + j);
             s[x][h][j] =
                 tok < end_col[x] && (tok >= beg_col[x] || tok < a.sinks) ? s[x][h][j] : -INFINITY;
           }
@@ -566,11 +594,19 @@ __global__ __launch_bounds__(kRowWaves * 64, 2) void window_rows_kernel(WindowAr
         l_run[x] += x0 + x1;
       }
     }
-    if constexpr (FP8) {
+    if constexpr (KV == kBf16) {
+      // high parts and residuals in the two halves of the contraction
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+#pragma unroll
+        for (int x = 0; x < CT; ++x)
+          acc[x][e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+              as_bf16x8(v[e]), as_bf16x8(ph[x][0], ph[x][1], pl[x][0], pl[x][1]), acc[x][e], 0, 0, 0);
+    } else {
       bf16x8 w[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        w[e] = as_bf16x8(fp8x8_to_bf16x8(v[e]));
+        w[e] = as_bf16x8(FP8 ? fp8x8_to_bf16x8(u32x2{v[e][0], v[e][1]}) : v[e]);
 #pragma unroll
         for (int x = 0; x < CT; ++x)
           acc[x][e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
@@ -582,84 +618,67 @@ __global__ __launch_bounds__(kRowWaves * 64, 2) void window_rows_kernel(WindowAr
         for (int x = 0; x < CT; ++x)
           acc[x][e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
               w[e], as_bf16x8(pl[x][0], pl[x][1], pl[x][2], pl[x][3]), acc[x][e], 0, 0, 0);
-    } else {
-      // high parts and residuals in the two halves of the contraction
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const bf16x8 w = as_bf16x8(v[e][0], v[e][1], v[e][0], v[e][1]);
-#pragma unroll
-        for (int x = 0; x < CT; ++x)
-          acc[x][e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-              w, as_bf16x8(ph[x][0], ph[x][1], pl[x][0], pl[x][1]), acc[x][e], 0, 0, 0);
-      }
     }
   };
 
   const uint32_t ring_at =
       (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)sm.slots[wave];
-  uint8_t *const slots = sm.slots[wave];
   bool bad = false;
   for (int i0 = 0; i0 == 0 || i0 < n; i0 += kPlaced) {
     const int c = min(kPlaced, n - i0);
     if (c > 0) locate(i0);
-    if constexpr (KV == kMx4) {
-      // registers of kAhead steps in flight
-      MxStage st[kAhead];
+    // (queries and index words have arrived: no wait of the compiler's in the walk)
 #pragma unroll
-      for (int u = 0; u < kAhead; ++u)
-        if (c > 0) fetch(min(u, c - 1), st[u]);
-      if (i0 == 0) bad = bad_pages(a, t, tid, W * 64);
-      for (int i = 0; i < c; i += kAhead) {
+    for (int x = 0; x < CT; ++x)
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u) {
-          if (u > 0 && i + u >= c) break;
-          wave_lds_fence();  // the slot's reads of the step before
-          const int g = (lane >> 2) & 3;
-          put_mx<Pipe, false>(slots + g * Pipe::kKGroup, lane, st[u].k, st[u].ks);
-          put_mx<Pipe, true>(slots + Slot::kVShift + Pipe::v_group(g), lane, st[u].v, st[u].vs);
-          fetch(min(i + u + kAhead, c - 1), st[u]);
-          wave_lds_fence();
-          process(i + u, slots);
-        }
+      for (int y = 0; y < 4; ++y) asm volatile("" : "+v"(pw.qf[x][y]));
+    asm volatile("" : "+v"(at_lo), "+v"(at_hi), "+v"(sc_lo), "+v"(sc_hi), "+v"(meta));
+    wait_reads();
+#pragma unroll
+    for (int i = 0; i < Slot::kSlots; ++i)
+      if (i < c) issue(i, ring_at + (uint32_t)(i * Slot::kBytes));
+    if (i0 == 0) {
+      bad = bad_pages(a, t, tid, W * 64);
+      asm volatile("" ::"s"(__builtin_amdgcn_ballot_w64(bad)));
+    }
+    int at = 0;  // the step's slot
+    for (int i = 0; i < c; ++i) {
+      // step i has arrived once at most the loads of those behind it are outstanding
+      if (i + Slot::kSlots <= c)
+        wait_loads<(Slot::kSlots - 1) * Slot::kLoads>();
+      else if (Slot::kSlots > 2 && i + 2 == c)
+        wait_loads<Slot::kLoads>();
+      else
+        wait_loads<0>();
+      process(i, slots + at);
+      if (i + Slot::kSlots < c) {
+        wait_reads();
+        issue(i + Slot::kSlots, ring_at + (uint32_t)at);
       }
-    } else {
-      // (queries and index words have arrived: no wait of the compiler's in the walk)
-#pragma unroll
-      for (int x = 0; x < CT; ++x)
-#pragma unroll
-        for (int c2 = 0; c2 < 4; ++c2) asm volatile("" : "+v"(pw.qf[x][c2]));
-      asm volatile("" : "+v"(at_lo), "+v"(at_hi), "+v"(meta));
-      wait_reads();
-      if (c > 0) issue(0, ring_at);
-      if (c > 1) issue(1, ring_at + (uint32_t)Slot::kBytes);
-      if (i0 == 0) {
-        bad = bad_pages(a, t, tid, W * 64);
-        asm volatile("" ::"s"(__builtin_amdgcn_ballot_w64(bad)));
-      }
-      for (int i = 0; i < c; ++i) {
-        if (i + 1 < c)
-          wait_loads<kStepLoads>();
-        else
-          wait_loads<0>();
-        process(i, slots + (i & 1) * Slot::kBytes);
-        if (i + 2 < c) {
-          wait_reads();
-          issue(i + 2, ring_at + (uint32_t)((i & 1) * Slot::kBytes));
-        }
-      }
+      at = at + Slot::kBytes == Slot::kSlots * Slot::kBytes ? 0 : at + Slot::kBytes;
     }
   }
 
   // The wave's columns to its slot.  acc[x][e][j] = O[column of the x-th 16][16 e + 4 quad + j]
+  // (MXFP4: [32 quad + 8 j + e])
   wait_reads();
   wave_lds_fence();
   float *const stash = reinterpret_cast<float *>(sm.slots[wave]);
 #pragma unroll
   for (int x = 0; x < CT; ++x) {
     const float l_col = quad_sum(l_run[x]);
+    float *const o = stash + (16 * x + col) * kStash;
+    if constexpr (KV == kMx4) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      *reinterpret_cast<f32x4 *>(stash + (16 * x + col) * kStash + 16 * e + 4 * quad) = acc[x][e];
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int e = 0; e < 8; e += 4)
+          *reinterpret_cast<f32x4 *>(o + 32 * quad + 8 * j + e) =
+              f32x4{acc[x][e][j], acc[x][e + 1][j], acc[x][e + 2][j], acc[x][e + 3][j]};
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) *reinterpret_cast<f32x4 *>(o + 16 * e + 4 * quad) = acc[x][e];
+    }
     if (quad == 0) {
       sm.m[wave][16 * x + col] = m_run[x];
       sm.l[wave][16 * x + col] = l_col;
@@ -780,6 +799,29 @@ __global__ __launch_bounds__(kRowWaves * 64, 2) void window_rows_kernel(WindowAr
 }
 
 // ---- long tiles --------------------------------------------------------------------
+// MXFP4 rows on their way to LDS as BF16 (lane l takes 32 values, block l & 3 of
+// row mx_row(l) of a 16-row block, and the row's scale word).
+// In this order of rows the 16 lanes that LDS writes at once meet each bank once: their
+// rows lie in four groups, 16 bytes further each in K, 32 in V (where lanes of the last two
+// groups write neighbouring units in turn).  With rows in order they shared a quarter of
+// the banks, and the writes took 257 cycles of a step's 310 in LDS.
+__device__ __forceinline__ int mx_row(int lane) { return 4 * ((lane >> 2) & 3) + (lane >> 4); }
+// A lane's 32 values to a slot as BF16; `group`: where the row's group (mx_row / 4) lies.
+template <class Pipe, bool V>
+__device__ __forceinline__ void put_mx(uint8_t *group, int lane, const u32x4 &w, uint32_t scales) {
+  const int b = lane & 3, r3 = lane >> 4;
+  const bool turn = V && (lane & 8);
+  uint8_t *const dst = group + r3 * 256 + ((4 * b) ^ Pipe::swizzle(r3)) * 16;
+  uint8_t *const even = dst + (turn ? 16 : 0), *const odd = dst + (turn ? 0 : 16);
+  const uint32_t scale = mx_scale(scales, b);
+#pragma unroll
+  for (int u = 0; u < 4; u += 2) {
+    const uint32_t x = turn ? w[u + 1] : w[u], y = turn ? w[u] : w[u + 1];
+    *reinterpret_cast<u32x4 *>(even + 16 * u) = mx4x8_to_bf16x8(x, scale);
+    *reinterpret_cast<u32x4 *>(odd + 16 * u) = mx4x8_to_bf16x8(y, scale);
+  }
+}
+
 // Many rows: the pipelined long tiles of paged prefill (PipeWave: 32 columns per wave, NW
 // waves over 32 * NW columns, G = W / NW groups of them that split the walk) over the
 // blocks of the walk, in 32-token steps of two blocks each.  Two steps at most at either end of
