@@ -349,8 +349,10 @@ constexpr float kHeadroomLog2 = 12.0f, kNearRefresh = 0.0625f;
 // HL: P enters the product as a BF16 high part and a BF16 residual (two MFMAs
 // per block of V), so the weights carry 16 significant bits and the
 // normalizer sums them in FP32.  Otherwise P is rounded once to BF16 and the
-// normalizer sums the rounded weights.
-template <int NW, bool FP8, bool HL, int G>
+// normalizer sums the rounded weights, or (XS) the weights before their rounding.  The
+// former keeps a weight that stands alone out of O's error, the latter all roundings out of
+// LSE's.
+template <int NW, bool FP8, bool HL, int G, bool XS = false>
 struct PipeWave {
   const PrefillArgs &a;
   int lane, col, quad;
@@ -505,6 +507,10 @@ struct PipeWave {
     } else {
       const uint32_t w = bf16x2_pack(x0, x1);
       p.hi[y >> 2][y & 3] = w;
+      if constexpr (XS) {
+        l += x0 + x1;
+        return;
+      }
       typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
       l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w),
                                           __builtin_bit_cast(bf16x2, 0x3F803F80u), l, false);

@@ -826,8 +826,11 @@ __device__ __forceinline__ void put_mx(uint8_t *group, int lane, const u32x4 &w,
 // waves over 32 * NW columns, G = W / NW groups of them that split the walk) over the
 // blocks of the walk, in 32-token steps of two blocks each.  Two steps at most at either end of
 // the window, and the sinks', hide tokens from some columns and are masked; the steps
-// between take PipeWave's unmasked path.  P is rounded once to BF16, and the normalizer sums
-// the rounded weights: the errors of many tokens average out below O's own rounding.
+// between take PipeWave's unmasked path.  P is rounded once to BF16 for the product: the errors
+// of many tokens average out below O's own rounding, and a token that stands alone, whose
+// score the column's reference was taken from, weighs a power of two.  The normalizer sums
+// the weights before their rounding, so LSE keeps FP32's precision.  (Two sums, one for each,
+// take 5 to 20% of the time: registers spill.)
 //
 // BF16 and FP8 blocks are loaded straight into the ring, NW slots deep.  MXFP4 codes go
 // through registers, 32 values and their scale per lane and block, two steps ahead, and are
@@ -848,7 +851,7 @@ __global__ __launch_bounds__(W * 64, 2) void window_long_kernel(WindowArgs args)
   constexpr int G = W / NW, TC = 32 * NW;
   constexpr int kOutRow = 256 + 16;  // bytes of a row of O in LDS
   constexpr bool FP8 = KV == kFp8, MX = KV == kMx4;
-  using Pipe = PipeWave<NW, FP8, false, G>;
+  using Pipe = PipeWave<NW, FP8, false, G, true>;
   constexpr int kSlot = Pipe::kSlotBytes, kSlots = MX ? 2 : Pipe::kSlots;
   constexpr int kRingBytes = G * kSlots * kSlot;
   constexpr int kMergeBytes = G > 1 ? W * 64 * 64 * 4 : 0;
