@@ -37,6 +37,7 @@ struct WindowArgs : PrefillArgs {
   int32_t head_tiles;   // one-row form: tiles per request
   uint32_t group_inv;   // 2^32 / group, rounded up, where that divides every column; 0: it does not
   uint32_t *arrived;    // splits: arrival words, loom::kMx4JoinBytes apart
+  int32_t sorted;       // tiles of the longest walks first (up to 64 requests)
   // Row tiles over MXFP4 pages with an even number of kv-heads: the workgroups of the command,
   // and its blocks are dealt so that two neighbouring heads, whose rows or scales share
   // cache lines, run on one XCD; 0: in order.
@@ -69,13 +70,14 @@ struct Tile {
   }
 };
 
-// The tile of this workgroup among those of up to 64 requests, the request of the longest
-// walks first and a request's last rows first: the launch does not end with a few long
-// walks alone (four chunks of 512 rows behind 2048-16384 tokens, the longest listed first
-// and so dispatched last: 481 us without the order).  Every wave holds the table, a request
-// per lane.  Rows belong to the requests before the first falling qo_indptr range.
+// The tile of this workgroup among those of up to 64 requests: every wave holds the table, a
+// request per lane.  Rows belong to the requests before the first falling qo_indptr range.
+// A request's last rows come first, and (`sorted`) the request of the longest walks: the
+// launch does not end with a few long walks alone (four chunks of 512 rows behind
+// 2048-16384 tokens, the longest listed first and so dispatched last: 481 us without the
+// order, 440 with it).  A grid of a workgroup per CU needs no order.
 template <int TC>
-__device__ __forceinline__ bool locate_longest_first(const WindowArgs &a, TileLoc &l, int split,
+__device__ __forceinline__ bool locate_lanes(const WindowArgs &a, TileLoc &l, int split,
                                                      uint32_t block) {
   const int lane = threadIdx.x & 63;
   const bool in = lane < a.batch;
@@ -93,16 +95,19 @@ __device__ __forceinline__ bool locate_longest_first(const WindowArgs &a, TileLo
   const int valid = falls ? __builtin_ctzll(falls) : a.batch;
   // (columns fit 31 bits: the plan checks it)
   const uint32_t cnt = lane < valid ? ((uint32_t)(s1 - s0) * (uint32_t)a.group + TC - 1) / TC : 0u;
-  // place among the requests, by tokens that the last row sees (pages, beyond the window)
-  const int64_t key = in ? min((int64_t)p1 - p0, (int64_t)(a.window / a.page_rows) + 1) : -1;
-  const int k32 = (int)max<int64_t>(-1, key);
-  int place = 0;
-  for (int r = 0; r < a.batch; ++r) {
-    const int other = __builtin_amdgcn_readlane(k32, r);
-    place += other > k32 || (other == k32 && r < lane) ? 1 : 0;
+  int place = lane;
+  uint32_t ordered = cnt;
+  if (a.sorted) {
+    // place among the requests, by pages that the last row sees (up to 2^24), no two alike
+    const int pages = max(0, min(min(p1 - p0, a.window / a.page_rows + 1), 1 << 24));
+    if (__builtin_amdgcn_ballot_w64(in && pages != __builtin_amdgcn_readfirstlane(pages))) {
+      const int key = in ? pages << 6 | (63 - lane) : -1;
+      if (in) place = 0;
+      for (int r = 0; r < a.batch; ++r) place += in && __builtin_amdgcn_readlane(key, r) > key ? 1 : 0;
+      // counts in that order, one per lane (lanes past the batch: places past it)
+      ordered = (uint32_t)__builtin_amdgcn_ds_permute(place * 4, (int)cnt);
+    }
   }
-  // counts in that order, one per lane (lanes past the batch: places past it)
-  const uint32_t ordered = (uint32_t)__builtin_amdgcn_ds_permute((in ? place : lane) * 4, (int)cnt);
   const uint32_t incl = wave_incl_add_sat_u32(ordered);
   const uint32_t before = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)incl, 0x138, 0xf, 0xf, false);
   const uint64_t who = __builtin_amdgcn_ballot_w64((uint32_t)l.rank >= before && (uint32_t)l.rank < incl);
@@ -131,7 +136,7 @@ __device__ __forceinline__ bool find_tile(const WindowArgs &a, LocateSmem<W> &sm
                                           uint32_t block) {
   TileLoc &l = t.loc;
   if (a.qo) {
-    if (a.batch <= 64 ? !locate_longest_first<TC>(a, l, split, block)
+    if (a.batch <= 64 ? !locate_lanes<TC>(a, l, split, block)
                       : !locate_tile<W, false, TC, false, true>(a, sm, l, split, block))
       return false;
   } else {
@@ -1474,6 +1479,7 @@ loom_status_t loom_window_attention_enqueue(const loom_window_attention_plan_t *
   if (a.pair_heads) workgroups = (workgroups + 15) / 16 * 16;
   const dim3 blocks((unsigned)workgroups), threads(plan->info.block_threads);
   hipStream_t stream = scope->queue->stream;
+  a.sorted = workgroups > (uint64_t)plan->cus;
   const uint64_t bytes = tokens * pg.batch_size * pg.num_kv_heads * 2 * (mx ? 68 : (uint64_t)row);
   const auto kernel = mx    ? kernel_of<kMx4>(*plan, bytes)
                       : fp8 ? kernel_of<kFp8>(*plan, bytes)
