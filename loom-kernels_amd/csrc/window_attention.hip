@@ -276,7 +276,6 @@ __device__ __forceinline__ void exact_column(const WindowArgs &a, const Tile &t,
 // Rows, codes and scales go straight to LDS.  Widened to BF16 on the way, as the long tiles
 // have them, MXFP4 rows cost a wave 360 cycles of LDS per 32 tokens, four times what the
 // codes take (64 single tokens under windows of 4096: 75 us).
-constexpr int kRowWaves = 8;
 constexpr int kStash = 132;  // floats between two columns' O in LDS, and of a split's state
 
 template <Kv KV>
@@ -306,15 +305,15 @@ struct RowSlot {
 // quads then lie in four neighbouring rows.
 __device__ __forceinline__ int mx_token(int c) { return 4 * (c & 3) + (c >> 2); }
 
-template <Kv KV, int CT>
+template <Kv KV, int CT, int W>
 struct RowsSmem {
   using Slot = RowSlot<KV>;
   // a wave's slots, and after its walk its columns' O
   static constexpr int kWaveBytes = (std::max(Slot::kSlots * Slot::kBytes, 16 * CT * kStash * 4) + 15) & ~15;
-  __align__(16) uint8_t slots[kRowWaves][kWaveBytes];
-  LocateSmem<kRowWaves> loc;
-  float m[kRowWaves][16 * CT], l[kRowWaves][16 * CT];
-  uint32_t bad[kRowWaves];
+  __align__(16) uint8_t slots[W][kWaveBytes];
+  LocateSmem<W> loc;
+  float m[W][16 * CT], l[W][16 * CT];
+  uint32_t bad[W];
   uint32_t arrived;
   uint32_t redo;  // columns whose O is not finite
 };
@@ -336,14 +335,14 @@ __device__ __forceinline__ f32x2 load_state(const float *p) {
                                                      __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
 }
 
-template <Kv KV, int CT, bool NT>
-__global__ __launch_bounds__(kRowWaves * 64, 2) void window_rows_kernel(WindowArgs args) {
-  constexpr int W = kRowWaves, TC = 16 * CT;
+template <Kv KV, int CT, int W, bool NT>
+__global__ __launch_bounds__(W * 64, 2) void window_rows_kernel(WindowArgs args) {
+  constexpr int TC = 16 * CT;
   constexpr bool FP8 = KV == kFp8;
   using Pipe = RowPipe<KV>;
   using Slot = RowSlot<KV>;
   constexpr int H = kStepBlocks<KV>, kPlaced = 64 / H;  // steps placed at once
-  __shared__ RowsSmem<KV, CT> sm;
+  __shared__ RowsSmem<KV, CT, W> sm;
   WindowArgs a = args;
   float v_scale = 1.0f;
   if constexpr (FP8) {
@@ -1269,15 +1268,21 @@ int row_splits(uint64_t grid, uint64_t tokens, int cus, bool mx) {
   const uint64_t most = std::min<uint64_t>(kMaxSplits, (uint64_t)cus / std::max<uint64_t>(grid, 1));
   // 16-row blocks per wave
   const uint64_t least = std::max<uint64_t>(1, grid * (mx ? 8 : 16) / (uint64_t)cus);
-  return (int)std::max<uint64_t>(1, std::min(most, blocks / (least * kRowWaves)));
+  return (int)std::max<uint64_t>(1, std::min(most, blocks / (least * 8)));
 }
 
 template <Kv KV>
 auto kernel_of(const loom_window_attention_plan &p, uint64_t bytes) {
-  if (p.info.algorithm != LOOM_PAGED_PREFILL_LONG_TILE)
-    return p.info.tile_cols == 32 ? window_rows_kernel<KV, 2, false>
-           : p.once && bytes >= kPastCaches ? window_rows_kernel<KV, 1, true>
-                                   : window_rows_kernel<KV, 1, false>;
+  if (p.info.algorithm != LOOM_PAGED_PREFILL_LONG_TILE) {
+    const bool past = p.once && bytes >= kPastCaches;
+    if (p.info.block_threads == 256)
+      return p.info.tile_cols == 32 ? window_rows_kernel<KV, 2, 4, false>
+             : past                 ? window_rows_kernel<KV, 1, 4, true>
+                                    : window_rows_kernel<KV, 1, 4, false>;
+    return p.info.tile_cols == 32 ? window_rows_kernel<KV, 2, 8, false>
+           : past                 ? window_rows_kernel<KV, 1, 8, true>
+                                  : window_rows_kernel<KV, 1, 8, false>;
+  }
   if (p.info.tile_cols == 128) return p.groups == 2 ? window_long_kernel<KV, 8, 4> : window_long_kernel<KV, 4, 4>;
   return p.groups == 4 ? window_long_kernel<KV, 8, 2> : window_long_kernel<KV, 4, 2>;
 }
@@ -1315,7 +1320,7 @@ loom_status_t make_plan(const loom::DeviceInfo &dev, const loom_window_attention
                                                       : 64;
   const uint64_t tiles = tiles_of(tc), grid = tiles * hkv;
   const uint32_t groups = long_tile ? long_groups(tc, cols * hkv / 128, grid, cus, s.window == 0) : 1;
-  const uint32_t waves = !long_tile ? kRowWaves : (uint32_t)tc / 32 * groups;
+  const uint32_t waves = !long_tile ? (grid > cus ? 4 : 8) : (uint32_t)tc / 32 * groups;
   if (grid * (waves * 64) >= (1ull << 32))
     return fail(err, LOOM_PLAN_STATE_COUNT_OUT_OF_RANGE, "window rows", s.rows);
   auto *p = new loom_window_attention_plan;
