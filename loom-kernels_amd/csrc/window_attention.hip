@@ -297,7 +297,6 @@ struct RowSlot {
   static constexpr int kBytes = KV == kMx4   ? kMxVs + 128
                                 : KV == kFp8 ? Pipe::kSlotBytes
                                              : kGroups * (Pipe::kKGroup + Pipe::kVGroup);
-  static constexpr int kSlots = KV == kMx4 ? 3 : 2;
   static constexpr int kLoads = KV == kMx4 ? 8 : 2 * kGroups;  // instructions of a step
 };
 // MXFP4: the row of a block that row c of the MFMA tile S = K.Q^T stands for.  S leaves lane
@@ -309,7 +308,7 @@ template <Kv KV, int CT, int W>
 struct RowsSmem {
   using Slot = RowSlot<KV>;
   // a wave's slots, and after its walk its columns' O
-  static constexpr int kWaveBytes = (std::max(Slot::kSlots * Slot::kBytes, 16 * CT * kStash * 4) + 15) & ~15;
+  static constexpr int kWaveBytes = (std::max(2 * Slot::kBytes, 16 * CT * kStash * 4) + 15) & ~15;
   __align__(16) uint8_t slots[W][kWaveBytes];
   LocateSmem<W> loc;
   float m[W][16 * CT], l[W][16 * CT];
@@ -336,7 +335,7 @@ __device__ __forceinline__ f32x2 load_state(const float *p) {
 }
 
 template <Kv KV, int CT, int W, bool NT>
-__global__ __launch_bounds__(W * 64, 2) void window_rows_kernel(WindowArgs args) {
+__global__ __launch_bounds__(W * 64, KV == kMx4 && CT == 1 && W == 4 ? 4 : 2) void window_rows_kernel(WindowArgs args) {
   constexpr int TC = 16 * CT;
   constexpr bool FP8 = KV == kFp8;
   using Pipe = RowPipe<KV>;
@@ -638,28 +637,24 @@ __global__ __launch_bounds__(W * 64, 2) void window_rows_kernel(WindowArgs args)
       for (int y = 0; y < 4; ++y) asm volatile("" : "+v"(pw.qf[x][y]));
     asm volatile("" : "+v"(at_lo), "+v"(at_hi), "+v"(sc_lo), "+v"(sc_hi), "+v"(meta));
     wait_reads();
-#pragma unroll
-    for (int i = 0; i < Slot::kSlots; ++i)
-      if (i < c) issue(i, ring_at + (uint32_t)(i * Slot::kBytes));
+    if (c > 0) issue(0, ring_at);
+    if (c > 1) issue(1, ring_at + (uint32_t)Slot::kBytes);
     if (i0 == 0) {
       bad = bad_pages(a, t, tid, W * 64);
       asm volatile("" ::"s"(__builtin_amdgcn_ballot_w64(bad)));
     }
-    int at = 0;  // the step's slot
     for (int i = 0; i < c; ++i) {
-      // step i has arrived once at most the loads of those behind it are outstanding
-      if (i + Slot::kSlots <= c)
-        wait_loads<(Slot::kSlots - 1) * Slot::kLoads>();
-      else if (Slot::kSlots > 2 && i + 2 == c)
+      // (of the loads, at most the next step's outstanding)
+      if (i + 1 < c)
         wait_loads<Slot::kLoads>();
       else
         wait_loads<0>();
+      const int at = (i & 1) * Slot::kBytes;
       process(i, slots + at);
-      if (i + Slot::kSlots < c) {
+      if (i + 2 < c) {
         wait_reads();
-        issue(i + Slot::kSlots, ring_at + (uint32_t)at);
+        issue(i + 2, ring_at + (uint32_t)at);
       }
-      at = at + Slot::kBytes == Slot::kSlots * Slot::kBytes ? 0 : at + Slot::kBytes;
     }
   }
 
@@ -1260,6 +1255,15 @@ uint32_t long_groups(uint64_t tile_cols, uint64_t tiles, uint64_t grid, uint64_t
   return grid <= cus ? 4 : 2;
 }
 
+// Waves of a row-tile workgroup: four where its walks do not wait for the CU, whose two to
+// four workgroups then begin and end beside each other's streams (128 single tokens under
+// windows of 128 26.2 -> 18.7 us, FP8 21.7 -> 15.6, MXFP4 21.4 -> 10.4; of 4096 337 / 335,
+// 194 / 189, 139 / 148); but with hardly more workgroups than CUs a long walk has eight (8
+// chunks of 1-32 rows, MXFP4, the whole prefixes of 300-5000 tokens: 31 / 41).
+uint32_t row_waves(uint64_t grid, uint64_t cus, uint64_t window) {
+  return grid >= 2 * cus || (grid > cus && window > 0 && window <= 2048) ? 4 : 8;
+}
+
 // Workgroups per (tile, kv-head) of a row-tile command of `grid` unsplit ones, whose walks
 // hold about `tokens` tokens: at most one per CU, and each with work for its join (2 us):
 // the more CUs stream already, the less another one adds.
@@ -1320,7 +1324,7 @@ loom_status_t make_plan(const loom::DeviceInfo &dev, const loom_window_attention
                                                       : 64;
   const uint64_t tiles = tiles_of(tc), grid = tiles * hkv;
   const uint32_t groups = long_tile ? long_groups(tc, cols * hkv / 128, grid, cus, s.window == 0) : 1;
-  const uint32_t waves = !long_tile ? (grid > cus ? 4 : 8) : (uint32_t)tc / 32 * groups;
+  const uint32_t waves = !long_tile ? row_waves(grid, cus, s.window) : (uint32_t)tc / 32 * groups;
   if (grid * (waves * 64) >= (1ull << 32))
     return fail(err, LOOM_PLAN_STATE_COUNT_OUT_OF_RANGE, "window rows", s.rows);
   auto *p = new loom_window_attention_plan;
