@@ -1218,6 +1218,7 @@ struct loom_window_attention_plan {
   int cus = 0;
   uint32_t groups = 1;  // long tiles: wave groups that split a walk
   bool once = false;    // row tiles: a request has one tile per kv-head, as a rule
+  uint64_t least_tiles = 0;  // that the command holds if no request's last one is in part empty
 };
 
 // Bytes of a command's rows from which they are loaded past the caches, where each is
@@ -1230,6 +1231,7 @@ namespace {
 
 constexpr uint64_t kMaxHeads = 4096;  // kv-heads: a row of all of them in a 32-bit stride
 constexpr int kMaxSplits = 16;
+constexpr uint64_t kLongWalk = 2048;  // tokens, from which a join costs little
 
 // Columns per workgroup, from the number of row tiles of 16 that the command holds (a
 // request's last one is about half full).  Microseconds, 16 / 32 / long, rows behind 5000
@@ -1264,12 +1266,15 @@ uint32_t row_waves(uint64_t grid, uint64_t cus, uint64_t window) {
   return grid >= 2 * cus || (grid > cus && window > 0 && window <= 2048) ? 4 : 8;
 }
 
-// Workgroups per (tile, kv-head) of a row-tile command of `grid` unsplit ones, whose walks
-// hold about `tokens` tokens: at most one per CU, and each with work for its join (2 us):
-// the more CUs stream already, the less another one adds.
-int row_splits(uint64_t grid, uint64_t tokens, int cus, bool mx) {
+// Workgroups per (tile, kv-head) of a row-tile command of `grid` unsplit ones (`least_grid` at
+// least), whose walks hold about `tokens` tokens: at most one per CU, and each with work for
+// its join (2 us): the more CUs stream already, the less another one adds.  (8 x 8 rows, 128
+// tiles of a grid of 192, over whole prefixes of 2500-5000 tokens 55 -> 37 us, FP8 26.6 ->
+// 20.5.)
+int row_splits(uint64_t grid, uint64_t least_grid, uint64_t tokens, int cus, bool mx) {
   const uint64_t blocks = (tokens + 15) / 16;
-  const uint64_t most = std::min<uint64_t>(kMaxSplits, (uint64_t)cus / std::max<uint64_t>(grid, 1));
+  const uint64_t most = std::min<uint64_t>(
+      kMaxSplits, (uint64_t)cus / std::max<uint64_t>(tokens >= kLongWalk ? least_grid : grid, 1));
   // 16-row blocks per wave
   const uint64_t least = std::max<uint64_t>(1, grid * (mx ? 8 : 16) / (uint64_t)cus);
   return (int)std::max<uint64_t>(1, std::min(most, blocks / (least * 8)));
@@ -1338,6 +1343,7 @@ loom_status_t make_plan(const loom::DeviceInfo &dev, const loom_window_attention
   p->cus = dev.cus;
   p->groups = groups;
   p->once = group_cols <= tc;
+  p->least_tiles = s.explicit_rows ? std::min(tiles, std::max(batch, (cols + tc - 1) / tc)) : tiles;
   *out = p;
   return loom::ok(err);
 }
@@ -1477,7 +1483,7 @@ loom_status_t loom_window_attention_enqueue(const loom_window_attention_plan_t *
                          (uint64_t)a.n_indices * page_rows / pg.batch_size);
   const uint64_t grid = plan->info.grid_blocks;
   const bool long_tile = plan->info.algorithm == LOOM_PAGED_PREFILL_LONG_TILE;
-  a.splits = long_tile ? 1 : row_splits(grid, tokens, plan->cus, mx);
+  a.splits = long_tile ? 1 : row_splits(grid, plan->least_tiles * pg.num_kv_heads, tokens, plan->cus, mx);
   if (a.splits > 1) {
     a.arrived = scope->queue->joins;
     a.states = (float *)loom::queue_shares(scope, (uint64_t)a.splits * grid * plan->info.tile_cols * kStash * 4);
