@@ -769,13 +769,14 @@ __global__ __launch_bounds__(W * 64, KV == kMx4 && CT == 1 && W == 4 ? 4 : 2) vo
       ls[y] = L;
     }
   }
-  // Columns that are not finite are found token by token.
+  // Columns that are not finite are found token by token.  (The normalizer alone overflows
+  // where a negative FP8 scale makes a reference of the lowest scores and V is zero.)
 #pragma unroll
   for (int y = 0; y < kItems; ++y) {
     const int c = (y * W * 64 + tid) >> 5;
     const float inv = 1.0f / ls[y] * v_scale;
     o[y] *= inv;
-    bool finite = true;
+    bool finite = ls[y] < INFINITY;
 #pragma unroll
     for (int e = 0; e < 4; ++e) finite &= fabsf(o[y][e]) < INFINITY;
     if (c < cols && !finite) atomicOr(&sm.redo, 1u << c);
@@ -1169,7 +1170,7 @@ __global__ __launch_bounds__(W * 64, 2) void window_long_kernel(WindowArgs args)
 #pragma unroll
         for (int i = 0; i < 4; ++i) z = fmaf(lw.acc[c][e][i], 0.0f, z);  // NaN: not finite
       }
-    const uint64_t b = __builtin_amdgcn_ballot_w64(colv_t[c] && !(z == 0.0f));
+    const uint64_t b = __builtin_amdgcn_ballot_w64(colv_t[c] && !(z == 0.0f && L[c] < INFINITY));
     redo |= (uint32_t)((b | b >> 16 | b >> 32 | b >> 48) & 0xffff) << (16 * c);
   }
   if constexpr (G > 1) {
@@ -1229,6 +1230,7 @@ constexpr uint64_t kPastCaches = 96ull << 20;
 
 namespace {
 
+constexpr float kLog2e = 1.44269504088896340736f;
 constexpr uint64_t kMaxHeads = 4096;  // kv-heads: a row of all of them in a 32-bit stride
 constexpr int kMaxSplits = 16;
 constexpr uint64_t kLongWalk = 2048;  // tokens, from which a join costs little
@@ -1304,7 +1306,7 @@ loom_status_t make_plan(const loom::DeviceInfo &dev, const loom_window_attention
                                      spec->sinks, &s, err);
   if (rc) return rc;
   const float scale = s.paged.softmax_scale;
-  if (!(scale > 0.0f) || !std::isfinite(scale))
+  if (!(scale > 0.0f) || !std::isfinite(scale * kLog2e))
     return fail(err, LOOM_PLAN_INVALID_OPTION, "softmax_scale");
   const uint64_t hq = s.paged.num_query_heads, hkv = s.paged.num_kv_heads, group = hq / hkv;
   const uint64_t batch = s.paged.batch_size;
@@ -1462,7 +1464,7 @@ loom_status_t loom_window_attention_enqueue(const loom_window_attention_plan_t *
   a.group = a.hq / a.hkv;
   a.pool = (int64_t)pg.max_num_pages;
   a.n_indices = (int64_t)l[4]->numel;
-  a.scale_log2 = pg.softmax_scale * 1.44269504088896340736f;
+  a.scale_log2 = pg.softmax_scale * kLog2e;
   a.indices_capacity = (plan->info.flags & LOOM_PLAN_PAGE_INDICES_CAPACITY) ? 1 : 0;
   a.page_rows = (int32_t)page_rows;
   a.blocks_lg = page_rows == 64 ? 2 : page_rows == 32 ? 1 : 0;

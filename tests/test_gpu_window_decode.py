@@ -138,6 +138,32 @@ def test_fp8_scales_that_do_not_keep_the_order(env, scale):
         window_util.K_SCALE = saved
 
 
+@pytest.mark.parametrize("rows", [None, [1]])
+def test_a_normalizer_past_fp32(env, rows):
+    """A negative k_scale: weights near FP32's end against the lowest score, whose sum passes
+    it, over V of zeros."""
+    torch, L = env
+    import window_util
+    c = Case(19, [30], rows, 1, 1, 0, 0, 16, "NHD", "fp8_e4m3")
+    c.q[:] = 0
+    c.q[..., 0] = 1
+    k, v = c.cache
+    k[:] = v[:] = 0
+    k[c.indices[0], 0, 0, 0] = 0x50  # 8.0, the other rows' is 0
+    scale = np.float32(-127.5 / 8 * np.log(2) * np.sqrt(128))
+    d = c.operands(torch)
+    d["kv_scales"][0] = float(scale)
+    saved, window_util.K_SCALE = window_util.K_SCALE, scale
+    try:
+        assert window_util.fp8_values()[0x50] == 8.0
+        assert abs(c.reference()[1][0, 0] - np.log2(29)) < 1e-6
+        for tile in (0,) if rows is None else (16, "long"):
+            c.check(*c.run(torch, L, d, **({} if rows is None else dict(tile_cols=tile))),
+                    long_tile=tile == "long")
+    finally:
+        window_util.K_SCALE = saved
+
+
 def test_scores_far_apart(env):
     """Scores of thousands: one token takes the whole weight."""
     c = Case(12, [300, 45], None, 4, 2, 200, 4, 16, "NHD", "bf16")

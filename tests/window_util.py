@@ -89,8 +89,11 @@ class Case:
                         top = s.max(1, keepdims=True)
                         w = np.exp(s - top)
                         total = w.sum(1, keepdims=True)
-                        o[at:at + m, g] = np.stack([
-                            (w[i, w[i] != 0] / total[i]) @ v[w[i] != 0] for i in range(m)])
+                        if np.isfinite(v).all():
+                            o[at:at + m, g] = w / total @ v
+                        else:  # (a weight of zero times an infinity)
+                            o[at:at + m, g] = np.stack([
+                                (w[i, w[i] != 0] / total[i]) @ v[w[i] != 0] for i in range(m)])
                         a[at:at + m, g] = w / total @ np.abs(np.where(np.isfinite(v), v, 0))
                         lse[at:at + m, g] = ((top + np.log(total)) * LOG2E)[:, 0]
                         sa = np.where(seen[:, used], np.abs(q) @ np.abs(k).T, 0)
