@@ -172,18 +172,28 @@ __device__ __forceinline__ bool find_tile(const WindowArgs &a, LocateSmem<W> &sm
   return true;
 }
 
-// Whether a page index of a token that some row of the request sees is out of range: this
-// thread's share of `threads`.  (The same for every tile of the request.)
-__device__ __forceinline__ bool bad_pages(const WindowArgs &a, const Tile &t, int tid, int threads) {
-  const int lg = a.blocks_lg + 4;
-  const int first = max(0, t.kv_len - t.group_rows + 1 - a.window) >> lg;
-  const int sinks = min((int)(((uint32_t)a.sinks + (1u << lg) - 1) >> lg), first);
-  const int n = sinks + (t.loc.pe - t.loc.ps) - first;
-  bool bad = false;
-  for (int i = tid; i < n; i += threads) {
-    const int32_t x = a.indices[t.loc.ps + (i < sinks ? i : i - sinks + first)];
-    bad |= x < 0 || (int64_t)x >= a.pool;
+// The page indices of tokens that some row of the request sees, in order.  (The same for
+// every tile of the request.)
+struct Pages {
+  int first, sinks, n;  // first page of the windows, the sinks' pages, all of them
+  __device__ __forceinline__ Pages(const WindowArgs &a, const Tile &t) {
+    const int lg = a.blocks_lg + 4;
+    first = max(0, t.kv_len - t.group_rows + 1 - a.window) >> lg;
+    sinks = min((int)(((uint32_t)a.sinks + (1u << lg) - 1) >> lg), first);
+    n = sinks + (t.loc.pe - t.loc.ps) - first;
   }
+  __device__ __forceinline__ int32_t index(const WindowArgs &a, const Tile &t, int i) const {
+    return a.indices[t.loc.ps + (i < sinks ? i : i - sinks + first)];
+  }
+};
+__device__ __forceinline__ bool bad_page(const WindowArgs &a, int32_t x) {
+  return x < 0 || (int64_t)x >= a.pool;
+}
+// Whether one is out of range: this thread's share, from `i` on, of `threads`.
+__device__ __forceinline__ bool bad_pages(const WindowArgs &a, const Tile &t, int i, int threads) {
+  const Pages p(a, t);
+  bool bad = false;
+  for (; i < p.n; i += threads) bad |= bad_page(a, p.index(a, t, i));
   return bad;
 }
 
@@ -314,7 +324,6 @@ struct RowsSmem {
   float m[W][16 * CT], l[W][16 * CT];
   uint32_t bad[W];
   uint32_t arrived;
-  uint32_t redo;  // columns whose O is not finite
 };
 
 template <int N>
@@ -626,10 +635,15 @@ __global__ __launch_bounds__(W * 64, KV == kMx4 && CT == 1 && W == 4 ? 4 : 2) vo
 
   const uint32_t ring_at =
       (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t *)sm.slots[wave];
+  // The thread's first page index comes with those of the walk, and is looked at before
+  // the first rows are under way: loads return in order.
+  const Pages pages(a, t);
+  const int32_t own_page = tid < pages.n ? pages.index(a, t, tid) : 0;
   bool bad = false;
   for (int i0 = 0; i0 == 0 || i0 < n; i0 += kPlaced) {
     const int c = min(kPlaced, n - i0);
     if (c > 0) locate(i0);
+    if (i0 == 0) bad = bad_page(a, own_page);
     // (queries and index words have arrived: no wait of the compiler's in the walk)
 #pragma unroll
     for (int x = 0; x < CT; ++x)
@@ -639,8 +653,8 @@ __global__ __launch_bounds__(W * 64, KV == kMx4 && CT == 1 && W == 4 ? 4 : 2) vo
     wait_reads();
     if (c > 0) issue(0, ring_at);
     if (c > 1) issue(1, ring_at + (uint32_t)Slot::kBytes);
-    if (i0 == 0) {
-      bad = bad_pages(a, t, tid, W * 64);
+    if (i0 == 0 && pages.n > W * 64) {
+      bad |= bad_pages(a, t, tid + W * 64, W * 64);
       asm volatile("" ::"s"(__builtin_amdgcn_ballot_w64(bad)));
     }
     for (int i = 0; i < c; ++i) {
@@ -683,7 +697,6 @@ __global__ __launch_bounds__(W * 64, KV == kMx4 && CT == 1 && W == 4 ? 4 : 2) vo
       sm.l[wave][16 * x + col] = l_col;
     }
   }
-  if (tid == 0) sm.redo = 0;
   if (block_or(bad, sm.bad)) return;
   const int cols = min(TC, t.fcols - t.col0);
   constexpr int kItems = TC * 32 / (W * 64);  // 4 dims of a column each
@@ -773,29 +786,25 @@ __global__ __launch_bounds__(W * 64, KV == kMx4 && CT == 1 && W == 4 ? 4 : 2) vo
   // where a negative FP8 scale makes a reference of the lowest scores and V is zero.)
 #pragma unroll
   for (int y = 0; y < kItems; ++y) {
-    const int c = (y * W * 64 + tid) >> 5;
-    const float inv = 1.0f / ls[y] * v_scale;
-    o[y] *= inv;
+    const int c0 = 2 * (y * W + wave);  // the wave's two columns
+    const int c = c0 + (lane >> 5), d = (lane & 31) * 4;
+    o[y] *= 1.0f / ls[y] * v_scale;
     bool finite = ls[y] < INFINITY;
 #pragma unroll
     for (int e = 0; e < 4; ++e) finite &= fabsf(o[y][e]) < INFINITY;
-    if (c < cols && !finite) atomicOr(&sm.redo, 1u << c);
+    const uint64_t redo = __builtin_amdgcn_ballot_w64(c < cols && !finite);
+    const bool mine = (lane < 32 ? (uint32_t)redo : (uint32_t)(redo >> 32)) == 0;
+    if (c < cols && mine) {
+      const int fc = t.col0 + c, rc = row_of(a, fc);
+      const int64_t row = (int64_t)(t.loc.qs + rc) * a.hq + (int64_t)kvh * a.group + (fc - rc * a.group);
+      *reinterpret_cast<u32x2 *>(a.out + row * 128 + d) =
+          u32x2{bf16x2_pack(o[y][0], o[y][1]), bf16x2_pack(o[y][2], o[y][3])};
+      if (d == 0) a.lse[row] = ms[y] + __log2f(ls[y]);
+    }
+    if (redo)
+      for (int x = 0; x < 2; ++x)
+        if ((uint32_t)(redo >> (32 * x))) exact_column<KV>(a, t, t.col0 + c0 + x, lane, v_scale);
   }
-  __syncthreads();
-  const uint32_t redo = uni((int)sm.redo);
-#pragma unroll
-  for (int y = 0; y < kItems; ++y) {
-    const int c = (y * W * 64 + tid) >> 5, d = (tid & 31) * 4;
-    if (c >= cols || (redo >> c & 1)) continue;
-    const int fc = t.col0 + c, rc = row_of(a, fc);
-    const int64_t row = (int64_t)(t.loc.qs + rc) * a.hq + (int64_t)kvh * a.group + (fc - rc * a.group);
-    *reinterpret_cast<u32x2 *>(a.out + row * 128 + d) =
-        u32x2{bf16x2_pack(o[y][0], o[y][1]), bf16x2_pack(o[y][2], o[y][3])};
-    if (d == 0) a.lse[row] = ms[y] + __log2f(ls[y]);
-  }
-  if (redo)
-    for (int c = wave; c < cols; c += W)
-      if (redo >> c & 1) exact_column<KV>(a, t, t.col0 + c, lane, v_scale);
 }
 
 // ---- long tiles --------------------------------------------------------------------
