@@ -1272,8 +1272,11 @@ uint32_t long_groups(uint64_t tile_cols, uint64_t tiles, uint64_t grid, uint64_t
 // four workgroups then begin and end beside each other's streams (128 single tokens under
 // windows of 128 26.2 -> 18.7 us, FP8 21.7 -> 15.6, MXFP4 21.4 -> 10.4; of 4096 337 / 335,
 // 194 / 189, 139 / 148); but with hardly more workgroups than CUs a long walk has eight (8
-// chunks of 1-32 rows, MXFP4, the whole prefixes of 300-5000 tokens: 31 / 41).
-uint32_t row_waves(uint64_t grid, uint64_t cus, uint64_t window) {
+// chunks of 1-32 rows, MXFP4, the whole prefixes of 300-5000 tokens: 31 / 41).  Four as well
+// for walks of few steps (`walk` tokens at most, as a rule; 8 x 10 rows under windows of 48
+// 5.4 / 5.1, but 8 single tokens under windows of 200 5.5 / 5.9).
+uint32_t row_waves(uint64_t grid, uint64_t cus, uint64_t window, uint64_t walk) {
+  if (walk <= 112) return 4;
   return grid >= 2 * cus || (grid > cus && window > 0 && window <= 2048) ? 4 : 8;
 }
 
@@ -1339,8 +1342,11 @@ loom_status_t make_plan(const loom::DeviceInfo &dev, const loom_window_attention
                       : (cols / 128) * hkv >= 2 * cus ? 128
                                                       : 64;
   const uint64_t tiles = tiles_of(tc), grid = tiles * hkv;
+  const uint64_t context = s.paged.max_num_pages * (s.paged.page_size ? s.paged.page_size : loom::kPageSize) / batch;
+  const uint64_t seen = s.window && s.window < context ? s.window + s.rows / batch : context;
+  const uint64_t walk = std::min(context, seen + std::min(s.sinks, context));
   const uint32_t groups = long_tile ? long_groups(tc, cols * hkv / 128, grid, cus, s.window == 0) : 1;
-  const uint32_t waves = !long_tile ? row_waves(grid, cus, s.window) : (uint32_t)tc / 32 * groups;
+  const uint32_t waves = !long_tile ? row_waves(grid, cus, s.window, walk) : (uint32_t)tc / 32 * groups;
   if (grid * (waves * 64) >= (1ull << 32))
     return fail(err, LOOM_PLAN_STATE_COUNT_OUT_OF_RANGE, "window rows", s.rows);
   auto *p = new loom_window_attention_plan;

@@ -48,12 +48,13 @@ def tiles(b, n, rows=None, hq=8, hkv=8, window=40):
 
 
 KERNELS = {
-    "16 columns, 8 waves": (*tiles(3, 150), 16, 512),
+    "16 columns, 8 waves": (*tiles(3, 200, window=120), 16, 512),
+    "16 columns, 4 waves, few steps": (*tiles(3, 150), 16, 256),
     "16 columns, 4 waves, windows": (*tiles(40, 90), 16, 256),
     "16 columns, 4 waves, whole": (*tiles(70, 60, window=0), 16, 256),
-    "32 columns, 8 waves": (*tiles(24, 90, 28, window=0), 32, 512),
+    "32 columns, 8 waves": (*tiles(24, 190, 28, window=0), 32, 512),
     "32 columns, 4 waves": (*tiles(33, 70, 21), 32, 256),
-    "one row, 32 columns, 8 waves": (*tiles(200, 40, hq=32, hkv=1), 32, 512),
+    "one row, 32 columns, 8 waves": (*tiles(200, 140, hq=32, hkv=1, window=0), 32, 512),
     "one row, 32 columns, 4 waves": (*tiles(500, 20, hq=32, hkv=1), 32, 256),
     "64 columns, 2 groups": (*tiles(40, 100, 70), 64, 256),
     "64 columns, 4 groups": (*tiles(1, 1500, 1400), 64, 512),
