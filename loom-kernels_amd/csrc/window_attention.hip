@@ -908,6 +908,8 @@ __global__ __launch_bounds__(W * 64, 2) void window_long_kernel(WindowArgs args)
   // The first page indices, then the queries: the first K/V loads wait for the former only.
   const int idx =
       lane < t.blocks ? a.indices[t.loc.ps + (t.block(lane) >> a.blocks_lg)] : 0;
+  const Pages pages(a, t);
+  const int32_t own_page = tid < pages.n ? pages.index(a, t, tid) : 0;
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
     const uint16_t *qp = colv_t[c] ? a.q + ((int64_t)(t.loc.qs + qi_t[c]) * a.hq +
@@ -958,7 +960,8 @@ __global__ __launch_bounds__(W * 64, 2) void window_long_kernel(WindowArgs args)
   // Checked and masked while the first blocks are on their way.
   bool bad = false;
   auto first = [&]() {
-    bad = bad_pages(a, t, tid, W * 64);
+    bad = bad_page(a, own_page);
+    if (pages.n > W * 64) bad |= bad_pages(a, t, tid + W * 64, W * 64);
 #pragma unroll
     for (int c = 0; c < 2; ++c)
 #pragma unroll
@@ -1171,14 +1174,15 @@ __global__ __launch_bounds__(W * 64, 2) void window_long_kernel(WindowArgs args)
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
     const float inv = 1.0f / L[c] * v_scale;
-    float z = 0.0f;
+    f32x4 zs = {};  // NaN: not finite
 #pragma unroll
     for (int e = 0; e < 8; ++e)
       if (e / kOwn == grp) {
         lw.acc[c][e] *= inv;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) z = fmaf(lw.acc[c][e][i], 0.0f, z);  // NaN: not finite
+        for (int i = 0; i < 4; ++i) zs[i] = fmaf(lw.acc[c][e][i], 0.0f, zs[i]);
       }
+    const float z = (zs[0] + zs[1]) + (zs[2] + zs[3]);
     const uint64_t b = __builtin_amdgcn_ballot_w64(colv_t[c] && !(z == 0.0f && L[c] < INFINITY));
     redo |= (uint32_t)((b | b >> 16 | b >> 32 | b >> 48) & 0xffff) << (16 * c);
   }
