@@ -883,17 +883,18 @@ __global__ __launch_bounds__(W * 64, 2) void window_long_kernel(WindowArgs args)
   const int own0 = t.col0 + 32 * wq;
   const int p0 = t.kv_len - t.group_rows;
   Pipe lw{a, lane, col, quad};
-  int beg_col[2], end_col[2], qi_t[2], gh_t[2];
-  bool colv_t[2];
+  // this lane's columns, one of each 16: their causal ends (0: no column)
+  int end_col[2];
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
     const int f = own0 + 16 * c + col;
-    colv_t[c] = f < t.fcols;
-    qi_t[c] = colv_t[c] ? row_of(a, f) : 0;
-    gh_t[c] = colv_t[c] ? f - qi_t[c] * a.group : 0;
-    end_col[c] = colv_t[c] ? p0 + qi_t[c] + 1 : 0;
-    beg_col[c] = max(0, end_col[c] - a.window);
+    end_col[c] = f < t.fcols ? p0 + row_of(a, f) + 1 : 0;
   }
+  // Output row of column f.
+  auto out_row = [&](int f) {
+    const int qi = row_of(a, f);
+    return (t.loc.qs + qi) * a.hq + kvh * a.group + (f - qi * a.group);
+  };
   lw.reset(ring + grp * kSlots * kSlot);
   // Steps that need no mask, [first_full, last_full): whose tokens every column of the
   // wave sees; and the steps up to the wave's last column's own token.
@@ -912,20 +913,18 @@ __global__ __launch_bounds__(W * 64, 2) void window_long_kernel(WindowArgs args)
   const int32_t own_page = tid < pages.n ? pages.index(a, t, tid) : 0;
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
-    const uint16_t *qp = colv_t[c] ? a.q + ((int64_t)(t.loc.qs + qi_t[c]) * a.hq +
-                                            (int64_t)kvh * a.group + gh_t[c]) * 128
-                                   : a.q;
+    const int f = own0 + 16 * c + col;
+    const uint16_t *qp = a.q + (f < t.fcols ? (int64_t)out_row(f) * 128 : 0);
 #pragma unroll
     for (int x = 0; x < 4; ++x) lw.qf[c][x] = load16(qp + Pipe::q_dim(x, quad));
   }
-  // Lane l holds the place of block 64 win + l of the walk in the wave's matrix (K or V):
-  // address of its first row, valid rows' bytes, and (MXFP4) its scales' address.
+  // Lane l holds the place of block 64 win + l of the walk in the wave's matrix (K or V): its
+  // first row's address (48 bits), above it the valid rows, and (MXFP4) the block of scales.
   const bool loads_k = wq < NW / 2;
   const uint64_t kv_base = (uint64_t)(loads_k ? a.k : a.v);
   const uint64_t mx_base = MX ? (uint64_t)(loads_k ? a.k_mx : a.v_mx) : 0;
   int win = -1;
-  uint32_t blk_lo = 0, blk_hi = 0, mx_lo = 0, mx_hi = 0;
-  int blk_rows = 0;
+  uint32_t blk_lo = 0, blk_hi = 0, blk_mx = 0;
   auto place = [&](int b) {
     if ((b >> 5) == win) return;
     win = b >> 5;
@@ -933,26 +932,28 @@ __global__ __launch_bounds__(W * 64, 2) void window_long_kernel(WindowArgs args)
     const int blk = t.block(x);
     int rows = x < t.blocks ? t.rows(a, x) : 0;
     const int pg = win == 0 ? idx : sm.next_idx[wave][lane];
-    if (pg < 0 || (int64_t)pg >= a.pool) rows = 0;  // (the request is refused)
+    if (bad_page(a, pg)) rows = 0;  // (the request is refused)
     const int row = (blk & ((1 << a.blocks_lg) - 1)) * 16;
     const uint64_t at = kv_base + row_at<KV>(a, pg, row, kvh);
     blk_lo = (uint32_t)at;
-    blk_hi = (uint32_t)(at >> 32);
-    blk_rows = rows;
-    if constexpr (MX) {
-      const uint64_t sc = mx_base + scale_at(a, pg, row, kvh);
-      mx_lo = (uint32_t)sc;
-      mx_hi = (uint32_t)(sc >> 32);
-    }
-    asm volatile("" ::"v"(blk_lo), "v"(blk_hi), "v"(blk_rows) : "memory");  // next_idx is read
+    blk_hi = ((uint32_t)(at >> 32) & 0xffffu) | (uint32_t)rows << 16;
+    if constexpr (MX) blk_mx = (uint32_t)(scale_at(a, pg, row, kvh) >> 6);
+    asm volatile("" ::"v"(blk_lo), "v"(blk_hi) : "memory");  // next_idx is read
     // (past the walk's end: past the buffer's, or of no use)
     lds_load4(__builtin_amdgcn_make_buffer_rsrc(const_cast<int32_t *>(a.indices + t.loc.ps), 0,
                                                 4 * (t.loc.pe - t.loc.ps), 0x00020000),
               &sm.next_idx[wave][0], (t.block(x + 64) >> a.blocks_lg) * 4);
   };
-  auto lane64 = [](uint32_t l, uint32_t h, int j) {
-    return ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)h, j) << 32) |
-           (uint32_t)__builtin_amdgcn_readlane((int)l, j);
+  struct Place {
+    uint64_t at, scales;  // addresses of its first row and its first scales
+    int rows;
+  };
+  auto block_at = [&](int x) {
+    const int l = x & 63;
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)blk_hi, l);
+    return Place{(uint64_t)(hi & 0xffffu) << 32 | (uint32_t)__builtin_amdgcn_readlane((int)blk_lo, l),
+                 MX ? mx_base + ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)blk_mx, l) << 6) : 0,
+                 (int)(hi >> 16)};
   };
   auto rsrc = [](uint64_t at, int bytes) {
     return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void *>(at), 0, bytes, 0x00020000);
@@ -965,20 +966,22 @@ __global__ __launch_bounds__(W * 64, 2) void window_long_kernel(WindowArgs args)
 #pragma unroll
     for (int c = 0; c < 2; ++c)
 #pragma unroll
-      for (int x = 0; x < 4; ++x) lw.qf[c][x] = colv_t[c] ? lw.qf[c][x] : u32x4{0, 0, 0, 0};
+      for (int x = 0; x < 4; ++x) lw.qf[c][x] = end_col[c] ? lw.qf[c][x] : u32x4{0, 0, 0, 0};
   };
   auto mask = [&](typename Pipe::Scores &s, int b) {
     const int t0 = 16 * t.block(2 * b) + 4 * quad, t1 = 16 * t.block(2 * b + 1) + 4 * quad;
 #pragma unroll
-    for (int c = 0; c < 2; ++c)
+    for (int c = 0; c < 2; ++c) {
+      const int beg = end_col[c] - a.window;
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int tok = (h ? t1 : t0) + i;
           s.s[c][h][i] =
-              tok < end_col[c] && (tok >= beg_col[c] || tok < a.sinks) ? s.s[c][h][i] : -INFINITY;
+              tok < end_col[c] && (tok >= beg || tok < a.sinks) ? s.s[c][h][i] : -INFINITY;
         }
+    }
   };
   const int nb = (t.blocks + 1) >> 1, steps = (nb + G - 1) / G;
   const int nbw = uni(max(0, (min(own_steps, nb) - grp + G - 1) / G));
@@ -1036,10 +1039,9 @@ __global__ __launch_bounds__(W * 64, 2) void window_long_kernel(WindowArgs args)
 #pragma unroll
       for (int y = 0; y < (NW == 4 ? 1 : 2); ++y) {
         const int h = NW == 4 ? (wq & 1) : y;
-        const int l = (2 * b + h) & 63;
-        const int rows = __builtin_amdgcn_readlane(blk_rows, l);
-        const __amdgpu_buffer_rsrc_t r = rsrc(lane64(blk_lo, blk_hi, l),
-                                              rows > 0 ? (rows - 1) * a.row_bytes + kRowBytes<KV> : 0);
+        const Place p = block_at(2 * b + h);
+        const __amdgpu_buffer_rsrc_t r =
+            rsrc(p.at, p.rows > 0 ? (p.rows - 1) * a.row_bytes + kRowBytes<KV> : 0);
         constexpr int kHalf = Pipe::kGroups / 2;
 #pragma unroll
         for (int x = 0; x < kHalf; ++x) {
@@ -1070,28 +1072,28 @@ __global__ __launch_bounds__(W * 64, 2) void window_long_kernel(WindowArgs args)
       place(b);
 #pragma unroll
       for (int y = 0; y < kHalves; ++y) {
-        const int l = (2 * b + (NW == 4 ? (wq & 1) : y)) & 63;
-        const int rows = __builtin_amdgcn_readlane(blk_rows, l);
-        g.w[y] = load16_rows<false>(
-            rsrc(lane64(blk_lo, blk_hi, l), rows > 0 ? (rows - 1) * a.row_bytes + 64 : 0),
-            mx_row(lane) * a.row_bytes + (lane & 3) * 16);
-        g.s[y] = __builtin_amdgcn_raw_buffer_load_b32(rsrc(lane64(mx_lo, mx_hi, l), 4 * rows),
-                                                      4 * mx_row(lane), 0, 0);
+        const Place p = block_at(2 * b + (NW == 4 ? (wq & 1) : y));
+        g.w[y] = load16_rows<false>(rsrc(p.at, p.rows > 0 ? (p.rows - 1) * a.row_bytes + 64 : 0),
+                                    mx_row(lane) * a.row_bytes + (lane & 3) * 16);
+        g.s[y] =
+            __builtin_amdgcn_raw_buffer_load_b32(rsrc(p.scales, 4 * p.rows), 4 * mx_row(lane), 0, 0);
       }
     };
     uint8_t *const group_ring = ring + grp * kSlots * kSlot;
     const int half_at = loads_k ? 4 * Pipe::kKGroup : Pipe::v_group(4) - Pipe::v_group(0);
-    const int put_group = (lane >> 2) & 3;
-    const int put_at = (loads_k ? put_group * Pipe::kKGroup : Pipe::v_group(put_group)) +
-                       (NW == 4 ? (wq & 1) * half_at : 0);
     auto put = [&](int slot, const Share &g) {
+      int l = lane;
+      // (with both halves of a block in flight, places are worked out anew: no registers)
+      if constexpr (kHalves > 1) asm volatile("" : "+v"(l));
+      const int group = (l >> 2) & 3;
+      uint8_t *const at = group_ring + slot + (NW == 4 ? (wq & 1) * half_at : 0) +
+                          (loads_k ? group * Pipe::kKGroup : Pipe::v_group(group));
 #pragma unroll
       for (int y = 0; y < kHalves; ++y) {
-        uint8_t *const at = group_ring + slot + put_at + (NW == 4 ? 0 : y * half_at);
         if (loads_k)
-          put_mx<Pipe, false>(at, lane, g.w[y], g.s[y]);
+          put_mx<Pipe, false>(at + y * half_at, l, g.w[y], g.s[y]);
         else
-          put_mx<Pipe, true>(at, lane, g.w[y], g.s[y]);
+          put_mx<Pipe, true>(at + y * half_at, l, g.w[y], g.s[y]);
       }
     };
     // K (j + 2) and V (j + 1) are written at step j, to slots read at step j - 1.
@@ -1183,7 +1185,7 @@ __global__ __launch_bounds__(W * 64, 2) void window_long_kernel(WindowArgs args)
         for (int i = 0; i < 4; ++i) zs[i] = fmaf(lw.acc[c][e][i], 0.0f, zs[i]);
       }
     const float z = (zs[0] + zs[1]) + (zs[2] + zs[3]);
-    const uint64_t b = __builtin_amdgcn_ballot_w64(colv_t[c] && !(z == 0.0f && L[c] < INFINITY));
+    const uint64_t b = __builtin_amdgcn_ballot_w64(end_col[c] && !(z == 0.0f && L[c] < INFINITY));
     redo |= (uint32_t)((b | b >> 16 | b >> 32 | b >> 48) & 0xffff) << (16 * c);
   }
   if constexpr (G > 1) {
@@ -1194,11 +1196,13 @@ __global__ __launch_bounds__(W * 64, 2) void window_long_kernel(WindowArgs args)
   // O through LDS, each wave its own 32 rows: whole rows go out 16 bytes per lane.
   static_assert(W * 32 * kOutRow <= sizeof(ring), "O staging");
   uint8_t *ot = ring + wave * 32 * kOutRow;
+  int own_col = col;  // (found again: held through the walk it would cost registers)
+  asm volatile("" : "+v"(own_col));
   int row_head[2];  // output row of each tile's column, -1: none
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
-    const bool mine = colv_t[c] && !(redo >> (16 * c + col) & 1);
-    row_head[c] = mine ? (t.loc.qs + qi_t[c]) * a.hq + kvh * a.group + gh_t[c] : -1;
+    const bool mine = end_col[c] && !(redo >> (16 * c + col) & 1);
+    row_head[c] = mine ? out_row(own0 + 16 * c + own_col) : -1;
 #pragma unroll
     for (int e = 0; e < 8; ++e)
       if (e / kOwn == grp)
