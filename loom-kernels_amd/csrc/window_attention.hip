@@ -1260,20 +1260,36 @@ constexpr uint64_t kLongWalk = 2048;  // tokens, from which a join costs little
 //  - two: 32, which share a walk's rows (8 x 32 rows 23.4 / 17.3 / 20.5, whole 94 / 59 / 80;
 //    MXFP4 27.2 / 19.1 / 26.3, whole 81 / 55 / 72, but 8 x 1-32, 300 tiles, 39 / 48: two
 //    workgroups of its 16 fit a CU);
-//  - more: long tiles (8 x 64 rows 42.0 / 30.2 / 21.9, whole 164 / 96 / 92).
-uint64_t row_tile_cols(uint64_t tiles, uint64_t cus, bool mx) {
+//  - more: long tiles (8 x 64 rows under windows of 1024 24 / 21), but where long walks
+//    differ (`uneven`), rows balance them: three per CU (8 x 48 rows, whole prefixes of
+//    1000-4000 tokens, 45 / 50, FP8 42 / 45, 3 x 100 34 / 43), MXFP4 up to seven (8 x 64 48 /
+//    59, 8 x 104 67 / 78, 8 x 128, eight, 76 / 80).
+uint64_t row_tile_cols(uint64_t tiles, uint64_t cus, bool mx, bool uneven) {
   if (4 * tiles <= (mx ? 6 : 5) * cus) return 16;
-  return 4 * tiles <= 9 * cus ? 32 : 0;
+  return 4 * tiles <= (uneven ? (mx ? 28 : 14) : 9) * cus ? 32 : 0;
 }
 
-// Wave groups of the long tiles: as many as `tiles` full ones of 128 columns (or a grid of
-// 64-column ones) leave room for.  Walks over the whole prefix differ, so the longest are
-// cut in two while two workgroups per CU hold all: 4 x 512 rows behind 2048-16384 tokens
-// 370 us in one group, 270 in two (MXFP4 442 / 311), but under windows of 4096, all alike, 142
-// / 160, and 8 x 512 528 / 574.
-uint32_t long_groups(uint64_t tile_cols, uint64_t tiles, uint64_t grid, uint64_t cus, bool whole) {
-  if (tile_cols == 128) return whole && 2 * tiles <= 5 * cus ? 2 : 1;
-  return grid <= cus ? 4 : 2;
+// Columns of the long tiles: 128 where they are two per CU, and for MXFP4, whose rows are
+// widened once per tile, wherever 64-column ones (a grid of `grid64`) are more than one (8 x
+// 80 rows under windows of 1024 30.5 / 37.6, 4 x 300 48 / 58).
+uint64_t long_tile_cols(uint64_t tiles128, uint64_t grid64, uint64_t cus, bool mx) {
+  return tiles128 >= 2 * cus || (mx && grid64 > cus) ? 128 : 64;
+}
+
+// Wave groups of the long tiles, which split a walk: of `tiles` full ones of 128 columns two
+// where walks over the whole prefix differ, while two workgroups per CU hold all (4 x 512
+// rows behind 2048-16384 tokens 330 us in one group, 253 in two, FP8 338 / 264, MXFP4 404 /
+// 290, but under windows of 4096, all alike, 134 / 144, and 8 x 512 277 / 302; with a window
+// past the contexts up to one and a half per CU: 4 x 512 of 600-2500 tokens, two per CU, 54 /
+// 59), or where one per CU holds them (8 x 128 MXFP4 rows under windows of 1024 37 / 33, 4 x
+// 300 48 / 59).  Of 64 columns four where a grid of one per CU holds them, or hardly more for uneven walks (8 x
+// 64 rows, whole prefixes of 1000-4000 tokens, 50 in four, 58 in two; FP8 45 / 53), else two
+// (8 x 80 rows under windows of 1024 28 / 39).
+uint32_t long_groups(uint64_t tile_cols, uint64_t tiles, uint64_t grid, uint64_t cus, uint64_t window,
+                     bool uneven) {
+  if (tile_cols == 128)
+    return tiles <= cus || 2 * tiles <= (window == 0 ? 5 : uneven ? 3 : 0) * cus ? 2 : 1;
+  return grid <= cus || (uneven && 2 * grid <= 3 * cus) ? 4 : 2;
 }
 
 // Waves of a row-tile workgroup: four where its walks do not wait for the CU, whose two to
@@ -1315,7 +1331,9 @@ auto kernel_of(const loom_window_attention_plan &p, uint64_t bytes) {
                                   : window_rows_kernel<KV, 1, 8, false>;
   }
   if (p.info.tile_cols == 128) return p.groups == 2 ? window_long_kernel<KV, 8, 4> : window_long_kernel<KV, 4, 4>;
-  return p.groups == 4 ? window_long_kernel<KV, 8, 2> : window_long_kernel<KV, 4, 2>;
+  if constexpr (KV != kMx4)  // (of 64 columns MXFP4 takes four groups always)
+    if (p.groups == 2) return window_long_kernel<KV, 4, 2>;
+  return window_long_kernel<KV, 8, 2>;
 }
 
 loom_status_t make_plan(const loom::DeviceInfo &dev, const loom_window_attention_spec_t *spec,
@@ -1341,19 +1359,24 @@ loom_status_t make_plan(const loom::DeviceInfo &dev, const loom_window_attention
                            : batch * ((group + tc - 1) / tc);
   };
   const bool mx = s.paged.kv_dtype == LOOM_KV_DTYPE_MXFP4;
+  // tokens of a request, as a rule (of a pool as large as what it holds), and whether long
+  // walks differ with them
+  const uint64_t context =
+      s.paged.max_num_pages * (s.paged.page_size ? s.paged.page_size : loom::kPageSize) / batch;
+  const bool uneven =
+      s.explicit_rows && batch > 1 && context >= 1024 && (s.window == 0 || s.window >= context);
   const uint64_t row_cols =
-      row_tile_cols((s.explicit_rows ? cols / 16 + (batch + 1) / 2 : tiles_of(16)) * hkv, cus, mx);
+      row_tile_cols((s.explicit_rows ? cols / 16 + (batch + 1) / 2 : tiles_of(16)) * hkv, cus, mx, uneven);
   const bool long_tile =
       flags & LOOM_PLAN_PREFILL_TILE_LONG ||
       (!(flags & LOOM_PLAN_PREFILL_TILE_16) && s.explicit_rows && row_cols == 0);
-  const uint64_t tc = !long_tile                      ? (row_cols == 16 || group_cols <= 16 ? 16 : 32)
-                      : (cols / 128) * hkv >= 2 * cus ? 128
-                                                      : 64;
+  const uint64_t tc = long_tile ? long_tile_cols(cols / 128 * hkv, tiles_of(64) * hkv, cus, mx)
+                      : row_cols == 16 || group_cols <= 16 ? 16
+                                                           : 32;
   const uint64_t tiles = tiles_of(tc), grid = tiles * hkv;
-  const uint64_t context = s.paged.max_num_pages * (s.paged.page_size ? s.paged.page_size : loom::kPageSize) / batch;
   const uint64_t seen = s.window && s.window < context ? s.window + s.rows / batch : context;
   const uint64_t walk = std::min(context, seen + std::min(s.sinks, context));
-  const uint32_t groups = long_tile ? long_groups(tc, cols * hkv / 128, grid, cus, s.window == 0) : 1;
+  const uint32_t groups = long_tile ? long_groups(tc, cols * hkv / 128, grid, cus, s.window, uneven) : 1;
   const uint32_t waves = !long_tile ? row_waves(grid, cus, s.window, walk) : (uint32_t)tc / 32 * groups;
   if (grid * (waves * 64) >= (1ull << 32))
     return fail(err, LOOM_PLAN_STATE_COUNT_OUT_OF_RANGE, "window rows", s.rows);

@@ -56,8 +56,10 @@ KERNELS = {
     "32 columns, 4 waves": (*tiles(33, 70, 21), 32, 256),
     "one row, 32 columns, 8 waves": (*tiles(200, 140, hq=32, hkv=1, window=0), 32, 512),
     "one row, 32 columns, 4 waves": (*tiles(500, 20, hq=32, hkv=1), 32, 256),
+    "32 columns, long walks that differ": (*tiles(2, 1100, 700, window=0), 32, 512),
     "64 columns, 2 groups": (*tiles(40, 100, 70), 64, 256),
     "64 columns, 4 groups": (*tiles(1, 1500, 1400), 64, 512),
+    "64 columns, 4 groups, long walks that differ": (*tiles(2, 1200, 1050, window=0), 64, 512),
     "128 columns, 1 group": (*tiles(16, 300, 260, 16, 16), 128, 256),
     "128 columns, 2 groups": (*tiles(16, 300, 260, 16, 16, window=0), 128, 512),
 }
@@ -69,6 +71,10 @@ def test_every_kernel(env, kernel, dtype):
     torch, L = env
     rows, lens, hq, hkv, window, cols, threads = KERNELS[kernel]
     c = Case(41, lens, rows, hq, hkv, window, 3, 16, "NHD", dtype)
+    if dtype == "mxfp4":  # other borders
+        cols, threads = {"64 columns, 2 groups": (128, 512),
+                         "64 columns, 4 groups, long walks that differ": (32, 256)}.get(
+                             kernel, (cols, threads))
     info = c.plan(L).info
     assert (info.tile_cols, info.block_threads) == (cols, threads)
     c.check(*c.run(torch, L), long_tile=cols > 32)
