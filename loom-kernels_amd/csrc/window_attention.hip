@@ -1308,13 +1308,17 @@ uint32_t row_waves(uint64_t grid, uint64_t cus, uint64_t window, uint64_t walk) 
 // least), whose walks hold about `tokens` tokens: at most one per CU, and each with work for
 // its join (2 us): the more CUs stream already, the less another one adds.  (8 x 8 rows, 128
 // tiles of a grid of 192, over whole prefixes of 2500-5000 tokens 55 -> 37 us, FP8 26.6 ->
-// 20.5.)
-int row_splits(uint64_t grid, uint64_t least_grid, uint64_t tokens, int cus, bool mx) {
+// 20.5.)  Walks that may differ (`uneven`) are cut in two up to four tiles on five CUs (24 single
+// tokens of 100-8000, 8 kv-heads, 97 -> 67 us, FP8 64 -> 45, MXFP4 43 -> 32; all of 8000 131 ->
+// 141, 80 -> 87, 60 -> 67; 32 of 100-8000 would take 105 -> 99, 68 -> 66, 54 -> 55, of 3000 64
+// both, 38 both, 27 -> 34).
+int row_splits(uint64_t grid, uint64_t least_grid, uint64_t tokens, bool uneven, uint64_t cus, bool mx) {
   const uint64_t blocks = (tokens + 15) / 16;
-  const uint64_t most = std::min<uint64_t>(
-      kMaxSplits, (uint64_t)cus / std::max<uint64_t>(tokens >= kLongWalk ? least_grid : grid, 1));
+  uint64_t most = cus / std::max<uint64_t>(tokens >= kLongWalk ? least_grid : grid, 1);
+  if (uneven && most == 1 && 5 * grid <= 4 * cus) most = 2;
+  most = std::min<uint64_t>(most, kMaxSplits);
   // 16-row blocks per wave
-  const uint64_t least = std::max<uint64_t>(1, grid * (mx ? 8 : 16) / (uint64_t)cus);
+  const uint64_t least = std::max<uint64_t>(1, grid * (mx ? 8 : 16) / cus);
   return (int)std::max<uint64_t>(1, std::min(most, blocks / (least * 8)));
 }
 
@@ -1526,12 +1530,15 @@ loom_status_t loom_window_attention_enqueue(const loom_window_attention_plan_t *
   if (a.group > 1 && s.rows * (uint64_t)a.group * (uint64_t)a.group < (1ull << 32))
     a.group_inv = (uint32_t)(((1ull << 32) + a.group - 1) / a.group);
   // the tokens that a request's rows see, at most: its window, or the average context
+  const uint64_t context = (uint64_t)a.n_indices * page_rows / pg.batch_size;
   const uint64_t tokens =
-      std::min<uint64_t>((uint64_t)a.window + (uint64_t)a.sinks + s.rows / pg.batch_size,
-                         (uint64_t)a.n_indices * page_rows / pg.batch_size);
+      std::min<uint64_t>((uint64_t)a.window + (uint64_t)a.sinks + s.rows / pg.batch_size, context);
   const uint64_t grid = plan->info.grid_blocks;
   const bool long_tile = plan->info.algorithm == LOOM_PAGED_PREFILL_LONG_TILE;
-  a.splits = long_tile ? 1 : row_splits(grid, plan->least_tiles * pg.num_kv_heads, tokens, plan->cus, mx);
+  a.splits = long_tile ? 1
+                       : row_splits(grid, plan->least_tiles * pg.num_kv_heads, tokens,
+                                    pg.batch_size > 1 && (uint64_t)a.window >= context,
+                                    (uint64_t)plan->cus, mx);
   if (a.splits > 1) {
     a.arrived = scope->queue->joins;
     a.states = (float *)loom::queue_shares(scope, (uint64_t)a.splits * grid * plan->info.tile_cols * kStash * 4);
