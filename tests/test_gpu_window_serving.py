@@ -120,6 +120,31 @@ def test_captured_beside_the_queues_own_commands(env, dtype, rows):
         other.check()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_graph_of_shared_walks(env, dtype):
+    """A graph queue's own capture has words and states of its private queue: every replay
+    is the eager command's, whatever runs between."""
+    torch, L = env
+    c = Case(47, [5000, 3100, 700], None, 8, 2, 0, 0, 16, "HND", dtype)
+    want = c.run(torch, L)
+    gq = L.GraphQueue(0, 2)
+    b = gq.bindings(16)
+    out, lse = c.outputs(torch)
+    plan, args = c.plan(L), c.args(L, b, c.operands(torch), out, lse)
+    torch.cuda.synchronize()
+    graph = gq.capture(b, lambda scope: (plan.enqueue_into(scope, args),
+                                         plan.enqueue_into(scope, args))).instantiate()
+    for i in range(4):
+        out.fill_(7.0)
+        lse.fill_(7.0)
+        torch.cuda.synchronize()
+        graph.launch().wait()
+        assert np.array_equal(host(out), want[0]) and np.array_equal(host(lse), want[1])
+        if i == 1:
+            graph.set_replay_mode("hip_graph_launch")
+        c.run(torch, L)
+
+
 def test_two_queues_at_once(env):
     """Shared walks on two streams: each queue has words and states of its own."""
     torch, L = env
