@@ -808,18 +808,21 @@ __global__ __launch_bounds__(W * 64, KV == kMx4 && CT == 1 && W == 4 ? 4 : 2) vo
 }
 
 // ---- long tiles --------------------------------------------------------------------
-// MXFP4 rows on their way to LDS as BF16 (lane l takes 32 values, block l & 3 of
-// row mx_row(l) of a 16-row block, and the row's scale word).
-// In this order of rows the 16 lanes that LDS writes at once meet each bank once: their
-// rows lie in four groups, 16 bytes further each in K, 32 in V (where lanes of the last two
-// groups write neighbouring units in turn).  With rows in order they shared a quarter of
-// the banks, and the writes took 257 cycles of a step's 310 in LDS.
-__device__ __forceinline__ int mx_row(int lane) { return 4 * ((lane >> 2) & 3) + (lane >> 4); }
-// A lane's 32 values to a slot as BF16; `group`: where the row's group (mx_row / 4) lies.
+// MXFP4 rows on their way to LDS as BF16: lane l takes 32 values, block mx_block(l) of row
+// mx_row(l) of a 16-row block, and the row's scale word.  LDS writes the 16 bytes of 8 lanes at
+// once, to 32 banks: two blocks, 64 bytes apart, of rows of the four groups, 16 bytes further
+// each in K, 32 in V (where lanes of the last two groups write neighbouring units in turn).
+// (Four blocks of two groups shared banks: 122 against 61 million conflict cycles, the rest
+// the fragments' reads, for 16384 rows under a window of 4096, 932 against 927 us; rows in
+// order took 1.1 ms.)
+__device__ __forceinline__ int mx_block(int lane) { return (lane & 1) + ((lane >> 2) & 2); }
+__device__ __forceinline__ int mx_group(int lane) { return (lane >> 1) & 3; }
+__device__ __forceinline__ int mx_row(int lane) { return 4 * mx_group(lane) + (lane >> 4); }
+// A lane's 32 values to a slot as BF16; `group`: where the row's group lies.
 template <class Pipe, bool V>
 __device__ __forceinline__ void put_mx(uint8_t *group, int lane, const u32x4 &w, uint32_t scales) {
-  const int b = lane & 3, r3 = lane >> 4;
-  const bool turn = V && (lane & 8);
+  const int b = mx_block(lane), r3 = lane >> 4;
+  const bool turn = V && (lane & 4);
   uint8_t *const dst = group + r3 * 256 + ((4 * b) ^ Pipe::swizzle(r3)) * 16;
   uint8_t *const even = dst + (turn ? 16 : 0), *const odd = dst + (turn ? 0 : 16);
   const uint32_t scale = mx_scale(scales, b);
@@ -1074,7 +1077,7 @@ __global__ __launch_bounds__(W * 64, 2) void window_long_kernel(WindowArgs args)
       for (int y = 0; y < kHalves; ++y) {
         const Place p = block_at(2 * b + (NW == 4 ? (wq & 1) : y));
         g.w[y] = load16_rows<false>(rsrc(p.at, p.rows > 0 ? (p.rows - 1) * a.row_bytes + 64 : 0),
-                                    mx_row(lane) * a.row_bytes + (lane & 3) * 16);
+                                    mx_row(lane) * a.row_bytes + mx_block(lane) * 16);
         g.s[y] =
             __builtin_amdgcn_raw_buffer_load_b32(rsrc(p.scales, 4 * p.rows), 4 * mx_row(lane), 0, 0);
       }
@@ -1085,7 +1088,7 @@ __global__ __launch_bounds__(W * 64, 2) void window_long_kernel(WindowArgs args)
       int l = lane;
       // (with both halves of a block in flight, places are worked out anew: no registers)
       if constexpr (kHalves > 1) asm volatile("" : "+v"(l));
-      const int group = (l >> 2) & 3;
+      const int group = mx_group(l);
       uint8_t *const at = group_ring + slot + (NW == 4 ? (wq & 1) * half_at : 0) +
                           (loads_k ? group * Pipe::kKGroup : Pipe::v_group(group));
 #pragma unroll
