@@ -276,16 +276,20 @@ __device__ __forceinline__ void exact_column(const WindowArgs &a, const Tile &t,
 }
 
 // ---- row tiles ---------------------------------------------------------------------
-// One workgroup of W waves per (16 or 32 columns, kv-head[, split]).  Wave w takes 32-token steps
-// w, w + W, ... of the walk (of its split's share of it), each through LDS of its own
-// (PipeWave's slot: whole rows, so a load instruction covers whole lines, in an order that
-// spreads the fragment reads over the banks), and the wave states merge in LDS.  Per step:
-// S = K.Q^T in 8 MFMAs of 16x16x32, the softmax with a running maximum that moves only when
-// a score passes it by 2^8, and O^T += V^T.P^T in 16, P as a BF16 high part and a BF16
-// residual (16 bits: few tokens carry a short window, whose errors do not average out).
+// One workgroup of W waves per (16 or 32 columns, kv-head[, split]).  Wave w takes steps w,
+// w + W, ... of the walk (of its split's share of it), of 16 tokens (BF16) or 32, each through
+// LDS of its own (PipeWave's slot: whole rows, so a load instruction covers whole lines, in an
+// order that spreads the fragment reads over the banks), two of them in flight, and the wave
+// states merge in LDS.  Per 32 tokens and 16 columns: S = K.Q^T in 8 MFMAs of 16x16x32, the
+// softmax with a running maximum that moves only when a score passes it by 2^8, and O^T +=
+// V^T.P^T in 16, P as a BF16 high part and a BF16 residual (16 bits: few tokens carry a short
+// window, whose errors do not average out).  Memory bounds the long walks (64 single tokens
+// under windows of 4096 151 us, 6.5 TB/s, FP8 97, MXFP4 71), three dependent round trips
+// (tables, page indices, rows) the short ones: one request's 128 tokens 5.0 us of which an
+// empty command is 3.9.
 // Rows, codes and scales go straight to LDS.  Widened to BF16 on the way, as the long tiles
 // have them, MXFP4 rows cost a wave 360 cycles of LDS per 32 tokens, four times what the
-// codes take (64 single tokens under windows of 4096: 75 us).
+// codes take (8 chunks of a few rows over 4-bit prefixes 39 us, 31 this way).
 constexpr int kStash = 132;  // floats between two columns' O in LDS, and of a split's state
 
 template <Kv KV>
@@ -344,7 +348,8 @@ __device__ __forceinline__ f32x2 load_state(const float *p) {
 }
 
 template <Kv KV, int CT, int W, bool NT>
-__global__ __launch_bounds__(W * 64, KV == kMx4 && CT == 1 && W == 4 ? 4 : 2) void window_rows_kernel(WindowArgs args) {
+__global__ __launch_bounds__(W * 64, KV == kMx4 && CT == 1 && W == 4 ? 4 : 2)
+void window_rows_kernel(WindowArgs args) {
   constexpr int TC = 16 * CT;
   constexpr bool FP8 = KV == kFp8;
   using Pipe = RowPipe<KV>;
@@ -842,7 +847,9 @@ __device__ __forceinline__ void put_mx(uint8_t *group, int lane, const u32x4 &w,
 // of many tokens average out below O's own rounding, and a token that stands alone, whose
 // score the column's reference was taken from, weighs a power of two.  The normalizer sums
 // the weights before their rounding, so LSE keeps FP32's precision.  (Two sums, one for each,
-// take 5 to 20% of the time: registers spill.)
+// take 5 to 20% of the time: registers spill.)  The waves' issue and LDS reads bound long
+// walks (16384 rows under a window of 4096, MXFP4: 927 us, 1040 TFLOP/s, MFMA busy 42%), a
+// tile's beginning and end the short ones (windows of 128: 9 of a tile's 16 us).
 //
 // BF16 and FP8 blocks are loaded straight into the ring, NW slots deep.  MXFP4 codes go
 // through registers, 32 values and their scale per lane and block, two steps ahead, and are
@@ -1285,9 +1292,9 @@ uint64_t long_tile_cols(uint64_t tiles128, uint64_t grid64, uint64_t cus, bool m
 // 290, but under windows of 4096, all alike, 134 / 144, and 8 x 512 277 / 302; with a window
 // past the contexts up to one and a half per CU: 4 x 512 of 600-2500 tokens, two per CU, 54 /
 // 59), or where one per CU holds them (8 x 128 MXFP4 rows under windows of 1024 37 / 33, 4 x
-// 300 48 / 59).  Of 64 columns four where a grid of one per CU holds them, or hardly more for uneven walks (8 x
-// 64 rows, whole prefixes of 1000-4000 tokens, 50 in four, 58 in two; FP8 45 / 53), else two
-// (8 x 80 rows under windows of 1024 28 / 39).
+// 300 48 / 59).  Of 64 columns four where a grid of one per CU holds them, or hardly more
+// for uneven walks (8 x 64 rows, whole prefixes of 1000-4000 tokens, 50 in four, 58 in two;
+// FP8 45 / 53), else two (8 x 80 rows under windows of 1024 28 / 39).
 uint32_t long_groups(uint64_t tile_cols, uint64_t tiles, uint64_t grid, uint64_t cus, uint64_t window,
                      bool uneven) {
   if (tile_cols == 128)
@@ -1337,7 +1344,8 @@ auto kernel_of(const loom_window_attention_plan &p, uint64_t bytes) {
            : past                 ? window_rows_kernel<KV, 1, 8, true>
                                   : window_rows_kernel<KV, 1, 8, false>;
   }
-  if (p.info.tile_cols == 128) return p.groups == 2 ? window_long_kernel<KV, 8, 4> : window_long_kernel<KV, 4, 4>;
+  if (p.info.tile_cols == 128)
+    return p.groups == 2 ? window_long_kernel<KV, 8, 4> : window_long_kernel<KV, 4, 4>;
   if constexpr (KV != kMx4)  // (of 64 columns MXFP4 takes four groups always)
     if (p.groups == 2) return window_long_kernel<KV, 4, 2>;
   return window_long_kernel<KV, 8, 2>;
@@ -1544,7 +1552,8 @@ loom_status_t loom_window_attention_enqueue(const loom_window_attention_plan_t *
                                     (uint64_t)plan->cus, mx);
   if (a.splits > 1) {
     a.arrived = scope->queue->joins;
-    a.states = (float *)loom::queue_shares(scope, (uint64_t)a.splits * grid * plan->info.tile_cols * kStash * 4);
+    a.states = (float *)loom::queue_shares(
+        scope, (uint64_t)a.splits * grid * plan->info.tile_cols * kStash * 4);
     if (!a.states || !a.arrived || grid > loom::kMx4Joins) a.splits = 1;
   }
   uint64_t workgroups = grid * a.splits;
