@@ -406,9 +406,9 @@ void window_rows_kernel(WindowArgs args) {
   const int n = hi - lo > wave ? (hi - lo - wave + W - 1) / W : 0;
 
   // Where the blocks of the wave's steps lie, 64 at a time, one per lane: byte offset of the
-  // first row in K and V (and in the MXFP4 scales), and block << 5 | rows.
-  uint32_t at_lo = 0, at_hi = 0, sc_lo = 0, sc_hi = 0;
-  int meta = 0;
+  // first row in K and V (and in the MXFP4 scales), and block << 5 | rows (blocks have up to
+  // 27 bits: unsigned).
+  uint32_t at_lo = 0, at_hi = 0, sc_lo = 0, sc_hi = 0, meta = 0;
   auto locate = [&](int i0) {
     const int x = H * (lo + wave + W * (i0 + lane / H)) + lane % H;
     const bool in = x < t.blocks;
@@ -425,7 +425,7 @@ void window_rows_kernel(WindowArgs args) {
       sc_lo = (uint32_t)sc;
       sc_hi = (uint32_t)(sc >> 32);
     }
-    meta = b << 5 | rows;
+    meta = (uint32_t)b << 5 | (uint32_t)rows;
   };
   auto lane64 = [&](uint32_t l, uint32_t h, int j) {
     return ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)h, j) << 32) |
@@ -451,7 +451,7 @@ void window_rows_kernel(WindowArgs args) {
 #pragma unroll
     for (int h = 0; h < H; ++h) {
       const int j = H * i + h;
-      const int rows = __builtin_amdgcn_readlane(meta, j) & 31;
+      const int rows = __builtin_amdgcn_readlane((int)meta, j) & 31;
       const uint64_t at = lane64(at_lo, at_hi, j);
       const int bytes = rows > 0 ? (rows - 1) * a.row_bytes + kRowBytes<KV> : 0;
       const __amdgpu_buffer_rsrc_t rk = rsrc(a.k, at, bytes), rv = rsrc(a.v, at, bytes);
@@ -556,7 +556,7 @@ void window_rows_kernel(WindowArgs args) {
     bool full = true;
 #pragma unroll
     for (int h = 0; h < H; ++h) {
-      t0[h] = (__builtin_amdgcn_readlane(meta, H * i + h) >> 5) * 16;
+      t0[h] = (int)((uint32_t)__builtin_amdgcn_readlane((int)meta, H * i + h) >> 5) * 16;
       full &= t0[h] >= full_beg && t0[h] + 16 <= full_end;
     }
     if (!full) {
