@@ -557,7 +557,7 @@ void window_rows_kernel(WindowArgs args) {
 #pragma unroll
     for (int h = 0; h < H; ++h) {
       t0[h] = (int)((uint32_t)__builtin_amdgcn_readlane((int)meta, H * i + h) >> 5) * 16;
-      full &= t0[h] >= full_beg && t0[h] + 16 <= full_end;
+      full &= t0[h] >= full_beg && t0[h] <= full_end - 16;  // (t0 + 16 may be 2^31)
     }
     if (!full) {
 #pragma unroll

@@ -45,3 +45,14 @@ def test_positions_past_2_30(env, length, window, sinks, dtype, form):
     count."""
     c = Case(61, [64 * 20 + length % 64], FORMS[form][0], 8, 2, window, sinks, 64, "HND", dtype)
     check(env, c, form, length)
+
+
+@pytest.mark.parametrize("form", ["one row", "rows", "rows, long tile"])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("sinks", [0, 4, 17])
+def test_the_last_position(env, sinks, dtype, form):
+    """The last token that a table of 16-row pages holds, walks of an odd number of blocks
+    and of an even one: behind the last block a pair's second half would begin at
+    2^31 - 16 and end at 2^31."""
+    c = Case(62, [16 * 9], FORMS[form][0] and [1], 8, 2, 40, sinks, 16, "NHD", dtype)
+    check(env, c, form, (1 << 31) - 16)
