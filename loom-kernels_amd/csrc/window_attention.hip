@@ -258,20 +258,21 @@ __device__ __forceinline__ void exact_column(const WindowArgs &a, const Tile &t,
       if (s == -INFINITY) continue;
       const float mn = fmax_nan(m, s), old = m == -INFINITY ? 0.0f : fast_exp2(m - mn);
       const float p = fast_exp2(s - mn);  // (NaN at +inf)
-      l = fmaf(l, old, p);
-      // (where a sum is infinite and its weight vanishes, it has no part either)
-      o0 = old == 0.0f ? 0.0f : o0 * old;
-      o1 = old == 0.0f ? 0.0f : o1 * old;
-      if (p != 0.0f) {
-        o0 = fmaf(p, v0, o0);
-        o1 = fmaf(p, v1, o1);
+      // The mean so far and the token's part of it: O stays within V's range, where sums
+      // of p v may pass FP32's.  (What weighs nothing has no part, infinite or not.)
+      const float ln = fmaf(l, old, p), keep = l * old / ln, part = p / ln;
+      o0 = keep == 0.0f ? 0.0f : o0 * keep;
+      o1 = keep == 0.0f ? 0.0f : o1 * keep;
+      if (part != 0.0f) {
+        o0 = fmaf(part, v0, o0);
+        o1 = fmaf(part, v1, o1);
       }
+      l = ln;
       m = mn;
     }
   }
-  const float inv = 1.0f / l;
   *reinterpret_cast<uint32_t *>(a.out + row * 128 + 2 * lane) =
-      bf16x2_pack(l == 0.0f ? NAN : o0 * inv * v_scale, l == 0.0f ? NAN : o1 * inv * v_scale);
+      bf16x2_pack(l == 0.0f ? NAN : o0 * v_scale, l == 0.0f ? NAN : o1 * v_scale);
   if (lane == 0) a.lse[row] = m + __log2f(l);
 }
 
