@@ -1333,6 +1333,13 @@ int row_splits(uint64_t grid, uint64_t least_grid, uint64_t tokens, bool uneven,
   return (int)std::max<uint64_t>(1, std::min(most, blocks / (least * 8)));
 }
 
+// Workgroups that are launched for `workgroups` with work: of MXFP4 row tiles over an even
+// number of kv-heads whole groups of 16, see WindowArgs::pair_heads.
+bool pairs_heads(bool mx_rows, uint64_t hkv) { return mx_rows && hkv % 2 == 0; }
+uint64_t launched(uint64_t workgroups, bool mx_rows, uint64_t hkv) {
+  return pairs_heads(mx_rows, hkv) ? (workgroups + 15) / 16 * 16 : workgroups;
+}
+
 template <Kv KV>
 auto kernel_of(const loom_window_attention_plan &p, uint64_t bytes) {
   if (p.info.algorithm != LOOM_PAGED_PREFILL_LONG_TILE) {
@@ -1394,7 +1401,7 @@ loom_status_t make_plan(const loom::DeviceInfo &dev, const loom_window_attention
   const uint64_t walk = std::min(context, seen + std::min(s.sinks, context));
   const uint32_t groups = long_tile ? long_groups(tc, cols * hkv / 128, grid, cus, s.window, uneven) : 1;
   const uint32_t waves = !long_tile ? row_waves(grid, cus, s.window, walk) : (uint32_t)tc / 32 * groups;
-  if (grid * (waves * 64) >= (1ull << 32))
+  if (launched(grid, mx && !long_tile, hkv) * (waves * 64) >= (1ull << 32))
     return fail(err, LOOM_PLAN_STATE_COUNT_OUT_OF_RANGE, "window rows", s.rows);
   auto *p = new loom_window_attention_plan;
   p->info.spec = s;
@@ -1557,9 +1564,8 @@ loom_status_t loom_window_attention_enqueue(const loom_window_attention_plan_t *
         scope, (uint64_t)a.splits * grid * plan->info.tile_cols * kStash * 4);
     if (!a.states || !a.arrived || grid > loom::kMx4Joins) a.splits = 1;
   }
-  uint64_t workgroups = grid * a.splits;
-  a.pair_heads = mx && !long_tile && a.hkv % 2 == 0 ? (int32_t)workgroups : 0;
-  if (a.pair_heads) workgroups = (workgroups + 15) / 16 * 16;
+  const uint64_t parts = grid * a.splits, workgroups = launched(parts, mx && !long_tile, pg.num_kv_heads);
+  a.pair_heads = pairs_heads(mx && !long_tile, pg.num_kv_heads) ? (int32_t)parts : 0;
   const dim3 blocks((unsigned)workgroups), threads(plan->info.block_threads);
   hipStream_t stream = scope->queue->stream;
   a.sorted = workgroups > (uint64_t)plan->cus;
