@@ -554,12 +554,14 @@ void window_rows_kernel(WindowArgs args) {
         }
     }
     int t0[H];
-    bool full = true;
+    int t_min = INT32_MAX, t_max = 0;
 #pragma unroll
     for (int h = 0; h < H; ++h) {
       t0[h] = (int)((uint32_t)__builtin_amdgcn_readlane((int)meta, H * i + h) >> 5) * 16;
-      full &= t0[h] >= full_beg && t0[h] <= full_end - 16;  // (t0 + 16 may be 2^31)
+      t_min = min(t_min, t0[h]);
+      t_max = max(t_max, t0[h]);
     }
+    const bool full = t_min >= full_beg && t_max <= full_end - 16;  // (t0 + 16 may be 2^31)
     if (!full) {
 #pragma unroll
       for (int x = 0; x < CT; ++x)
