@@ -209,19 +209,38 @@ __device__ __forceinline__ uint64_t scale_at(const WindowArgs &a, int page, int 
           (uint32_t)row) * 4;
 }
 
+// FP8: takes the pages' k_scale into scale_log2 and returns what the queries are multiplied
+// with besides, exactly: 1, and for a scale of 0 or below 0 or -1.  The kernels mask and
+// compare scores before the scale is multiplied in, which has to keep their order.
+template <Kv KV>
+__device__ __forceinline__ float take_key_scale(WindowArgs &a) {
+  if constexpr (KV != kFp8) return 1.0f;
+  const float scale = a.scale_log2 * a.kv_scales[0];
+  if (scale != 0.0f) a.scale_log2 = fabsf(scale);
+  return scale < 0.0f ? -1.0f : scale == 0.0f ? 0.0f : 1.0f;
+}
+__device__ __forceinline__ u32x4 times(const u32x4 &q, float factor) {
+  u32x4 r;
+#pragma unroll
+  for (int x = 0; x < 4; ++x)
+    r[x] = pack_hi16(__float_as_uint(bf16_lo(q[x]) * factor), __float_as_uint(bf16_hi(q[x]) * factor));
+  return r;
+}
+
 // One column's O and LSE token by token, by one wave: for columns whose O is not finite.
 // The tiles' products multiply a hidden token's V with a weight of zero, which is not
 // zero where V is infinite or NaN; here hidden tokens, and weights of zero, have no part.
 // (Not made to be fast: about 0.15 us per token.)
 template <Kv KV>
-__device__ __forceinline__ void exact_column(const WindowArgs &a, const Tile &t, int f, int lane,
-                                             float v_scale) {
+__device__ __forceinline__ void exact_column(const WindowArgs &args, const Tile &t, int f, int lane) {
+  WindowArgs a = args;
+  const float factor = take_key_scale<KV>(a), v_scale = KV == kFp8 ? a.kv_scales[1] : 1.0f;
   const int qi = row_of(a, f);
   const int64_t row = (int64_t)(t.loc.qs + qi) * a.hq + (int64_t)t.loc.kvh * a.group + (f - qi * a.group);
   const int end = t.kv_len - t.group_rows + qi + 1, beg = max(0, end - a.window);
   const int sinks = min(a.sinks, beg), n = sinks + end - beg;
   const uint32_t qw = *reinterpret_cast<const uint32_t *>(a.q + row * 128 + 2 * lane);
-  const float q0 = bf16_lo(qw), q1 = bf16_hi(qw);
+  const float q0 = bf16_lo(qw) * factor, q1 = bf16_hi(qw) * factor;
   float m = -INFINITY, l = 0.0f, o0 = 0.0f, o1 = 0.0f;
   auto pair = [&](const uint16_t *base, const uint8_t *mx, uint64_t at, uint64_t sc, float &x, float &y) {
     const uint8_t *b = reinterpret_cast<const uint8_t *>(base) + at;
@@ -358,11 +377,7 @@ void window_rows_kernel(WindowArgs args) {
   constexpr int H = kStepBlocks<KV>, kPlaced = 64 / H;  // steps placed at once
   __shared__ RowsSmem<KV, CT, W> sm;
   WindowArgs a = args;
-  float v_scale = 1.0f;
-  if constexpr (FP8) {
-    a.scale_log2 *= a.kv_scales[0];
-    v_scale = a.kv_scales[1];
-  }
+  const float q_factor = take_key_scale<KV>(a), v_scale = FP8 ? a.kv_scales[1] : 1.0f;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = uni(tid >> 6);
   const int col = lane & 15, quad = lane >> 4;
@@ -652,6 +667,11 @@ void window_rows_kernel(WindowArgs args) {
     const int c = min(kPlaced, n - i0);
     if (c > 0) locate(i0);
     if (i0 == 0) bad = bad_page(a, own_page);
+    if (i0 == 0 && q_factor != 1.0f)
+#pragma unroll
+      for (int x = 0; x < CT; ++x)
+#pragma unroll
+        for (int y = 0; y < 4; ++y) pw.qf[x][y] = times(pw.qf[x][y], q_factor);
     // (queries and index words have arrived: no wait of the compiler's in the walk)
 #pragma unroll
     for (int x = 0; x < CT; ++x)
@@ -791,7 +811,7 @@ void window_rows_kernel(WindowArgs args) {
     }
   }
   // Columns that are not finite are found token by token.  (The normalizer alone overflows
-  // where a negative FP8 scale makes a reference of the lowest scores and V is zero.)
+  // over a V of zeros where scores of 2^31 are off by more than 2^7 in FP32.)
 #pragma unroll
   for (int y = 0; y < kItems; ++y) {
     const int c0 = 2 * (y * W + wave);  // the wave's two columns
@@ -810,8 +830,9 @@ void window_rows_kernel(WindowArgs args) {
       if (d == 0) a.lse[row] = ms[y] + __log2f(ls[y]);
     }
     if (redo)
+#pragma unroll 1
       for (int x = 0; x < 2; ++x)
-        if ((uint32_t)(redo >> (32 * x))) exact_column<KV>(a, t, t.col0 + c0 + x, lane, v_scale);
+        if ((uint32_t)(redo >> (32 * x))) exact_column<KV>(args, t, t.col0 + c0 + x, lane);
   }
 }
 
@@ -881,11 +902,7 @@ __global__ __launch_bounds__(W * 64, 2) void window_long_kernel(WindowArgs args)
   __shared__ LongSmem<W, NW> sm;
   __shared__ __align__(16) uint8_t ring[std::max({kRingBytes, kMergeBytes, kOutBytes})];
   WindowArgs a = args;
-  float v_scale = 1.0f;
-  if constexpr (FP8) {
-    a.scale_log2 *= a.kv_scales[0];
-    v_scale = a.kv_scales[1];
-  }
+  const float q_factor = take_key_scale<KV>(a), v_scale = FP8 ? a.kv_scales[1] : 1.0f;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = uni(tid >> 6);
   const int col = lane & 15, quad = lane >> 4;
@@ -980,6 +997,11 @@ __global__ __launch_bounds__(W * 64, 2) void window_long_kernel(WindowArgs args)
     for (int c = 0; c < 2; ++c)
 #pragma unroll
       for (int x = 0; x < 4; ++x) lw.qf[c][x] = end_col[c] ? lw.qf[c][x] : u32x4{0, 0, 0, 0};
+    if (q_factor != 1.0f)
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) lw.qf[c][x] = times(lw.qf[c][x], q_factor);
   };
   auto mask = [&](typename Pipe::Scores &s, int b) {
     const int t0 = 16 * t.block(2 * b) + 4 * quad, t1 = 16 * t.block(2 * b + 1) + 4 * quad;
@@ -1238,7 +1260,7 @@ __global__ __launch_bounds__(W * 64, 2) void window_long_kernel(WindowArgs args)
   }
   if (redo)
     for (int c = grp; c < 32; c += G)
-      if (redo >> c & 1) exact_column<KV>(a, t, own0 + c, lane, v_scale);
+      if (redo >> c & 1) exact_column<KV>(args, t, own0 + c, lane);
 }
 
 }  // namespace
