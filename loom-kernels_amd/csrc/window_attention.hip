@@ -259,11 +259,11 @@ __device__ __forceinline__ void exact_column(const WindowArgs &args, const Tile 
       y = bf16_hi(w);
     }
   };
-  for (int i0 = 0; i0 < n; i0 += 64) {
-    const int i = min(i0 + lane, n - 1), tok = i < sinks ? i : i - sinks + beg;
+  for (int left = n; left > 0; left -= 64) {  // (counted down: a count up may pass 2^31 - 1)
+    const int i = n - left + min(lane, left - 1), tok = i < sinks ? i : i - sinks + beg;
     const int pages = a.indices[t.loc.ps + (tok >> (a.blocks_lg + 4))];
     const int in_page = tok & (a.page_rows - 1);
-    const int c = min(64, n - i0);
+    const int c = min(64, left);
     for (int j = 0; j < c; ++j) {
       const int page = __builtin_amdgcn_readlane(pages, j), r = __builtin_amdgcn_readlane(in_page, j);
       const uint64_t at = row_at<KV>(a, page, r, t.loc.kvh), sc = scale_at(a, page, r, t.loc.kvh);
