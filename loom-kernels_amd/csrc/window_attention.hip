@@ -230,7 +230,7 @@ __device__ __forceinline__ u32x4 times(const u32x4 &q, float factor) {
 // One column's O and LSE token by token, by one wave: for columns whose O is not finite.
 // The tiles' products multiply a hidden token's V with a weight of zero, which is not
 // zero where V is infinite or NaN; here hidden tokens, and weights of zero, have no part.
-// (Not made to be fast: about 0.15 us per token.)
+// (Not made to be fast: 0.5 us per token, up to the first score that is no number.)
 template <Kv KV>
 __device__ __forceinline__ void exact_column(const WindowArgs &args, const Tile &t, int f, int lane) {
   WindowArgs a = args;
@@ -288,6 +288,10 @@ __device__ __forceinline__ void exact_column(const WindowArgs &args, const Tile 
       }
       l = ln;
       m = mn;
+      if (!(l == l)) {  // no number, which no later token changes
+        left = 0;
+        break;
+      }
     }
   }
   *reinterpret_cast<uint32_t *>(a.out + row * 128 + 2 * lane) =
