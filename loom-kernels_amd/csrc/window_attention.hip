@@ -306,8 +306,8 @@ __device__ __forceinline__ void exact_column(const WindowArgs &args, const Tile 
 // order that spreads the fragment reads over the banks), two of them in flight, and the wave
 // states merge in LDS.  Per 32 tokens and 16 columns: S = K.Q^T in 8 MFMAs of 16x16x32, the
 // softmax with a running maximum that moves only when a score passes it by 2^8, and O^T +=
-// V^T.P^T in 16, P as a BF16 high part and a BF16 residual (16 bits: few tokens carry a short
-// window, whose errors do not average out).  Memory bounds the long walks (64 single tokens
+// V^T.P^T in 16, P as a BF16 high part and a BF16 residual (16 bits: the roundings of a short
+// window's few weights do not average out, see the long tiles').  Memory bounds the long walks (64 single tokens
 // under windows of 4096 151 us, 6.5 TB/s, FP8 97, MXFP4 71), three dependent round trips
 // (tables, page indices, rows) the short ones: one request's 128 tokens 5.0 us of which an
 // empty command is 3.9.
@@ -869,15 +869,19 @@ __device__ __forceinline__ void put_mx(uint8_t *group, int lane, const u32x4 &w,
 
 // Many rows: the pipelined long tiles of paged prefill (PipeWave: 32 columns per wave, NW
 // waves over 32 * NW columns, G = W / NW groups of them that split the walk) over the
-// blocks of the walk, in 32-token steps of two blocks each.  Two steps at most at either end of
-// the window, and the sinks', hide tokens from some columns and are masked; the steps
-// between take PipeWave's unmasked path.  P is rounded once to BF16 for the product: the errors
-// of many tokens average out below O's own rounding, and a token that stands alone, whose
-// score the column's reference was taken from, weighs a power of two.  The normalizer sums
-// the weights before their rounding, so LSE keeps FP32's precision.  (Two sums, one for each,
-// take 5 to 20% of the time: registers spill.)  The waves' issue and LDS reads bound long
-// walks (16384 rows under a window of 4096, MXFP4: 927 us, 1040 TFLOP/s, MFMA busy 42%), a
-// tile's beginning and end the short ones (windows of 128: 9 of a tile's 16 us).
+// blocks of the walk, in 32-token steps of two blocks each.  A wave masks the sinks' steps,
+// those from the walk's begin (the tile's first row's window) to its own last row's, up to
+// five where a group is one head, and two at the end; the steps between take PipeWave's
+// unmasked path.  (A step whose tokens are all hidden from a column that has seen none yet
+// takes the branch that moves the reference.)  P is rounded once to BF16 for the product, as
+// in the other long tiles, which adds to O's error against 64 bits (rms, O's own rounding
+// among it) 6 to 9% under windows of 2-16 tokens, 3% of 64, 2% of 128 and 1% from 1024 on,
+// where the errors of many tokens average out; row tiles (tile_cols 16) add nothing.  The
+// normalizer sums the weights before their rounding, so LSE keeps FP32's precision.  (Two
+// sums, one for each, take 5 to 20% of the time: registers spill.)  The waves' issue and LDS
+// reads bound long walks (16384 rows under a window of 4096, MXFP4: 926 us, 1040 TFLOP/s,
+// MFMA busy 42%), a tile's beginning and end the short ones (windows of 128: 9 of a tile's
+// 16 us).
 //
 // BF16 and FP8 blocks are loaded straight into the ring, NW slots deep.  MXFP4 codes go
 // through registers, 32 values and their scale per lane and block, two steps ahead, and are
@@ -1303,6 +1307,11 @@ constexpr uint64_t kLongWalk = 2048;  // tokens, from which a join costs little
 //    differ (`uneven`), rows balance them: three per CU (8 x 48 rows, whole prefixes of
 //    1000-4000 tokens, 45 / 50, FP8 42 / 45, 3 x 100 34 / 43), MXFP4 up to seven (8 x 64 48 /
 //    59, 8 x 104 67 / 78, 8 x 128, eight, 76 / 80).
+// `uneven` is a guess: the plan sees no lengths, and takes the pool for what the requests
+// hold.  Walks over whole prefixes that are all alike lose by it (8 x 48 rows behind 3000
+// tokens 58 / 37, MXFP4 58 / 45, 8 x 100 92 / 61), and so do short ones in a pool ten times
+// what they need (8 x 48 behind 300 17 / 13, MXFP4 8 x 100 22 / 17, 8 x 64 14 / 16); a
+// caller who knows them sets the tile.
 uint64_t row_tile_cols(uint64_t tiles, uint64_t cus, bool mx, bool uneven) {
   if (4 * tiles <= (mx ? 6 : 5) * cus) return 16;
   return 4 * tiles <= (uneven ? (mx ? 28 : 14) : 9) * cus ? 32 : 0;
